@@ -13,6 +13,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libkda_mi355x.so"
 HEADER = PKG.parent / "include" / "kda_mi355x.h"
+LATENT_HEADER = PKG.parent / "include" / "latent_mi355x.h"
 
 KDA_OK = 0
 KDA_ERR_INVALID_ARGUMENT = -1
@@ -30,6 +31,7 @@ KDA_STATUS_NONFINITE = 65536
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
 
@@ -75,11 +77,24 @@ _SIGNATURES = {
     "kda_abi_version": (_i, []),
 }
 
-# Entry points of this binding's own, outside the C ABI of the header: the two
+# The C ABI of include/latent_mi355x.h
+_LATENT = {
+    "kda_latent_attn_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp] + [_i] * 7 + [_f, _i]),
+    "kda_latent_attn_bwd": (_i, [_vp] * 7 + [_i32] + [_vp] * 6 + [_i] * 7 + [_f, _i, _vp, _sz]),
+    "kda_latent_attn_bwd_workspace": (_sz, [_i] * 5),
+    "kda_latent_append": (_i, [_vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _f, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                               _i, _i, _i, _i, _i, _i]),
+    "kda_latent_decode": (_i, [_vp] * 7 + [_i] * 5 + [_i64, _i, _i, _f, _i, _vp, _sz]),
+    "kda_latent_decode_workspace": (_sz, [_i] * 8),
+}
+
+# Entry points outside the C ABI of kda_mi355x.h: those of latent_mi355x.h, and
+# the binding's own (neither header's): the two
 # backward calls whose outputs may be rounded to the primals' 16-bit types by
 # the kernels that form them, and the seam's backward with the workspace its
 # direct form needs (axiom_amd/csrc/kda_internal.h)
 _PRIVATE = {
+    **_LATENT,
     "axiom_chunk_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                              _vp, _vp, _vp, _vp, _vp, _vp,
                              _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _i, _vp, _sz]),
@@ -90,9 +105,9 @@ _PRIVATE = {
 _lib = None
 
 
-def header_symbols() -> list[str]:
-    """Names of every entry point ``include/kda_mi355x.h`` declares."""
-    text = HEADER.read_text()
+def header_symbols(header: Path = HEADER) -> list[str]:
+    """Names of every entry point a header (``include/kda_mi355x.h``) declares."""
+    text = header.read_text()
     return re.findall(r"^KDA_API\s+[\w\s\*]+?\b(kda_\w+)\s*\(", text, flags=re.M)
 
 

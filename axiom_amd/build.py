@@ -33,7 +33,8 @@ HIPCC_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wno-unused-command-line-argument",
 ]
-SOURCES = ["kda_chunk.hip", "kda_varlen.hip", "kda_decode.hip", "kda_bwd.hip", "kda_ut.hip", "kda_prologue.hip", "kda_api.hip"]
+SOURCES = ["kda_chunk.hip", "kda_varlen.hip", "kda_decode.hip", "kda_bwd.hip", "kda_ut.hip", "kda_prologue.hip",
+           "kda_latent_fwd.hip", "kda_latent_bwd.hip", "kda_latent_decode.hip", "kda_latent_api.hip", "kda_api.hip"]
 
 
 def _hipcc() -> str:

@@ -689,6 +689,8 @@ int scratch_for_stream(hipStream_t stream, void** out) {
   return KDA_OK;
 }
 
+int kda::api_fail(int code, const char* msg) { return fail(code, "%s", msg); }
+
 extern "C" {
 
 int kda_abi_version(void) { return 102; }

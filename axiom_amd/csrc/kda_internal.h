@@ -288,6 +288,76 @@ struct CcFinishArgs {
 };
 hipError_t launch_cc_finish(const CcFinishArgs& a, hipStream_t s);
 
+// Sets the calling thread's error message and returns `code` (kda_last_error).
+int api_fail(int code, const char* msg);
+
+// Latent attention, expanded form.  Strides in elements; the last axis of every
+// tensor is contiguous.  o, dout, dq are [B,Tq,H,*] and dkv [B,Tk,H,2 dn],
+// dkr [B,Tk,dr] contiguous; lse, D are [B,H,Tq] fp32.  Packed calls (cu_q
+// non-null): B == 1 and n_seqs sequences, rows cu[i] .. cu[i+1].
+struct LatentArgs {
+  const void* q;           // [B,Tq,H,dn+dr]
+  const void* kv;          // [B,Tk,H,dn+dn]: nope key | value
+  const void* kr;          // [B,Tk,dr]: the rotary key of all heads
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int n_seqs;
+  int B, Tq, Tk, H;
+  int64_t q_b, q_t, q_h, kv_b, kv_t, kv_h, kr_b, kr_t;
+  int causal;
+  float scale;
+  void* o;
+  float* lse;
+  // backward
+  const void* o_in;
+  const void* dout;
+  const float* lse_in;
+  float* D;                // sum over dn of do * o
+  float* dmax;             // fp16: largest |do| of each 128-row block, [B*H][ceil(Tq / 128)]
+  int dmax_n;              // its blocks
+  float* dkr_part;         // [B,H,Tk,dr]: each head's share of the rotary key's gradient
+  void* dq;
+  void* dkv;
+  void* dkr;
+};
+hipError_t launch_latent_fwd(const LatentArgs& a, int dn, int dr, int dt, hipStream_t s);
+hipError_t launch_latent_bwd(const LatentArgs& a, int dn, int dr, int dt, hipStream_t s);
+
+// New rows of the latent cache: RMS norm of the first R elements (w null: none),
+// rotation of the last dr, stored at row slots[i] of the cache (outside
+// [0, n_slots): not stored); the queries' rotary parts rotated to q_out.
+struct LatentAppendArgs {
+  const void* rows;        // [N, R+dr], row stride rows_t
+  const int64_t* positions;  // [N]
+  const int64_t* slots;    // [N]
+  const float* cos_sin;    // [P, dr]: cos of the dr/2 angles | sin
+  const float* w;          // [R] or null
+  void* cache;             // [n_slots, R+dr]
+  const void* q;           // [N, H, dr] with strides, or null
+  void* q_out;
+  int64_t rows_t, q_t, q_h, qo_t, qo_h, n_slots, P;
+  int N, H, interleaved;
+  float eps;
+};
+hipError_t launch_latent_append(const LatentAppendArgs& a, int R, int dr, int dt, hipStream_t s);
+
+// Latent attention, absorbed form over the paged cache.
+struct LatentDecodeArgs {
+  const void* q;           // [B,Tq,H,R+dr]
+  const void* cache;       // [n_pages, page, R+dr]
+  const int32_t* table;    // [B, per]
+  const int32_t* lens;     // [B]
+  void* o;                 // [B,Tq,H,R]
+  float* lse;              // [B,Tq,H]
+  float* part_o;           // partial results of split sequences
+  float* part_ml;
+  int B, Tq, H, per, page_shift;
+  int64_t n_pages;
+  int groups, wgs;         // row groups of a sequence; workgroups along the cache
+  float scale;
+};
+hipError_t launch_latent_decode(const LatentDecodeArgs& a, int R, int dr, int dt, int nb, hipStream_t s);
+
 }  // namespace kda
 
 // Entry points of the package's own binding (axiom_amd/_lib.py), outside the C

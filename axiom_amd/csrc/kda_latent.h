@@ -1,0 +1,220 @@
+// Device helpers of the latent-attention kernels (gfx950 / CDNA4 only).
+//
+// The kernels work on 32 x 32 score tiles (v_mfma_f32_32x32x16, fp32: eight
+// v_mfma_f32_32x32x2 on the same registers).  Lane l of a wave has m = l & 31
+// and half h = l >> 5; an operand fragment is 8 elements of a 16-wide
+// contraction block, and the accumulator's 16 values of a lane are rows
+// 8 (i >> 2) + 4 h + (i & 3), i = 0..15, of column m.  Two fragment orders:
+//   * row fragment (contraction along a row): element j is column 8 h + j;
+//   * column fragment (contraction over rows): element j is row
+//     8 (j >> 2) + 4 h + (j & 3), the accumulator's own row order, so a score
+//     tile (or its adjoint) is the second operand of the next product with
+//     no exchange between lanes, and the first operand is read with its rows
+//     transposed (ds_read_b64_tr_b16: a group of 16 lanes reads 4 rows of 16
+//     columns and each lane gets one column).
+//
+// LDS tiles are row-major without padding, because direct global->LDS copies
+// write 1 KiB of consecutive bytes per wave instruction; bank conflicts are
+// kept out by a permutation of the 16-byte chunks inside each row instead
+// (chunk c of row r sits at c ^ swz(r)), applied to the copies' source
+// addresses.  swz is distinct over 8 consecutive rows (row fragments) and
+// differs above its lowest bit over 4 (transposed reads of chunk pairs).
+#pragma once
+
+#include "kda_common.h"
+
+namespace kda {
+namespace latent {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4v* lds_s4;
+
+constexpr float kLn2 = 0.6931471805599453f;
+// finite start of the running maximum: exp2 of a masked (-inf) score minus it is 0
+constexpr float kMaxInit = -1e30f;
+// The running maximum is raised (and the accumulators rescaled) only when a
+// tile exceeds it by more than 2^kLazy: probabilities then reach at most
+// 2^8, in range for the 16-bit operands and without loss, since the row sum is
+// kept in fp32 and both are divided at the end.
+constexpr float kLazy = 8.f;
+
+template <int DT> struct El;
+template <> struct El<0> { typedef float t; typedef f8 frag; static constexpr int ES = 4; };
+template <> struct El<1> { typedef u16 t; typedef b8 frag; static constexpr int ES = 2; };
+template <> struct El<2> { typedef u16 t; typedef h8 frag; static constexpr int ES = 2; };
+
+__device__ __forceinline__ f16v mma(f16v c, const f8& a, const f8& b) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ f16v mma(f16v c, const b8& a, const b8& b) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mma(f16v c, const h8& a, const h8& b) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// the 16 x 16 forms (32-wide contraction; same fragment rules with four lane groups)
+__device__ __forceinline__ f4 mma_s(f4 c, const f8& a, const f8& b) { return mma32(c, a, b); }
+__device__ __forceinline__ f4 mma_s(f4 c, const b8& a, const b8& b) { return mma32_bf16(c, a, b); }
+__device__ __forceinline__ f4 mma_s(f4 c, const h8& a, const h8& b) { return mma32(c, a, b); }
+
+// eight fp32 values to a fragment (round to nearest even)
+template <int DT>
+__device__ __forceinline__ typename El<DT>::frag to_frag(const float (&x)[8]) {
+  typename El<DT>::frag r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if constexpr (DT == 0) r[j] = x[j];
+    else if constexpr (DT == 1) r[j] = static_cast<__bf16>(x[j]);
+    else r[j] = static_cast<_Float16>(x[j]);
+  }
+  return r;
+}
+
+// four fp32 values to four consecutive elements of global memory
+template <int DT>
+__device__ __forceinline__ void store4(void* p, int64_t i, float a, float b, float c, float d) {
+  if constexpr (DT == 0) {
+    *reinterpret_cast<f4*>(static_cast<float*>(p) + i) = f4{a, b, c, d};
+  } else if constexpr (DT == 1) {
+    *reinterpret_cast<uint2*>(static_cast<u16*>(p) + i) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+  } else {
+    const h4 v = {static_cast<_Float16>(a), static_cast<_Float16>(b), static_cast<_Float16>(c), static_cast<_Float16>(d)};
+    *reinterpret_cast<uint2*>(static_cast<u16*>(p) + i) = __builtin_bit_cast(uint2, v);
+  }
+}
+
+// value combined over the two halves of the wave (lane l and l ^ 32)
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Direct global->LDS copy of 16 or 4 bytes a lane, to 64 consecutive places from
+// dst on (wave-uniform).
+__device__ __forceinline__ void copy16(const char* src, char* dst) { __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0); }
+__device__ __forceinline__ void copy4(const void* src, char* dst) { __builtin_amdgcn_global_load_lds(src, dst, 4, 0, 0); }
+
+// An LDS tile of rows of W elements of ES bytes.
+template <int W, int ES>
+struct Tile {
+  static constexpr int RB = W * ES;       // bytes of a row
+  static constexpr int CPR = RB / 16;     // 16-byte chunks of a row
+  static_assert(RB % 64 == 0, "whole groups of chunks");
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (CPR >= 16 && CPR % 16 == 0) return ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8);
+    else if constexpr (CPR % 8 == 0) return ((r & 3) << 1) | ((r >> 2) & 1);
+    else return (r & 2) | ((r >> 2) & 1);   // 4 chunks: two rows per 128 bytes
+  }
+  static __device__ __forceinline__ int off(int r, int c) { return r * RB + ((c ^ swz(r)) << 4); }
+  static constexpr int bytes(int rows) { return rows * RB; }
+
+  // row fragment of contraction block ks: row `row`, elements 16 ks + 8 h ..
+  template <class F>
+  static __device__ __forceinline__ F row_frag(const char* base, int row, int ks, int h) {
+    if constexpr (ES == 2) {
+      return *reinterpret_cast<const F*>(base + off(row, 2 * ks + h));
+    } else {
+      F f;
+      const f4 a = *reinterpret_cast<const f4*>(base + off(row, 4 * ks + 2 * h));
+      const f4 b = *reinterpret_cast<const f4*>(base + off(row, 4 * ks + 2 * h + 1));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { f[j] = a[j]; f[4 + j] = b[j]; }
+      return f;
+    }
+  }
+  // column fragment: column col0 + m, rows row0 + 8 (j >> 2) + 4 h + (j & 3)
+  template <class F>
+  static __device__ __forceinline__ F col_frag(const char* base, int row0, int col0, int lane) {
+    if constexpr (ES == 2) {
+      const int g = lane >> 4, i = lane & 15;
+      const int r = row0 + 4 * (g >> 1) + (i >> 2);
+      const int c = (col0 >> 3) + 2 * (g & 1) + ((i & 3) >> 1);
+      const int sub = 8 * (i & 1);
+      union { s4v s[2]; F f; } u;
+      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + off(r, c) + sub));
+      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + off(r + 8, c) + sub));
+      return u.f;
+    } else {
+      const int m = lane & 31, h = lane >> 5;
+      const int c = (col0 + m) >> 2, sub = ((col0 + m) & 3) * 4;
+      F f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        f[j] = *reinterpret_cast<const float*>(base + off(row0 + 8 * (j >> 2) + 4 * h + (j & 3), c) + sub);
+      return f;
+    }
+  }
+};
+
+// Direct global->LDS copy of ROWS rows into a tile by NW waves: the wave's
+// share of 1 KiB pieces.  Rows past `last` repeat row `last` (a row the mask
+// already excludes reads no memory outside the tensor).
+template <class TL, int ROWS, int NW>
+struct Copy {
+  static constexpr int PIECES = ROWS * TL::CPR / 64;
+  static constexpr int PER = (PIECES + NW - 1) / NW;
+  static_assert(ROWS * TL::CPR % 64 == 0, "whole pieces");
+  unsigned offs[PER];
+  __device__ __forceinline__ void init(int wave, int lane, unsigned row_bytes, int last) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int s = (wave + p * NW) * 64 + lane;
+      const int r = s / TL::CPR, c = (s % TL::CPR) ^ TL::swz(r);
+      offs[p] = static_cast<unsigned>(min(r, last)) * row_bytes + c * 16;
+    }
+  }
+  // src: the tile's first row (wave-uniform)
+  __device__ __forceinline__ void issue(const char* src, char* dst, int wave) const {
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      if (PIECES % NW == 0 || wave + p * NW < PIECES)
+        copy16(src + offs[p], dst + (wave + p * NW) * 1024);
+  }
+};
+
+// The sequence and block of a workgroup.  Dense: block `id` of one batch
+// element.  Packed (cu non-null): blocks are numbered sequence by sequence,
+// ceil(len / BLK) of each; found by the wave, 64 sequences at a time.  Offsets
+// are clamped into [0, T] and made non-decreasing pairwise, so no access
+// leaves the tensors whatever they hold.
+struct Span { int seq, blk, a, e; };   // rows [a, e) of the packed axis
+__device__ __forceinline__ bool find_span(const int32_t* cu, int n_seqs, int T, int BLK, int id, Span& s) {
+  const int lane = __lane_id();
+  int base = 0;
+  for (int s0 = 0; s0 < n_seqs; s0 += 64) {
+    const int i = s0 + lane;
+    int a = 0, e = 0;
+    if (i < n_seqs) {
+      a = min(max(cu[i], 0), T);
+      e = min(max(cu[i + 1], a), T);
+    }
+    const int nb = (e - a + BLK - 1) / BLK;
+    int inc = nb;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(inc, d, 64);
+      inc += lane >= d ? up : 0;
+    }
+    const unsigned long long hit = __ballot(base + inc > id);
+    if (hit) {
+      const int w = __ffsll(static_cast<long long>(hit)) - 1;
+      s.seq = s0 + w;
+      s.blk = __builtin_amdgcn_readfirstlane(id - base - (__shfl(inc, w, 64) - __shfl(nb, w, 64)));
+      s.a = __builtin_amdgcn_readfirstlane(__shfl(a, w, 64));
+      s.e = __builtin_amdgcn_readfirstlane(__shfl(e, w, 64));
+      return true;
+    }
+    base += __builtin_amdgcn_readfirstlane(__shfl(inc, 63, 64));
+  }
+  return false;
+}
+
+}  // namespace latent
+}  // namespace kda

@@ -1,0 +1,225 @@
+// C ABI of the latent attention: argument validation, workspace layout, dispatch.
+#include "latent_mi355x.h"
+
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <initializer_list>
+
+#include "kda_internal.h"
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+  char msg[400];
+  va_list ap;
+  va_start(ap, fmt);
+  std::vsnprintf(msg, sizeof(msg), fmt, ap);
+  va_end(ap);
+  return kda::api_fail(code, msg);
+}
+int launched(hipError_t e, const char* what) {
+  return e == hipSuccess ? KDA_OK : fail(KDA_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+size_t align_up(size_t x) { return (x + 255) / 256 * 256; }
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+size_t elem(int dtype) { return dtype == KDA_DTYPE_F32 ? 4 : 2; }
+bool dtype_ok(int dtype) { return dtype == KDA_DTYPE_F32 || dtype == KDA_DTYPE_BF16 || dtype == KDA_DTYPE_F16; }
+
+// A tile's rows are addressed with 32-bit offsets from its first row: 64 rows at most.
+constexpr int64_t kMaxRowBytes = int64_t{1} << 25;
+constexpr int64_t kMaxBlocks = int64_t{1} << 23;   // 256 threads each
+
+int check_attn(const void* q, const void* kv, const void* kr, const int64_t* st, const int32_t* cu_q, const int32_t* cu_k,
+               int32_t n_seqs, int B, int Tq, int Tk, int H, int dn, int dr, float scale, int dtype) {
+  if (!dtype_ok(dtype)) return fail(KDA_ERR_INVALID_ARGUMENT, "dtype=%d must be F32, BF16 or F16", dtype);
+  if (B < 0 || Tq < 0 || Tk < 0 || H < 1) return fail(KDA_ERR_INVALID_ARGUMENT, "sizes B=%d Tq=%d Tk=%d H=%d out of range", B, Tq, Tk, H);
+  if ((dn != 64 && dn != 128) || (dr != 32 && dr != 64))
+    return fail(KDA_ERR_UNSUPPORTED, "head dims dn=%d, dr=%d unsupported (dn in {64, 128}, dr in {32, 64})", dn, dr);
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(KDA_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  if ((cu_q == nullptr) != (cu_k == nullptr)) return fail(KDA_ERR_INVALID_ARGUMENT, "cu_q and cu_k go together");
+  if (cu_q && (B != 1 || n_seqs < 1)) return fail(KDA_ERR_INVALID_ARGUMENT, "packed sequences need B == 1 and n_seqs >= 1");
+  if (static_cast<int64_t>(B) * H > 65535) return fail(KDA_ERR_UNSUPPORTED, "B * H = %lld over 65535", static_cast<long long>(B) * H);
+  const int64_t blocks = (static_cast<int64_t>(Tq > Tk ? Tq : Tk) / 128 + 1 + (cu_q ? n_seqs : 0)) * B * H;
+  if (blocks > kMaxBlocks) return fail(KDA_ERR_UNSUPPORTED, "%lld blocks of 128 rows over %lld", static_cast<long long>(blocks),
+                                       static_cast<long long>(kMaxBlocks));
+  if (!st) return fail(KDA_ERR_INVALID_ARGUMENT, "null strides");
+  if (static_cast<int64_t>(B) * Tq > 0 && !q) return fail(KDA_ERR_INVALID_ARGUMENT, "null q");
+  if (static_cast<int64_t>(B) * Tk > 0 && (!kv || !kr)) return fail(KDA_ERR_INVALID_ARGUMENT, "null kv or k_rope");
+  for (const void* p : {q, kv, kr})
+    if (!aligned(p, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "q, kv and k_rope must be aligned to 16 bytes");
+  const int64_t es = static_cast<int64_t>(elem(dtype));
+  for (int i = 0; i < 8; ++i)
+    if (st[i] < 0 || st[i] * es % 16 != 0)
+      return fail(KDA_ERR_INVALID_ARGUMENT, "strides must be non-negative multiples of 16 bytes (stride %d is %lld elements)", i,
+                  static_cast<long long>(st[i]));
+  if (st[1] * es >= kMaxRowBytes || st[4] * es >= kMaxRowBytes || st[7] * es >= kMaxRowBytes)
+    return fail(KDA_ERR_UNSUPPORTED, "token strides of 32 MiB or more are unsupported");
+  return KDA_OK;
+}
+
+kda::LatentArgs attn_args(const void* q, const void* kv, const void* kr, const int64_t* st, const int32_t* cu_q,
+                          const int32_t* cu_k, int32_t n_seqs, int B, int Tq, int Tk, int H, int causal, float scale) {
+  kda::LatentArgs a{};
+  a.q = q; a.kv = kv; a.kr = kr;
+  a.cu_q = cu_q; a.cu_k = cu_k; a.n_seqs = cu_q ? n_seqs : 0;
+  a.B = B; a.Tq = Tq; a.Tk = Tk; a.H = H;
+  a.q_b = st[0]; a.q_t = st[1]; a.q_h = st[2];
+  a.kv_b = st[3]; a.kv_t = st[4]; a.kv_h = st[5];
+  a.kr_b = st[6]; a.kr_t = st[7];
+  a.causal = causal != 0;
+  a.scale = scale;
+  return a;
+}
+
+struct BwdLayout { size_t D, dmax, part, total; };
+BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dr) {
+  BwdLayout L{};
+  const size_t bh = static_cast<size_t>(B) * H;
+  L.D = 0;
+  L.dmax = align_up(bh * Tq * 4);
+  L.part = L.dmax + align_up(bh * ((Tq + 127) / 128) * 4);
+  L.total = L.part + align_up(bh * Tk * dr * 4) + 256;
+  return L;
+}
+
+// Decode: query rows of a workgroup in 16-row blocks (as few as hold the
+// sequence's Tq * H rows, at most 64; fp32: 32, whose operands take twice
+// the registers), the row groups of a sequence, and the workgroups along the
+// cache: one a CU (its two key tiles take the LDS), and no more than there
+// can be key tiles.
+constexpr int kCUs = 256;
+struct DecodePlan { int nb, groups, wgs; size_t part_o, total; };
+bool decode_plan(int B, int Tq, int H, int R, int page_size, int max_pages, int dtype, DecodePlan* P) {
+  const int64_t rows = static_cast<int64_t>(Tq) * H, cap = static_cast<int64_t>(page_size) * max_pages;
+  const int kt = dtype == KDA_DTYPE_F32 ? 32 : 64;
+  const int64_t tiles = (cap + kt - 1) / kt * B;
+  if (rows > (1 << 20) || cap >= (int64_t{1} << 31) || tiles >= (int64_t{1} << 30)) return false;
+  P->nb = rows <= 16 ? 1 : (rows <= 32 || dtype == KDA_DTYPE_F32 ? 2 : 4);
+  P->groups = static_cast<int>((rows + 16 * P->nb - 1) / (16 * P->nb));
+  int64_t wgs = kCUs / P->groups > 8 ? kCUs / P->groups / 8 * 8 : 8;
+  P->wgs = static_cast<int>(wgs < tiles ? wgs : (tiles > 0 ? tiles : 1));
+  const size_t slots = 2 * static_cast<size_t>(P->wgs) * P->groups * 16 * P->nb;
+  P->part_o = align_up(slots * 8);
+  P->total = P->part_o + align_up(slots * R * 4);
+  return true;
+}
+bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
+
+}  // namespace
+
+extern "C" {
+
+int kda_latent_attn_fwd(hipStream_t stream, const void* q, const void* kv, const void* k_rope, const int64_t* strides,
+                        const int32_t* cu_q, const int32_t* cu_k, int32_t n_seqs, void* o, float* lse, int B, int Tq, int Tk,
+                        int H, int dn, int dr, int causal, float scale, int dtype) {
+  if (const int rc = check_attn(q, kv, k_rope, strides, cu_q, cu_k, n_seqs, B, Tq, Tk, H, dn, dr, scale, dtype)) return rc;
+  if (static_cast<int64_t>(B) * Tq == 0) return KDA_OK;
+  if (!o || !lse) return fail(KDA_ERR_INVALID_ARGUMENT, "null o or lse");
+  if (!aligned(o, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "o must be aligned to 16 bytes");
+  kda::LatentArgs a = attn_args(q, kv, k_rope, strides, cu_q, cu_k, n_seqs, B, Tq, Tk, H, causal, scale);
+  a.o = o;
+  a.lse = lse;
+  return launched(kda::launch_latent_fwd(a, dn, dr, dtype, stream), "kda_latent_attn_fwd");
+}
+
+size_t kda_latent_attn_bwd_workspace(int B, int Tq, int Tk, int H, int dr) {
+  if (B < 0 || Tq < 0 || Tk < 0 || H < 1 || (dr != 32 && dr != 64)) return 0;
+  return bwd_layout(B, Tq, Tk, H, dr).total;
+}
+
+int kda_latent_attn_bwd(hipStream_t stream, const void* q, const void* kv, const void* k_rope, const int64_t* strides,
+                        const int32_t* cu_q, const int32_t* cu_k, int32_t n_seqs, const void* o, const float* lse,
+                        const void* d_o, void* dq, void* dkv, void* dk_rope, int B, int Tq, int Tk, int H, int dn, int dr,
+                        int causal, float scale, int dtype, void* workspace, size_t workspace_bytes) {
+  if (const int rc = check_attn(q, kv, k_rope, strides, cu_q, cu_k, n_seqs, B, Tq, Tk, H, dn, dr, scale, dtype)) return rc;
+  if (B == 0) return KDA_OK;
+  if (Tq > 0 && (!o || !lse || !d_o || !dq)) return fail(KDA_ERR_INVALID_ARGUMENT, "null o, lse, d_o or dq");
+  if (Tk > 0 && (!dkv || !dk_rope)) return fail(KDA_ERR_INVALID_ARGUMENT, "null dkv or dk_rope");
+  for (const void* p : {o, d_o, static_cast<const void*>(dq), static_cast<const void*>(dkv), static_cast<const void*>(dk_rope)})
+    if (!aligned(p, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "o, d_o, dq, dkv and dk_rope must be aligned to 16 bytes");
+  if (static_cast<int64_t>(H) * dn * elem(dtype) >= kMaxRowBytes) return fail(KDA_ERR_UNSUPPORTED, "H * dn too large");
+  const BwdLayout L = bwd_layout(B, Tq, Tk, H, dr);
+  if (!workspace || workspace_bytes < L.total)
+    return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0}, L.total);
+  if (!aligned(workspace, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "workspace must be aligned to 16 bytes");
+  kda::LatentArgs a = attn_args(q, kv, k_rope, strides, cu_q, cu_k, n_seqs, B, Tq, Tk, H, causal, scale);
+  char* ws = static_cast<char*>(workspace);
+  a.o_in = o; a.lse_in = lse; a.dout = d_o;
+  a.D = reinterpret_cast<float*>(ws + L.D);
+  a.dmax = reinterpret_cast<float*>(ws + L.dmax);
+  a.dmax_n = (Tq + 127) / 128;
+  a.dkr_part = reinterpret_cast<float*>(ws + L.part);
+  a.dq = dq; a.dkv = dkv; a.dkr = dk_rope;
+  return launched(kda::launch_latent_bwd(a, dn, dr, dtype, stream), "kda_latent_attn_bwd");
+}
+
+int kda_latent_append(hipStream_t stream, const void* rows, int64_t rows_stride, const int64_t* positions, const int64_t* slots,
+                      const float* cos_sin, int64_t n_positions, const float* norm_weight, float eps, void* cache,
+                      int64_t n_slots, const void* q, int64_t q_stride_t, int64_t q_stride_h, void* q_out, int64_t qo_stride_t,
+                      int64_t qo_stride_h, int N, int H, int R, int dr, int interleaved, int dtype) {
+  if (!dtype_ok(dtype)) return fail(KDA_ERR_INVALID_ARGUMENT, "dtype=%d must be F32, BF16 or F16", dtype);
+  if ((R != 256 && R != 512) || (dr != 32 && dr != 64))
+    return fail(KDA_ERR_UNSUPPORTED, "R=%d, dr=%d unsupported (R in {256, 512}, dr in {32, 64})", R, dr);
+  if (N < 0 || n_slots < 0 || (q && H < 1)) return fail(KDA_ERR_INVALID_ARGUMENT, "sizes out of range");
+  if (N == 0) return KDA_OK;
+  if (N > kMaxBlocks) return fail(KDA_ERR_UNSUPPORTED, "N=%d over %lld", N, static_cast<long long>(kMaxBlocks));
+  if (!rows || !positions || !slots || !cos_sin || n_positions < 1) return fail(KDA_ERR_INVALID_ARGUMENT, "null rows, positions, slots or cos_sin");
+  if (n_slots > 0 && !cache) return fail(KDA_ERR_INVALID_ARGUMENT, "null cache");
+  if ((q == nullptr) != (q_out == nullptr)) return fail(KDA_ERR_INVALID_ARGUMENT, "q and q_out go together");
+  if (norm_weight && !(eps >= 0.f)) return fail(KDA_ERR_INVALID_ARGUMENT, "eps must not be negative");
+  const int64_t es = static_cast<int64_t>(elem(dtype));
+  for (const void* p : {rows, static_cast<const void*>(cache), static_cast<const void*>(cos_sin), static_cast<const void*>(norm_weight)})
+    if (!aligned(p, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "rows, cache, cos_sin and norm_weight must be aligned to 16 bytes");
+  if (rows_stride < 0 || rows_stride * es % 16 != 0) return fail(KDA_ERR_INVALID_ARGUMENT, "rows_stride must be a multiple of 16 bytes");
+  if (!aligned(q, 4 * es) || !aligned(q_out, 4 * es) || q_stride_t % 4 || q_stride_h % 4 || qo_stride_t % 4 || qo_stride_h % 4)
+    return fail(KDA_ERR_INVALID_ARGUMENT, "q and q_out must be aligned to 4 elements, their strides too");
+  kda::LatentAppendArgs a{};
+  a.rows = rows; a.positions = positions; a.slots = slots; a.cos_sin = cos_sin; a.w = norm_weight;
+  a.cache = cache; a.q = q; a.q_out = q_out;
+  a.rows_t = rows_stride; a.q_t = q_stride_t; a.q_h = q_stride_h; a.qo_t = qo_stride_t; a.qo_h = qo_stride_h;
+  a.n_slots = n_slots; a.P = n_positions; a.N = N; a.H = H; a.interleaved = interleaved != 0; a.eps = eps;
+  return launched(kda::launch_latent_append(a, R, dr, dtype, stream), "kda_latent_append");
+}
+
+size_t kda_latent_decode_workspace(int B, int Tq, int H, int R, int dr, int page_size, int max_pages, int dtype) {
+  DecodePlan P;
+  if (B < 0 || Tq < 1 || H < 1 || (R != 256 && R != 512) || (dr != 32 && dr != 64) || !pow2(page_size) || max_pages < 0 ||
+      !dtype_ok(dtype) || !decode_plan(B, Tq, H, R, page_size, max_pages, dtype, &P))
+    return 0;
+  return P.total;
+}
+
+int kda_latent_decode(hipStream_t stream, const void* q, const void* cache, const int32_t* block_table, const int32_t* seq_lens,
+                      void* o, float* lse, int B, int Tq, int H, int R, int dr, int64_t n_pages, int page_size, int max_pages,
+                      float scale, int dtype, void* workspace, size_t workspace_bytes) {
+  if (!dtype_ok(dtype)) return fail(KDA_ERR_INVALID_ARGUMENT, "dtype=%d must be F32, BF16 or F16", dtype);
+  if ((R != 256 && R != 512) || (dr != 32 && dr != 64))
+    return fail(KDA_ERR_UNSUPPORTED, "R=%d, dr=%d unsupported (R in {256, 512}, dr in {32, 64})", R, dr);
+  if (B < 0 || Tq < 1 || H < 1 || max_pages < 0 || n_pages < 0) return fail(KDA_ERR_INVALID_ARGUMENT, "sizes out of range");
+  if (!pow2(page_size)) return fail(KDA_ERR_INVALID_ARGUMENT, "page_size=%d must be a power of two", page_size);
+  if (n_pages >= (int64_t{1} << 31) / page_size) return fail(KDA_ERR_UNSUPPORTED, "n_pages * page_size must be below 2^31");
+  if (B > 65535) return fail(KDA_ERR_UNSUPPORTED, "B=%d over 65535", B);
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(KDA_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  if (B == 0) return KDA_OK;
+  if (n_pages == 0) max_pages = 0;      // no page: every length is 0
+  if (!q || !seq_lens || !o || !lse || (max_pages > 0 && (!cache || !block_table)))
+    return fail(KDA_ERR_INVALID_ARGUMENT, "null q, cache, block_table, seq_lens, o or lse");
+  for (const void* p : {q, cache, static_cast<const void*>(o), static_cast<const void*>(workspace)})
+    if (!aligned(p, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "q, cache, o and workspace must be aligned to 16 bytes");
+  DecodePlan P;
+  if (!decode_plan(B, Tq, H, R, page_size, max_pages, dtype, &P))
+    return fail(KDA_ERR_UNSUPPORTED, "Tq * H = %lld rows or B * max_pages * page_size too large", static_cast<long long>(Tq) * H);
+  if (!workspace || workspace_bytes < P.total)
+    return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0}, P.total);
+  kda::LatentDecodeArgs a{};
+  a.q = q; a.cache = cache; a.table = block_table; a.lens = seq_lens; a.o = o; a.lse = lse;
+  a.part_ml = static_cast<float*>(workspace);
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + P.part_o);
+  a.B = B; a.Tq = Tq; a.H = H; a.per = max_pages; a.n_pages = n_pages;
+  for (a.page_shift = 0; (1 << a.page_shift) < page_size;) ++a.page_shift;
+  a.groups = P.groups; a.wgs = P.wgs; a.scale = scale;
+  return launched(kda::launch_latent_decode(a, R, dr, dtype, P.nb, stream), "kda_latent_decode");
+}
+
+}  // extern "C"

@@ -1,0 +1,469 @@
+// Latent attention, expanded form, backward.
+//
+//   D_i = sum_d do_id o_id,   p_ij = exp(scale s_ij - lse_i),
+//   g_ij = p_ij (do_i . v_j - D_i),
+//   dq_i = scale sum_j g_ij k_j,  dk_j = scale sum_i g_ij q_i,  dv_j = sum_i p_ij do_i,
+// the rotary key's gradient summed over the heads.
+//
+// Three launches and one more for the sum over heads, no atomics, so a gradient
+// is the same bits in every run: the row pass (D, and for fp16 the largest
+// |do|), the query pass (a workgroup owns 128 queries and walks the keys; dq),
+// the key pass (a workgroup owns 128 keys and walks the queries; dk, dv, the
+// head's share of the rotary key's gradient in fp32), then that share's sum in
+// head order.  Both passes form p and g again: seven products instead of five,
+// against an fp32 dq kept in memory and added to by every key block.
+//
+// p and g are rounded to the inputs' type for the products they enter; sums
+// are fp32.  For fp16, whose smallest value is 6e-8, g is formed from do
+// scaled by a power of two that brings the head's largest |do| near 1, and the
+// sums are scaled back: p of a long row times a small do would vanish otherwise.
+
+#include "kda_internal.h"
+#include "kda_latent.h"
+
+namespace kda {
+namespace latent {
+
+// ---------------------------------------------------------------- row pass
+template <int DT, int DN>
+__global__ __launch_bounds__(256) void kda_latent_rows_kernel(LatentArgs a) {
+  constexpr int LPR = DN / 8;             // lanes of a row, eight elements each
+  constexpr int RPP = 256 / LPR;          // rows at a time
+  __shared__ float red[4];
+  const int bh = blockIdx.y, b = bh / a.H, head = bh - b * a.H;
+  const int e0 = (threadIdx.x % LPR) * 8;
+  float top = 0.f;
+#pragma unroll 2
+  for (int r = threadIdx.x / LPR; r < 128; r += RPP) {
+    const int row = blockIdx.x * 128 + r;
+    if (row >= a.Tq) break;
+    const int64_t i = ((static_cast<int64_t>(b) * a.Tq + row) * a.H + head) * DN + e0;
+    float d = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const f4 x = ld4<DT>(a.dout, i + 4 * t), y = ld4<DT>(a.o_in, i + 4 * t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d = fmaf(x[e], y[e], d);
+        if constexpr (DT == 2) top = fmaxf(top, fabsf(x[e]));
+      }
+    }
+#pragma unroll
+    for (int s = 1; s < LPR; s <<= 1) d += __shfl_xor(d, s, 64);
+    if (e0 == 0) a.D[static_cast<int64_t>(bh) * a.Tq + row] = d;
+  }
+  if constexpr (DT == 2) {
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0)
+      a.dmax[static_cast<int64_t>(bh) * a.dmax_n + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
+}
+
+// fp16: the power of two that brings the head's largest |do| into [1, 2);
+// 1 where there is none (zeros, or a value that is not finite)
+__device__ __forceinline__ float do_factor(const LatentArgs& a, int bh) {
+  float t = 0.f;
+  for (int i = __lane_id(); i < a.dmax_n; i += 64) t = fmaxf(t, a.dmax[static_cast<int64_t>(bh) * a.dmax_n + i]);
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) t = fmaxf(t, __shfl_xor(t, s, 64));
+  if (!(t > 0.f) || t > 65504.f) return 1.f;
+  return __uint_as_float((254u << 23) - (__float_as_uint(t) & 0x7F800000u));
+}
+
+template <int DT, int DN, int DR>
+struct BwdCfg {
+  static constexpr int ES = El<DT>::ES;
+  static constexpr int NW = 4, BM = 32 * NW;     // rows that a workgroup owns
+  static constexpr int BN = ES == 2 ? 64 : 32;   // rows of the other side at a time
+  typedef Tile<DN, ES> TN;
+  typedef Tile<DR, ES> TR;
+  static constexpr int OFF_V = TN::bytes(BN), OFF_R = 2 * TN::bytes(BN);
+  static constexpr int OFF_L = OFF_R + TR::bytes(BN);          // key pass: lse, then D, 64 floats each
+  static constexpr int BUF_Q = OFF_L, BUF_K = OFF_L + 512;
+};
+
+struct Where { int b, head, bh, r0, re, k0, ke, off; };   // rows owned from r0 to re, the other side k0 to ke
+// q_side: the workgroup owns queries, else keys.  off: owned query row i sees the
+// keys of the sequence with index <= i + off; owned key row j is seen by the
+// queries of the sequence with index >= j + off.
+__device__ __forceinline__ bool locate(const LatentArgs& a, int nb, int BM, bool q_side, bool reverse, Where& w) {
+  const int id = blockIdx.x, bh_n = a.B * a.H;
+  int blk;
+  if (bh_n % 8 == 0) {
+    const int slot = id >> 3;
+    w.bh = (id & 7) + 8 * (slot / nb);
+    blk = slot % nb;
+  } else {
+    w.bh = id % bh_n;
+    blk = id / bh_n;
+  }
+  if (reverse) blk = nb - 1 - blk;
+  w.b = w.bh / a.H;
+  w.head = w.bh - w.b * a.H;
+  if (a.cu_q) {
+    Span s;
+    if (!find_span(q_side ? a.cu_q : a.cu_k, a.n_seqs, q_side ? a.Tq : a.Tk, BM, blk, s)) return false;
+    const int32_t* o = q_side ? a.cu_k : a.cu_q;
+    const int T = q_side ? a.Tk : a.Tq;
+    w.r0 = s.a + s.blk * BM;
+    w.re = s.e;
+    w.k0 = min(max(o[s.seq], 0), T);
+    w.ke = min(max(o[s.seq + 1], w.k0), T);
+    const int nr = s.e - s.a, no = w.ke - w.k0;
+    w.off = no - nr - s.a;   // keys - queries, or queries - keys
+  } else {
+    w.r0 = blk * BM;
+    w.re = q_side ? a.Tq : a.Tk;
+    w.k0 = 0;
+    w.ke = q_side ? a.Tk : a.Tq;
+    w.off = q_side ? a.Tk - a.Tq : a.Tq - a.Tk;
+  }
+  return true;
+}
+
+// -------------------------------------------------------------- query pass
+// As the forward: scores transposed, one query a lane column.  g^T is the second
+// operand of dq^T += K^T g^T, whose first operand is the key tile read transposed.
+template <int DT, int DN, int DR>
+__global__ __launch_bounds__(256, 1) void kda_latent_dq_kernel(LatentArgs a, int nqb) {
+  typedef BwdCfg<DT, DN, DR> C;
+  typedef typename El<DT>::frag F;
+  typedef typename El<DT>::t E;
+  constexpr int ES = C::ES, BN = C::BN, KN = DN / 16, KR = DR / 16, ND = DN / 32, NR = DR / 32;
+  __shared__ __attribute__((aligned(1024))) char buf0[C::BUF_Q];
+  __shared__ __attribute__((aligned(1024))) char buf1[C::BUF_Q];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 31, h = lane >> 5;
+  Where w;
+  if (!locate(a, nqb, C::BM, true, true, w)) return;
+  const int nk = w.ke - w.k0;
+  const int row = w.r0 + wave * 32 + m;
+  const bool live = row < w.re;
+  const int crow = min(row, w.re - 1);
+  const int kmax = a.causal ? min(nk - 1, row + w.off) : nk - 1;
+  const int wave_lo = a.causal ? min(nk - 1, w.r0 + wave * 32 + w.off) : nk - 1;
+  const int wave_hi = a.causal ? min(nk - 1, min(w.r0 + wave * 32 + 31, w.re - 1) + w.off) : nk - 1;
+  const int blk_hi = a.causal ? min(nk - 1, min(w.r0 + C::BM - 1, w.re - 1) + w.off) : nk - 1;
+  const int nt = (blk_hi + BN) / BN;
+
+  F qn[KN], qr[KR], dO[KN];
+  {
+    const E* qp = static_cast<const E*>(a.q) + w.b * a.q_b + static_cast<int64_t>(crow) * a.q_t + w.head * a.q_h;
+    const E* dp = static_cast<const E*>(a.dout) + ((static_cast<int64_t>(w.b) * a.Tq + crow) * a.H + w.head) * DN;
+#pragma unroll
+    for (int s = 0; s < KN; ++s) {
+      qn[s] = *reinterpret_cast<const F*>(qp + 16 * s + 8 * h);
+      dO[s] = *reinterpret_cast<const F*>(dp + 16 * s + 8 * h);
+    }
+#pragma unroll
+    for (int s = 0; s < KR; ++s) qr[s] = *reinterpret_cast<const F*>(qp + DN + 16 * s + 8 * h);
+  }
+  const int64_t ri = static_cast<int64_t>(w.bh) * a.Tq + crow;
+  const float lse2 = a.lse_in[ri] * kLog2e, D = a.D[ri];
+  const float gf = DT == 2 ? do_factor(a, w.bh) : 1.f;
+
+  const char* kvp = static_cast<const char*>(a.kv) + (w.b * a.kv_b + w.k0 * a.kv_t + w.head * a.kv_h) * ES;
+  const char* krp = static_cast<const char*>(a.kr) + (w.b * a.kr_b + w.k0 * a.kr_t) * ES;
+  const unsigned kv_rb = static_cast<unsigned>(a.kv_t * ES), kr_rb = static_cast<unsigned>(a.kr_t * ES);
+  Copy<typename C::TN, BN, C::NW> cn;
+  Copy<typename C::TR, BN, C::NW> cr;
+  cn.init(wave, lane, kv_rb, BN);
+  cr.init(wave, lane, kr_rb, BN);
+  auto fetch = [&](int j, char* dst) {
+    const char* s = kvp + static_cast<int64_t>(j) * BN * kv_rb;
+    const char* r = krp + static_cast<int64_t>(j) * BN * kr_rb;
+    if (j * BN + BN <= nk) {
+      cn.issue(s, dst, wave);
+      cn.issue(s + DN * ES, dst + C::OFF_V, wave);
+      cr.issue(r, dst + C::OFF_R, wave);
+    } else {
+      Copy<typename C::TN, BN, C::NW> tn;
+      Copy<typename C::TR, BN, C::NW> tr;
+      tn.init(wave, lane, kv_rb, nk - 1 - j * BN);
+      tr.init(wave, lane, kr_rb, nk - 1 - j * BN);
+      tn.issue(s, dst, wave);
+      tn.issue(s + DN * ES, dst + C::OFF_V, wave);
+      tr.issue(r, dst + C::OFF_R, wave);
+    }
+  };
+
+  const float c = a.scale * kLog2e;
+  f16v acc[ND + NR];
+#pragma unroll
+  for (int n = 0; n < ND + NR; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
+
+  auto step = [&](int j, const char* cur, char* nxt) {
+    wait_vmem_all();
+    lds_barrier();
+    if (j + 1 < nt) fetch(j + 1, nxt);
+    const int kt = j * BN;
+    if (kt > wave_hi) return;
+#pragma unroll
+    for (int t = 0; t < BN / 32; ++t) {
+      f16v s, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KN; ++k) {
+        s = mma(s, C::TN::template row_frag<F>(cur, 32 * t + m, k, h), qn[k]);
+        dp = mma(dp, C::TN::template row_frag<F>(cur + C::OFF_V, 32 * t + m, k, h), dO[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < KR; ++k) s = mma(s, C::TR::template row_frag<F>(cur + C::OFF_R, 32 * t + m, k, h), qr[k]);
+      const bool edge = kt + 32 * t + 31 > wave_lo;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float g[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int i = 8 * u + e;
+          g[e] = fast_exp2(fmaf(s[i], c, -lse2)) * (dp[i] - D);
+          if constexpr (DT == 2) g[e] *= gf;
+        }
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (kt + 32 * t + 8 * ((8 * u + e) >> 2) + 4 * h + (e & 3) > kmax) g[e] = 0.f;
+        }
+        const F gq = to_frag<DT>(g);
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+          acc[n] = mma(acc[n], C::TN::template col_frag<F>(cur, 32 * t + 16 * u, 32 * n, lane), gq);
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+          acc[ND + n] = mma(acc[ND + n], C::TR::template col_frag<F>(cur + C::OFF_R, 32 * t + 16 * u, 32 * n, lane), gq);
+      }
+    }
+  };
+  if (nt > 0) fetch(0, buf0);
+  for (int j = 0; j < nt;) {
+    step(j, buf0, buf1);
+    if (++j >= nt) break;
+    step(j, buf1, buf0);
+    ++j;
+  }
+  if (!live) return;
+  const float f = a.scale / gf;
+  const int64_t ob = ((static_cast<int64_t>(w.b) * a.Tq + row) * a.H + w.head) * (DN + DR) + 4 * h;
+#pragma unroll
+  for (int n = 0; n < ND + NR; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      store4<DT>(a.dq, ob + 32 * n + 8 * i, acc[n][4 * i] * f, acc[n][4 * i + 1] * f, acc[n][4 * i + 2] * f,
+                 acc[n][4 * i + 3] * f);
+}
+
+// ---------------------------------------------------------------- key pass
+// Scores untransposed: a lane column is one key, whose key, rotary key and value
+// rows stay in registers; the query tile (nope, rotary, do) is in LDS, read by
+// rows for the two score products and transposed for dk^T and dv^T.
+template <int DT, int DN, int DR>
+__global__ __launch_bounds__(256, 1) void kda_latent_dkv_kernel(LatentArgs a, int nkb) {
+  typedef BwdCfg<DT, DN, DR> C;
+  typedef typename El<DT>::frag F;
+  typedef typename El<DT>::t E;
+  constexpr int ES = C::ES, BN = C::BN, KN = DN / 16, KR = DR / 16, ND = DN / 32, NR = DR / 32;
+  __shared__ __attribute__((aligned(1024))) char buf0[C::BUF_K];
+  __shared__ __attribute__((aligned(1024))) char buf1[C::BUF_K];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 31, h = lane >> 5;
+  Where w;
+  if (!locate(a, nkb, C::BM, false, false, w)) return;
+  const int nq = w.ke - w.k0;                   // queries of the sequence
+  const int key = w.r0 + wave * 32 + m;         // this lane's key (packed axis)
+  const bool live = key < w.re;
+  const int ckey = min(key, w.re - 1);
+  const int first = a.causal ? max(0, key + w.off) : 0;                      // first query that sees this lane's key
+  const int wave_first = a.causal ? max(0, w.r0 + wave * 32 + w.off) : 0;    // ... any of the wave's keys
+  const int wave_full = a.causal ? max(0, min(w.r0 + wave * 32 + 31, w.re - 1) + w.off) : 0;   // ... all of them
+  const int j0 = (a.causal ? max(0, w.r0 + w.off) : 0) / BN;
+  const int nt = (nq + BN - 1) / BN;
+
+  F kn[KN], kr[KR], vv[KN];
+  {
+    const E* p = static_cast<const E*>(a.kv) + w.b * a.kv_b + static_cast<int64_t>(ckey) * a.kv_t + w.head * a.kv_h;
+    const E* r = static_cast<const E*>(a.kr) + w.b * a.kr_b + static_cast<int64_t>(ckey) * a.kr_t;
+#pragma unroll
+    for (int s = 0; s < KN; ++s) {
+      kn[s] = *reinterpret_cast<const F*>(p + 16 * s + 8 * h);
+      vv[s] = *reinterpret_cast<const F*>(p + DN + 16 * s + 8 * h);
+    }
+#pragma unroll
+    for (int s = 0; s < KR; ++s) kr[s] = *reinterpret_cast<const F*>(r + 16 * s + 8 * h);
+  }
+  const float gf = DT == 2 ? do_factor(a, w.bh) : 1.f;
+
+  const char* qp = static_cast<const char*>(a.q) + (w.b * a.q_b + w.k0 * a.q_t + w.head * a.q_h) * ES;
+  const char* dp_ = static_cast<const char*>(a.dout) + ((static_cast<int64_t>(w.b) * a.Tq + w.k0) * a.H + w.head) * DN * ES;
+  const float* lsep = a.lse_in + static_cast<int64_t>(w.bh) * a.Tq + w.k0;
+  const float* Dp = a.D + static_cast<int64_t>(w.bh) * a.Tq + w.k0;
+  const unsigned q_rb = static_cast<unsigned>(a.q_t * ES), d_rb = static_cast<unsigned>(a.H * DN * ES);
+  Copy<typename C::TN, BN, C::NW> cq, cd;
+  Copy<typename C::TR, BN, C::NW> cr;
+  cq.init(wave, lane, q_rb, BN);
+  cd.init(wave, lane, d_rb, BN);
+  cr.init(wave, lane, q_rb, BN);
+  auto fetch = [&](int j, char* dst) {
+    const char* s = qp + static_cast<int64_t>(j) * BN * q_rb;
+    const char* d = dp_ + static_cast<int64_t>(j) * BN * d_rb;
+    if (j * BN + BN <= nq) {
+      cq.issue(s, dst, wave);
+      cd.issue(d, dst + C::OFF_V, wave);
+      cr.issue(s + DN * ES, dst + C::OFF_R, wave);
+    } else {
+      Copy<typename C::TN, BN, C::NW> tq, td;
+      Copy<typename C::TR, BN, C::NW> tr;
+      tq.init(wave, lane, q_rb, nq - 1 - j * BN);
+      td.init(wave, lane, d_rb, nq - 1 - j * BN);
+      tr.init(wave, lane, q_rb, nq - 1 - j * BN);
+      tq.issue(s, dst, wave);
+      td.issue(d, dst + C::OFF_V, wave);
+      tr.issue(s + DN * ES, dst + C::OFF_R, wave);
+    }
+    if (wave < 2) {
+      const float* x = wave == 0 ? lsep : Dp;
+      copy4(x + min(j * BN + lane, nq - 1), dst + C::OFF_L + 256 * wave);
+    }
+  };
+
+  const float c = a.scale * kLog2e;
+  f16v dk[ND + NR], dv[ND];
+#pragma unroll
+  for (int n = 0; n < ND + NR; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dk[n][i] = 0.f;
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dv[n][i] = 0.f;
+
+  auto step = [&](int j, const char* cur, char* nxt) {
+    wait_vmem_all();
+    lds_barrier();
+    if (j + 1 < nt) fetch(j + 1, nxt);
+    const int qt = j * BN;
+    if (qt + BN - 1 < wave_first) return;       // none of these queries sees a key of this wave
+#pragma unroll
+    for (int t = 0; t < BN / 32; ++t) {
+      f16v s, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KN; ++k) {
+        s = mma(s, C::TN::template row_frag<F>(cur, 32 * t + m, k, h), kn[k]);
+        dp = mma(dp, C::TN::template row_frag<F>(cur + C::OFF_V, 32 * t + m, k, h), vv[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < KR; ++k) s = mma(s, C::TR::template row_frag<F>(cur + C::OFF_R, 32 * t + m, k, h), kr[k]);
+      const int q0 = qt + 32 * t;
+      const bool edge = q0 < wave_full || q0 + 31 >= nq;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float p[8], g[8];
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const f4 ls = *reinterpret_cast<const f4*>(cur + C::OFF_L + (32 * t + 16 * u + 8 * v + 4 * h) * 4);
+          const f4 dd = *reinterpret_cast<const f4*>(cur + C::OFF_L + 256 + (32 * t + 16 * u + 8 * v + 4 * h) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 8 * u + 4 * v + e;
+            p[4 * v + e] = fast_exp2(fmaf(s[i], c, -ls[e] * kLog2e));
+            g[4 * v + e] = p[4 * v + e] * (dp[i] - dd[e]);
+            if constexpr (DT == 2) g[4 * v + e] *= gf;
+          }
+        }
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int qi = q0 + 16 * u + 8 * (e >> 2) + 4 * h + (e & 3);
+            if (qi < first || qi >= nq) p[e] = g[e] = 0.f;
+          }
+        }
+        const F pf = to_frag<DT>(p), gq = to_frag<DT>(g);
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          dv[n] = mma(dv[n], C::TN::template col_frag<F>(cur + C::OFF_V, 32 * t + 16 * u, 32 * n, lane), pf);
+          dk[n] = mma(dk[n], C::TN::template col_frag<F>(cur, 32 * t + 16 * u, 32 * n, lane), gq);
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+          dk[ND + n] = mma(dk[ND + n], C::TR::template col_frag<F>(cur + C::OFF_R, 32 * t + 16 * u, 32 * n, lane), gq);
+      }
+    }
+  };
+  if (j0 < nt) fetch(j0, buf0);
+  for (int j = j0; j < nt;) {
+    step(j, buf0, buf1);
+    if (++j >= nt) break;
+    step(j, buf1, buf0);
+    ++j;
+  }
+  if (!live) return;
+  const float f = a.scale / gf;
+  const int64_t ob = ((static_cast<int64_t>(w.b) * a.Tk + key) * a.H + w.head) * (2 * DN) + 4 * h;
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      store4<DT>(a.dkv, ob + 32 * n + 8 * i, dk[n][4 * i] * f, dk[n][4 * i + 1] * f, dk[n][4 * i + 2] * f, dk[n][4 * i + 3] * f);
+      store4<DT>(a.dkv, ob + DN + 32 * n + 8 * i, dv[n][4 * i], dv[n][4 * i + 1], dv[n][4 * i + 2], dv[n][4 * i + 3]);
+    }
+  const int64_t rb = (static_cast<int64_t>(w.bh) * a.Tk + key) * DR + 4 * h;
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      store4<0>(a.dkr_part, rb + 32 * n + 8 * i, dk[ND + n][4 * i] * f, dk[ND + n][4 * i + 1] * f, dk[ND + n][4 * i + 2] * f,
+                dk[ND + n][4 * i + 3] * f);
+}
+
+// ------------------------------------- the rotary key's gradient: sum over heads
+template <int DT>
+__global__ __launch_bounds__(256) void kda_latent_dkr_kernel(LatentArgs a, int64_t per_b) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;   // element of [Tk, dr]
+  if (i >= per_b) return;
+  const float* p = a.dkr_part + static_cast<int64_t>(blockIdx.y) * a.H * per_b + i;
+  f4 s = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int hd = 0; hd < a.H; ++hd) s += *reinterpret_cast<const f4*>(p + hd * per_b);
+  store4<DT>(a.dkr, blockIdx.y * per_b + i, s[0], s[1], s[2], s[3]);
+}
+
+template <int DT, int DN, int DR>
+hipError_t run_bwd(const LatentArgs& a, hipStream_t s) {
+  constexpr int BM = BwdCfg<DT, DN, DR>::BM;
+  const int64_t bh = static_cast<int64_t>(a.B) * a.H;
+  const int64_t nqb = a.cu_q ? static_cast<int64_t>(a.Tq) / BM + a.n_seqs : (static_cast<int64_t>(a.Tq) + BM - 1) / BM;
+  const int64_t nkb = a.cu_q ? static_cast<int64_t>(a.Tk) / BM + a.n_seqs : (static_cast<int64_t>(a.Tk) + BM - 1) / BM;
+  if (bh <= 0) return hipSuccess;
+  if (a.Tq > 0) {
+    kda_latent_rows_kernel<DT, DN><<<dim3((a.Tq + 127) / 128, bh), dim3(256), 0, s>>>(a);
+    kda_latent_dq_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(nqb * bh)), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
+  }
+  if (a.Tk > 0) {
+    kda_latent_dkv_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(nkb * bh)), dim3(256), 0, s>>>(a, static_cast<int>(nkb));
+    const int64_t per_b = static_cast<int64_t>(a.Tk) * DR;
+    kda_latent_dkr_kernel<DT><<<dim3(static_cast<unsigned>((per_b + 1023) / 1024), a.B), dim3(256), 0, s>>>(a, per_b);
+  }
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t bwd_by_dims(const LatentArgs& a, int dn, int dr, hipStream_t s) {
+  if (dn == 128) return dr == 64 ? run_bwd<DT, 128, 64>(a, s) : run_bwd<DT, 128, 32>(a, s);
+  return dr == 64 ? run_bwd<DT, 64, 64>(a, s) : run_bwd<DT, 64, 32>(a, s);
+}
+
+}  // namespace latent
+
+hipError_t launch_latent_bwd(const LatentArgs& a, int dn, int dr, int dt, hipStream_t s) {
+  return dt == 0 ? latent::bwd_by_dims<0>(a, dn, dr, s) : dt == 1 ? latent::bwd_by_dims<1>(a, dn, dr, s)
+                                                                  : latent::bwd_by_dims<2>(a, dn, dr, s);
+}
+
+}  // namespace kda

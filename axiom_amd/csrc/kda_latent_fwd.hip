@@ -1,0 +1,230 @@
+// Latent attention, expanded form, forward: o = softmax(scale (q_n k_n^T + q_r k_r^T)) v.
+//
+// One pass over the keys with a running maximum and sum.  A workgroup of four
+// waves owns 128 queries of one head, a wave 32 of them; key tiles of 64 rows
+// (fp32: 32) are copied straight to LDS, the next one while the present one is
+// used.  Scores are formed transposed (S^T = K Q^T), so a lane holds one
+// query's column: its maximum and sum need one exchange with the lane's other
+// half, and the probabilities are the second operand of O^T += V^T P^T in the
+// registers they were made in.  The rotary key's tile is read once per head from
+// the tensor all heads share; no broadcast copy of it exists anywhere.
+// P is rounded to the inputs' type for the second product (the matrix cores'
+// operand); the row sum adds the unrounded values.
+
+#include "kda_internal.h"
+#include "kda_latent.h"
+
+namespace kda {
+namespace latent {
+
+template <int DT, int DN, int DR>
+struct FwdCfg {
+  static constexpr int ES = El<DT>::ES;
+  static constexpr int NW = 4, BM = 32 * NW;
+  static constexpr int BN = ES == 2 ? 64 : 32;
+  typedef Tile<DN, ES> TN;
+  typedef Tile<DR, ES> TR;
+  static constexpr int OFF_V = TN::bytes(BN), OFF_R = 2 * TN::bytes(BN);
+  static constexpr int BUF = 2 * TN::bytes(BN) + TR::bytes(BN);
+};
+
+template <int DT, int DN, int DR>
+__global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_kernel(LatentArgs a, int nqb) {
+  typedef FwdCfg<DT, DN, DR> C;
+  typedef typename El<DT>::frag F;
+  typedef typename El<DT>::t E;
+  constexpr int ES = C::ES, BN = C::BN, NB = BN / 32, KN = DN / 16, KR = DR / 16, ND = DN / 32;
+  __shared__ __attribute__((aligned(1024))) char buf0[C::BUF];
+  __shared__ __attribute__((aligned(1024))) char buf1[C::BUF];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 31, h = lane >> 5;
+
+  // block -> (batch, head, queries).  Heads are spread over the eight XCDs
+  // (consecutive workgroups go round them), so that one XCD's L2 serves a
+  // head's keys; the longest causal blocks of a head start first.
+  int b = 0, head, q0, qe, k0, ke, off;
+  {
+    const int id = blockIdx.x, bh_n = a.B * a.H;
+    int bh, blk;
+    if (bh_n % 8 == 0) {
+      const int slot = id >> 3;
+      bh = (id & 7) + 8 * (slot / nqb);
+      blk = nqb - 1 - slot % nqb;
+    } else {
+      bh = id % bh_n;
+      blk = nqb - 1 - id / bh_n;
+    }
+    b = bh / a.H;
+    head = bh - b * a.H;
+    if (a.cu_q) {
+      Span s;
+      if (!find_span(a.cu_q, a.n_seqs, a.Tq, C::BM, blk, s)) return;
+      q0 = s.a + s.blk * C::BM;
+      qe = s.e;
+      k0 = min(max(a.cu_k[s.seq], 0), a.Tk);
+      ke = min(max(a.cu_k[s.seq + 1], k0), a.Tk);
+      off = (ke - k0) - (s.e - s.a) - s.a;    // key index inside the sequence <= query row + off
+    } else {
+      q0 = blk * C::BM;
+      qe = a.Tq;
+      k0 = 0;
+      ke = a.Tk;
+      off = a.Tk - a.Tq;
+    }
+  }
+  const int nk = ke - k0;
+  const int row = q0 + wave * 32 + m;         // this lane's query
+  const bool live = row < qe;
+  const int kmax = a.causal ? min(nk - 1, row + off) : nk - 1;   // last key it sees
+  const int wave_lo = a.causal ? min(nk - 1, q0 + wave * 32 + off) : nk - 1;   // last key that all of the wave's queries see
+  const int wave_hi = a.causal ? min(nk - 1, min(q0 + wave * 32 + 31, qe - 1) + off) : nk - 1;
+  const int blk_hi = a.causal ? min(nk - 1, min(q0 + C::BM - 1, qe - 1) + off) : nk - 1;
+  const int nt = (blk_hi + BN) / BN;          // key tiles of the workgroup (0 when no query sees a key)
+
+  F qn[KN], qr[KR];
+  {
+    const E* qp = static_cast<const E*>(a.q) + b * a.q_b + static_cast<int64_t>(min(row, qe - 1)) * a.q_t + head * a.q_h;
+#pragma unroll
+    for (int s = 0; s < KN; ++s) qn[s] = *reinterpret_cast<const F*>(qp + 16 * s + 8 * h);
+#pragma unroll
+    for (int s = 0; s < KR; ++s) qr[s] = *reinterpret_cast<const F*>(qp + DN + 16 * s + 8 * h);
+  }
+
+  const char* kvp = static_cast<const char*>(a.kv) + (b * a.kv_b + k0 * a.kv_t + head * a.kv_h) * ES;
+  const char* krp = static_cast<const char*>(a.kr) + (b * a.kr_b + k0 * a.kr_t) * ES;
+  const unsigned kv_rb = static_cast<unsigned>(a.kv_t * ES), kr_rb = static_cast<unsigned>(a.kr_t * ES);
+  Copy<typename C::TN, BN, C::NW> cn;
+  Copy<typename C::TR, BN, C::NW> cr;
+  cn.init(wave, lane, kv_rb, BN);
+  cr.init(wave, lane, kr_rb, BN);
+  auto fetch = [&](int j, char* dst) {
+    const char* s = kvp + static_cast<int64_t>(j) * BN * kv_rb;
+    const char* r = krp + static_cast<int64_t>(j) * BN * kr_rb;
+    if (j * BN + BN <= nk) {
+      cn.issue(s, dst, wave);
+      cn.issue(s + DN * ES, dst + C::OFF_V, wave);
+      cr.issue(r, dst + C::OFF_R, wave);
+    } else {
+      Copy<typename C::TN, BN, C::NW> tn;
+      Copy<typename C::TR, BN, C::NW> tr;
+      tn.init(wave, lane, kv_rb, nk - 1 - j * BN);
+      tr.init(wave, lane, kr_rb, nk - 1 - j * BN);
+      tn.issue(s, dst, wave);
+      tn.issue(s + DN * ES, dst + C::OFF_V, wave);
+      tr.issue(r, dst + C::OFF_R, wave);
+    }
+  };
+
+  const float c = a.scale * kLog2e;
+  float mx = kMaxInit, mc = kMaxInit * c, l = 0.f;   // running maximum (raw score units, and times c) and sum
+  const float lazy = kLazy / c;
+  f16v acc[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
+
+  auto step = [&](int j, const char* cur, char* nxt) {
+    wait_vmem_all();
+    lds_barrier();
+    if (j + 1 < nt) fetch(j + 1, nxt);
+    const int kt = j * BN;
+    if (kt > wave_hi) return;                 // nothing of this tile for this wave's queries
+    f16v s[NB];
+#pragma unroll
+    for (int t = 0; t < NB; ++t) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KN; ++k) s[t] = mma(s[t], C::TN::template row_frag<F>(cur, 32 * t + m, k, h), qn[k]);
+#pragma unroll
+      for (int k = 0; k < KR; ++k) s[t] = mma(s[t], C::TR::template row_frag<F>(cur + C::OFF_R, 32 * t + m, k, h), qr[k]);
+    }
+    if (kt + BN - 1 > wave_lo) {
+#pragma unroll
+      for (int t = 0; t < NB; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = kt + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
+          s[t][i] = key <= kmax ? s[t][i] : -INFINITY;
+        }
+    }
+    float tm = s[0][0];
+#pragma unroll
+    for (int t = 0; t < NB; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) tm = fmaxf(tm, s[t][i]);
+    tm = half_max(tm);
+    if (__any(tm > mx + lazy)) {
+      const float nm = fmaxf(mx, tm);
+      const float al = fast_exp2((mx - nm) * c);
+      mx = nm;
+      mc = nm * c;
+      l *= al;
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[n][i] *= al;
+    }
+#pragma unroll
+    for (int t = 0; t < NB; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = fast_exp2(fmaf(s[t][8 * u + e], c, -mc));
+          l += p[e];
+        }
+        const F pf = to_frag<DT>(p);
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+          acc[n] = mma(acc[n], C::TN::template col_frag<F>(cur + C::OFF_V, 32 * t + 16 * u, 32 * n, lane), pf);
+      }
+  };
+  if (nt > 0) fetch(0, buf0);
+  for (int j = 0; j < nt;) {
+    step(j, buf0, buf1);
+    if (++j >= nt) break;
+    step(j, buf1, buf0);
+    ++j;
+  }
+
+  l = half_sum(l);
+  if (!live) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // no visible key: zeros; NaN stays NaN
+  const int64_t ob = ((static_cast<int64_t>(b) * a.Tq + row) * a.H + head) * DN + 4 * h;
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      store4<DT>(a.o, ob + 32 * n + 8 * i, acc[n][4 * i] * inv, acc[n][4 * i + 1] * inv, acc[n][4 * i + 2] * inv,
+                 acc[n][4 * i + 3] * inv);
+  if (h == 0) a.lse[(static_cast<int64_t>(b) * a.H + head) * a.Tq + row] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * kLn2;
+}
+
+template <int DT, int DN, int DR>
+hipError_t run_fwd(const LatentArgs& a, hipStream_t s) {
+  constexpr int BM = FwdCfg<DT, DN, DR>::BM;
+  // packed: every sequence ends in at most one partial block
+  const int64_t nqb = a.cu_q ? static_cast<int64_t>(a.Tq) / BM + a.n_seqs : (static_cast<int64_t>(a.Tq) + BM - 1) / BM;
+  const int64_t grid = nqb * a.B * a.H;
+  if (grid <= 0) return hipSuccess;
+  kda_latent_fwd_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(grid)), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t by_dims(const LatentArgs& a, int dn, int dr, hipStream_t s) {
+  if (dn == 128) return dr == 64 ? run_fwd<DT, 128, 64>(a, s) : run_fwd<DT, 128, 32>(a, s);
+  return dr == 64 ? run_fwd<DT, 64, 64>(a, s) : run_fwd<DT, 64, 32>(a, s);
+}
+
+}  // namespace latent
+
+hipError_t launch_latent_fwd(const LatentArgs& a, int dn, int dr, int dt, hipStream_t s) {
+  return dt == 0 ? latent::by_dims<0>(a, dn, dr, s) : dt == 1 ? latent::by_dims<1>(a, dn, dr, s) : latent::by_dims<2>(a, dn, dr, s);
+}
+
+}  // namespace kda
