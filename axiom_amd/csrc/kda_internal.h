@@ -351,12 +351,17 @@ struct LatentDecodeArgs {
   float* lse;              // [B,Tq,H]
   float* part_o;           // partial results of split sequences
   float* part_ml;
+  int* line;               // tiles of a run, then each sequence's first tile on the line
+  int whole;               // a workgroup a sequence: nothing to join
+  int least;               // fewest places of a run
+  int pad;                 // places of a sequence beside its tiles
   int B, Tq, H, per, page_shift;
   int64_t n_pages;
   int groups, wgs;         // row groups of a sequence; workgroups along the cache
   float scale;
 };
-hipError_t launch_latent_decode(const LatentDecodeArgs& a, int R, int dr, int dt, int nb, hipStream_t s);
+int latent_decode_tile(int m_rows);   // keys of a tile, by the query rows of a workgroup
+hipError_t launch_latent_decode(const LatentDecodeArgs& a, int R, int dr, int dt, int m_rows, hipStream_t s);
 
 }  // namespace kda
 

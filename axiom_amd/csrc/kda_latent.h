@@ -86,6 +86,27 @@ __device__ __forceinline__ void store4(void* p, int64_t i, float a, float b, flo
   }
 }
 
+// x, of which the compiler knows nothing: addresses derived from it inside a loop
+// are formed there (a few integer instructions) instead of being held in dozens
+// of registers across it, which the accumulators need
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// all but the newest N vector memory operations of the wave are done
+template <int N>
+__device__ __forceinline__ void wait_vmem_but() {
+  static_assert(N >= 0 && N < 64, "vmcnt is six bits");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
+// every LDS read of the wave has returned (before its buffer is copied into again)
+__device__ __forceinline__ void lds_reads_done() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // value combined over the two halves of the wave (lane l and l ^ 32)
 __device__ __forceinline__ float half_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -94,6 +115,16 @@ __device__ __forceinline__ float half_max(float x) {
 __device__ __forceinline__ float half_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// maximum over the four 16-lane groups
+__device__ __forceinline__ float group_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float group_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
 // Direct global->LDS copy of 16 or 4 bytes a lane, to 64 consecutive places from
@@ -107,23 +138,30 @@ struct Tile {
   static constexpr int RB = W * ES;       // bytes of a row
   static constexpr int CPR = RB / 16;     // 16-byte chunks of a row
   static_assert(RB % 64 == 0, "whole groups of chunks");
+  // the permutation stays inside aligned groups of SWZ + 1 chunks
+  static constexpr int SWZ = CPR % 16 == 0 ? 15 : CPR % 8 == 0 ? 7 : 3;
   static __device__ __forceinline__ int swz(int r) {
-    if constexpr (CPR >= 16 && CPR % 16 == 0) return ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8);
-    else if constexpr (CPR % 8 == 0) return ((r & 3) << 1) | ((r >> 2) & 1);
+    if constexpr (SWZ == 15) return ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8);
+    else if constexpr (SWZ == 7) return ((r & 3) << 1) | ((r >> 2) & 1);
     else return (r & 2) | ((r >> 2) & 1);   // 4 chunks: two rows per 128 bytes
   }
-  static __device__ __forceinline__ int off(int r, int c) { return r * RB + ((c ^ swz(r)) << 4); }
+  // byte offset of chunk cc + cl of row r: cc the part that unrolling makes a
+  // constant, cl the lane's part in bits that cc has clear, so that the part of
+  // cc above the permutation goes into the instruction's offset field
+  static __device__ __forceinline__ int off(int r, int cc, int cl = 0) {
+    return r * RB + ((cc & ~SWZ) << 4) + ((((cc & SWZ) | cl) ^ swz(r)) << 4);
+  }
   static constexpr int bytes(int rows) { return rows * RB; }
 
   // row fragment of contraction block ks: row `row`, elements 16 ks + 8 h ..
   template <class F>
   static __device__ __forceinline__ F row_frag(const char* base, int row, int ks, int h) {
     if constexpr (ES == 2) {
-      return *reinterpret_cast<const F*>(base + off(row, 2 * ks + h));
+      return *reinterpret_cast<const F*>(base + off(row, 2 * ks, h));
     } else {
       F f;
-      const f4 a = *reinterpret_cast<const f4*>(base + off(row, 4 * ks + 2 * h));
-      const f4 b = *reinterpret_cast<const f4*>(base + off(row, 4 * ks + 2 * h + 1));
+      const f4 a = *reinterpret_cast<const f4*>(base + off(row, 4 * ks, 2 * h));
+      const f4 b = *reinterpret_cast<const f4*>(base + off(row, 4 * ks + 1, 2 * h));
 #pragma unroll
       for (int j = 0; j < 4; ++j) { f[j] = a[j]; f[4 + j] = b[j]; }
       return f;
@@ -135,19 +173,19 @@ struct Tile {
     if constexpr (ES == 2) {
       const int g = lane >> 4, i = lane & 15;
       const int r = row0 + 4 * (g >> 1) + (i >> 2);
-      const int c = (col0 >> 3) + 2 * (g & 1) + ((i & 3) >> 1);
+      const int cc = col0 >> 3, cl = 2 * (g & 1) + ((i & 3) >> 1);
       const int sub = 8 * (i & 1);
       union { s4v s[2]; F f; } u;
-      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + off(r, c) + sub));
-      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + off(r + 8, c) + sub));
+      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + off(r, cc, cl) + sub));
+      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + off(r + 8, cc, cl) + sub));
       return u.f;
     } else {
       const int m = lane & 31, h = lane >> 5;
-      const int c = (col0 + m) >> 2, sub = ((col0 + m) & 3) * 4;
+      const int cc = col0 >> 2, cl = m >> 2, sub = (m & 3) * 4;
       F f;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        f[j] = *reinterpret_cast<const float*>(base + off(row0 + 8 * (j >> 2) + 4 * h + (j & 3), c) + sub);
+        f[j] = *reinterpret_cast<const float*>(base + off(row0 + 8 * (j >> 2) + 4 * h + (j & 3), cc, cl) + sub);
       return f;
     }
   }

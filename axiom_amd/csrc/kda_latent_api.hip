@@ -83,24 +83,28 @@ BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dr) {
   return L;
 }
 
-// Decode: query rows of a workgroup in 16-row blocks (as few as hold the
-// sequence's Tq * H rows, at most 64; fp32: 32, whose operands take twice
-// the registers), the row groups of a sequence, and the workgroups along the
-// cache: one a CU (its two key tiles take the LDS), and no more than there
-// can be key tiles.
+// Decode: query rows of a workgroup (16, or 64 where there are more than 16;
+// fp32 16, whose operands take twice the registers and LDS), the row groups
+// of a sequence, and the workgroups along the cache: one a CU (its buffers take
+// the LDS), and no more than there can be runs of `least` tiles (a tile for each
+// of the eight waves, or one of 64 keys).  Sequences whose table holds at most
+// kWholeTokens tokens get a workgroup each instead and no join launch.
 constexpr int kCUs = 256;
-struct DecodePlan { int nb, groups, wgs; size_t part_o, total; };
+constexpr int kWholeTokens = 256;
+struct DecodePlan { int rows, groups, wgs, whole, least; size_t part_ml, part_o, total; };
 bool decode_plan(int B, int Tq, int H, int R, int page_size, int max_pages, int dtype, DecodePlan* P) {
   const int64_t rows = static_cast<int64_t>(Tq) * H, cap = static_cast<int64_t>(page_size) * max_pages;
-  const int kt = dtype == KDA_DTYPE_F32 ? 32 : 64;
-  const int64_t tiles = (cap + kt - 1) / kt * B;
+  P->rows = rows <= 16 || dtype == KDA_DTYPE_F32 ? 16 : 64;
+  P->least = P->rows == 64 ? 1 : dtype == KDA_DTYPE_F32 ? 4 : 8;
+  const int64_t kt = kda::latent_decode_tile(P->rows), tiles = ((cap + kt - 1) / kt + 2 * P->least) * B;
   if (rows > (1 << 20) || cap >= (int64_t{1} << 31) || tiles >= (int64_t{1} << 30)) return false;
-  P->nb = rows <= 16 ? 1 : (rows <= 32 || dtype == KDA_DTYPE_F32 ? 2 : 4);
-  P->groups = static_cast<int>((rows + 16 * P->nb - 1) / (16 * P->nb));
-  int64_t wgs = kCUs / P->groups > 8 ? kCUs / P->groups / 8 * 8 : 8;
-  P->wgs = static_cast<int>(wgs < tiles ? wgs : (tiles > 0 ? tiles : 1));
-  const size_t slots = 2 * static_cast<size_t>(P->wgs) * P->groups * 16 * P->nb;
-  P->part_o = align_up(slots * 8);
+  P->groups = static_cast<int>((rows + P->rows - 1) / P->rows);
+  P->whole = cap <= kWholeTokens;
+  const int64_t wgs = kCUs / P->groups > 8 ? kCUs / P->groups / 8 * 8 : 8, runs = (tiles + P->least - 1) / P->least;
+  P->wgs = P->whole ? (B > 0 ? B : 1) : static_cast<int>(wgs < runs ? wgs : runs);
+  const size_t slots = P->whole ? 0 : 2 * static_cast<size_t>(P->wgs) * P->groups * P->rows;
+  P->part_ml = align_up(4 * (static_cast<size_t>(B) + 1));
+  P->part_o = P->part_ml + align_up(slots * 8);
   P->total = P->part_o + align_up(slots * R * 4);
   return true;
 }
@@ -214,12 +218,13 @@ int kda_latent_decode(hipStream_t stream, const void* q, const void* cache, cons
     return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0}, P.total);
   kda::LatentDecodeArgs a{};
   a.q = q; a.cache = cache; a.table = block_table; a.lens = seq_lens; a.o = o; a.lse = lse;
-  a.part_ml = static_cast<float*>(workspace);
+  a.line = static_cast<int*>(workspace);
+  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + P.part_ml);
   a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + P.part_o);
   a.B = B; a.Tq = Tq; a.H = H; a.per = max_pages; a.n_pages = n_pages;
   for (a.page_shift = 0; (1 << a.page_shift) < page_size;) ++a.page_shift;
-  a.groups = P.groups; a.wgs = P.wgs; a.scale = scale;
-  return launched(kda::launch_latent_decode(a, R, dr, dtype, P.nb, stream), "kda_latent_decode");
+  a.groups = P.groups; a.wgs = P.wgs; a.whole = P.whole; a.least = P.least; a.pad = 2 * P.least; a.scale = scale;
+  return launched(kda::launch_latent_decode(a, R, dr, dtype, P.rows, stream), "kda_latent_decode");
 }
 
 }  // extern "C"

@@ -79,57 +79,73 @@ __global__ __launch_bounds__(256) void kda_latent_append_kernel(LatentAppendArgs
 }
 
 // ------------------------------------------------------------------ decode
-// A workgroup of four waves holds a group of 16 NB query rows (row = token *
-// H + head) of one sequence and walks a run of key tiles.  All sequences'
-// tiles form one line that is cut into equal runs, so workgroups carry equal
-// work whatever the lengths are; a run that covers only part of a sequence
-// leaves its unnormalised sum, maximum and row sum for the join kernel.
-// The cache is read once per row group: a tile's rows go straight to LDS and
-// serve as keys (rows) and as values (the same rows transposed).
-// Waves share the tile: for the scores a wave takes 16 keys, for the output a
-// quarter of the R columns; the probabilities cross through LDS.
-template <int DT, int R, int DR, int NB>
+// All sequences' key tiles form one line that is cut into equal runs, one a
+// workgroup, so workgroups carry equal work whatever the lengths are; a run
+// that covers only part of a sequence leaves its unnormalised sum, maximum and
+// row sum for the join kernel.  A workgroup holds 16 or 64 query rows (row =
+// token * H + head) in registers; the cache is read once for them.
+//
+// Up to 16 rows: bound by the cache's bytes (30 flop a byte), so the waves work
+// alone, without a barrier in the loop: each takes every NW-th group of 16 keys
+// of the run through an LDS buffer of its own, and a SIMD's second wave computes
+// while the first waits for its copies (147 KB a CU in buffers).  S^T = K Q^T
+// (16x16x32) leaves a lane four keys of one query, which is the second operand of
+// O^T += V^T P^T (16x16x16) as it stands, V^T being the same rows read
+// transposed.  The waves' sums meet once a run, in LDS.
+template <int DT, int R, int DR>
 struct DecCfg {
   static constexpr int ES = El<DT>::ES;
-  static constexpr int KT = ES == 2 ? 64 : 32;
+  static constexpr int NW = ES == 2 ? 8 : 4;               // a buffer a wave fills the LDS (R = 512)
+  static constexpr int KT = 16;                            // keys of a tile
   typedef Tile<R, ES> TN;
   typedef Tile<DR, ES> TR;
-  typedef Tile<KT, ES> TP;
-  static constexpr int OFF_R = TN::bytes(KT);
-  static constexpr int BUF = OFF_R + TR::bytes(KT);
+  static constexpr int OFF_R = TN::bytes(16);
+  static constexpr int WBUF = OFF_R + TR::bytes(16);       // one wave's buffer
+  static constexpr int PN = 16 * TN::CPR / 64, PR = 16 * TR::CPR / 64;   // its 1 KiB pieces
+  static constexpr int NVR = NW * WBUF / (NW * 1024);      // 16-column blocks of all waves' sums that the LDS holds
 };
 
-// Fragments of the 16 x 16 products: lane m = l & 15, group gq = l >> 4; element
-// j is contraction index 32 s + 8 gq + j.
+// Row fragment of the 16 x 16 x 32 product: lane m = l & 15, group gq = l >> 4;
+// element j is column 32 s + 8 gq + j.
 template <class TL, class F>
 __device__ __forceinline__ F row_frag16(const char* base, int row, int s, int gq) {
   if constexpr (sizeof(F) == 16) {
-    return *reinterpret_cast<const F*>(base + TL::off(row, 4 * s + gq));
+    return *reinterpret_cast<const F*>(base + TL::off(row, 4 * s, gq));
   } else {
     F f;
-    const f4 a = *reinterpret_cast<const f4*>(base + TL::off(row, 8 * s + 2 * gq));
-    const f4 b = *reinterpret_cast<const f4*>(base + TL::off(row, 8 * s + 2 * gq + 1));
+    const f4 a = *reinterpret_cast<const f4*>(base + TL::off(row, 8 * s, 2 * gq));
+    const f4 b = *reinterpret_cast<const f4*>(base + TL::off(row, 8 * s + 1, 2 * gq));
 #pragma unroll
     for (int j = 0; j < 4; ++j) { f[j] = a[j]; f[4 + j] = b[j]; }
     return f;
   }
 }
-template <class TL, class F>
-__device__ __forceinline__ F col_frag16(const char* base, int s, int col0, int lane) {
-  if constexpr (sizeof(F) == 16) {
-    const int i = lane & 15, r = 32 * s + 8 * (lane >> 4) + (i >> 2);
-    const int c = (col0 >> 3) + ((i & 3) >> 1), sub = 8 * (i & 1);
-    union { s4v v[2]; F f; } u;
-    u.v[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + TL::off(r, c) + sub));
-    u.v[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + TL::off(r + 4, c) + sub));
-    return u.f;
-  } else {
-    const int m = lane & 15, r = 32 * s + 8 * (lane >> 4);
-    const int c = (col0 + m) >> 2, sub = ((col0 + m) & 3) * 4;
-    F f;
+// The lane's four probabilities (keys 4 gq ..) as the second operand of the 16 x 16 x 16 product.
+template <int DT> struct P4 { typedef f4 t; };
+template <> struct P4<1> { typedef s4v t; };
+template <> struct P4<2> { typedef h4 t; };
+template <int DT>
+__device__ __forceinline__ typename P4<DT>::t to_p4(const float (&p)[4]) {
+  if constexpr (DT == 0) return f4{p[0], p[1], p[2], p[3]};
+  else if constexpr (DT == 1) return __builtin_bit_cast(s4v, make_uint2(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])));
+  else return h4{static_cast<_Float16>(p[0]), static_cast<_Float16>(p[1]), static_cast<_Float16>(p[2]), static_cast<_Float16>(p[3])};
+}
+__device__ __forceinline__ f4 mma_p(f4 c, const f4& a, const f4& b) { return mma16(c, a, b); }
+__device__ __forceinline__ f4 mma_p(f4 c, const h4& a, const h4& b) { return mma16(c, a, b); }
+__device__ __forceinline__ f4 mma_p(f4 c, const s4v& a, const s4v& b) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
+// First operand of O^T += V^T P^T: column col0 + m of V, keys 4 gq + j.
+template <int DT, class TL>
+__device__ __forceinline__ typename P4<DT>::t v_frag(const char* base, int col0, int lane) {
+  const int i = lane & 15, gq = lane >> 4;
+  if constexpr (DT == 0) {
+    f4 v;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float*>(base + TL::off(r + j, c) + sub);
-    return f;
+    for (int j = 0; j < 4; ++j)
+      v[j] = *reinterpret_cast<const float*>(base + TL::off(4 * gq + j, col0 >> 2, i >> 2) + 4 * (i & 3));
+    return v;
+  } else {
+    return __builtin_bit_cast(typename P4<DT>::t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s4)(base + TL::off(4 * gq + (i >> 2), col0 >> 3, (i & 3) >> 1) + 8 * (i & 1))));
   }
 }
 
@@ -139,31 +155,79 @@ __device__ __forceinline__ int seq_len(const LatentDecodeArgs& a, int b) {
   const int n = a.lens[b];
   return n < 0 ? 0 : (n > cap ? static_cast<int>(cap) : n);
 }
-// Tiles of sequences [0, b1), summed by the wave.
-template <int KT>
-__device__ __forceinline__ int tiles_before(const LatentDecodeArgs& a, int b1) {
-  int n = 0;
-  for (int i = __lane_id(); i < b1; i += 64) n += (seq_len(a, i) + KT - 1) / KT;
+__device__ __forceinline__ int wave_sum(int n) {
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) n += __shfl_xor(n, s, 64);
   return __builtin_amdgcn_readfirstlane(n);
 }
+// inclusive prefix sum over the lanes
+__device__ __forceinline__ int wave_scan(int n) {
+  const int lane = __lane_id();
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(n, d, 64);
+    n += lane >= d ? up : 0;
+  }
+  return n;
+}
 
-template <int DT, int R, int DR, int NB>
-__global__ __launch_bounds__(256, 1) void kda_latent_decode_kernel(LatentDecodeArgs a) {
-  typedef DecCfg<DT, R, DR, NB> C;
-  typedef typename El<DT>::frag F;
-  typedef typename El<DT>::t E;
-  constexpr int ES = C::ES, KT = C::KT, W = R + DR, KS = W / 32, KSN = R / 32, NV = R / 64, M16 = 16 * NB;
-  __shared__ __attribute__((aligned(1024))) char buf0[C::BUF];
-  __shared__ __attribute__((aligned(1024))) char buf1[C::BUF];
-  __shared__ __attribute__((aligned(1024))) char sp[C::TP::bytes(M16)];
-  __shared__ float red[4][M16];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m = lane & 15, gq = lane >> 4;
+// Places of a sequence on the line: its tiles, and a.pad for what a workgroup
+// spends on a sequence beside them (queries, first copies, the waves' sums), so
+// that one run does not collect many short sequences.
+__device__ __forceinline__ int places(const LatentDecodeArgs& a, int len, int KT) {
+  return len > 0 ? (len + KT - 1) / KT + a.pad : 0;
+}
+// The part of the line that workgroup w covers: places [g, g1), the first of them
+// place t of sequence b.
+struct Run {
+  int g, g1, b, t, len;              // len: sequence b's length
+  __device__ __forceinline__ Run uniform() const {   // in scalar registers
+    return {__builtin_amdgcn_readfirstlane(g), __builtin_amdgcn_readfirstlane(g1), __builtin_amdgcn_readfirstlane(b),
+            __builtin_amdgcn_readfirstlane(t), __builtin_amdgcn_readfirstlane(len)};
+  }
+};
+__device__ __forceinline__ Run find_run(const LatentDecodeArgs& a, int w, int KT) {
+  const int lane = __lane_id();
+  Run r{0, 0, 0, 0, 0};
+  if (a.whole) {                     // a workgroup a sequence
+    r.b = w;
+    r.len = seq_len(a, w);
+    r.g1 = (r.len + KT - 1) / KT;
+    return r;
+  }
+  int n = lane < a.B ? seq_len(a, lane) : 0, nt = places(a, n, KT), sum = nt;
+  for (int i = lane + 64; i < a.B; i += 64) sum += places(a, seq_len(a, i), KT);
+  const int total = wave_sum(sum), per = max(a.least, (total + a.wgs - 1) / a.wgs);
+  r.g = w * per;
+  r.g1 = min(total, r.g + per);
+  const bool tell = blockIdx.x == 0 && threadIdx.x < 64;   // the join kernel's starts of the sequences
+  if (tell && lane == 0) a.line[0] = per;
+  int base = 0;
+  bool found = false;
+  for (int s0 = 0; s0 < a.B; s0 += 64) {
+    if (s0 > 0) {
+      n = s0 + lane < a.B ? seq_len(a, s0 + lane) : 0;
+      nt = places(a, n, KT);
+    }
+    const int inc = wave_scan(nt);
+    if (tell && s0 + lane < a.B) a.line[1 + s0 + lane] = base + inc - nt;
+    const unsigned long long hit = __ballot(base + inc > r.g);
+    if (hit && !found) {
+      const int x = __ffsll(static_cast<long long>(hit)) - 1;
+      r.b = s0 + x;
+      r.t = r.g - base - (__builtin_amdgcn_readlane(inc, x) - __builtin_amdgcn_readlane(nt, x));
+      r.len = __builtin_amdgcn_readlane(n, x);
+      found = true;
+    }
+    if (found && !tell) break;
+    base += __builtin_amdgcn_readlane(inc, 63);
+  }
+  return r;
+}
 
-  // the row groups of one run are eight workgroups apart, on one XCD, whose L2 serves the second
-  int w, grp;
+// workgroup -> run and row group; the groups of one run are eight workgroups
+// apart, on one XCD, whose L2 then serves all but the first
+__device__ __forceinline__ void run_group(const LatentDecodeArgs& a, int& w, int& grp) {
   if (a.wgs % 8 == 0) {
     grp = (blockIdx.x >> 3) % a.groups;
     w = (blockIdx.x / (8 * a.groups)) * 8 + (blockIdx.x & 7);
@@ -171,160 +235,356 @@ __global__ __launch_bounds__(256, 1) void kda_latent_decode_kernel(LatentDecodeA
     grp = blockIdx.x % a.groups;
     w = blockIdx.x / a.groups;
   }
-  const int total = tiles_before<KT>(a, a.B);
-  const int per = (total + a.wgs - 1) / a.wgs;
-  int g = w * per;
-  const int g1 = min(total, g + per);
-  if (g >= g1) return;
-  // sequence and tile of the run's first tile
-  int b = 0, t = 0;
-  {
-    int base = 0;
-    for (int s0 = 0; s0 < a.B; s0 += 64) {
-      const int nt_ = s0 + lane < a.B ? (seq_len(a, s0 + lane) + KT - 1) / KT : 0;
-      int inc = nt_;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int up = __shfl_up(inc, d, 64);
-        inc += lane >= d ? up : 0;
-      }
-      const unsigned long long hit = __ballot(base + inc > g);
-      if (hit) {
-        const int x = __ffsll(static_cast<long long>(hit)) - 1;
-        b = s0 + x;
-        t = __builtin_amdgcn_readfirstlane(g - base - (__shfl(inc, x, 64) - __shfl(nt_, x, 64)));
-        break;
-      }
-      base += __builtin_amdgcn_readfirstlane(__shfl(inc, 63, 64));
-    }
-  }
+}
 
-  const int rows = a.Tq * a.H;
+// zeros for the rows of an empty sequence
+template <int DT, int R>
+__device__ __forceinline__ void empty_rows(const LatentDecodeArgs& a, int b, int r0, int r1, int threads) {
+  for (int i = threadIdx.x; i < (r1 - r0) * (R / 4); i += threads) {
+    const int64_t row = static_cast<int64_t>(b) * a.Tq * a.H + r0 + i / (R / 4);
+    store4<DT>(a.o, row * R + 4 * (i % (R / 4)), 0.f, 0.f, 0.f, 0.f);
+    if (i % (R / 4) == 0) a.lse[row] = -INFINITY;
+  }
+}
+
+// page of token tok, inside the cache; row of a token from it
+__device__ __forceinline__ int page_of(const LatentDecodeArgs& a, const int32_t* table, int tok) {
+  return table[tok >> a.page_shift];
+}
+__device__ __forceinline__ int slot_of(const LatentDecodeArgs& a, int page, int tok) {
+  return (min(max(page, 0), static_cast<int>(a.n_pages - 1)) << a.page_shift) + (tok & ((1 << a.page_shift) - 1));
+}
+
+// Order of a product's instructions: AHEAD fragment reads of RPF LDS reads each
+// first, then a product for each further fragment read, then the rest.
+template <int N, int AHEAD, int RPF>
+__device__ __forceinline__ void pace() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * RPF, 0);
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, RPF > 2 ? 4 : 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, RPF, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, RPF > 2 ? 4 * AHEAD : AHEAD, 0);
+}
+
+template <int DT, int R, int DR>
+__global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decode16_kernel(LatentDecodeArgs a) {
+  typedef DecCfg<DT, R, DR> C;
+  typedef typename El<DT>::frag F;
+  typedef typename El<DT>::t E;
+  constexpr int ES = C::ES, NW = C::NW, KT = C::KT, W = R + DR, KS = W / 32, KSN = R / 32, NV = R / 16;
+  __shared__ __attribute__((aligned(1024))) char buf[NW * C::WBUF];
+  __shared__ float red_m[NW][16], red_l[NW][16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 15, gq = lane >> 4;
+  int w, grp;
+  run_group(a, w, grp);
+  Run run = find_run(a, w, KT).uniform();
+  const int rows = a.Tq * a.H, r = grp * 16 + m;
+  if (a.whole && run.g1 == 0) empty_rows<DT, R>(a, w, grp * 16, min(rows, grp * 16 + 16), 64 * NW);
+
   const float c = a.scale * kLog2e, lazy = kLazy / c;
   const char* cache = static_cast<const char*>(a.cache);
+  char* const mine = buf + wave * C::WBUF;
 
-  while (g < g1) {
-    const int len = seq_len(a, b), n_all = (len + KT - 1) / KT;
-    if (n_all == 0) { ++b; t = 0; continue; }
-    const int ta = t, tb = min(n_all, t + (g1 - g));   // this segment's tiles
+  while (run.g < run.g1) {
+    const int b = run.b, len = run.len, n_all = (len + KT - 1) / KT;
+    const int ta = run.t, tb = min(n_all, ta + (run.g1 - run.g));   // this segment's tiles
+    if (ta < tb) {
     const int32_t* table = a.table + static_cast<int64_t>(b) * a.per;
 
-    // cache row of this lane's key of a tile (KT <= 64 keys, one a lane)
-    auto slot_of = [&](int j) {
-      const int tok = min(j * KT + (lane & (KT - 1)), len - 1);
-      const int page = min(max(table[tok >> a.page_shift], 0), static_cast<int>(a.n_pages - 1));
-      return (page << a.page_shift) + (tok & ((1 << a.page_shift) - 1));
+    auto token = [&](int j) { return min(j * KT + m, len - 1); };   // key m of tile j
+    auto fetch = [&](int slot) {
+      const int ln = fresh(lane);
+#pragma unroll
+      for (int p = 0; p < C::PN; ++p) {
+        const int s = p * 64 + ln, rr = s / C::TN::CPR;
+        const int64_t at = C::TN::CPR % 64 == 0 ? __builtin_amdgcn_readlane(slot, p * 64 / C::TN::CPR) : __shfl(slot, rr, 64);
+        copy16(cache + at * (W * ES) + (((s % C::TN::CPR) ^ C::TN::swz(rr)) << 4), mine + p * 1024);
+      }
+#pragma unroll
+      for (int p = 0; p < C::PR; ++p) {
+        const int s = p * 64 + ln, rr = s / C::TR::CPR;
+        copy16(cache + static_cast<int64_t>(__shfl(slot, rr, 64)) * (W * ES) + R * ES +
+                   (((s % C::TR::CPR) ^ C::TR::swz(rr)) << 4), mine + C::OFF_R + p * 1024);
+      }
     };
+
+    int page = page_of(a, table, token(ta + wave));   // of the next tile to copy
+    if (ta + wave < tb) {
+      fetch(slot_of(a, page, token(ta + wave)));
+      page = page_of(a, table, token(ta + wave + NW));
+    }
+    F q[KS];
+    {
+      const E* qp = static_cast<const E*>(a.q) + (static_cast<int64_t>(b) * rows + min(r, rows - 1)) * W;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const F*>(qp + 32 * s + 8 * gq);
+    }
+    const int seen = len - (a.Tq - 1 - min(r, rows - 1) / a.H);
+
+    f4 acc[NV];
+    float mx = kMaxInit, mc = kMaxInit * c, l = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) acc[v] = f4{0, 0, 0, 0};
+
+    for (int j = ta + wave; j < tb; j += NW) {
+      wait_vmem_all();
+      const int ln = fresh(lane), fm = ln & 15, fg = ln >> 4;
+      f4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};     // two chains
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const F kf = k < KSN ? row_frag16<typename C::TN, F>(mine, fm, k, fg)
+                             : row_frag16<typename C::TR, F>(mine + C::OFF_R, fm, k - KSN, fg);
+        if (k & 1) s1 = mma_s(s1, kf, q[k]);
+        else s0 = mma_s(s0, kf, q[k]);
+      }
+      if constexpr (ES == 2) pace<KS, 8, 1>();
+      const int key0 = j * KT + 4 * gq;
+      f4 s = s0 + s1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = key0 + i < seen ? s[i] : -INFINITY;
+      const float tm = group_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+      if (__any(tm > mx + lazy)) {
+        const float nm = fmaxf(mx, tm), al = fast_exp2((mx - nm) * c);
+        mx = nm;
+        mc = nm * c;
+        l *= al;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) acc[v] *= al;
+      }
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = fast_exp2(fmaf(s[i], c, -mc));
+        l += e[i];
+      }
+      const auto p = to_p4<DT>(e);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) acc[v] = mma_p(acc[v], v_frag<DT, typename C::TN>(mine, 16 * v, ln), p);
+      if constexpr (ES == 2) pace<NV, 8, 1>();
+      if (j + NW < tb) {
+        lds_reads_done();                    // the buffer is read out
+        fetch(slot_of(a, page, token(j + NW)));
+        page = page_of(a, table, token(j + 2 * NW));
+      }
+    }
+
+    // the waves' sums: scaled to the common maximum, added in wave order by the wave that
+    // owns a share of the columns, as many columns at a time as the buffers hold
+    l = group_sum(l);
+    if (gq == 0) {
+      red_m[wave][m] = mc;
+      red_l[wave][m] = l;
+    }
+    lds_barrier();                           // also: every wave has left its buffer
+    const bool whole = ta == 0 && tb == n_all;
+    float mt = red_m[0][m], ls = 0.f;
+#pragma unroll
+    for (int x = 1; x < NW; ++x) mt = fmaxf(mt, red_m[x][m]);
+#pragma unroll
+    for (int x = 0; x < NW; ++x) ls = fmaf(fast_exp2(red_m[x][m] - mt), red_l[x][m], ls);
+    const float f = fast_exp2(mc - mt);
+    const int64_t row = static_cast<int64_t>(b) * rows + r;
+    const int64_t sr = (static_cast<int64_t>(2 * w + (ta > 0 ? 0 : 1)) * a.groups + grp) * 16 + m;
+    const float inv = whole ? (ls > 0.f ? 1.f / ls : ls) : 1.f;   // nothing visible: zeros; NaN stays NaN
+    constexpr int VR = C::NVR < NV ? (C::NVR >= NV / 2 ? NV / 2 : NV / 4) : NV;   // column blocks of a round
+    static_assert(VR % NW == 0 && NV % VR == 0 && VR * NW * 1024 <= NW * C::WBUF, "rounds of columns");
+#pragma unroll
+    for (int v0 = 0; v0 < NV; v0 += VR) {
+      if (v0 > 0) lds_barrier();             // the round before has been read
+#pragma unroll
+      for (int v = 0; v < VR; ++v)
+        *reinterpret_cast<f4*>(buf + (wave * VR + v) * 1024 + lane * 16) = acc[v0 + v] * f;
+      lds_barrier();
+#pragma unroll
+      for (int v = 0; v < VR / NW; ++v) {
+        const int vb = wave * (VR / NW) + v;
+        f4 o = {0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < NW; ++x) o += *reinterpret_cast<const f4*>(buf + (x * VR + vb) * 1024 + lane * 16);
+        o *= inv;
+        const int col = 16 * (v0 + vb) + 4 * gq;
+        if (r < rows) {
+          if (whole) store4<DT>(a.o, row * R + col, o[0], o[1], o[2], o[3]);
+          else *reinterpret_cast<f4*>(a.part_o + sr * R + col) = o;
+        }
+      }
+    }
+    if (wave == 0 && gq == 0 && r < rows) {
+      if (whole) {
+        a.lse[row] = ls == 0.f ? -INFINITY : (mt + __log2f(ls)) * kLn2;
+      } else {
+        a.part_ml[2 * sr] = mt;
+        a.part_ml[2 * sr + 1] = ls;
+      }
+    }
+    lds_barrier();                           // the sums have been read: the buffers are free
+    }
+    run.g += places(a, len, KT) - ta;
+    ++run.b;
+    run.t = 0;
+    if (run.g < run.g1) run.len = seq_len(a, run.b);
+  }
+}
+
+// More than 16 rows: 64 a workgroup (16-bit types).  120 flop a byte and more, so
+// the waves share each tile of 64 keys: for the scores a wave takes 32 keys by 32
+// rows (32x32x16, its rows' queries in 144 registers), for the output a
+// quarter of the R columns by all 64 rows.  A wave's probabilities go to LDS in
+// the fragment order that they are made in.  They are formed against the
+// maximum that the waves agreed on last; only a tile that exceeds it by 2^8 costs
+// the extra exchange, so a tile takes two barriers.
+template <int DT, int R, int DR>
+__global__ __launch_bounds__(256, 1) void kda_latent_decode64_kernel(LatentDecodeArgs a) {
+  typedef typename El<DT>::frag F;
+  typedef typename El<DT>::t E;
+  typedef Tile<R, 2> TN;
+  typedef Tile<DR, 2> TR;
+  typedef Tile<64, 2> TP;
+  constexpr int KT = 64, W = R + DR, KN = R / 16, KR = DR / 16, NV = R / 128;
+  constexpr int OFF_R = TN::bytes(KT), BUF = OFF_R + TR::bytes(KT);
+  __shared__ __attribute__((aligned(1024))) char buf0[BUF];
+  __shared__ __attribute__((aligned(1024))) char buf1[BUF];
+  __shared__ __attribute__((aligned(1024))) char sp[TP::bytes(64)];
+  __shared__ float red[2][64];
+  __shared__ int raise[2];                   // whether a tile exceeds the agreed maximum; by tile parity
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 31, h = lane >> 5, kh = wave >> 1, rh = wave & 1;   // key and row halves of the scores
+  int w, grp;
+  run_group(a, w, grp);
+  Run run = find_run(a, w, KT).uniform();
+  const int rows = a.Tq * a.H, r0 = grp * 64;
+  if (a.whole && run.g1 == 0) empty_rows<DT, R>(a, w, r0, min(rows, r0 + 64), 256);
+
+  const float c = a.scale * kLog2e, lazy = kLazy / c;
+  const char* cache = static_cast<const char*>(a.cache);
+  const int qrow = min(r0 + 32 * rh + m, rows - 1);
+
+  while (run.g < run.g1) {
+    const int b = run.b, len = run.len, n_all = (len + KT - 1) / KT;
+    const int ta = run.t, tb = min(n_all, ta + (run.g1 - run.g));
+    if (ta < tb) {
+    const int32_t* table = a.table + static_cast<int64_t>(b) * a.per;
+    auto token = [&](int j) { return min(j * KT + lane, len - 1); };   // a key a lane
     auto fetch = [&](int slot, char* dst) {
-      constexpr int PN = KT * C::TN::CPR / 64, PR = KT * C::TR::CPR / 64;
+      const int ln = fresh(lane);
 #pragma unroll
-      for (int p = 0; p < PN / 4; ++p) {
-        const int s = (wave + 4 * p) * 64 + lane, r = s / C::TN::CPR;
-        const char* src = cache + static_cast<int64_t>(__shfl(slot, r, 64)) * (W * ES) + (((s % C::TN::CPR) ^ C::TN::swz(r)) << 4);
-        copy16(src, dst + (wave + 4 * p) * 1024);
+      for (int p = 0; p < KT * TN::CPR / 256; ++p) {
+        const int s = (wave + 4 * p) * 64 + ln, rr = s / TN::CPR;
+        const int64_t at = TN::CPR == 64 ? __builtin_amdgcn_readlane(slot, wave + 4 * p) : __shfl(slot, rr, 64);
+        copy16(cache + at * (W * 2) + (((s % TN::CPR) ^ TN::swz(rr)) << 4), dst + (wave + 4 * p) * 1024);
       }
 #pragma unroll
-      for (int p = 0; p < (PR + 3) / 4; ++p) {
-        if (PR % 4 != 0 && wave + 4 * p >= PR) break;
-        const int s = (wave + 4 * p) * 64 + lane, r = s / C::TR::CPR;
-        const char* src = cache + static_cast<int64_t>(__shfl(slot, r, 64)) * (W * ES) + R * ES +
-                          (((s % C::TR::CPR) ^ C::TR::swz(r)) << 4);
-        copy16(src, dst + C::OFF_R + (wave + 4 * p) * 1024);
+      for (int p = 0; p < KT * TR::CPR / 256; ++p) {
+        const int s = (wave + 4 * p) * 64 + ln, rr = s / TR::CPR;
+        copy16(cache + static_cast<int64_t>(__shfl(slot, rr, 64)) * (W * 2) + R * 2 + (((s % TR::CPR) ^ TR::swz(rr)) << 4),
+               dst + OFF_R + (wave + 4 * p) * 1024);
       }
     };
-
-    int next_slot = slot_of(ta);
-    // queries of the group: lane column m of each 16-row block
-    F q[NB][KS];
-    int seen[NB];
+    const int tok0 = token(ta);
+    const int page0 = page_of(a, table, tok0);
+    int page = page_of(a, table, token(ta + 1));
+    F q[KN + KR];
+    {
+      const E* qp = static_cast<const E*>(a.q) + (static_cast<int64_t>(b) * rows + qrow) * W;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const int r = min(grp * M16 + 16 * n + m, rows - 1);
-      seen[n] = len - (a.Tq - 1 - r / a.H);
-      const E* qp = static_cast<const E*>(a.q) + (static_cast<int64_t>(b) * rows + r) * W;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) q[n][s] = *reinterpret_cast<const F*>(qp + 32 * s + 8 * gq);
+      for (int s = 0; s < KN + KR; ++s) q[s] = *reinterpret_cast<const F*>(qp + 16 * s + 8 * h);
     }
-    lds_barrier();                          // the last segment's reads of the buffers are done
-    fetch(next_slot, buf0);
-    if (ta + 1 < tb) next_slot = slot_of(ta + 1);
+    const int seen = len - (a.Tq - 1 - qrow / a.H);
+    if (threadIdx.x < 2) raise[threadIdx.x] = 0;
+    lds_barrier();                           // the last segment has left the buffers
+    fetch(slot_of(a, page0, tok0), buf0);
 
-    f4 acc[NB][NV];
-    float mx[NB], mc[NB], l[NB];
+    f16v acc[NV][2];
+    float mx = kMaxInit, l = 0.f;            // of row 32 rh + m; l over this wave's keys
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      mx[n] = kMaxInit;
-      mc[n] = kMaxInit * c;
-      l[n] = 0.f;
+    for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int v = 0; v < NV; ++v) acc[n][v] = f4{0, 0, 0, 0};
-    }
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[v][n][i] = 0.f;
 
     auto step = [&](int j, const char* cur, char* nxt) {
       wait_vmem_all();
       lds_barrier();
+      if (threadIdx.x == 0) raise[(j + 1) & 1] = 0;
       if (j + 1 < tb) {
-        fetch(next_slot, nxt);
-        if (j + 2 < tb) next_slot = slot_of(j + 2);
+        const int slot = slot_of(a, page, token(j + 1));
+        page = page_of(a, table, token(j + 2));
+        fetch(slot, nxt);
       }
-      f4 s[NB];
+      const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
+      f16v s, s1;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) s[n] = f4{0, 0, 0, 0};
-      if (16 * wave < KT) {
+      for (int i = 0; i < 16; ++i) s[i] = s1[i] = 0.f;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const F kf = k < KSN ? row_frag16<typename C::TN, F>(cur, 16 * wave + m, k, gq)
-                               : row_frag16<typename C::TR, F>(cur + C::OFF_R, 16 * wave + m, k - KSN, gq);
-#pragma unroll
-          for (int n = 0; n < NB; ++n) s[n] = mma_s(s[n], kf, q[n][k]);
-        }
-        const int key0 = j * KT + 16 * wave + 4 * gq;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][i] = key0 + i < seen[n] ? s[n][i] : -INFINITY;
-          float tm = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3]));
-          tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
-          tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-          if (gq == 0) red[wave][16 * n + m] = tm;
-        }
+      for (int k = 0; k < KN; k += 2) {
+        s = mma(s, TN::template row_frag<F>(cur, 32 * kh + fm, k, fh), q[k]);
+        s1 = mma(s1, TN::template row_frag<F>(cur, 32 * kh + fm, k + 1, fh), q[k + 1]);
       }
-      lds_barrier();
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        float tm = red[0][16 * n + m];
+      for (int k = 0; k < KR; k += 2) {
+        s = mma(s, TR::template row_frag<F>(cur + OFF_R, 32 * kh + fm, k, fh), q[KN + k]);
+        s1 = mma(s1, TR::template row_frag<F>(cur + OFF_R, 32 * kh + fm, k + 1, fh), q[KN + k + 1]);
+      }
+      const int key0 = j * KT + 32 * kh + 4 * h;
+      float tm = -INFINITY;
 #pragma unroll
-        for (int x = 1; x < KT / 16; ++x) tm = fmaxf(tm, red[x][16 * n + m]);
-        if (__any(tm > mx[n] + lazy)) {
-          const float nm = fmaxf(mx[n], tm), al = fast_exp2((mx[n] - nm) * c);
-          mx[n] = nm;
-          mc[n] = nm * c;
-          l[n] *= al;
+      for (int i = 0; i < 16; ++i) {
+        s[i] += s1[i];
+        s[i] = key0 + 8 * (i >> 2) + (i & 3) < seen ? s[i] : -INFINITY;
+        tm = fmaxf(tm, s[i]);
+      }
+      tm = half_max(tm);
+      float lt = 0.f;
+      auto probs = [&] {
+        const float mc = mx * c;
+        lt = 0.f;
 #pragma unroll
-          for (int v = 0; v < NV; ++v) acc[n][v] *= al;
-        }
-        if (16 * wave < KT) {
-          float p[4];
+        for (int u = 0; u < 2; ++u) {
+          float p[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[i] = fast_exp2(fmaf(s[n][i], c, -mc[n]));
-            l[n] += p[i];
+          for (int e = 0; e < 8; ++e) {
+            p[e] = fast_exp2(fmaf(s[8 * u + e], c, -mc));
+            lt += p[e];
           }
-          const int key = 16 * wave + 4 * gq;
-          store4<DT>(sp + C::TP::off(16 * n + m, key * ES / 16) + (key * ES) % 16, 0, p[0], p[1], p[2], p[3]);
+          *reinterpret_cast<F*>(sp + TP::off(32 * rh + fm, 4 * kh + 2 * u, fh)) = to_frag<DT>(p);
+        }
+      };
+      probs();
+      if (h == 0) red[kh][32 * rh + m] = tm;
+      if (__any(tm > mx + lazy) && lane == 0) raise[j & 1] = 1;
+      lds_barrier();
+      if (raise[j & 1]) {                    // the whole workgroup: new maxima, sums scaled, probabilities again
+        const float o0 = mx;
+        // the output's columns are rows m and 32 + m: their old and new maxima, from the score waves
+        const float nm = fmaxf(mx, fmaxf(red[0][32 * rh + m], red[1][32 * rh + m]));
+        mx = nm;
+        l *= fast_exp2((o0 - nm) * c);
+        lds_barrier();
+        probs();
+        if (kh == 0 && h == 0) red[0][32 * rh + m] = fast_exp2((o0 - nm) * c);
+        lds_barrier();
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float al = red[0][32 * n + m];
+#pragma unroll
+          for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[v][n][i] *= al;
         }
       }
-      lds_barrier();
+      l += lt;
 #pragma unroll
-      for (int k = 0; k < KT / 32; ++k) {
-        F pf[NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) pf[n] = row_frag16<typename C::TP, F>(sp, 16 * n + m, k, gq);
+      for (int k = 0; k < 4; ++k) {
+        const F p0 = TP::template row_frag<F>(sp, fm, k, fh), p1 = TP::template row_frag<F>(sp, 32 + fm, k, fh);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          const F vf = col_frag16<typename C::TN, F>(cur, k, wave * (R / 4) + 16 * v, lane);
-#pragma unroll
-          for (int n = 0; n < NB; ++n) acc[n][v] = mma_s(acc[n][v], vf, pf[n]);
+          const F vf = TN::template col_frag<F>(cur, 16 * k, wave * (R / 4) + 32 * v, ln);
+          acc[v][0] = mma(acc[v][0], vf, p0);
+          acc[v][1] = mma(acc[v][1], vf, p1);
         }
       }
     };
@@ -335,81 +595,94 @@ __global__ __launch_bounds__(256, 1) void kda_latent_decode_kernel(LatentDecodeA
       ++j;
     }
 
-    // row sums over the four lane groups and the four waves
     lds_barrier();
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      l[n] += __shfl_xor(l[n], 16, 64);
-      l[n] += __shfl_xor(l[n], 32, 64);
-      if (gq == 0) red[wave][16 * n + m] = l[n];
-    }
+    l = half_sum(l);
+    if (h == 0) red[kh][32 * rh + m] = l;
+    float* ms = reinterpret_cast<float*>(sp);   // the rows' maxima
+    if (kh == 0 && h == 0) ms[32 * rh + m] = mx * c;
     lds_barrier();
     const bool whole = ta == 0 && tb == n_all;
-    const int64_t slot = (static_cast<int64_t>(2 * w + (ta > 0 ? 0 : 1)) * a.groups + grp) * M16;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const int r = grp * M16 + 16 * n + m;
-      const float ls = red[0][16 * n + m] + red[1][16 * n + m] + red[2][16 * n + m] + red[3][16 * n + m];
-      if (r < rows) {
-        const int64_t row = static_cast<int64_t>(b) * rows + r;
-        const int col = wave * (R / 4) + 4 * gq;
+    for (int n = 0; n < 2; ++n) {
+      const int r = r0 + 32 * n + m;
+      const float ls = red[0][32 * n + m] + red[1][32 * n + m], mc = ms[32 * n + m];
+      if (r >= rows) continue;
+      const int64_t row = static_cast<int64_t>(b) * rows + r;
+      const int64_t sr = (static_cast<int64_t>(2 * w + (ta > 0 ? 0 : 1)) * a.groups + grp) * 64 + 32 * n + m;
+      const int col = wave * (R / 4) + 4 * h;
+      const float inv = ls > 0.f ? 1.f / ls : ls;   // nothing visible: zeros; NaN stays NaN
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f4 o = {acc[v][n][4 * i], acc[v][n][4 * i + 1], acc[v][n][4 * i + 2], acc[v][n][4 * i + 3]};
+          if (whole) store4<DT>(a.o, row * R + col + 32 * v + 8 * i, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+          else *reinterpret_cast<f4*>(a.part_o + sr * R + col + 32 * v + 8 * i) = o;
+        }
+      if (wave == 0 && h == 0) {
         if (whole) {
-          const float inv = ls > 0.f ? 1.f / ls : ls;   // nothing visible: zeros; NaN stays NaN
-#pragma unroll
-          for (int v = 0; v < NV; ++v)
-            store4<DT>(a.o, row * R + col + 16 * v, acc[n][v][0] * inv, acc[n][v][1] * inv, acc[n][v][2] * inv,
-                       acc[n][v][3] * inv);
-          if (wave == 0 && gq == 0) a.lse[row] = ls == 0.f ? -INFINITY : (mc[n] + __log2f(ls)) * kLn2;
+          a.lse[row] = ls == 0.f ? -INFINITY : (mc + __log2f(ls)) * kLn2;
         } else {
-          const int64_t sr = slot + 16 * n + m;
-#pragma unroll
-          for (int v = 0; v < NV; ++v) *reinterpret_cast<f4*>(a.part_o + sr * R + col + 16 * v) = acc[n][v];
-          if (wave == 0 && gq == 0) {
-            a.part_ml[2 * sr] = mc[n];
-            a.part_ml[2 * sr + 1] = ls;
-          }
+          a.part_ml[2 * sr] = mc;
+          a.part_ml[2 * sr + 1] = ls;
         }
       }
     }
-    g += tb - ta;
-    ++b;
-    t = 0;
+    lds_barrier();
+    }
+    run.g += places(a, len, KT) - ta;
+    ++run.b;
+    run.t = 0;
+    if (run.g < run.g1) run.len = seq_len(a, run.b);
   }
 }
 
-// Joins the parts of a split sequence in run order; writes the rows of a sequence of length zero.
+// Joins the parts of a split sequence in run order, one row a workgroup; writes
+// the rows of an empty sequence.  Two halves of the workgroup take every second part.
 template <int DT, int R, int KT>
-__global__ __launch_bounds__(256) void kda_latent_join_kernel(LatentDecodeArgs a, int M16) {
-  constexpr int TPR = R / 4, RPB = 256 / TPR;
-  const int rows = a.Tq * a.H;
-  const int b = blockIdx.y, r = blockIdx.x * RPB + threadIdx.x / TPR, col = (threadIdx.x % TPR) * 4;
+__global__ __launch_bounds__(R / 2) void kda_latent_join_kernel(LatentDecodeArgs a, int M16) {
+  __shared__ float fac[64];
+  __shared__ f4 other[R / 4];
+  const int rows = a.Tq * a.H, lane = threadIdx.x & 63;
+  const int b = blockIdx.y, r = blockIdx.x, half = threadIdx.x / (R / 4), col = (threadIdx.x % (R / 4)) * 4;
   const int n = (seq_len(a, b) + KT - 1) / KT;
-  const int g0 = tiles_before<KT>(a, b), total = tiles_before<KT>(a, a.B);
-  if (r >= rows) return;
   const int64_t row = static_cast<int64_t>(b) * rows + r;
   if (n == 0) {
-    store4<DT>(a.o, row * R + col, 0.f, 0.f, 0.f, 0.f);
-    if (col == 0) a.lse[row] = -INFINITY;
+    if (half == 0) store4<DT>(a.o, row * R + col, 0.f, 0.f, 0.f, 0.f);
+    if (threadIdx.x == 0) a.lse[row] = -INFINITY;
     return;
   }
-  const int per = (total + a.wgs - 1) / a.wgs;
+  const int per = a.line[0], g0 = a.line[1 + b];
   const int w0 = g0 / per, w1 = (g0 + n - 1) / per;
   if (w0 == w1) return;
   const int grp = r / M16;
   auto at = [&](int w) { return (static_cast<int64_t>(2 * w + (w == w0 ? 1 : 0)) * a.groups + grp) * M16 + (r - grp * M16); };
   float mx = kMaxInit;
-  for (int w = w0; w <= w1; ++w) mx = fmaxf(mx, a.part_ml[2 * at(w)]);
+  for (int w = w0 + lane; w <= w1; w += 64) mx = fmaxf(mx, a.part_ml[2 * at(w)]);
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) mx = fmaxf(mx, __shfl_xor(mx, s, 64));
   f4 o = {0, 0, 0, 0};
   float l = 0.f;
-  for (int w = w0; w <= w1; ++w) {
-    const int64_t s = at(w);
-    const float f = fast_exp2(a.part_ml[2 * s] - mx);
-    l = fmaf(f, a.part_ml[2 * s + 1], l);
-    o += f * *reinterpret_cast<const f4*>(a.part_o + s * R + col);
+  for (int wb = w0; wb <= w1; wb += 64) {
+    const int cnt = min(64, w1 - wb + 1);
+    __syncthreads();
+    if (threadIdx.x < 64) fac[lane] = lane < cnt ? fast_exp2(a.part_ml[2 * at(wb + lane)] - mx) : 0.f;
+    const float pl = lane < cnt ? a.part_ml[2 * at(wb + lane) + 1] : 0.f;
+    __syncthreads();
+    float x = fac[lane] * pl;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) x += __shfl_xor(x, s, 64);
+    l += x;
+#pragma unroll 8
+    for (int i = half; i < cnt; i += 2) o += fac[i] * *reinterpret_cast<const f4*>(a.part_o + at(wb + i) * R + col);
   }
+  if (half == 1) other[col / 4] = o;
+  __syncthreads();
+  if (half == 1) return;
+  o += other[col / 4];
   const float inv = l > 0.f ? 1.f / l : l;
   store4<DT>(a.o, row * R + col, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-  if (col == 0) a.lse[row] = l == 0.f ? -INFINITY : (mx + __log2f(l)) * kLn2;
+  if (threadIdx.x == 0) a.lse[row] = l == 0.f ? -INFINITY : (mx + __log2f(l)) * kLn2;
 }
 
 template <int DT, int R, int DR>
@@ -421,27 +694,27 @@ hipError_t run_append(const LatentAppendArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int DT, int R, int DR, int NB>
-hipError_t run_decode(const LatentDecodeArgs& a, hipStream_t s) {
-  kda_latent_decode_kernel<DT, R, DR, NB><<<dim3(a.wgs * a.groups), dim3(256), 0, s>>>(a);
-  constexpr int RPB = 256 / (R / 4);
-  kda_latent_join_kernel<DT, R, DecCfg<DT, R, DR, NB>::KT>
-      <<<dim3((a.Tq * a.H + RPB - 1) / RPB, a.B), dim3(256), 0, s>>>(a, 16 * NB);
+template <int DT, int R, int DR>
+hipError_t run_decode(const LatentDecodeArgs& a, int m_rows, hipStream_t s) {
+  typedef DecCfg<DT, R, DR> C;
+  if (m_rows == 16) {
+    kda_latent_decode16_kernel<DT, R, DR><<<dim3(a.wgs * a.groups), dim3(64 * C::NW), 0, s>>>(a);
+  } else if constexpr (DT != 0) {
+    kda_latent_decode64_kernel<DT, R, DR><<<dim3(a.wgs * a.groups), dim3(256), 0, s>>>(a);
+  } else {
+    return hipErrorInvalidValue;
+  }
+  if (a.whole) return hipGetLastError();
+  const dim3 grid(a.Tq * a.H, a.B), block(R / 2);
+  if (m_rows == 16) kda_latent_join_kernel<DT, R, 16><<<grid, block, 0, s>>>(a, 16);
+  else kda_latent_join_kernel<DT, R, 64><<<grid, block, 0, s>>>(a, 64);
   return hipGetLastError();
 }
 
-template <int DT, int R, int DR>
-hipError_t decode_by_rows(const LatentDecodeArgs& a, int nb, hipStream_t s) {
-  if (nb == 1) return run_decode<DT, R, DR, 1>(a, s);
-  if (nb == 2) return run_decode<DT, R, DR, 2>(a, s);
-  if constexpr (DT != 0) return run_decode<DT, R, DR, 4>(a, s);
-  return hipErrorInvalidValue;
-}
-
 template <int DT>
-hipError_t decode_by_dims(const LatentDecodeArgs& a, int R, int dr, int nb, hipStream_t s) {
-  if (R == 512) return dr == 64 ? decode_by_rows<DT, 512, 64>(a, nb, s) : decode_by_rows<DT, 512, 32>(a, nb, s);
-  return dr == 64 ? decode_by_rows<DT, 256, 64>(a, nb, s) : decode_by_rows<DT, 256, 32>(a, nb, s);
+hipError_t decode_by_dims(const LatentDecodeArgs& a, int R, int dr, int m_rows, hipStream_t s) {
+  if (R == 512) return dr == 64 ? run_decode<DT, 512, 64>(a, m_rows, s) : run_decode<DT, 512, 32>(a, m_rows, s);
+  return dr == 64 ? run_decode<DT, 256, 64>(a, m_rows, s) : run_decode<DT, 256, 32>(a, m_rows, s);
 }
 template <int DT>
 hipError_t append_by_dims(const LatentAppendArgs& a, int R, int dr, hipStream_t s) {
@@ -455,9 +728,10 @@ hipError_t launch_latent_append(const LatentAppendArgs& a, int R, int dr, int dt
   return dt == 0 ? latent::append_by_dims<0>(a, R, dr, s) : dt == 1 ? latent::append_by_dims<1>(a, R, dr, s)
                                                                     : latent::append_by_dims<2>(a, R, dr, s);
 }
-hipError_t launch_latent_decode(const LatentDecodeArgs& a, int R, int dr, int dt, int nb, hipStream_t s) {
-  return dt == 0 ? latent::decode_by_dims<0>(a, R, dr, nb, s) : dt == 1 ? latent::decode_by_dims<1>(a, R, dr, nb, s)
-                                                                        : latent::decode_by_dims<2>(a, R, dr, nb, s);
+int latent_decode_tile(int m_rows) { return m_rows; }
+hipError_t launch_latent_decode(const LatentDecodeArgs& a, int R, int dr, int dt, int m_rows, hipStream_t s) {
+  return dt == 0 ? latent::decode_by_dims<0>(a, R, dr, m_rows, s) : dt == 1 ? latent::decode_by_dims<1>(a, R, dr, m_rows, s)
+                                                                        : latent::decode_by_dims<2>(a, R, dr, m_rows, s);
 }
 
 }  // namespace kda

@@ -98,7 +98,7 @@ def test_append_refuses(L, kw, code):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(q=None), -1), (dict(cache=None), -1), (dict(table=None), -1), (dict(lens=None), -1), (dict(o=None), -1), (dict(lse=None), -1),
-    (dict(q=OK + 8), -1), (dict(cache=OK + 4), -1), (dict(o=OK + 2), -1), (dict(ws=OK + 8), -1), (dict(ws=None), -3), (dict(bytes=1000), -3),
+    (dict(q=OK + 8), -1), (dict(cache=OK + 4), -1), (dict(o=OK + 2), -1), (dict(ws=OK + 8), -1), (dict(ws=None), -3), (dict(bytes=100), -3),
     (dict(B=-1), -1), (dict(B=70000), -2), (dict(Tq=0), -1), (dict(H=0), -1), (dict(R=128), -2), (dict(dr=128), -2), (dict(page=48), -1),
     (dict(page=0), -1), (dict(pages=1 << 27), -2), (dict(per=-1), -1), (dict(per=1 << 27), -2), (dict(scale=0.0), -1), (dict(dtype=3), -1)])
 def test_decode_refuses(L, kw, code):
