@@ -17,8 +17,11 @@
 // write 1 KiB of consecutive bytes per wave instruction; bank conflicts are
 // kept out by a permutation of the 16-byte chunks inside each row instead
 // (chunk c of row r sits at c ^ swz(r)), applied to the copies' source
-// addresses.  swz is distinct over 8 consecutive rows (row fragments) and
-// differs above its lowest bit over 4 (transposed reads of chunk pairs).
+// addresses.  A 16-byte read takes 16 lanes at a time, lanes 0-3, 12-15, 20-27 of
+// 32 and then the others, an 8-byte one 32: swz gives each such set, of 16
+// or 32 rows a fragment and of transposed reads of 4 rows, different banks
+// (measured: 37 % of the LDS cycles were conflicts with a permutation that was
+// distinct over 8 consecutive rows only).
 #pragma once
 
 #include "kda_common.h"
@@ -94,6 +97,33 @@ __device__ __forceinline__ int fresh(int x) {
   return x;
 }
 
+// Order of a product's instructions, from here up to the last barrier of the
+// scheduler: the reads of AHEAD fragments (RPF LDS reads each) first, then MPF
+// products for each further fragment read, then the rest.
+template <int N, int AHEAD, int RPF, int MPF>
+__device__ __forceinline__ void pace() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * RPF, 0);
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, MPF, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, RPF, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * MPF, 0);
+}
+
+// The same with VPM vector instructions and one exponential beside each product.
+template <int N, int AHEAD, int RPF, int VPM>
+__device__ __forceinline__ void pace_mixed() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * RPF, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (i < N - AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, RPF, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, VPM, 0);
+    __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+  }
+}
+
 // all but the newest N vector memory operations of the wave are done
 template <int N>
 __device__ __forceinline__ void wait_vmem_but() {
@@ -141,27 +171,29 @@ struct Tile {
   // the permutation stays inside aligned groups of SWZ + 1 chunks
   static constexpr int SWZ = CPR % 16 == 0 ? 15 : CPR % 8 == 0 ? 7 : 3;
   static __device__ __forceinline__ int swz(int r) {
-    if constexpr (SWZ == 15) return ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8);
-    else if constexpr (SWZ == 7) return ((r & 3) << 1) | ((r >> 2) & 1);
-    else return (r & 2) | ((r >> 2) & 1);   // 4 chunks: two rows per 128 bytes
+    const int lo = (((r >> 2) ^ (r >> 3)) & 1) << 1 | ((r >> 3) & 1);
+    if constexpr (SWZ == 15) return ((r & 3) << 2) | lo;
+    else if constexpr (SWZ == 7) return ((r & 2) << 1) | lo;   // two rows per 256 bytes
+    else return lo;                                            // four
   }
-  // byte offset of chunk cc + cl of row r: cc the part that unrolling makes a
-  // constant, cl the lane's part in bits that cc has clear, so that the part of
-  // cc above the permutation goes into the instruction's offset field
-  static __device__ __forceinline__ int off(int r, int cc, int cl = 0) {
-    return r * RB + ((cc & ~SWZ) << 4) + ((((cc & SWZ) | cl) ^ swz(r)) << 4);
+  // byte offset of chunk cc + cl of row r0 + r: r0 (a multiple of 16) and cc are
+  // the parts that unrolling makes constants, r and cl the lane's (cl in bits
+  // that cc has clear), so that what the constants add outside the permutation
+  // goes into the instruction's offset field
+  static __device__ __forceinline__ int off(int r, int cc, int cl = 0, int r0 = 0) {
+    return r0 * RB + ((cc & ~SWZ) << 4) + (r * RB + ((((cc & SWZ) | cl) ^ swz(r)) << 4));
   }
   static constexpr int bytes(int rows) { return rows * RB; }
 
-  // row fragment of contraction block ks: row `row`, elements 16 ks + 8 h ..
+  // row fragment of contraction block ks: row r0 + row, elements 16 ks + 8 h ..
   template <class F>
-  static __device__ __forceinline__ F row_frag(const char* base, int row, int ks, int h) {
+  static __device__ __forceinline__ F row_frag(const char* base, int row, int ks, int h, int r0 = 0) {
     if constexpr (ES == 2) {
-      return *reinterpret_cast<const F*>(base + off(row, 2 * ks, h));
+      return *reinterpret_cast<const F*>(base + off(row, 2 * ks, h, r0));
     } else {
       F f;
-      const f4 a = *reinterpret_cast<const f4*>(base + off(row, 4 * ks, 2 * h));
-      const f4 b = *reinterpret_cast<const f4*>(base + off(row, 4 * ks + 1, 2 * h));
+      const f4 a = *reinterpret_cast<const f4*>(base + off(row, 4 * ks, 2 * h, r0));
+      const f4 b = *reinterpret_cast<const f4*>(base + off(row, 4 * ks + 1, 2 * h, r0));
 #pragma unroll
       for (int j = 0; j < 4; ++j) { f[j] = a[j]; f[4 + j] = b[j]; }
       return f;
@@ -172,12 +204,12 @@ struct Tile {
   static __device__ __forceinline__ F col_frag(const char* base, int row0, int col0, int lane) {
     if constexpr (ES == 2) {
       const int g = lane >> 4, i = lane & 15;
-      const int r = row0 + 4 * (g >> 1) + (i >> 2);
+      const int r = 4 * (g >> 1) + (i >> 2);
       const int cc = col0 >> 3, cl = 2 * (g & 1) + ((i & 3) >> 1);
       const int sub = 8 * (i & 1);
       union { s4v s[2]; F f; } u;
-      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + off(r, cc, cl) + sub));
-      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + off(r + 8, cc, cl) + sub));
+      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + off(r, cc, cl, row0) + sub));
+      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + off(r + 8, cc, cl, row0) + sub));
       return u.f;
     } else {
       const int m = lane & 31, h = lane >> 5;
@@ -185,7 +217,7 @@ struct Tile {
       F f;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        f[j] = *reinterpret_cast<const float*>(base + off(row0 + 8 * (j >> 2) + 4 * h + (j & 3), cc, cl) + sub);
+        f[j] = *reinterpret_cast<const float*>(base + off(8 * (j >> 2) + 4 * h + (j & 3), cc, cl, row0) + sub);
       return f;
     }
   }
@@ -196,24 +228,38 @@ struct Tile {
 // already excludes reads no memory outside the tensor).
 template <class TL, int ROWS, int NW>
 struct Copy {
-  static constexpr int PIECES = ROWS * TL::CPR / 64;
+  static constexpr int PIECES = ROWS * TL::CPR / 64, RPP = 64 / TL::CPR > 0 ? 64 / TL::CPR : 1;
   static constexpr int PER = (PIECES + NW - 1) / NW;
-  static_assert(ROWS * TL::CPR % 64 == 0, "whole pieces");
-  unsigned offs[PER];
-  __device__ __forceinline__ void init(int wave, int lane, unsigned row_bytes, int last) {
+  static_assert(ROWS * TL::CPR % 64 == 0 && (PIECES % NW == 0 || PIECES < NW), "whole pieces, a share a wave");
+  // the permutation repeats every 16 rows: where a wave's pieces are that far
+  // apart, one offset a lane serves all of them
+  static constexpr bool ONE = RPP * NW % 16 == 0;
+  static __device__ __forceinline__ unsigned offset(int p, int wave, int lane, unsigned row_bytes, int last) {
+    const int s = (wave + p * NW) * 64 + lane;
+    const int r = s / TL::CPR, c = (s % TL::CPR) ^ TL::swz(r);
+    return static_cast<unsigned>(min(r, last)) * row_bytes + c * 16;
+  }
+  unsigned offs[ONE ? 1 : PER];
+  __device__ __forceinline__ void init(int wave, int lane, unsigned row_bytes) {
+#pragma unroll
+    for (int p = 0; p < (ONE ? 1 : PER); ++p) offs[p] = offset(p, wave, lane, row_bytes, ROWS);
+  }
+  // all rows there; src: the tile's first row (wave-uniform)
+  __device__ __forceinline__ void issue(const char* src, char* dst, int wave, unsigned row_bytes) const {
+    if (PIECES < NW && wave >= PIECES) return;
+    unsigned o = 0;
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
-      const int s = (wave + p * NW) * 64 + lane;
-      const int r = s / TL::CPR, c = (s % TL::CPR) ^ TL::swz(r);
-      offs[p] = static_cast<unsigned>(min(r, last)) * row_bytes + c * 16;
+      if (p == 0 || !ONE) o = static_cast<unsigned>(fresh(static_cast<int>(offs[p])));   // scalar base, 32-bit lane offset
+      copy16((ONE ? src + static_cast<size_t>(p * RPP * NW) * row_bytes : src) + o, dst + (wave + p * NW) * 1024);
     }
   }
-  // src: the tile's first row (wave-uniform)
-  __device__ __forceinline__ void issue(const char* src, char* dst, int wave) const {
+  // the sequence's last rows
+  static __device__ __forceinline__ void issue_last(const char* src, char* dst, int wave, int lane, unsigned row_bytes, int last) {
+    if (PIECES < NW && wave >= PIECES) return;
+    const int ln = fresh(lane);
 #pragma unroll
-    for (int p = 0; p < PER; ++p)
-      if (PIECES % NW == 0 || wave + p * NW < PIECES)
-        copy16(src + offs[p], dst + (wave + p * NW) * 1024);
+    for (int p = 0; p < PER; ++p) copy16(src + offset(p, wave, ln, row_bytes, last), dst + (wave + p * NW) * 1024);
   }
 };
 

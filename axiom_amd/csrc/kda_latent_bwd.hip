@@ -128,7 +128,7 @@ __device__ __forceinline__ bool locate(const LatentArgs& a, int nb, int BM, bool
 // As the forward: scores transposed, one query a lane column.  g^T is the second
 // operand of dq^T += K^T g^T, whose first operand is the key tile read transposed.
 template <int DT, int DN, int DR>
-__global__ __launch_bounds__(256, 1) void kda_latent_dq_kernel(LatentArgs a, int nqb) {
+__global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_kernel(LatentArgs a, int nqb) {
   typedef BwdCfg<DT, DN, DR> C;
   typedef typename El<DT>::frag F;
   typedef typename El<DT>::t E;
@@ -170,23 +170,20 @@ __global__ __launch_bounds__(256, 1) void kda_latent_dq_kernel(LatentArgs a, int
   const unsigned kv_rb = static_cast<unsigned>(a.kv_t * ES), kr_rb = static_cast<unsigned>(a.kr_t * ES);
   Copy<typename C::TN, BN, C::NW> cn;
   Copy<typename C::TR, BN, C::NW> cr;
-  cn.init(wave, lane, kv_rb, BN);
-  cr.init(wave, lane, kr_rb, BN);
+  cn.init(wave, lane, kv_rb);
+  cr.init(wave, lane, kr_rb);
   auto fetch = [&](int j, char* dst) {
     const char* s = kvp + static_cast<int64_t>(j) * BN * kv_rb;
     const char* r = krp + static_cast<int64_t>(j) * BN * kr_rb;
     if (j * BN + BN <= nk) {
-      cn.issue(s, dst, wave);
-      cn.issue(s + DN * ES, dst + C::OFF_V, wave);
-      cr.issue(r, dst + C::OFF_R, wave);
+      cn.issue(s, dst, wave, kv_rb);
+      cn.issue(s + DN * ES, dst + C::OFF_V, wave, kv_rb);
+      cr.issue(r, dst + C::OFF_R, wave, kr_rb);
     } else {
-      Copy<typename C::TN, BN, C::NW> tn;
-      Copy<typename C::TR, BN, C::NW> tr;
-      tn.init(wave, lane, kv_rb, nk - 1 - j * BN);
-      tr.init(wave, lane, kr_rb, nk - 1 - j * BN);
-      tn.issue(s, dst, wave);
-      tn.issue(s + DN * ES, dst + C::OFF_V, wave);
-      tr.issue(r, dst + C::OFF_R, wave);
+      const int last = nk - 1 - j * BN;
+      cn.issue_last(s, dst, wave, lane, kv_rb, last);
+      cn.issue_last(s + DN * ES, dst + C::OFF_V, wave, lane, kv_rb, last);
+      cr.issue_last(r, dst + C::OFF_R, wave, lane, kr_rb, last);
     }
   };
 
@@ -203,41 +200,52 @@ __global__ __launch_bounds__(256, 1) void kda_latent_dq_kernel(LatentArgs a, int
     if (j + 1 < nt) fetch(j + 1, nxt);
     const int kt = j * BN;
     if (kt > wave_hi) return;
+    const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
 #pragma unroll
     for (int t = 0; t < BN / 32; ++t) {
       f16v s, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < KN; ++k) {
-        s = mma(s, C::TN::template row_frag<F>(cur, 32 * t + m, k, h), qn[k]);
-        dp = mma(dp, C::TN::template row_frag<F>(cur + C::OFF_V, 32 * t + m, k, h), dO[k]);
+        s = mma(s, C::TN::template row_frag<F>(cur, fm, k, fh, 32 * t), qn[k]);
+        dp = mma(dp, C::TN::template row_frag<F>(cur + C::OFF_V, fm, k, fh, 32 * t), dO[k]);
       }
 #pragma unroll
-      for (int k = 0; k < KR; ++k) s = mma(s, C::TR::template row_frag<F>(cur + C::OFF_R, 32 * t + m, k, h), qr[k]);
-      const bool edge = kt + 32 * t + 31 > wave_lo;
+      for (int k = 0; k < KR; ++k) s = mma(s, C::TR::template row_frag<F>(cur + C::OFF_R, fm, k, fh, 32 * t), qr[k]);
+      if constexpr (ES == 2) pace<2 * KN + KR, 4, 1, 1>();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = fast_exp2(fmaf(s[i], c, -lse2)) * (dp[i] - D);
+        if constexpr (DT == 2) s[i] *= gf;
+      }
+      if (kt + 32 * t + 31 > wave_lo) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (kt + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) > kmax) s[i] = 0.f;
+      }
+      F gq[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float g[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int i = 8 * u + e;
-          g[e] = fast_exp2(fmaf(s[i], c, -lse2)) * (dp[i] - D);
-          if constexpr (DT == 2) g[e] *= gf;
-        }
-        if (edge) {
+        for (int e = 0; e < 8; ++e) g[e] = s[8 * u + e];
+        gq[u] = to_frag<DT>(g);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (kt + 32 * t + 8 * ((8 * u + e) >> 2) + 4 * h + (e & 3) > kmax) g[e] = 0.f;
-        }
-        const F gq = to_frag<DT>(g);
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int n = 0; n < ND; ++n)
-          acc[n] = mma(acc[n], C::TN::template col_frag<F>(cur, 32 * t + 16 * u, 32 * n, lane), gq);
+          acc[n] = mma(acc[n], C::TN::template col_frag<F>(cur, 32 * t + 16 * u, 32 * n, ln), gq[u]);
 #pragma unroll
         for (int n = 0; n < NR; ++n)
-          acc[ND + n] = mma(acc[ND + n], C::TR::template col_frag<F>(cur + C::OFF_R, 32 * t + 16 * u, 32 * n, lane), gq);
+          acc[ND + n] = mma(acc[ND + n], C::TR::template col_frag<F>(cur + C::OFF_R, 32 * t + 16 * u, 32 * n, ln), gq[u]);
       }
+      if constexpr (ES == 2) pace<2 * (ND + NR), 3, 2, 1>();
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   if (nt > 0) fetch(0, buf0);
@@ -259,43 +267,49 @@ __global__ __launch_bounds__(256, 1) void kda_latent_dq_kernel(LatentArgs a, int
 }
 
 // ---------------------------------------------------------------- key pass
-// Scores untransposed: a lane column is one key, whose key, rotary key and value
-// rows stay in registers; the query tile (nope, rotary, do) is in LDS, read by
-// rows for the two score products and transposed for dk^T and dv^T.
+// Scores untransposed: a lane column is one key; the query tile (nope, rotary,
+// do) is in LDS, read by rows for the two score products and transposed for
+// dk^T and dv^T.
+//
+// 16-bit types: a pair of waves owns 32 keys and splits the work by what it
+// holds.  The first wave holds the keys and dv (112 registers): s, p, dv += p
+// do.  The second holds the values and dk (128): do v^T, and with p from the
+// first, in fp32 through LDS, g and dk += g q.  Each has half of the products,
+// the two share a SIMD, and one wave's exponentials run under the other's
+// products; a wave that holds all of it (240 registers and the scores) is alone
+// on its SIMD and had the matrix cores busy 32 % of the time.
+// fp32: operands twice as large and products 16 times as slow, so one wave does it all.
 template <int DT, int DN, int DR>
-__global__ __launch_bounds__(256, 1) void kda_latent_dkv_kernel(LatentArgs a, int nkb) {
-  typedef BwdCfg<DT, DN, DR> C;
+struct KeyCfg : BwdCfg<DT, DN, DR> {
+  typedef BwdCfg<DT, DN, DR> B;
+  static constexpr bool PAIR = B::ES == 2;
+  static constexpr int NT = PAIR ? 512 : 256, NWV = NT / 64;
+  static constexpr int P_BYTES = PAIR ? 4 * 8192 : 16;    // p of a tile: 64 x 32 fp32 a pair
+};
+
+template <int DT, int DN, int DR>
+__global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kernel(LatentArgs a, int nkb) {
+  typedef KeyCfg<DT, DN, DR> C;
   typedef typename El<DT>::frag F;
   typedef typename El<DT>::t E;
-  constexpr int ES = C::ES, BN = C::BN, KN = DN / 16, KR = DR / 16, ND = DN / 32, NR = DR / 32;
+  constexpr int ES = C::ES, BN = C::BN, KN = DN / 16, KR = DR / 16, ND = DN / 32, NR = DR / 32, NWV = C::NWV, NTL = BN / 32;
   __shared__ __attribute__((aligned(1024))) char buf0[C::BUF_K];
   __shared__ __attribute__((aligned(1024))) char buf1[C::BUF_K];
+  __shared__ __attribute__((aligned(1024))) char pbuf[C::P_BYTES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m = lane & 31, h = lane >> 5;
+  const int m = lane & 31, h = lane >> 5, own = wave & 3, role = wave >> 2;
   Where w;
   if (!locate(a, nkb, C::BM, false, false, w)) return;
   const int nq = w.ke - w.k0;                   // queries of the sequence
-  const int key = w.r0 + wave * 32 + m;         // this lane's key (packed axis)
+  const int key = w.r0 + own * 32 + m;          // this lane's key (packed axis)
   const bool live = key < w.re;
   const int ckey = min(key, w.re - 1);
-  const int first = a.causal ? max(0, key + w.off) : 0;                      // first query that sees this lane's key
-  const int wave_first = a.causal ? max(0, w.r0 + wave * 32 + w.off) : 0;    // ... any of the wave's keys
-  const int wave_full = a.causal ? max(0, min(w.r0 + wave * 32 + 31, w.re - 1) + w.off) : 0;   // ... all of them
+  const int first = a.causal ? max(0, key + w.off) : 0;                     // first query that sees this lane's key
+  const int wave_first = a.causal ? max(0, w.r0 + own * 32 + w.off) : 0;    // ... any of the wave's keys
+  const int wave_full = a.causal ? max(0, min(w.r0 + own * 32 + 31, w.re - 1) + w.off) : 0;   // ... all of them
   const int j0 = (a.causal ? max(0, w.r0 + w.off) : 0) / BN;
   const int nt = (nq + BN - 1) / BN;
-
-  F kn[KN], kr[KR], vv[KN];
-  {
-    const E* p = static_cast<const E*>(a.kv) + w.b * a.kv_b + static_cast<int64_t>(ckey) * a.kv_t + w.head * a.kv_h;
-    const E* r = static_cast<const E*>(a.kr) + w.b * a.kr_b + static_cast<int64_t>(ckey) * a.kr_t;
-#pragma unroll
-    for (int s = 0; s < KN; ++s) {
-      kn[s] = *reinterpret_cast<const F*>(p + 16 * s + 8 * h);
-      vv[s] = *reinterpret_cast<const F*>(p + DN + 16 * s + 8 * h);
-    }
-#pragma unroll
-    for (int s = 0; s < KR; ++s) kr[s] = *reinterpret_cast<const F*>(r + 16 * s + 8 * h);
-  }
+  const float c = a.scale * kLog2e;
   const float gf = DT == 2 ? do_factor(a, w.bh) : 1.f;
 
   const char* qp = static_cast<const char*>(a.q) + (w.b * a.q_b + w.k0 * a.q_t + w.head * a.q_h) * ES;
@@ -303,123 +317,291 @@ __global__ __launch_bounds__(256, 1) void kda_latent_dkv_kernel(LatentArgs a, in
   const float* lsep = a.lse_in + static_cast<int64_t>(w.bh) * a.Tq + w.k0;
   const float* Dp = a.D + static_cast<int64_t>(w.bh) * a.Tq + w.k0;
   const unsigned q_rb = static_cast<unsigned>(a.q_t * ES), d_rb = static_cast<unsigned>(a.H * DN * ES);
-  Copy<typename C::TN, BN, C::NW> cq, cd;
-  Copy<typename C::TR, BN, C::NW> cr;
-  cq.init(wave, lane, q_rb, BN);
-  cd.init(wave, lane, d_rb, BN);
-  cr.init(wave, lane, q_rb, BN);
+  Copy<typename C::TN, BN, NWV> cq, cd;
+  Copy<typename C::TR, BN, NWV> cr;
+  cq.init(wave, lane, q_rb);
+  cd.init(wave, lane, d_rb);
+  cr.init(wave, lane, q_rb);
   auto fetch = [&](int j, char* dst) {
     const char* s = qp + static_cast<int64_t>(j) * BN * q_rb;
     const char* d = dp_ + static_cast<int64_t>(j) * BN * d_rb;
     if (j * BN + BN <= nq) {
-      cq.issue(s, dst, wave);
-      cd.issue(d, dst + C::OFF_V, wave);
-      cr.issue(s + DN * ES, dst + C::OFF_R, wave);
+      cq.issue(s, dst, wave, q_rb);
+      cd.issue(d, dst + C::OFF_V, wave, d_rb);
+      cr.issue(s + DN * ES, dst + C::OFF_R, wave, q_rb);
     } else {
-      Copy<typename C::TN, BN, C::NW> tq, td;
-      Copy<typename C::TR, BN, C::NW> tr;
-      tq.init(wave, lane, q_rb, nq - 1 - j * BN);
-      td.init(wave, lane, d_rb, nq - 1 - j * BN);
-      tr.init(wave, lane, q_rb, nq - 1 - j * BN);
-      tq.issue(s, dst, wave);
-      td.issue(d, dst + C::OFF_V, wave);
-      tr.issue(s + DN * ES, dst + C::OFF_R, wave);
+      const int last = nq - 1 - j * BN;
+      cq.issue_last(s, dst, wave, lane, q_rb, last);
+      cd.issue_last(d, dst + C::OFF_V, wave, lane, d_rb, last);
+      cr.issue_last(s + DN * ES, dst + C::OFF_R, wave, lane, q_rb, last);
     }
     if (wave < 2) {
       const float* x = wave == 0 ? lsep : Dp;
       copy4(x + min(j * BN + lane, nq - 1), dst + C::OFF_L + 256 * wave);
     }
   };
-
-  const float c = a.scale * kLog2e;
-  f16v dk[ND + NR], dv[ND];
-#pragma unroll
-  for (int n = 0; n < ND + NR; ++n)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) dk[n][i] = 0.f;
-#pragma unroll
-  for (int n = 0; n < ND; ++n)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) dv[n][i] = 0.f;
-
-  auto step = [&](int j, const char* cur, char* nxt) {
+  // a tile's turn: its copies are there, the next ones are on their way
+  auto turn = [&](int j, char* nxt) {
     wait_vmem_all();
     lds_barrier();
     if (j + 1 < nt) fetch(j + 1, nxt);
-    const int qt = j * BN;
-    if (qt + BN - 1 < wave_first) return;       // none of these queries sees a key of this wave
+  };
+
+  const E* kp = static_cast<const E*>(a.kv) + w.b * a.kv_b + static_cast<int64_t>(ckey) * a.kv_t + w.head * a.kv_h + 8 * h;
+  const E* rp = static_cast<const E*>(a.kr) + w.b * a.kr_b + static_cast<int64_t>(ckey) * a.kr_t + 8 * h;
+  const int64_t ob = ((static_cast<int64_t>(w.b) * a.Tk + key) * a.H + w.head) * (2 * DN) + 4 * h;
+  const float f = a.scale / gf;
+
+  // p of a score tile, from s; rows q0 .. of the sequence, rows 32 t .. of the tile
+  auto probs = [&](const char* cur, int q0, int t, int fh, bool edge, f16v& s) {
 #pragma unroll
-    for (int t = 0; t < BN / 32; ++t) {
-      f16v s, dp;
+    for (int v = 0; v < 4; ++v) {
+      const f4 ls = *reinterpret_cast<const f4*>(cur + C::OFF_L + (32 * t + 8 * v + 4 * fh) * 4);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+      for (int e = 0; e < 4; ++e) s[4 * v + e] = fast_exp2(fmaf(s[4 * v + e], c, -ls[e] * kLog2e));
+    }
+    if (edge) {
 #pragma unroll
-      for (int k = 0; k < KN; ++k) {
-        s = mma(s, C::TN::template row_frag<F>(cur, 32 * t + m, k, h), kn[k]);
-        dp = mma(dp, C::TN::template row_frag<F>(cur + C::OFF_V, 32 * t + m, k, h), vv[k]);
-      }
-#pragma unroll
-      for (int k = 0; k < KR; ++k) s = mma(s, C::TR::template row_frag<F>(cur + C::OFF_R, 32 * t + m, k, h), kr[k]);
-      const int q0 = qt + 32 * t;
-      const bool edge = q0 < wave_full || q0 + 31 >= nq;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float p[8], g[8];
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const f4 ls = *reinterpret_cast<const f4*>(cur + C::OFF_L + (32 * t + 16 * u + 8 * v + 4 * h) * 4);
-          const f4 dd = *reinterpret_cast<const f4*>(cur + C::OFF_L + 256 + (32 * t + 16 * u + 8 * v + 4 * h) * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 8 * u + 4 * v + e;
-            p[4 * v + e] = fast_exp2(fmaf(s[i], c, -ls[e] * kLog2e));
-            g[4 * v + e] = p[4 * v + e] * (dp[i] - dd[e]);
-            if constexpr (DT == 2) g[4 * v + e] *= gf;
-          }
-        }
-        if (edge) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int qi = q0 + 16 * u + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (qi < first || qi >= nq) p[e] = g[e] = 0.f;
-          }
-        }
-        const F pf = to_frag<DT>(p), gq = to_frag<DT>(g);
-#pragma unroll
-        for (int n = 0; n < ND; ++n) {
-          dv[n] = mma(dv[n], C::TN::template col_frag<F>(cur + C::OFF_V, 32 * t + 16 * u, 32 * n, lane), pf);
-          dk[n] = mma(dk[n], C::TN::template col_frag<F>(cur, 32 * t + 16 * u, 32 * n, lane), gq);
-        }
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
-          dk[ND + n] = mma(dk[ND + n], C::TR::template col_frag<F>(cur + C::OFF_R, 32 * t + 16 * u, 32 * n, lane), gq);
+      for (int i = 0; i < 16; ++i) {
+        const int qi = q0 + 8 * (i >> 2) + 4 * h + (i & 3);
+        if (qi < first || qi >= nq) s[i] = 0.f;
       }
     }
   };
-  if (j0 < nt) fetch(j0, buf0);
-  for (int j = j0; j < nt;) {
-    step(j, buf0, buf1);
-    if (++j >= nt) break;
-    step(j, buf1, buf0);
-    ++j;
-  }
-  if (!live) return;
-  const float f = a.scale / gf;
-  const int64_t ob = ((static_cast<int64_t>(w.b) * a.Tk + key) * a.H + w.head) * (2 * DN) + 4 * h;
+  // g from p and do v^T (0 where p is: a masked pair's do v^T need not be finite)
+  auto adjoint = [&](const char* cur, int t, int fh, bool edge, const f16v& p, f16v& dp) {
 #pragma unroll
-  for (int n = 0; n < ND; ++n)
+    for (int v = 0; v < 4; ++v) {
+      const f4 dd = *reinterpret_cast<const f4*>(cur + C::OFF_L + 256 + (32 * t + 8 * v + 4 * fh) * 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      store4<DT>(a.dkv, ob + 32 * n + 8 * i, dk[n][4 * i] * f, dk[n][4 * i + 1] * f, dk[n][4 * i + 2] * f, dk[n][4 * i + 3] * f);
-      store4<DT>(a.dkv, ob + DN + 32 * n + 8 * i, dv[n][4 * i], dv[n][4 * i + 1], dv[n][4 * i + 2], dv[n][4 * i + 3]);
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * v + e;
+        float g = p[i] * (dp[i] - dd[e]);
+        if constexpr (DT == 2) g *= gf;
+        dp[i] = edge && p[i] == 0.f ? 0.f : g;
+      }
     }
-  const int64_t rb = (static_cast<int64_t>(w.bh) * a.Tk + key) * DR + 4 * h;
+  };
+  auto frags = [&](const f16v& x, F (&out)[2]) {
 #pragma unroll
-  for (int n = 0; n < NR; ++n)
+    for (int u = 0; u < 2; ++u) {
+      float y[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      store4<0>(a.dkr_part, rb + 32 * n + 8 * i, dk[ND + n][4 * i] * f, dk[ND + n][4 * i + 1] * f, dk[ND + n][4 * i + 2] * f,
-                dk[ND + n][4 * i + 3] * f);
+      for (int e = 0; e < 8; ++e) y[e] = x[8 * u + e];
+      out[u] = to_frag<DT>(y);
+    }
+  };
+  auto zero = [](f16v& x) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+  };
+  // dkr_part and dkv of this lane's key
+  auto put_dv = [&](const f16v (&dv)[ND]) {
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store4<DT>(a.dkv, ob + DN + 32 * n + 8 * i, dv[n][4 * i], dv[n][4 * i + 1], dv[n][4 * i + 2], dv[n][4 * i + 3]);
+  };
+  auto put_dk = [&](const f16v (&dk)[ND + NR]) {
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store4<DT>(a.dkv, ob + 32 * n + 8 * i, dk[n][4 * i] * f, dk[n][4 * i + 1] * f, dk[n][4 * i + 2] * f, dk[n][4 * i + 3] * f);
+    const int64_t rb = (static_cast<int64_t>(w.bh) * a.Tk + key) * DR + 4 * h;
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store4<0>(a.dkr_part, rb + 32 * n + 8 * i, dk[ND + n][4 * i] * f, dk[ND + n][4 * i + 1] * f, dk[ND + n][4 * i + 2] * f,
+                  dk[ND + n][4 * i + 3] * f);
+  };
+
+  if (j0 < nt) fetch(j0, buf0);
+  if constexpr (C::PAIR) {
+    char* const mine = pbuf + own * 8192 + lane * 16;
+    if (role == 0) {
+      F kn[KN], kr[KR];
+#pragma unroll
+      for (int s = 0; s < KN; ++s) kn[s] = *reinterpret_cast<const F*>(kp + 16 * s);
+#pragma unroll
+      for (int s = 0; s < KR; ++s) kr[s] = *reinterpret_cast<const F*>(rp + 16 * s);
+      f16v dv[ND];
+#pragma unroll
+      for (int n = 0; n < ND; ++n) zero(dv[n]);
+      auto step = [&](int j, const char* cur, char* nxt) {
+        turn(j, nxt);
+        const int qt = j * BN;
+        const bool busy = qt + BN > wave_first;
+        const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
+        F pf[2][2];
+        if (busy) {
+          f16v s[2];
+          zero(s[0]);
+          zero(s[1]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int k = 0; k < KN; ++k)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) s[t] = mma(s[t], C::TN::template row_frag<F>(cur, fm, k, fh, 32 * t), kn[k]);
+#pragma unroll
+          for (int k = 0; k < KR; ++k)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) s[t] = mma(s[t], C::TR::template row_frag<F>(cur + C::OFF_R, fm, k, fh, 32 * t), kr[k]);
+          pace<2 * (KN + KR), 6, 1, 1>();
+          __builtin_amdgcn_sched_barrier(0);
+          const bool edge = qt < wave_full || qt + BN > nq;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (edge) probs(cur, qt + 32 * t, t, fh, true, s[t]);
+            else probs(cur, qt + 32 * t, t, fh, false, s[t]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<f4*>(mine + (4 * t + i) * 1024) = f4{s[t][4 * i], s[t][4 * i + 1], s[t][4 * i + 2], s[t][4 * i + 3]};
+            frags(s[t], pf[t]);
+          }
+        }
+        lds_barrier();
+        if (busy) {
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+              dv[n] = mma(dv[n], C::TN::template col_frag<F>(cur + C::OFF_V, 16 * u, 32 * n, ln), pf[u >> 1][u & 1]);
+          pace<4 * ND, 4, 2, 1>();
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      for (int j = j0; j < nt;) {
+        step(j, buf0, buf1);
+        if (++j >= nt) break;
+        step(j, buf1, buf0);
+        ++j;
+      }
+      if (live) put_dv(dv);
+    } else {
+      F vv[KN];
+#pragma unroll
+      for (int s = 0; s < KN; ++s) vv[s] = *reinterpret_cast<const F*>(kp + DN + 16 * s);
+      f16v dk[ND + NR];
+#pragma unroll
+      for (int n = 0; n < ND + NR; ++n) zero(dk[n]);
+      auto step = [&](int j, const char* cur, char* nxt) {
+        turn(j, nxt);
+        const int qt = j * BN;
+        const bool busy = qt + BN > wave_first;
+        const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
+        f16v dp[2];
+        if (busy) {
+          zero(dp[0]);
+          zero(dp[1]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int k = 0; k < KN; ++k)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) dp[t] = mma(dp[t], C::TN::template row_frag<F>(cur + C::OFF_V, fm, k, fh, 32 * t), vv[k]);
+          pace<2 * KN, 6, 1, 1>();
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        lds_barrier();
+        if (busy) {
+          F gq[2][2];
+          const bool edge = qt < wave_full || qt + BN > nq;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            f16v p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const f4 x = *reinterpret_cast<const f4*>(mine + (4 * t + i) * 1024);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) p[4 * i + e] = x[e];
+            }
+            if (edge) adjoint(cur, t, fh, true, p, dp[t]);
+            else adjoint(cur, t, fh, false, p, dp[t]);
+            frags(dp[t], gq[t]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+              dk[n] = mma(dk[n], C::TN::template col_frag<F>(cur, 16 * u, 32 * n, ln), gq[u >> 1][u & 1]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+              dk[ND + n] = mma(dk[ND + n], C::TR::template col_frag<F>(cur + C::OFF_R, 16 * u, 32 * n, ln), gq[u >> 1][u & 1]);
+          }
+          pace<4 * (ND + NR), 4, 2, 1>();
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      for (int j = j0; j < nt;) {
+        step(j, buf0, buf1);
+        if (++j >= nt) break;
+        step(j, buf1, buf0);
+        ++j;
+      }
+      if (live) put_dk(dk);
+    }
+  } else {
+    F kn[KN], kr[KR], vv[KN];
+#pragma unroll
+    for (int s = 0; s < KN; ++s) {
+      kn[s] = *reinterpret_cast<const F*>(kp + 16 * s);
+      vv[s] = *reinterpret_cast<const F*>(kp + DN + 16 * s);
+    }
+#pragma unroll
+    for (int s = 0; s < KR; ++s) kr[s] = *reinterpret_cast<const F*>(rp + 16 * s);
+    f16v dk[ND + NR], dv[ND];
+#pragma unroll
+    for (int n = 0; n < ND + NR; ++n) zero(dk[n]);
+#pragma unroll
+    for (int n = 0; n < ND; ++n) zero(dv[n]);
+    auto step = [&](int j, const char* cur, char* nxt) {
+      turn(j, nxt);
+      const int qt = j * BN;
+      if (qt + BN <= wave_first) return;        // none of these queries sees a key of this wave
+      const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
+      f16v s, dp;
+      zero(s);
+      zero(dp);
+#pragma unroll
+      for (int k = 0; k < KN; ++k) {
+        s = mma(s, C::TN::template row_frag<F>(cur, fm, k, fh), kn[k]);
+        dp = mma(dp, C::TN::template row_frag<F>(cur + C::OFF_V, fm, k, fh), vv[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < KR; ++k) s = mma(s, C::TR::template row_frag<F>(cur + C::OFF_R, fm, k, fh), kr[k]);
+      const bool edge = qt < wave_full || qt + BN > nq;
+      probs(cur, qt, 0, fh, edge, s);
+      adjoint(cur, 0, fh, edge, s, dp);
+      F pf[2], gq[2];
+      frags(s, pf);
+      frags(dp, gq);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          dv[n] = mma(dv[n], C::TN::template col_frag<F>(cur + C::OFF_V, 16 * u, 32 * n, ln), pf[u]);
+          dk[n] = mma(dk[n], C::TN::template col_frag<F>(cur, 16 * u, 32 * n, ln), gq[u]);
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+          dk[ND + n] = mma(dk[ND + n], C::TR::template col_frag<F>(cur + C::OFF_R, 16 * u, 32 * n, ln), gq[u]);
+      }
+    };
+    for (int j = j0; j < nt;) {
+      step(j, buf0, buf1);
+      if (++j >= nt) break;
+      step(j, buf1, buf0);
+      ++j;
+    }
+    if (live) {
+      put_dv(dv);
+      put_dk(dk);
+    }
+  }
 }
 
 // ------------------------------------- the rotary key's gradient: sum over heads
@@ -446,7 +628,7 @@ hipError_t run_bwd(const LatentArgs& a, hipStream_t s) {
     kda_latent_dq_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(nqb * bh)), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
   }
   if (a.Tk > 0) {
-    kda_latent_dkv_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(nkb * bh)), dim3(256), 0, s>>>(a, static_cast<int>(nkb));
+    kda_latent_dkv_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(nkb * bh)), dim3(KeyCfg<DT, DN, DR>::NT), 0, s>>>(a, static_cast<int>(nkb));
     const int64_t per_b = static_cast<int64_t>(a.Tk) * DR;
     kda_latent_dkr_kernel<DT><<<dim3(static_cast<unsigned>((per_b + 1023) / 1024), a.B), dim3(256), 0, s>>>(a, per_b);
   }

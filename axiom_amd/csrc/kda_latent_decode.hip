@@ -255,19 +255,6 @@ __device__ __forceinline__ int slot_of(const LatentDecodeArgs& a, int page, int 
   return (min(max(page, 0), static_cast<int>(a.n_pages - 1)) << a.page_shift) + (tok & ((1 << a.page_shift) - 1));
 }
 
-// Order of a product's instructions: AHEAD fragment reads of RPF LDS reads each
-// first, then a product for each further fragment read, then the rest.
-template <int N, int AHEAD, int RPF>
-__device__ __forceinline__ void pace() {
-  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * RPF, 0);
-#pragma unroll
-  for (int i = 0; i < N - AHEAD; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, RPF > 2 ? 4 : 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, RPF, 0);
-  }
-  __builtin_amdgcn_sched_group_barrier(0x008, RPF > 2 ? 4 * AHEAD : AHEAD, 0);
-}
-
 template <int DT, int R, int DR>
 __global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decode16_kernel(LatentDecodeArgs a) {
   typedef DecCfg<DT, R, DR> C;
@@ -340,7 +327,7 @@ __global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decod
         if (k & 1) s1 = mma_s(s1, kf, q[k]);
         else s0 = mma_s(s0, kf, q[k]);
       }
-      if constexpr (ES == 2) pace<KS, 8, 1>();
+      if constexpr (ES == 2) pace<KS, 8, 1, 1>();
       const int key0 = j * KT + 4 * gq;
       f4 s = s0 + s1;
 #pragma unroll
@@ -363,7 +350,7 @@ __global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decod
       const auto p = to_p4<DT>(e);
 #pragma unroll
       for (int v = 0; v < NV; ++v) acc[v] = mma_p(acc[v], v_frag<DT, typename C::TN>(mine, 16 * v, ln), p);
-      if constexpr (ES == 2) pace<NV, 8, 1>();
+      if constexpr (ES == 2) pace<NV, 8, 1, 1>();
       if (j + NW < tb) {
         lds_reads_done();                    // the buffer is read out
         fetch(slot_of(a, page, token(j + NW)));
@@ -521,13 +508,13 @@ __global__ __launch_bounds__(256, 1) void kda_latent_decode64_kernel(LatentDecod
       for (int i = 0; i < 16; ++i) s[i] = s1[i] = 0.f;
 #pragma unroll
       for (int k = 0; k < KN; k += 2) {
-        s = mma(s, TN::template row_frag<F>(cur, 32 * kh + fm, k, fh), q[k]);
-        s1 = mma(s1, TN::template row_frag<F>(cur, 32 * kh + fm, k + 1, fh), q[k + 1]);
+        s = mma(s, TN::template row_frag<F>(cur, fm, k, fh, 32 * kh), q[k]);
+        s1 = mma(s1, TN::template row_frag<F>(cur, fm, k + 1, fh, 32 * kh), q[k + 1]);
       }
 #pragma unroll
       for (int k = 0; k < KR; k += 2) {
-        s = mma(s, TR::template row_frag<F>(cur + OFF_R, 32 * kh + fm, k, fh), q[KN + k]);
-        s1 = mma(s1, TR::template row_frag<F>(cur + OFF_R, 32 * kh + fm, k + 1, fh), q[KN + k + 1]);
+        s = mma(s, TR::template row_frag<F>(cur + OFF_R, fm, k, fh, 32 * kh), q[KN + k]);
+        s1 = mma(s1, TR::template row_frag<F>(cur + OFF_R, fm, k + 1, fh, 32 * kh), q[KN + k + 1]);
       }
       const int key0 = j * KT + 32 * kh + 4 * h;
       float tm = -INFINITY;
@@ -550,7 +537,7 @@ __global__ __launch_bounds__(256, 1) void kda_latent_decode64_kernel(LatentDecod
             p[e] = fast_exp2(fmaf(s[8 * u + e], c, -mc));
             lt += p[e];
           }
-          *reinterpret_cast<F*>(sp + TP::off(32 * rh + fm, 4 * kh + 2 * u, fh)) = to_frag<DT>(p);
+          *reinterpret_cast<F*>(sp + TP::off(fm, 4 * kh + 2 * u, fh, 32 * rh)) = to_frag<DT>(p);
         }
       };
       probs();
@@ -579,7 +566,7 @@ __global__ __launch_bounds__(256, 1) void kda_latent_decode64_kernel(LatentDecod
       l += lt;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const F p0 = TP::template row_frag<F>(sp, fm, k, fh), p1 = TP::template row_frag<F>(sp, 32 + fm, k, fh);
+        const F p0 = TP::template row_frag<F>(sp, fm, k, fh), p1 = TP::template row_frag<F>(sp, fm, k, fh, 32);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           const F vf = TN::template col_frag<F>(cur, 16 * k, wave * (R / 4) + 32 * v, ln);

@@ -96,23 +96,20 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
   const unsigned kv_rb = static_cast<unsigned>(a.kv_t * ES), kr_rb = static_cast<unsigned>(a.kr_t * ES);
   Copy<typename C::TN, BN, C::NW> cn;
   Copy<typename C::TR, BN, C::NW> cr;
-  cn.init(wave, lane, kv_rb, BN);
-  cr.init(wave, lane, kr_rb, BN);
+  cn.init(wave, lane, kv_rb);
+  cr.init(wave, lane, kr_rb);
   auto fetch = [&](int j, char* dst) {
     const char* s = kvp + static_cast<int64_t>(j) * BN * kv_rb;
     const char* r = krp + static_cast<int64_t>(j) * BN * kr_rb;
     if (j * BN + BN <= nk) {
-      cn.issue(s, dst, wave);
-      cn.issue(s + DN * ES, dst + C::OFF_V, wave);
-      cr.issue(r, dst + C::OFF_R, wave);
+      cn.issue(s, dst, wave, kv_rb);
+      cn.issue(s + DN * ES, dst + C::OFF_V, wave, kv_rb);
+      cr.issue(r, dst + C::OFF_R, wave, kr_rb);
     } else {
-      Copy<typename C::TN, BN, C::NW> tn;
-      Copy<typename C::TR, BN, C::NW> tr;
-      tn.init(wave, lane, kv_rb, nk - 1 - j * BN);
-      tr.init(wave, lane, kr_rb, nk - 1 - j * BN);
-      tn.issue(s, dst, wave);
-      tn.issue(s + DN * ES, dst + C::OFF_V, wave);
-      tr.issue(r, dst + C::OFF_R, wave);
+      const int last = nk - 1 - j * BN;
+      cn.issue_last(s, dst, wave, lane, kv_rb, last);
+      cn.issue_last(s + DN * ES, dst + C::OFF_V, wave, lane, kv_rb, last);
+      cr.issue_last(r, dst + C::OFF_R, wave, lane, kr_rb, last);
     }
   };
 
@@ -131,16 +128,24 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
     if (j + 1 < nt) fetch(j + 1, nxt);
     const int kt = j * BN;
     if (kt > wave_hi) return;                 // nothing of this tile for this wave's queries
+    const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
     f16v s[NB];
 #pragma unroll
-    for (int t = 0; t < NB; ++t) {
+    for (int t = 0; t < NB; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < KN; ++k) s[t] = mma(s[t], C::TN::template row_frag<F>(cur, 32 * t + m, k, h), qn[k]);
+    for (int k = 0; k < KN; ++k)
 #pragma unroll
-      for (int k = 0; k < KR; ++k) s[t] = mma(s[t], C::TR::template row_frag<F>(cur + C::OFF_R, 32 * t + m, k, h), qr[k]);
-    }
+      for (int t = 0; t < NB; ++t) s[t] = mma(s[t], C::TN::template row_frag<F>(cur, fm, k, fh, 32 * t), qn[k]);
+#pragma unroll
+    for (int k = 0; k < KR; ++k)
+#pragma unroll
+      for (int t = 0; t < NB; ++t)
+        s[t] = mma(s[t], C::TR::template row_frag<F>(cur + C::OFF_R, fm, k, fh, 32 * t), qr[k]);
+    if constexpr (ES == 2) pace<NB * (KN + KR), 6, 1, 1>();
+    __builtin_amdgcn_sched_barrier(0);
     if (kt + BN - 1 > wave_lo) {
 #pragma unroll
       for (int t = 0; t < NB; ++t)
@@ -167,21 +172,25 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[n][i] *= al;
     }
+    F pf[2 * NB];
 #pragma unroll
-    for (int t = 0; t < NB; ++t)
+    for (int u = 0; u < 2 * NB; ++u) {
+      float p[8];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = fast_exp2(fmaf(s[t][8 * u + e], c, -mc));
-          l += p[e];
-        }
-        const F pf = to_frag<DT>(p);
-#pragma unroll
-        for (int n = 0; n < ND; ++n)
-          acc[n] = mma(acc[n], C::TN::template col_frag<F>(cur + C::OFF_V, 32 * t + 16 * u, 32 * n, lane), pf);
+      for (int e = 0; e < 8; ++e) {
+        p[e] = fast_exp2(fmaf(s[u >> 1][8 * (u & 1) + e], c, -mc));
+        l += p[e];
       }
+      pf[u] = to_frag<DT>(p);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 2 * NB; ++u)
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+        acc[n] = mma(acc[n], C::TN::template col_frag<F>(cur + C::OFF_V, 16 * u, 32 * n, ln), pf[u]);
+    if constexpr (ES == 2) pace<2 * NB * ND, 4, 2, 1>();
+    __builtin_amdgcn_sched_barrier(0);
   };
   if (nt > 0) fetch(0, buf0);
   for (int j = 0; j < nt;) {
