@@ -79,9 +79,10 @@ _SIGNATURES = {
 
 # The C ABI of include/latent_mi355x.h
 _LATENT = {
-    "kda_latent_attn_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp] + [_i] * 7 + [_f, _i]),
+    "kda_latent_attn_fwd": (_i, [_vp] * 7 + [_i32, _vp, _vp] + [_i] * 7 + [_f, _i, _vp, _sz]),
+    "kda_latent_attn_fwd_workspace": (_sz, [_i] * 6 + [_i32, _i]),
     "kda_latent_attn_bwd": (_i, [_vp] * 7 + [_i32] + [_vp] * 6 + [_i] * 7 + [_f, _i, _vp, _sz]),
-    "kda_latent_attn_bwd_workspace": (_sz, [_i] * 5),
+    "kda_latent_attn_bwd_workspace": (_sz, [_i] * 6 + [_i32, _i]),
     "kda_latent_append": (_i, [_vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _f, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
                                _i, _i, _i, _i, _i, _i]),
     "kda_latent_decode": (_i, [_vp] * 7 + [_i] * 5 + [_i64, _i, _i, _f, _i, _vp, _sz]),

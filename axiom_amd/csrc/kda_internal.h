@@ -308,6 +308,12 @@ struct LatentArgs {
   float scale;
   void* o;
   float* lse;
+  // Few blocks: up to `splits` workgroups a block, each with a share of the
+  // other axis, leave fp32 parts that a join adds (forward: also the maxima
+  // and sums); part index z, then [B*H][rows][width].
+  int splits;
+  float* part;
+  float* part_ml;
   // backward
   const void* o_in;
   const void* dout;
@@ -315,7 +321,8 @@ struct LatentArgs {
   float* D;                // sum over dn of do * o
   float* dmax;             // fp16: largest |do| of each 128-row block, [B*H][ceil(Tq / 128)]
   int dmax_n;              // its blocks
-  float* dkr_part;         // [B,H,Tk,dr]: each head's share of the rotary key's gradient
+  float* dkr_part;         // [splits][B,H,Tk,dr]: each head's share of the rotary key's gradient
+  int splits_k;            // the key pass' splits (`splits` is the query pass')
   void* dq;
   void* dkv;
   void* dkr;

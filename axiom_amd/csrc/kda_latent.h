@@ -25,6 +25,7 @@
 #pragma once
 
 #include "kda_common.h"
+#include "kda_internal.h"
 
 namespace kda {
 namespace latent {
@@ -263,6 +264,18 @@ struct Copy {
   }
 };
 
+// A block's share z of its n tiles along the other axis: [j0, j1) of `parts`
+// shares of at least two tiles each.
+struct Share {
+  int j0, j1, parts;
+  __device__ __forceinline__ Share(int n, int splits, int z) {
+    const int c = splits > 1 ? max(2, (n + splits - 1) / splits) : max(n, 1);
+    parts = max(1, (n + c - 1) / c);
+    j0 = z * c;
+    j1 = min(n, j0 + c);
+  }
+};
+
 // The sequence and block of a workgroup.  Dense: block `id` of one batch
 // element.  Packed (cu non-null): blocks are numbered sequence by sequence,
 // ceil(len / BLK) of each; found by the wave, 64 sequences at a time.  Offsets
@@ -298,6 +311,48 @@ __device__ __forceinline__ bool find_span(const int32_t* cu, int n_seqs, int T, 
     base += __builtin_amdgcn_readfirstlane(__shfl(inc, 63, 64));
   }
   return false;
+}
+
+struct Where { int b, head, bh, r0, re, k0, ke, off; };   // rows owned from r0 to re, the other side k0 to ke
+// q_side: the workgroup owns queries, else keys.  off: owned query row i sees the
+// keys of the sequence with index <= i + off; owned key row j is seen by the
+// queries of the sequence with index >= j + off.
+// Heads are spread over the eight XCDs (consecutive workgroups go round them), so
+// that one XCD's L2 serves a head's rows; reverse: the last block of a head
+// first (the one with the longest causal walk).
+__device__ __forceinline__ bool locate(const LatentArgs& a, int nb, int BM, bool q_side, bool reverse, Where& w) {
+  const int id = blockIdx.x, bh_n = a.B * a.H;
+  int blk;
+  if (bh_n % 8 == 0) {
+    const int slot = id >> 3;
+    w.bh = (id & 7) + 8 * (slot / nb);
+    blk = slot % nb;
+  } else {
+    w.bh = id % bh_n;
+    blk = id / bh_n;
+  }
+  if (reverse) blk = nb - 1 - blk;
+  w.b = w.bh / a.H;
+  w.head = w.bh - w.b * a.H;
+  if (a.cu_q) {
+    Span s;
+    if (!find_span(q_side ? a.cu_q : a.cu_k, a.n_seqs, q_side ? a.Tq : a.Tk, BM, blk, s)) return false;
+    const int32_t* o = q_side ? a.cu_k : a.cu_q;
+    const int T = q_side ? a.Tk : a.Tq;
+    w.r0 = s.a + s.blk * BM;
+    w.re = s.e;
+    w.k0 = min(max(o[s.seq], 0), T);
+    w.ke = min(max(o[s.seq + 1], w.k0), T);
+    const int nr = s.e - s.a, no = w.ke - w.k0;
+    w.off = no - nr - s.a;   // keys - queries, or queries - keys
+  } else {
+    w.r0 = blk * BM;
+    w.re = q_side ? a.Tq : a.Tk;
+    w.k0 = 0;
+    w.ke = q_side ? a.Tk : a.Tq;
+    w.off = q_side ? a.Tk - a.Tq : a.Tq - a.Tk;
+  }
+  return true;
 }
 
 }  // namespace latent

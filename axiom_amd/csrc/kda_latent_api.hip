@@ -58,6 +58,10 @@ int check_attn(const void* q, const void* kv, const void* kr, const int64_t* st,
   return KDA_OK;
 }
 
+bool sizes_ok(int B, int Tq, int Tk, int H, int dn, int dr, int n_seqs, int dtype) {
+  return B >= 0 && Tq >= 0 && Tk >= 0 && H >= 1 && (dn == 64 || dn == 128) && (dr == 32 || dr == 64) && n_seqs >= 0 && dtype_ok(dtype);
+}
+
 kda::LatentArgs attn_args(const void* q, const void* kv, const void* kr, const int64_t* st, const int32_t* cu_q,
                           const int32_t* cu_k, int32_t n_seqs, int B, int Tq, int Tk, int H, int causal, float scale) {
   kda::LatentArgs a{};
@@ -72,22 +76,50 @@ kda::LatentArgs attn_args(const void* q, const void* kv, const void* kr, const i
   return a;
 }
 
-struct BwdLayout { size_t D, dmax, part, total; };
-BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dr) {
+// Workgroups of a block of 128 rows along the other axis.  A launch of fewer
+// blocks than the chip runs at once leaves CUs idle while each block walks its
+// whole row of tiles, so the walk is shared out, up to 16 ways, until there are
+// `slots` workgroups; a join adds their fp32 parts.
+int splits_of(int64_t T, int64_t T_other, int B, int H, int n_seqs, int slots) {
+  const int64_t blocks = (n_seqs > 0 ? T / 128 + n_seqs : (T + 127) / 128) * B * H;
+  if (blocks <= 0) return 1;
+  const int64_t s = slots / blocks, most = (T_other + 127) / 128;   // shares of at least 128 rows
+  return static_cast<int>(s < 1 || most <= 1 ? 1 : (s < most ? (s < 16 ? s : 16) : (most < 16 ? most : 16)));
+}
+// Workgroups at once on 256 CUs: two a CU where registers and LDS allow.
+constexpr int kSlots16 = 512, kSlots32 = 256, kSlotsKeys = 256;
+int q_slots(int dtype) { return dtype == KDA_DTYPE_F32 ? kSlots32 : kSlots16; }
+
+struct FwdLayout { int splits; size_t ml, total; };
+FwdLayout fwd_layout(int B, int Tq, int Tk, int H, int dn, int n_seqs, int dtype) {
+  FwdLayout L{};
+  L.splits = splits_of(Tq, Tk, B, H, n_seqs, q_slots(dtype));
+  const size_t rows = L.splits > 1 ? static_cast<size_t>(L.splits) * B * H * Tq : 0;
+  L.ml = align_up(rows * dn * 4);
+  L.total = L.ml + align_up(rows * 8);
+  return L;
+}
+struct BwdLayout { int splits, splits_k; size_t D, dmax, dkr, part, total; };
+BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dn, int dr, int n_seqs, int dtype) {
   BwdLayout L{};
   const size_t bh = static_cast<size_t>(B) * H;
+  L.splits = splits_of(Tq, Tk, B, H, n_seqs, q_slots(dtype));
+  L.splits_k = splits_of(Tk, Tq, B, H, n_seqs, kSlotsKeys);
   L.D = 0;
   L.dmax = align_up(bh * Tq * 4);
-  L.part = L.dmax + align_up(bh * ((Tq + 127) / 128) * 4);
-  L.total = L.part + align_up(bh * Tk * dr * 4) + 256;
+  L.dkr = L.dmax + align_up(bh * ((Tq + 127) / 128) * 4);
+  L.part = L.dkr + align_up(L.splits_k * bh * Tk * dr * 4);
+  const size_t pq = L.splits > 1 ? L.splits * bh * Tq * (dn + dr) * 4 : 0;        // used in turn
+  const size_t pk = L.splits_k > 1 ? L.splits_k * bh * Tk * 2 * dn * 4 : 0;
+  L.total = L.part + align_up(pq > pk ? pq : pk) + 256;
   return L;
 }
 
 // Decode: query rows of a workgroup (16, or 64 where there are more than 16;
 // fp32 16, whose operands take twice the registers and LDS), the row groups
 // of a sequence, and the workgroups along the cache: one a CU (its buffers take
-// the LDS), and no more than there can be runs of `least` tiles (a tile for each
-// of the eight waves, or one of 64 keys).  Sequences whose table holds at most
+// the LDS), and no more than there can be runs of `least` tiles (a tile
+// of each wave, or two of 32 keys).  Sequences whose table holds at most
 // kWholeTokens tokens get a workgroup each instead and no join launch.
 constexpr int kCUs = 256;
 constexpr int kWholeTokens = 256;
@@ -95,7 +127,7 @@ struct DecodePlan { int rows, groups, wgs, whole, least; size_t part_ml, part_o,
 bool decode_plan(int B, int Tq, int H, int R, int page_size, int max_pages, int dtype, DecodePlan* P) {
   const int64_t rows = static_cast<int64_t>(Tq) * H, cap = static_cast<int64_t>(page_size) * max_pages;
   P->rows = rows <= 16 || dtype == KDA_DTYPE_F32 ? 16 : 64;
-  P->least = P->rows == 64 ? 1 : dtype == KDA_DTYPE_F32 ? 4 : 8;
+  P->least = P->rows == 64 ? 2 : dtype == KDA_DTYPE_F32 ? 4 : 8;
   const int64_t kt = kda::latent_decode_tile(P->rows), tiles = ((cap + kt - 1) / kt + 2 * P->least) * B;
   if (rows > (1 << 20) || cap >= (int64_t{1} << 31) || tiles >= (int64_t{1} << 30)) return false;
   P->groups = static_cast<int>((rows + P->rows - 1) / P->rows);
@@ -116,20 +148,32 @@ extern "C" {
 
 int kda_latent_attn_fwd(hipStream_t stream, const void* q, const void* kv, const void* k_rope, const int64_t* strides,
                         const int32_t* cu_q, const int32_t* cu_k, int32_t n_seqs, void* o, float* lse, int B, int Tq, int Tk,
-                        int H, int dn, int dr, int causal, float scale, int dtype) {
+                        int H, int dn, int dr, int causal, float scale, int dtype, void* workspace, size_t workspace_bytes) {
   if (const int rc = check_attn(q, kv, k_rope, strides, cu_q, cu_k, n_seqs, B, Tq, Tk, H, dn, dr, scale, dtype)) return rc;
   if (static_cast<int64_t>(B) * Tq == 0) return KDA_OK;
   if (!o || !lse) return fail(KDA_ERR_INVALID_ARGUMENT, "null o or lse");
   if (!aligned(o, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "o must be aligned to 16 bytes");
+  const FwdLayout L = fwd_layout(B, Tq, Tk, H, dn, cu_q ? n_seqs : 0, dtype);
+  if (L.total > 0 && (!workspace || workspace_bytes < L.total))
+    return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0}, L.total);
+  if (!aligned(workspace, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "workspace must be aligned to 16 bytes");
   kda::LatentArgs a = attn_args(q, kv, k_rope, strides, cu_q, cu_k, n_seqs, B, Tq, Tk, H, causal, scale);
   a.o = o;
   a.lse = lse;
+  a.splits = L.splits;
+  a.part = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + L.ml);
   return launched(kda::launch_latent_fwd(a, dn, dr, dtype, stream), "kda_latent_attn_fwd");
 }
 
-size_t kda_latent_attn_bwd_workspace(int B, int Tq, int Tk, int H, int dr) {
-  if (B < 0 || Tq < 0 || Tk < 0 || H < 1 || (dr != 32 && dr != 64)) return 0;
-  return bwd_layout(B, Tq, Tk, H, dr).total;
+size_t kda_latent_attn_fwd_workspace(int B, int Tq, int Tk, int H, int dn, int dr, int32_t n_seqs, int dtype) {
+  if (!sizes_ok(B, Tq, Tk, H, dn, dr, n_seqs, dtype)) return 0;
+  return fwd_layout(B, Tq, Tk, H, dn, n_seqs, dtype).total;
+}
+
+size_t kda_latent_attn_bwd_workspace(int B, int Tq, int Tk, int H, int dn, int dr, int32_t n_seqs, int dtype) {
+  if (!sizes_ok(B, Tq, Tk, H, dn, dr, n_seqs, dtype)) return 0;
+  return bwd_layout(B, Tq, Tk, H, dn, dr, n_seqs, dtype).total;
 }
 
 int kda_latent_attn_bwd(hipStream_t stream, const void* q, const void* kv, const void* k_rope, const int64_t* strides,
@@ -143,7 +187,7 @@ int kda_latent_attn_bwd(hipStream_t stream, const void* q, const void* kv, const
   for (const void* p : {o, d_o, static_cast<const void*>(dq), static_cast<const void*>(dkv), static_cast<const void*>(dk_rope)})
     if (!aligned(p, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "o, d_o, dq, dkv and dk_rope must be aligned to 16 bytes");
   if (static_cast<int64_t>(H) * dn * elem(dtype) >= kMaxRowBytes) return fail(KDA_ERR_UNSUPPORTED, "H * dn too large");
-  const BwdLayout L = bwd_layout(B, Tq, Tk, H, dr);
+  const BwdLayout L = bwd_layout(B, Tq, Tk, H, dn, dr, cu_q ? n_seqs : 0, dtype);
   if (!workspace || workspace_bytes < L.total)
     return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0}, L.total);
   if (!aligned(workspace, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "workspace must be aligned to 16 bytes");
@@ -153,7 +197,10 @@ int kda_latent_attn_bwd(hipStream_t stream, const void* q, const void* kv, const
   a.D = reinterpret_cast<float*>(ws + L.D);
   a.dmax = reinterpret_cast<float*>(ws + L.dmax);
   a.dmax_n = (Tq + 127) / 128;
-  a.dkr_part = reinterpret_cast<float*>(ws + L.part);
+  a.dkr_part = reinterpret_cast<float*>(ws + L.dkr);
+  a.part = reinterpret_cast<float*>(ws + L.part);
+  a.splits = L.splits;
+  a.splits_k = L.splits_k;
   a.dq = dq; a.dkv = dkv; a.dkr = dk_rope;
   return launched(kda::launch_latent_bwd(a, dn, dr, dtype, stream), "kda_latent_attn_bwd");
 }

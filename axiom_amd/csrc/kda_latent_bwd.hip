@@ -85,45 +85,6 @@ struct BwdCfg {
   static constexpr int BUF_Q = OFF_L, BUF_K = OFF_L + 512;
 };
 
-struct Where { int b, head, bh, r0, re, k0, ke, off; };   // rows owned from r0 to re, the other side k0 to ke
-// q_side: the workgroup owns queries, else keys.  off: owned query row i sees the
-// keys of the sequence with index <= i + off; owned key row j is seen by the
-// queries of the sequence with index >= j + off.
-__device__ __forceinline__ bool locate(const LatentArgs& a, int nb, int BM, bool q_side, bool reverse, Where& w) {
-  const int id = blockIdx.x, bh_n = a.B * a.H;
-  int blk;
-  if (bh_n % 8 == 0) {
-    const int slot = id >> 3;
-    w.bh = (id & 7) + 8 * (slot / nb);
-    blk = slot % nb;
-  } else {
-    w.bh = id % bh_n;
-    blk = id / bh_n;
-  }
-  if (reverse) blk = nb - 1 - blk;
-  w.b = w.bh / a.H;
-  w.head = w.bh - w.b * a.H;
-  if (a.cu_q) {
-    Span s;
-    if (!find_span(q_side ? a.cu_q : a.cu_k, a.n_seqs, q_side ? a.Tq : a.Tk, BM, blk, s)) return false;
-    const int32_t* o = q_side ? a.cu_k : a.cu_q;
-    const int T = q_side ? a.Tk : a.Tq;
-    w.r0 = s.a + s.blk * BM;
-    w.re = s.e;
-    w.k0 = min(max(o[s.seq], 0), T);
-    w.ke = min(max(o[s.seq + 1], w.k0), T);
-    const int nr = s.e - s.a, no = w.ke - w.k0;
-    w.off = no - nr - s.a;   // keys - queries, or queries - keys
-  } else {
-    w.r0 = blk * BM;
-    w.re = q_side ? a.Tq : a.Tk;
-    w.k0 = 0;
-    w.ke = q_side ? a.Tk : a.Tq;
-    w.off = q_side ? a.Tk - a.Tq : a.Tq - a.Tk;
-  }
-  return true;
-}
-
 // -------------------------------------------------------------- query pass
 // As the forward: scores transposed, one query a lane column.  g^T is the second
 // operand of dq^T += K^T g^T, whose first operand is the key tile read transposed.
@@ -147,7 +108,9 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   const int wave_lo = a.causal ? min(nk - 1, w.r0 + wave * 32 + w.off) : nk - 1;
   const int wave_hi = a.causal ? min(nk - 1, min(w.r0 + wave * 32 + 31, w.re - 1) + w.off) : nk - 1;
   const int blk_hi = a.causal ? min(nk - 1, min(w.r0 + C::BM - 1, w.re - 1) + w.off) : nk - 1;
-  const int nt = (blk_hi + BN) / BN;
+  const Share part(max(0, (blk_hi + BN) / BN), a.splits, blockIdx.y);
+  const int nt = part.j1;
+  if (static_cast<int>(blockIdx.y) >= part.parts) return;
 
   F qn[KN], qr[KR], dO[KN];
   {
@@ -248,8 +211,8 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  if (nt > 0) fetch(0, buf0);
-  for (int j = 0; j < nt;) {
+  if (part.j0 < nt) fetch(part.j0, buf0);
+  for (int j = part.j0; j < nt;) {
     step(j, buf0, buf1);
     if (++j >= nt) break;
     step(j, buf1, buf0);
@@ -257,6 +220,16 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   }
   if (!live) return;
   const float f = a.scale / gf;
+  if (part.parts > 1) {
+    const int64_t pb = ((static_cast<int64_t>(blockIdx.y) * a.B * a.H + w.bh) * a.Tq + row) * (DN + DR) + 4 * h;
+#pragma unroll
+    for (int n = 0; n < ND + NR; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store4<0>(a.part, pb + 32 * n + 8 * i, acc[n][4 * i] * f, acc[n][4 * i + 1] * f, acc[n][4 * i + 2] * f,
+                  acc[n][4 * i + 3] * f);
+    return;
+  }
   const int64_t ob = ((static_cast<int64_t>(w.b) * a.Tq + row) * a.H + w.head) * (DN + DR) + 4 * h;
 #pragma unroll
   for (int n = 0; n < ND + NR; ++n)
@@ -307,8 +280,10 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   const int first = a.causal ? max(0, key + w.off) : 0;                     // first query that sees this lane's key
   const int wave_first = a.causal ? max(0, w.r0 + own * 32 + w.off) : 0;    // ... any of the wave's keys
   const int wave_full = a.causal ? max(0, min(w.r0 + own * 32 + 31, w.re - 1) + w.off) : 0;   // ... all of them
-  const int j0 = (a.causal ? max(0, w.r0 + w.off) : 0) / BN;
-  const int nt = (nq + BN - 1) / BN;
+  const int jf = (a.causal ? max(0, w.r0 + w.off) : 0) / BN;                // the block's first query tile
+  const Share part(max(0, (nq + BN - 1) / BN - jf), a.splits_k, blockIdx.y);
+  if (static_cast<int>(blockIdx.y) >= part.parts) return;
+  const int j0 = jf + part.j0, nt = jf + part.j1;
   const float c = a.scale * kLog2e;
   const float gf = DT == 2 ? do_factor(a, w.bh) : 1.f;
 
@@ -395,27 +370,31 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = 0.f;
   };
-  // dkr_part and dkv of this lane's key
+  // dv, dk and the rotary part of this lane's key, or this share's parts of them
+  const bool parted = part.parts > 1;
+  const int64_t prow = (static_cast<int64_t>(blockIdx.y) * a.B * a.H + w.bh) * a.Tk + key;
+  auto put4 = [&](int col, float x, float y, float z, float u) {
+    if (parted) store4<0>(a.part, prow * (2 * DN) + 4 * h + col, x, y, z, u);
+    else store4<DT>(a.dkv, ob + col, x, y, z, u);
+  };
   auto put_dv = [&](const f16v (&dv)[ND]) {
 #pragma unroll
     for (int n = 0; n < ND; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        store4<DT>(a.dkv, ob + DN + 32 * n + 8 * i, dv[n][4 * i], dv[n][4 * i + 1], dv[n][4 * i + 2], dv[n][4 * i + 3]);
+      for (int i = 0; i < 4; ++i) put4(DN + 32 * n + 8 * i, dv[n][4 * i], dv[n][4 * i + 1], dv[n][4 * i + 2], dv[n][4 * i + 3]);
   };
   auto put_dk = [&](const f16v (&dk)[ND + NR]) {
 #pragma unroll
     for (int n = 0; n < ND; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        store4<DT>(a.dkv, ob + 32 * n + 8 * i, dk[n][4 * i] * f, dk[n][4 * i + 1] * f, dk[n][4 * i + 2] * f, dk[n][4 * i + 3] * f);
-    const int64_t rb = (static_cast<int64_t>(w.bh) * a.Tk + key) * DR + 4 * h;
+        put4(32 * n + 8 * i, dk[n][4 * i] * f, dk[n][4 * i + 1] * f, dk[n][4 * i + 2] * f, dk[n][4 * i + 3] * f);
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        store4<0>(a.dkr_part, rb + 32 * n + 8 * i, dk[ND + n][4 * i] * f, dk[ND + n][4 * i + 1] * f, dk[ND + n][4 * i + 2] * f,
-                  dk[ND + n][4 * i + 3] * f);
+        store4<0>(a.dkr_part, prow * DR + 4 * h + 32 * n + 8 * i, dk[ND + n][4 * i] * f, dk[ND + n][4 * i + 1] * f,
+                  dk[ND + n][4 * i + 2] * f, dk[ND + n][4 * i + 3] * f);
   };
 
   if (j0 < nt) fetch(j0, buf0);
@@ -616,6 +595,43 @@ __global__ __launch_bounds__(256) void kda_latent_dkr_kernel(LatentArgs a, int64
   store4<DT>(a.dkr, blockIdx.y * per_b + i, s[0], s[1], s[2], s[3]);
 }
 
+// Adds the parts of split blocks in part order; a quarter of a block a
+// workgroup.  Q: dq's blocks, else dkv's and (in place, in part 0) the rotary key's.
+template <int DT, int DN, int DR, bool Q>
+__global__ __launch_bounds__(256) void kda_latent_bwd_join_kernel(LatentArgs a, int nb) {
+  typedef BwdCfg<DT, DN, DR> C;
+  constexpr int WID = Q ? DN + DR : 2 * DN;
+  Where w;
+  if (!locate(a, nb, C::BM, Q, Q, w)) return;
+  const int n_o = w.ke - w.k0;
+  int tiles;
+  if (Q) {
+    const int hi = a.causal ? min(n_o - 1, min(w.r0 + C::BM - 1, w.re - 1) + w.off) : n_o - 1;
+    tiles = max(0, (hi + C::BN) / C::BN);
+  } else {
+    tiles = max(0, (n_o + C::BN - 1) / C::BN - (a.causal ? max(0, w.r0 + w.off) : 0) / C::BN);
+  }
+  const int parts = Share(tiles, Q ? a.splits : a.splits_k, 0).parts;
+  if (parts == 1) return;
+  const int T = Q ? a.Tq : a.Tk, ra = w.r0 + blockIdx.y * 32, n = min(32, w.re - ra);
+  const int64_t step = static_cast<int64_t>(a.B) * a.H * T, row0 = static_cast<int64_t>(w.bh) * T + ra;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < n * (WID / 4); i += 256) {
+    const int r = i / (WID / 4), col = i % (WID / 4) * 4;
+    f4 s = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int z = 0; z < parts; ++z) s += *reinterpret_cast<const f4*>(a.part + (z * step + row0 + r) * WID + col);
+    store4<DT>(Q ? a.dq : a.dkv, ((static_cast<int64_t>(w.b) * T + ra + r) * a.H + w.head) * WID + col, s[0], s[1], s[2], s[3]);
+  }
+  if constexpr (!Q)
+    for (int i = threadIdx.x; i < n * (DR / 4); i += 256) {
+      float* p = a.dkr_part + row0 * DR + i * 4;
+      f4 s = {0, 0, 0, 0};
+      for (int z = 0; z < parts; ++z) s += *reinterpret_cast<const f4*>(p + z * step * DR);
+      *reinterpret_cast<f4*>(p) = s;
+    }
+}
+
 template <int DT, int DN, int DR>
 hipError_t run_bwd(const LatentArgs& a, hipStream_t s) {
   constexpr int BM = BwdCfg<DT, DN, DR>::BM;
@@ -625,10 +641,14 @@ hipError_t run_bwd(const LatentArgs& a, hipStream_t s) {
   if (bh <= 0) return hipSuccess;
   if (a.Tq > 0) {
     kda_latent_rows_kernel<DT, DN><<<dim3((a.Tq + 127) / 128, bh), dim3(256), 0, s>>>(a);
-    kda_latent_dq_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(nqb * bh)), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
+    const unsigned gx = static_cast<unsigned>(nqb * bh);
+    kda_latent_dq_kernel<DT, DN, DR><<<dim3(gx, a.splits), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
+    if (a.splits > 1) kda_latent_bwd_join_kernel<DT, DN, DR, true><<<dim3(gx, 4), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
   }
   if (a.Tk > 0) {
-    kda_latent_dkv_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(nkb * bh)), dim3(KeyCfg<DT, DN, DR>::NT), 0, s>>>(a, static_cast<int>(nkb));
+    const unsigned gx = static_cast<unsigned>(nkb * bh);
+    kda_latent_dkv_kernel<DT, DN, DR><<<dim3(gx, a.splits_k), dim3(KeyCfg<DT, DN, DR>::NT), 0, s>>>(a, static_cast<int>(nkb));
+    if (a.splits_k > 1) kda_latent_bwd_join_kernel<DT, DN, DR, false><<<dim3(gx, 4), dim3(256), 0, s>>>(a, static_cast<int>(nkb));
     const int64_t per_b = static_cast<int64_t>(a.Tk) * DR;
     kda_latent_dkr_kernel<DT><<<dim3(static_cast<unsigned>((per_b + 1023) / 1024), a.B), dim3(256), 0, s>>>(a, per_b);
   }

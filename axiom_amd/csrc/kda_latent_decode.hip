@@ -417,205 +417,240 @@ __global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decod
 }
 
 // More than 16 rows: 64 a workgroup (16-bit types).  120 flop a byte and more, so
-// the waves share each tile of 64 keys: for the scores a wave takes 32 keys by 32
-// rows (32x32x16, its rows' queries in 144 registers), for the output a
-// quarter of the R columns by all 64 rows.  A wave's probabilities go to LDS in
-// the fragment order that they are made in.  They are formed against the
-// maximum that the waves agreed on last; only a tile that exceeds it by 2^8 costs
-// the extra exchange, so a tile takes two barriers.
+// the tile is shared and the work split by what a wave holds: four waves hold
+// the queries (16 rows each, 72 registers) and make a tile's probabilities,
+// four hold the output (64 rows by a quarter of the R columns, 128 registers)
+// and add the tile before.  The two on a SIMD have about as many products
+// (16x16x32 and 32x32x16); one's softmax runs under the other's products, and a
+// tile of 32 keys takes one barrier.  A row's keys of a tile are all in one wave,
+// so its maximum needs no exchange; where it rises (by 2^8, seldom) the factor
+// goes to the output waves beside the probabilities.  Four buffers: one each
+// is written to, arrived, scored and added.
 template <int DT, int R, int DR>
-__global__ __launch_bounds__(256, 1) void kda_latent_decode64_kernel(LatentDecodeArgs a) {
+__global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeArgs a) {
   typedef typename El<DT>::frag F;
   typedef typename El<DT>::t E;
   typedef Tile<R, 2> TN;
   typedef Tile<DR, 2> TR;
-  typedef Tile<64, 2> TP;
-  constexpr int KT = 64, W = R + DR, KN = R / 16, KR = DR / 16, NV = R / 128;
+  constexpr int KT = 32;
+  typedef Tile<KT, 2> TP;
+  constexpr int W = R + DR, KS = W / 32, KSN = R / 32, NV = R / 128;
   constexpr int OFF_R = TN::bytes(KT), BUF = OFF_R + TR::bytes(KT);
+  constexpr int PN = KT * TN::CPR / 64 / 8, PR = KT * TR::CPR / 64;   // pieces: latents a wave; rotary parts in all
   __shared__ __attribute__((aligned(1024))) char buf0[BUF];
   __shared__ __attribute__((aligned(1024))) char buf1[BUF];
-  __shared__ __attribute__((aligned(1024))) char sp[TP::bytes(64)];
-  __shared__ float red[2][64];
-  __shared__ int raise[2];                   // whether a tile exceeds the agreed maximum; by tile parity
+  __shared__ __attribute__((aligned(1024))) char buf2[BUF];
+  __shared__ __attribute__((aligned(1024))) char buf3[BUF];
+  __shared__ __attribute__((aligned(1024))) char sp[2][TP::bytes(64)];   // probabilities, by tile parity
+  __shared__ float fac[2][64];               // factor of the rows' sums before this tile
+  __shared__ int4 rose[2];                   // whether a score wave's rows have one
+  __shared__ float ml[2][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m = lane & 31, h = lane >> 5, kh = wave >> 1, rh = wave & 1;   // key and row halves of the scores
+  const int own = wave & 3;
+  const bool scoring = wave < 4;
   int w, grp;
   run_group(a, w, grp);
   Run run = find_run(a, w, KT).uniform();
   const int rows = a.Tq * a.H, r0 = grp * 64;
-  if (a.whole && run.g1 == 0) empty_rows<DT, R>(a, w, r0, min(rows, r0 + 64), 256);
+  if (a.whole && run.g1 == 0) empty_rows<DT, R>(a, w, r0, min(rows, r0 + 64), 512);
 
   const float c = a.scale * kLog2e, lazy = kLazy / c;
   const char* cache = static_cast<const char*>(a.cache);
-  const int qrow = min(r0 + 32 * rh + m, rows - 1);
 
   while (run.g < run.g1) {
     const int b = run.b, len = run.len, n_all = (len + KT - 1) / KT;
     const int ta = run.t, tb = min(n_all, ta + (run.g1 - run.g));
     if (ta < tb) {
     const int32_t* table = a.table + static_cast<int64_t>(b) * a.per;
-    auto token = [&](int j) { return min(j * KT + lane, len - 1); };   // a key a lane
+    auto token = [&](int j) { return min(j * KT + (lane & 31), len - 1); };   // a key a lane
     auto fetch = [&](int slot, char* dst) {
       const int ln = fresh(lane);
 #pragma unroll
-      for (int p = 0; p < KT * TN::CPR / 256; ++p) {
-        const int s = (wave + 4 * p) * 64 + ln, rr = s / TN::CPR;
-        const int64_t at = TN::CPR == 64 ? __builtin_amdgcn_readlane(slot, wave + 4 * p) : __shfl(slot, rr, 64);
-        copy16(cache + at * (W * 2) + (((s % TN::CPR) ^ TN::swz(rr)) << 4), dst + (wave + 4 * p) * 1024);
+      for (int p = 0; p < PN; ++p) {
+        const int s = (wave + 8 * p) * 64 + ln, rr = s / TN::CPR;
+        const int64_t at = TN::CPR == 64 ? __builtin_amdgcn_readlane(slot, wave + 8 * p) : __shfl(slot, rr, 64);
+        copy16(cache + at * (W * 2) + (((s % TN::CPR) ^ TN::swz(rr)) << 4), dst + (wave + 8 * p) * 1024);
       }
-#pragma unroll
-      for (int p = 0; p < KT * TR::CPR / 256; ++p) {
-        const int s = (wave + 4 * p) * 64 + ln, rr = s / TR::CPR;
+      if (wave < PR) {
+        const int s = wave * 64 + ln, rr = s / TR::CPR;
         copy16(cache + static_cast<int64_t>(__shfl(slot, rr, 64)) * (W * 2) + R * 2 + (((s % TR::CPR) ^ TR::swz(rr)) << 4),
-               dst + OFF_R + (wave + 4 * p) * 1024);
+               dst + OFF_R + wave * 1024);
       }
     };
-    const int tok0 = token(ta);
-    const int page0 = page_of(a, table, tok0);
-    int page = page_of(a, table, token(ta + 1));
-    F q[KN + KR];
-    {
-      const E* qp = static_cast<const E*>(a.q) + (static_cast<int64_t>(b) * rows + qrow) * W;
-#pragma unroll
-      for (int s = 0; s < KN + KR; ++s) q[s] = *reinterpret_cast<const F*>(qp + 16 * s + 8 * h);
-    }
-    const int seen = len - (a.Tq - 1 - qrow / a.H);
-    if (threadIdx.x < 2) raise[threadIdx.x] = 0;
-    lds_barrier();                           // the last segment has left the buffers
+    const int tok0 = token(ta), tok1 = token(ta + 1);
+    const int page0 = page_of(a, table, tok0), page1 = page_of(a, table, tok1);
+    int page = page_of(a, table, token(ta + 2));
     fetch(slot_of(a, page0, tok0), buf0);
+    if (ta + 1 < tb) fetch(slot_of(a, page1, tok1), buf1);
 
-    f16v acc[NV][2];
-    float mx = kMaxInit, l = 0.f;            // of row 32 rh + m; l over this wave's keys
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[v][n][i] = 0.f;
-
-    auto step = [&](int j, const char* cur, char* nxt) {
-      wait_vmem_all();
+    // interval i: tile i is scored, tile i - 1 added, tile i + 2 copied
+    auto turn = [&](int i, char* nxt) {
+      if (i + 1 < tb) wait_vmem_but<PN>();
+      else wait_vmem_all();
       lds_barrier();
-      if (threadIdx.x == 0) raise[(j + 1) & 1] = 0;
-      if (j + 1 < tb) {
-        const int slot = slot_of(a, page, token(j + 1));
-        page = page_of(a, table, token(j + 2));
+      if (i + 2 < tb) {
+        const int slot = slot_of(a, page, token(i + 2));
+        page = page_of(a, table, token(i + 3));
         fetch(slot, nxt);
       }
-      const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
-      f16v s, s1;
+    };
+    const bool whole = ta == 0 && tb == n_all;
+    const int64_t srow = (static_cast<int64_t>(2 * w + (ta > 0 ? 0 : 1)) * a.groups + grp) * 64;
+
+    if (scoring) {
+      const int m = lane & 15, gq = lane >> 4, r = min(r0 + 16 * own + m, rows - 1);
+      F q[KS];
+      {
+        const E* qp = static_cast<const E*>(a.q) + (static_cast<int64_t>(b) * rows + r) * W;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = s1[i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KN; k += 2) {
-        s = mma(s, TN::template row_frag<F>(cur, fm, k, fh, 32 * kh), q[k]);
-        s1 = mma(s1, TN::template row_frag<F>(cur, fm, k + 1, fh, 32 * kh), q[k + 1]);
+        for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const F*>(qp + 32 * s + 8 * gq);
       }
+      const int seen = len - (a.Tq - 1 - r / a.H);
+      float mx = kMaxInit, mc = kMaxInit * c, l = 0.f;
+      auto step = [&](int i, const char* cur, char* nxt) {
+        turn(i, nxt);
+        if (i >= tb) return;
+        const int ln = fresh(lane), fm = ln & 15, fg = ln >> 4;
+        f4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < KR; k += 2) {
-        s = mma(s, TR::template row_frag<F>(cur + OFF_R, fm, k, fh, 32 * kh), q[KN + k]);
-        s1 = mma(s1, TR::template row_frag<F>(cur + OFF_R, fm, k + 1, fh, 32 * kh), q[KN + k + 1]);
-      }
-      const int key0 = j * KT + 32 * kh + 4 * h;
-      float tm = -INFINITY;
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] += s1[i];
-        s[i] = key0 + 8 * (i >> 2) + (i & 3) < seen ? s[i] : -INFINITY;
-        tm = fmaxf(tm, s[i]);
-      }
-      tm = half_max(tm);
-      float lt = 0.f;
-      auto probs = [&] {
-        const float mc = mx * c;
-        lt = 0.f;
+          for (int t = 0; t < 2; ++t)
+            s[t] = mma_s(s[t], k < KSN ? row_frag16<TN, F>(cur + TN::bytes(16 * t), fm, k, fg)
+                                       : row_frag16<TR, F>(cur + OFF_R + TR::bytes(16 * t), fm, k - KSN, fg), q[k]);
+        pace<2 * KS, 8, 1, 1>();
+        __builtin_amdgcn_sched_barrier(0);
+        const int key0 = i * KT + 4 * gq;
+        float tm = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float p[8];
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            p[e] = fast_exp2(fmaf(s[8 * u + e], c, -mc));
-            lt += p[e];
+          for (int e = 0; e < 4; ++e) {
+            s[t][e] = key0 + 16 * t + e < seen ? s[t][e] : -INFINITY;
+            tm = fmaxf(tm, s[t][e]);
           }
-          *reinterpret_cast<F*>(sp + TP::off(fm, 4 * kh + 2 * u, fh, 32 * rh)) = to_frag<DT>(p);
+        tm = group_max(tm);
+        const bool up = __any(tm > mx + lazy);
+        if (up) {
+          const float nm = fmaxf(mx, tm), al = fast_exp2((mx - nm) * c);
+          mx = nm;
+          mc = nm * c;
+          l *= al;
+          if (gq == 0) fac[i & 1][16 * own + m] = al;
+        }
+        if (lane == 0) reinterpret_cast<int*>(&rose[i & 1])[own] = up;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[e] = fast_exp2(fmaf(s[t][e], c, -mc));
+            l += p[e];
+          }
+          // the output waves' fragment order: chunk 2 t + half, first or second four keys
+          store4<DT>(sp[i & 1] + TP::off(fm, 2 * t, fg & 1, 16 * own) + 8 * (fg >> 1), 0, p[0], p[1], p[2], p[3]);
         }
       };
-      probs();
-      if (h == 0) red[kh][32 * rh + m] = tm;
-      if (__any(tm > mx + lazy) && lane == 0) raise[j & 1] = 1;
+      for (int i = ta; i <= tb;) {
+        step(i, buf0, buf2);
+        if (++i > tb) break;
+        step(i, buf1, buf3);
+        if (++i > tb) break;
+        step(i, buf2, buf0);
+        if (++i > tb) break;
+        step(i, buf3, buf1);
+        ++i;
+      }
+      l = group_sum(l);
+      if (gq == 0) {
+        ml[0][16 * own + m] = mc;
+        ml[1][16 * own + m] = l;
+      }
       lds_barrier();
-      if (raise[j & 1]) {                    // the whole workgroup: new maxima, sums scaled, probabilities again
-        const float o0 = mx;
-        // the output's columns are rows m and 32 + m: their old and new maxima, from the score waves
-        const float nm = fmaxf(mx, fmaxf(red[0][32 * rh + m], red[1][32 * rh + m]));
-        mx = nm;
-        l *= fast_exp2((o0 - nm) * c);
-        lds_barrier();
-        probs();
-        if (kh == 0 && h == 0) red[0][32 * rh + m] = fast_exp2((o0 - nm) * c);
-        lds_barrier();
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float al = red[0][32 * n + m];
-#pragma unroll
-          for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[v][n][i] *= al;
+      if (gq == 0 && r0 + 16 * own + m < rows) {
+        if (whole) {
+          a.lse[static_cast<int64_t>(b) * rows + r] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * kLn2;
+        } else {
+          a.part_ml[2 * (srow + 16 * own + m)] = mc;
+          a.part_ml[2 * (srow + 16 * own + m) + 1] = l;
         }
       }
-      l += lt;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const F p0 = TP::template row_frag<F>(sp, fm, k, fh), p1 = TP::template row_frag<F>(sp, fm, k, fh, 32);
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          const F vf = TN::template col_frag<F>(cur, 16 * k, wave * (R / 4) + 32 * v, ln);
-          acc[v][0] = mma(acc[v][0], vf, p0);
-          acc[v][1] = mma(acc[v][1], vf, p1);
-        }
-      }
-    };
-    for (int j = ta; j < tb;) {
-      step(j, buf0, buf1);
-      if (++j >= tb) break;
-      step(j, buf1, buf0);
-      ++j;
-    }
-
-    lds_barrier();
-    l = half_sum(l);
-    if (h == 0) red[kh][32 * rh + m] = l;
-    float* ms = reinterpret_cast<float*>(sp);   // the rows' maxima
-    if (kh == 0 && h == 0) ms[32 * rh + m] = mx * c;
-    lds_barrier();
-    const bool whole = ta == 0 && tb == n_all;
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int r = r0 + 32 * n + m;
-      const float ls = red[0][32 * n + m] + red[1][32 * n + m], mc = ms[32 * n + m];
-      if (r >= rows) continue;
-      const int64_t row = static_cast<int64_t>(b) * rows + r;
-      const int64_t sr = (static_cast<int64_t>(2 * w + (ta > 0 ? 0 : 1)) * a.groups + grp) * 64 + 32 * n + m;
-      const int col = wave * (R / 4) + 4 * h;
-      const float inv = ls > 0.f ? 1.f / ls : ls;   // nothing visible: zeros; NaN stays NaN
+    } else {
+      const int m = lane & 31, h = lane >> 5;
+      f16v acc[NV][2];
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f4 o = {acc[v][n][4 * i], acc[v][n][4 * i + 1], acc[v][n][4 * i + 2], acc[v][n][4 * i + 3]};
-          if (whole) store4<DT>(a.o, row * R + col + 32 * v + 8 * i, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-          else *reinterpret_cast<f4*>(a.part_o + sr * R + col + 32 * v + 8 * i) = o;
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[v][n][e] = 0.f;
+      auto step = [&](int i, const char* prev, char* nxt) {
+        turn(i, nxt);
+        if (i == ta) return;
+        const int par = (i - 1) & 1;
+        const int4 up = rose[par];
+        if (__builtin_amdgcn_readfirstlane(up.x | up.y | up.z | up.w)) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int mine = n == 0 ? (m < 16 ? up.x : up.y) : (m < 16 ? up.z : up.w);
+            const float al = mine ? fac[par][32 * n + m] : 1.f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[v][n][e] *= al;
+          }
         }
-      if (wave == 0 && h == 0) {
-        if (whole) {
-          a.lse[row] = ls == 0.f ? -INFINITY : (mc + __log2f(ls)) * kLn2;
-        } else {
-          a.part_ml[2 * sr] = mc;
-          a.part_ml[2 * sr + 1] = ls;
+        const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const F p0 = TP::template row_frag<F>(sp[par], fm, k, fh), p1 = TP::template row_frag<F>(sp[par], fm, k, fh, 32);
+#pragma unroll
+          for (int v = 0; v < NV; ++v) {
+            const F vf = TN::template col_frag<F>(prev, 16 * k, own * (R / 4) + 32 * v, ln);
+            acc[v][0] = mma(acc[v][0], vf, p0);
+            acc[v][1] = mma(acc[v][1], vf, p1);
+          }
         }
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+        for (int k = 0; k < 2 * NV; ++k) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      for (int i = ta; i <= tb;) {
+        step(i, buf3, buf2);
+        if (++i > tb) break;
+        step(i, buf0, buf3);
+        if (++i > tb) break;
+        step(i, buf1, buf0);
+        if (++i > tb) break;
+        step(i, buf2, buf1);
+        ++i;
+      }
+      lds_barrier();
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int r = r0 + 32 * n + m;
+        if (r >= rows) continue;
+        const float ls = ml[1][32 * n + m];
+        const int64_t row = static_cast<int64_t>(b) * rows + r;
+        const int col = own * (R / 4) + 4 * h;
+        const float inv = ls > 0.f ? 1.f / ls : ls;   // nothing visible: zeros; NaN stays NaN
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f4 o = {acc[v][n][4 * e], acc[v][n][4 * e + 1], acc[v][n][4 * e + 2], acc[v][n][4 * e + 3]};
+            if (whole) store4<DT>(a.o, row * R + col + 32 * v + 8 * e, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+            else *reinterpret_cast<f4*>(a.part_o + (srow + 32 * n + m) * R + col + 32 * v + 8 * e) = o;
+          }
       }
     }
-    lds_barrier();
+    lds_barrier();                           // the sums have been read
     }
     run.g += places(a, len, KT) - ta;
     ++run.b;
@@ -687,14 +722,14 @@ hipError_t run_decode(const LatentDecodeArgs& a, int m_rows, hipStream_t s) {
   if (m_rows == 16) {
     kda_latent_decode16_kernel<DT, R, DR><<<dim3(a.wgs * a.groups), dim3(64 * C::NW), 0, s>>>(a);
   } else if constexpr (DT != 0) {
-    kda_latent_decode64_kernel<DT, R, DR><<<dim3(a.wgs * a.groups), dim3(256), 0, s>>>(a);
+    kda_latent_decode64_kernel<DT, R, DR><<<dim3(a.wgs * a.groups), dim3(512), 0, s>>>(a);
   } else {
     return hipErrorInvalidValue;
   }
   if (a.whole) return hipGetLastError();
   const dim3 grid(a.Tq * a.H, a.B), block(R / 2);
   if (m_rows == 16) kda_latent_join_kernel<DT, R, 16><<<grid, block, 0, s>>>(a, 16);
-  else kda_latent_join_kernel<DT, R, 64><<<grid, block, 0, s>>>(a, 64);
+  else kda_latent_join_kernel<DT, R, 32><<<grid, block, 0, s>>>(a, 64);
   return hipGetLastError();
 }
 
@@ -715,7 +750,7 @@ hipError_t launch_latent_append(const LatentAppendArgs& a, int R, int dr, int dt
   return dt == 0 ? latent::append_by_dims<0>(a, R, dr, s) : dt == 1 ? latent::append_by_dims<1>(a, R, dr, s)
                                                                     : latent::append_by_dims<2>(a, R, dr, s);
 }
-int latent_decode_tile(int m_rows) { return m_rows; }
+int latent_decode_tile(int m_rows) { return m_rows == 16 ? 16 : 32; }
 hipError_t launch_latent_decode(const LatentDecodeArgs& a, int R, int dr, int dt, int m_rows, hipStream_t s) {
   return dt == 0 ? latent::decode_by_dims<0>(a, R, dr, m_rows, s) : dt == 1 ? latent::decode_by_dims<1>(a, R, dr, m_rows, s)
                                                                         : latent::decode_by_dims<2>(a, R, dr, m_rows, s);

@@ -40,47 +40,19 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 31, h = lane >> 5;
 
-  // block -> (batch, head, queries).  Heads are spread over the eight XCDs
-  // (consecutive workgroups go round them), so that one XCD's L2 serves a
-  // head's keys; the longest causal blocks of a head start first.
-  int b = 0, head, q0, qe, k0, ke, off;
-  {
-    const int id = blockIdx.x, bh_n = a.B * a.H;
-    int bh, blk;
-    if (bh_n % 8 == 0) {
-      const int slot = id >> 3;
-      bh = (id & 7) + 8 * (slot / nqb);
-      blk = nqb - 1 - slot % nqb;
-    } else {
-      bh = id % bh_n;
-      blk = nqb - 1 - id / bh_n;
-    }
-    b = bh / a.H;
-    head = bh - b * a.H;
-    if (a.cu_q) {
-      Span s;
-      if (!find_span(a.cu_q, a.n_seqs, a.Tq, C::BM, blk, s)) return;
-      q0 = s.a + s.blk * C::BM;
-      qe = s.e;
-      k0 = min(max(a.cu_k[s.seq], 0), a.Tk);
-      ke = min(max(a.cu_k[s.seq + 1], k0), a.Tk);
-      off = (ke - k0) - (s.e - s.a) - s.a;    // key index inside the sequence <= query row + off
-    } else {
-      q0 = blk * C::BM;
-      qe = a.Tq;
-      k0 = 0;
-      ke = a.Tk;
-      off = a.Tk - a.Tq;
-    }
-  }
-  const int nk = ke - k0;
+  Where w;
+  if (!locate(a, nqb, C::BM, true, true, w)) return;
+  const int b = w.b, head = w.head, q0 = w.r0, qe = w.re, off = w.off, nk = w.ke - w.k0;
   const int row = q0 + wave * 32 + m;         // this lane's query
   const bool live = row < qe;
   const int kmax = a.causal ? min(nk - 1, row + off) : nk - 1;   // last key it sees
   const int wave_lo = a.causal ? min(nk - 1, q0 + wave * 32 + off) : nk - 1;   // last key that all of the wave's queries see
   const int wave_hi = a.causal ? min(nk - 1, min(q0 + wave * 32 + 31, qe - 1) + off) : nk - 1;
   const int blk_hi = a.causal ? min(nk - 1, min(q0 + C::BM - 1, qe - 1) + off) : nk - 1;
-  const int nt = (blk_hi + BN) / BN;          // key tiles of the workgroup (0 when no query sees a key)
+  // key tiles of the block (none when no query sees a key) and this workgroup's
+  const Share part(max(0, (blk_hi + BN) / BN), a.splits, blockIdx.y);
+  const int nt = part.j1;
+  if (static_cast<int>(blockIdx.y) >= part.parts) return;
 
   F qn[KN], qr[KR];
   {
@@ -91,8 +63,8 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
     for (int s = 0; s < KR; ++s) qr[s] = *reinterpret_cast<const F*>(qp + DN + 16 * s + 8 * h);
   }
 
-  const char* kvp = static_cast<const char*>(a.kv) + (b * a.kv_b + k0 * a.kv_t + head * a.kv_h) * ES;
-  const char* krp = static_cast<const char*>(a.kr) + (b * a.kr_b + k0 * a.kr_t) * ES;
+  const char* kvp = static_cast<const char*>(a.kv) + (b * a.kv_b + w.k0 * a.kv_t + head * a.kv_h) * ES;
+  const char* krp = static_cast<const char*>(a.kr) + (b * a.kr_b + w.k0 * a.kr_t) * ES;
   const unsigned kv_rb = static_cast<unsigned>(a.kv_t * ES), kr_rb = static_cast<unsigned>(a.kr_t * ES);
   Copy<typename C::TN, BN, C::NW> cn;
   Copy<typename C::TR, BN, C::NW> cr;
@@ -128,7 +100,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
     if (j + 1 < nt) fetch(j + 1, nxt);
     const int kt = j * BN;
     if (kt > wave_hi) return;                 // nothing of this tile for this wave's queries
-    const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
+    const int ln = lane, fm = m, fh = h;
     f16v s[NB];
 #pragma unroll
     for (int t = 0; t < NB; ++t)
@@ -192,8 +164,8 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
     if constexpr (ES == 2) pace<2 * NB * ND, 4, 2, 1>();
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (nt > 0) fetch(0, buf0);
-  for (int j = 0; j < nt;) {
+  if (part.j0 < nt) fetch(part.j0, buf0);
+  for (int j = part.j0; j < nt;) {
     step(j, buf0, buf1);
     if (++j >= nt) break;
     step(j, buf1, buf0);
@@ -202,7 +174,17 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
 
   l = half_sum(l);
   if (!live) return;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // no visible key: zeros; NaN stays NaN
+  if (part.parts > 1) {
+    const int64_t pr = (static_cast<int64_t>(blockIdx.y) * a.B * a.H + w.bh) * a.Tq + row;
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store4<0>(a.part, pr * DN + 4 * h + 32 * n + 8 * i, acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]);
+    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(mc, l);
+    return;
+  }
+  const float inv = l > 0.f ? 1.f / l : l;      // no visible key: zeros; NaN stays NaN
   const int64_t ob = ((static_cast<int64_t>(b) * a.Tq + row) * a.H + head) * DN + 4 * h;
 #pragma unroll
   for (int n = 0; n < ND; ++n)
@@ -210,7 +192,41 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
     for (int i = 0; i < 4; ++i)
       store4<DT>(a.o, ob + 32 * n + 8 * i, acc[n][4 * i] * inv, acc[n][4 * i + 1] * inv, acc[n][4 * i + 2] * inv,
                  acc[n][4 * i + 3] * inv);
-  if (h == 0) a.lse[(static_cast<int64_t>(b) * a.H + head) * a.Tq + row] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * kLn2;
+  if (h == 0) a.lse[static_cast<int64_t>(w.bh) * a.Tq + row] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * kLn2;
+}
+
+// Joins the parts of split blocks, in part order; a quarter of a block a workgroup.
+template <int DT, int DN, int DR>
+__global__ __launch_bounds__(256) void kda_latent_fwd_join_kernel(LatentArgs a, int nqb) {
+  typedef FwdCfg<DT, DN, DR> C;
+  constexpr int LPR = DN / 4, RPP = 256 / LPR;
+  Where w;
+  if (!locate(a, nqb, C::BM, true, true, w)) return;
+  const int nk = w.ke - w.k0, blk_hi = a.causal ? min(nk - 1, min(w.r0 + C::BM - 1, w.re - 1) + w.off) : nk - 1;
+  const int parts = Share(max(0, (blk_hi + C::BN) / C::BN), a.splits, 0).parts;
+  if (parts == 1) return;
+  const int col = (threadIdx.x % LPR) * 4;
+  const int64_t step = static_cast<int64_t>(a.B) * a.H * a.Tq;
+#pragma unroll 2
+  for (int r = threadIdx.x / LPR; r < 32; r += RPP) {
+    const int row = w.r0 + blockIdx.y * 32 + r;
+    if (row >= w.re) break;
+    const int64_t pr = static_cast<int64_t>(w.bh) * a.Tq + row;
+    float mx = kMaxInit, l = 0.f;
+    for (int z = 0; z < parts; ++z) mx = fmaxf(mx, a.part_ml[2 * (z * step + pr)]);
+    f4 o = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int z = 0; z < parts; ++z) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (z * step + pr));
+      const float f = fast_exp2(ml.x - mx);
+      l = fmaf(f, ml.y, l);
+      o += f * *reinterpret_cast<const f4*>(a.part + (z * step + pr) * DN + col);
+    }
+    const float inv = l > 0.f ? 1.f / l : l;
+    store4<DT>(a.o, ((static_cast<int64_t>(w.b) * a.Tq + row) * a.H + w.head) * DN + col, o[0] * inv, o[1] * inv, o[2] * inv,
+               o[3] * inv);
+    if (col == 0) a.lse[pr] = l == 0.f ? -INFINITY : (mx + __log2f(l)) * kLn2;
+  }
 }
 
 template <int DT, int DN, int DR>
@@ -220,7 +236,9 @@ hipError_t run_fwd(const LatentArgs& a, hipStream_t s) {
   const int64_t nqb = a.cu_q ? static_cast<int64_t>(a.Tq) / BM + a.n_seqs : (static_cast<int64_t>(a.Tq) + BM - 1) / BM;
   const int64_t grid = nqb * a.B * a.H;
   if (grid <= 0) return hipSuccess;
-  kda_latent_fwd_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(grid)), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
+  const unsigned gx = static_cast<unsigned>(grid);
+  kda_latent_fwd_kernel<DT, DN, DR><<<dim3(gx, a.splits), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
+  if (a.splits > 1) kda_latent_fwd_join_kernel<DT, DN, DR><<<dim3(gx, 4), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
   return hipGetLastError();
 }
 

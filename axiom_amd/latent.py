@@ -75,7 +75,8 @@ def _output(name, what, t, shape, dtype, dev):
     return t
 
 
-def latent_attn_fwd(q, kv, k_rope, cu_seqlens=None, cu_seqlens_k=None, causal: bool = True, scale=None, out=None, lse=None):
+def latent_attn_fwd(q, kv, k_rope, cu_seqlens=None, cu_seqlens_k=None, causal: bool = True, scale=None, out=None, lse=None,
+                    workspace=None):
     """Latent attention, expanded form; returns ``(o, lse)``.
 
     ``q [B,Tq,H,dn+dr]`` (nope part, then the rotated part), ``kv [B,Tk,H,2 dn]``
@@ -87,15 +88,22 @@ def latent_attn_fwd(q, kv, k_rope, cu_seqlens=None, cu_seqlens_k=None, causal: b
     gets zeros and ``-inf``.  ``cu_seqlens`` (int32 ``[N+1]`` on the device, B ==
     1) packs N sequences; ``cu_seqlens_k`` its key offsets where they differ.
     ``scale``: default ``(dn + dr) ** -0.5``.  dn in {64, 128}, dr in {32, 64}.
+    ``out`` / ``lse``: optional preallocated outputs; ``workspace``: an optional
+    uint8 device buffer (a call of few blocks needs one; a smaller one than
+    needed is replaced by a new one).
     """
     what = "latent_attn_fwd"
     B, Tq, Tk, H, dn, dr, st, cu_q, cu_k, n_seqs, scale = _attn_check(what, q, kv, k_rope, cu_seqlens, cu_seqlens_k, scale)
     dev = _require_gpu([q, kv, k_rope, cu_q, cu_k], what)
     o = _output("out", what, out, (B, Tq, H, dn), q.dtype, dev)
     lse = _output("lse", what, lse, (B, H, Tq), torch.float32, dev)
+    code = _IN_CODES[q.dtype]
+    ws_bytes = _ws_bytes("kda_latent_attn_fwd_workspace", B, Tq, Tk, H, dn, dr, n_seqs, code)
+    if ws_bytes and (workspace is None or workspace.numel() * workspace.element_size() < ws_bytes):
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     rc = _lib.lib().kda_latent_attn_fwd(_stream(dev), _ptr(q), _ptr(kv), _ptr(k_rope), st, _ptr(cu_q), _ptr(cu_k), n_seqs,
-                                        _ptr(o), _ptr(lse), B, Tq, Tk, H, dn, dr, 1 if causal else 0, scale,
-                                        _IN_CODES[q.dtype])
+                                        _ptr(o), _ptr(lse), B, Tq, Tk, H, dn, dr, 1 if causal else 0, scale, code,
+                                        _ptr(workspace), ws_bytes)
     _lib.check(rc, what)
     return o, lse
 
@@ -119,7 +127,7 @@ def latent_attn_bwd(q, kv, k_rope, o, lse, do, cu_seqlens=None, cu_seqlens_k=Non
         raise ValueError(f"{what}: lse must be fp32 [{B},{H},{Tq}]")
     _contig("lse", lse)
     dev = _require_gpu([q, kv, k_rope, o, lse, do, cu_q, cu_k], what)
-    ws_bytes = _ws_bytes("kda_latent_attn_bwd_workspace", B, Tq, Tk, H, dr)
+    ws_bytes = _ws_bytes("kda_latent_attn_bwd_workspace", B, Tq, Tk, H, dn, dr, n_seqs, _IN_CODES[q.dtype])
     if workspace is None or workspace.numel() * workspace.element_size() < ws_bytes:
         workspace = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
     dq = torch.empty((B, Tq, H, dn + dr), dtype=q.dtype, device=dev)

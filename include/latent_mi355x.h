@@ -37,12 +37,19 @@ extern "C" {
  * dn in {64, 128}, dr in {32, 64}, scale > 0 and finite, Tq, Tk >= 0.
  * Products run in the inputs' precision (probabilities rounded to it for the
  * second), sums and softmax statistics in fp32.  Pointers are aligned to 16
- * bytes and strides are multiples of 16 bytes.
+ * bytes and strides are multiples of 16 bytes.  Calls of few blocks of 128
+ * queries share each block's keys out over workgroups and join their parts:
+ * caller workspace of kda_latent_attn_fwd_workspace bytes.
  */
 KDA_API int kda_latent_attn_fwd(hipStream_t stream, const void* q, const void* kv, const void* k_rope,
                 const int64_t* strides, const int32_t* cu_q, const int32_t* cu_k, int32_t n_seqs,
                 void* o, float* lse, int B, int Tq, int Tk, int H, int dn, int dr, int causal, float scale,
-                int dtype);
+                int dtype, void* workspace, size_t workspace_bytes);
+
+/* Workspace bytes kda_latent_attn_fwd needs (n_seqs 0: dense).  0 where it
+ * needs none (enough blocks of 128 queries to fill the chip; also on bad
+ * input): then workspace may be null.  Host-only. */
+KDA_API size_t kda_latent_attn_fwd_workspace(int B, int Tq, int Tk, int H, int dn, int dr, int32_t n_seqs, int dtype);
 
 /*
  * Gradients of o of kda_latent_attn_fwd: given its inputs, o, lse and the
@@ -57,8 +64,8 @@ KDA_API int kda_latent_attn_bwd(hipStream_t stream, const void* q, const void* k
                 int B, int Tq, int Tk, int H, int dn, int dr, int causal, float scale, int dtype,
                 void* workspace, size_t workspace_bytes);
 
-/* Workspace bytes kda_latent_attn_bwd needs (0 on bad input).  Host-only. */
-KDA_API size_t kda_latent_attn_bwd_workspace(int B, int Tq, int Tk, int H, int dr);
+/* Workspace bytes kda_latent_attn_bwd needs (n_seqs 0: dense; 0 on bad input).  Host-only. */
+KDA_API size_t kda_latent_attn_bwd_workspace(int B, int Tq, int Tk, int H, int dn, int dr, int32_t n_seqs, int dtype);
 
 /*
  * New tokens into the latent cache: row i of `rows` [N, R+dr] (the

@@ -39,9 +39,9 @@ DENSE = (192 * 100 * 2, 192 * 2, 192, 256 * 100 * 2, 256 * 2, 256, 6400, 64)
 
 
 def _fwd(L, q=OK, kv=OK, kr=OK, st=DENSE, cu_q=None, cu_k=None, n=0, o=OK, lse=OK, B=1, Tq=100, Tk=100, H=2, dn=128, dr=64,
-         causal=1, scale=0.1, dtype=1):
+         causal=1, scale=0.1, dtype=1, ws=None, bytes=0):
     return L.kda_latent_attn_fwd(None, q, kv, kr, None if st is None else _st(*st), cu_q, cu_k, n, o, lse, B, Tq, Tk, H, dn,
-                                 dr, causal, scale, dtype)
+                                 dr, causal, scale, dtype, ws, bytes)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -51,7 +51,8 @@ def _fwd(L, q=OK, kv=OK, kr=OK, st=DENSE, cu_q=None, cu_k=None, n=0, o=OK, lse=O
     (dict(scale=0.0), -1), (dict(scale=-1.0), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1),
     (dict(dtype=3), -1), (dict(dtype=-1), -1), (dict(cu_q=OK), -1), (dict(cu_q=OK, cu_k=OK, n=0), -1),
     (dict(cu_q=OK, cu_k=OK, n=2, B=2), -1), (dict(st=DENSE[:1] + (193,) + DENSE[2:]), -1), (dict(st=DENSE[:7] + (-64,)), -1),
-    (dict(st=DENSE[:4] + (1 << 24,) + DENSE[5:]), -2), (dict(B=70000, H=1), -2), (dict(Tq=1 << 30, H=128), -2)])
+    (dict(st=DENSE[:4] + (1 << 24,) + DENSE[5:]), -2), (dict(B=70000, H=1), -2), (dict(Tq=1 << 30, H=128), -2),
+    (dict(Tk=1000), -3), (dict(Tk=1000, ws=OK, bytes=64), -3), (dict(Tk=1000, ws=OK + 4, bytes=1 << 40), -1)])
 def test_forward_refuses(L, kw, code):
     assert _fwd(L, **kw) == code
     assert _lib.last_error()
@@ -63,17 +64,39 @@ def test_empty_calls_do_nothing(L):
     assert L.kda_latent_decode(None, None, None, None, None, None, None, 0, 1, 1, 512, 64, 1, 16, 1, 0.1, 1, None, 0) == 0
 
 
-def test_backward_workspace(L):
-    # D, the blocks' largest |do|, each head's share of the rotary key's gradient
-    up = lambda x: -(-x // 256) * 256  # noqa: E731
-    assert L.kda_latent_attn_bwd_workspace(2, 300, 400, 3, 64) == up(6 * 300 * 4) + up(6 * 3 * 4) + up(6 * 400 * 64 * 4) + 256
-    for bad in ((-1, 1, 1, 1, 64), (1, -1, 1, 1, 64), (1, 1, 1, 0, 64), (1, 1, 1, 1, 48)):
-        assert L.kda_latent_attn_bwd_workspace(*bad) == 0
+def _up(x):
+    return -(-x // 256) * 256
+
+
+def _splits(T, other, B, H, n, slots):
+    """Workgroups of a block of 128 rows along the other axis: until `slots` workgroups, 16 at most, 128 rows each at least."""
+    blocks = (T // 128 + n if n else -(-T // 128)) * B * H
+    return max(1, min(slots // blocks, -(-other // 128), 16)) if blocks else 1
+
+
+@pytest.mark.parametrize("B,Tq,Tk,H,dn,dr,n", [(2, 300, 400, 3, 128, 64, 0), (1, 1, 5000, 16, 128, 64, 0), (4, 4096, 4096, 16, 128, 64, 0),
+                                               (1, 700, 700, 2, 64, 32, 9), (1, 0, 50, 2, 64, 32, 0), (1, 50, 0, 2, 64, 32, 0)])
+@pytest.mark.parametrize("code", [0, 1, 2])
+def test_attention_workspaces(L, B, Tq, Tk, H, dn, dr, n, code):
+    s = _splits(Tq, Tk, B, H, n, 256 if code == 0 else 512)
+    rows = s * B * H * Tq if s > 1 else 0
+    assert L.kda_latent_attn_fwd_workspace(B, Tq, Tk, H, dn, dr, n, code) == _up(rows * dn * 4) + _up(rows * 8)
+    # D, the blocks' largest |do|, each head's (and part's) share of the rotary key's gradient, the parts of dq, then of dkv
+    k = _splits(Tk, Tq, B, H, n, 256)
+    want = _up(B * H * Tq * 4) + _up(B * H * -(-Tq // 128) * 4) + _up(k * B * H * Tk * dr * 4)
+    want += _up(max(rows * (dn + dr) * 4, k * B * H * Tk * 2 * dn * 4 if k > 1 else 0)) + 256
+    assert L.kda_latent_attn_bwd_workspace(B, Tq, Tk, H, dn, dr, n, code) == want
+
+
+@pytest.mark.parametrize("bad", [(-1, 1, 1, 1, 64, 64, 0, 1), (1, -1, 1, 1, 64, 64, 0, 1), (1, 1, 1, 0, 64, 64, 0, 1),
+                                 (1, 1, 1, 1, 96, 64, 0, 1), (1, 1, 1, 1, 64, 48, 0, 1), (1, 1, 1, 1, 64, 64, -1, 1), (1, 1, 1, 1, 64, 64, 0, 3)])
+def test_attention_workspaces_refuse(L, bad):
+    assert L.kda_latent_attn_fwd_workspace(*bad) == 0 and L.kda_latent_attn_bwd_workspace(*bad) == 0
 
 
 def test_backward_refuses(L):
     def bwd(ws=OK, n=None, o=OK, do=OK, dq=OK, dkv=OK, dkr=OK):
-        need = L.kda_latent_attn_bwd_workspace(1, 100, 100, 2, 64)
+        need = L.kda_latent_attn_bwd_workspace(1, 100, 100, 2, 128, 64, 0, 1)
         return L.kda_latent_attn_bwd(None, OK, OK, OK, _st(*DENSE), None, None, 0, o, OK, do, dq, dkv, dkr, 1, 100, 100, 2, 128,
                                      64, 1, 0.1, 1, ws, need - 1 if n is None else n)
     assert bwd() == -3 and bwd(ws=None, n=1 << 30) == -3
