@@ -255,6 +255,23 @@ __device__ __forceinline__ int slot_of(const LatentDecodeArgs& a, int page, int 
   return (min(max(page, 0), static_cast<int>(a.n_pages - 1)) << a.page_shift) + (tok & ((1 << a.page_shift) - 1));
 }
 
+// One 1 KiB piece (number s / 64 of a buffer's tile) of cache rows to LDS: the
+// part of the rows from byte `from` on that tile TL holds.  slot: the cache row
+// of key `lane`.  A piece inside one row has its row in scalar registers.
+template <class TL>
+__device__ __forceinline__ void copy_piece(const char* cache, int row_bytes, int from, int slot, int piece, int lane, char* dst) {
+  if constexpr (TL::CPR % 64 == 0) {
+    constexpr int PPR = TL::CPR / 64;      // pieces of a row
+    const int r = piece / PPR;
+    const char* src = cache + static_cast<int64_t>(__builtin_amdgcn_readlane(slot, r)) * row_bytes + (from + piece % PPR * 1024);
+    copy16(src + static_cast<unsigned>((lane ^ TL::swz(r)) << 4), dst + piece * 1024);
+  } else {
+    const int r = piece * (64 / TL::CPR) + lane / TL::CPR;
+    const unsigned off = static_cast<unsigned>(from + (((lane % TL::CPR) ^ TL::swz(r)) << 4));
+    copy16(cache + static_cast<int64_t>(__shfl(slot, r, 64)) * row_bytes + off, dst + piece * 1024);
+  }
+}
+
 template <int DT, int R, int DR>
 __global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decode16_kernel(LatentDecodeArgs a) {
   typedef DecCfg<DT, R, DR> C;
@@ -283,19 +300,11 @@ __global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decod
 
     auto token = [&](int j) { return min(j * KT + m, len - 1); };   // key m of tile j
     auto fetch = [&](int slot) {
-      const int ln = fresh(lane);
+      const int ln = fresh(lane) & 63;
 #pragma unroll
-      for (int p = 0; p < C::PN; ++p) {
-        const int s = p * 64 + ln, rr = s / C::TN::CPR;
-        const int64_t at = C::TN::CPR % 64 == 0 ? __builtin_amdgcn_readlane(slot, p * 64 / C::TN::CPR) : __shfl(slot, rr, 64);
-        copy16(cache + at * (W * ES) + (((s % C::TN::CPR) ^ C::TN::swz(rr)) << 4), mine + p * 1024);
-      }
+      for (int p = 0; p < C::PN; ++p) copy_piece<typename C::TN>(cache, W * ES, 0, slot, p, ln, mine);
 #pragma unroll
-      for (int p = 0; p < C::PR; ++p) {
-        const int s = p * 64 + ln, rr = s / C::TR::CPR;
-        copy16(cache + static_cast<int64_t>(__shfl(slot, rr, 64)) * (W * ES) + R * ES +
-                   (((s % C::TR::CPR) ^ C::TR::swz(rr)) << 4), mine + C::OFF_R + p * 1024);
-      }
+      for (int p = 0; p < C::PR; ++p) copy_piece<typename C::TR>(cache, W * ES, R * ES, slot, p, ln, mine + C::OFF_R);
     };
 
     int page = page_of(a, table, token(ta + wave));   // of the next tile to copy
@@ -464,18 +473,10 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
     const int32_t* table = a.table + static_cast<int64_t>(b) * a.per;
     auto token = [&](int j) { return min(j * KT + (lane & 31), len - 1); };   // a key a lane
     auto fetch = [&](int slot, char* dst) {
-      const int ln = fresh(lane);
+      const int ln = fresh(lane) & 63;
 #pragma unroll
-      for (int p = 0; p < PN; ++p) {
-        const int s = (wave + 8 * p) * 64 + ln, rr = s / TN::CPR;
-        const int64_t at = TN::CPR == 64 ? __builtin_amdgcn_readlane(slot, wave + 8 * p) : __shfl(slot, rr, 64);
-        copy16(cache + at * (W * 2) + (((s % TN::CPR) ^ TN::swz(rr)) << 4), dst + (wave + 8 * p) * 1024);
-      }
-      if (wave < PR) {
-        const int s = wave * 64 + ln, rr = s / TR::CPR;
-        copy16(cache + static_cast<int64_t>(__shfl(slot, rr, 64)) * (W * 2) + R * 2 + (((s % TR::CPR) ^ TR::swz(rr)) << 4),
-               dst + OFF_R + wave * 1024);
-      }
+      for (int p = 0; p < PN; ++p) copy_piece<TN>(cache, W * 2, 0, slot, wave + 8 * p, ln, dst);
+      if (wave < PR) copy_piece<TR>(cache, W * 2, R * 2, slot, wave, ln, dst + OFF_R);
     };
     const int tok0 = token(ta), tok1 = token(ta + 1);
     const int page0 = page_of(a, table, tok0), page1 = page_of(a, table, tok1);
