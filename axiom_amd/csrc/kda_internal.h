@@ -319,10 +319,11 @@ struct LatentArgs {
   const void* dout;
   const float* lse_in;
   float* D;                // sum over dn of do * o
-  float* dmax;             // fp16: largest |do| of each 128-row block, [B*H][ceil(Tq / 128)]
-  int dmax_n;              // its blocks
+  float* dmax;             // fp16: largest |do| of each query block, [B*H][dmax_n]
+  int dmax_n;
   float* dkr_part;         // [splits][B,H,Tk,dr]: each head's share of the rotary key's gradient
-  int splits_k;            // the key pass' splits (`splits` is the query pass')
+  int splits_k;            // the key pass' splits and parts (`splits`, `part` are the query pass')
+  float* part_k;
   void* dq;
   void* dkv;
   void* dkr;

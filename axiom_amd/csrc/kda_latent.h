@@ -313,15 +313,15 @@ __device__ __forceinline__ bool find_span(const int32_t* cu, int n_seqs, int T, 
   return false;
 }
 
-struct Where { int b, head, bh, r0, re, k0, ke, off; };   // rows owned from r0 to re, the other side k0 to ke
+struct Where { int b, head, bh, blk, r0, re, k0, ke, off; };   // rows owned from r0 to re, the other side k0 to ke
 // q_side: the workgroup owns queries, else keys.  off: owned query row i sees the
 // keys of the sequence with index <= i + off; owned key row j is seen by the
 // queries of the sequence with index >= j + off.
 // Heads are spread over the eight XCDs (consecutive workgroups go round them), so
 // that one XCD's L2 serves a head's rows; reverse: the last block of a head
 // first (the one with the longest causal walk).
-__device__ __forceinline__ bool locate(const LatentArgs& a, int nb, int BM, bool q_side, bool reverse, Where& w) {
-  const int id = blockIdx.x, bh_n = a.B * a.H;
+__device__ __forceinline__ bool locate(const LatentArgs& a, int id, int nb, int BM, bool q_side, bool reverse, Where& w) {
+  const int bh_n = a.B * a.H;
   int blk;
   if (bh_n % 8 == 0) {
     const int slot = id >> 3;
@@ -332,6 +332,7 @@ __device__ __forceinline__ bool locate(const LatentArgs& a, int nb, int BM, bool
     blk = id / bh_n;
   }
   if (reverse) blk = nb - 1 - blk;
+  w.blk = blk;
   w.b = w.bh / a.H;
   w.head = w.bh - w.b * a.H;
   if (a.cu_q) {

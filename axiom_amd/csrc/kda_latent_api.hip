@@ -80,38 +80,39 @@ kda::LatentArgs attn_args(const void* q, const void* kv, const void* kr, const i
 // blocks than the chip runs at once leaves CUs idle while each block walks its
 // whole row of tiles, so the walk is shared out, up to 16 ways, until there are
 // `slots` workgroups; a join adds their fp32 parts.
+// blocks of 128 rows of one head; packed: every sequence ends in at most one partial block
+int64_t blocks_of(int64_t T, int n_seqs) { return n_seqs > 0 ? T / 128 + n_seqs : (T + 127) / 128; }
 int splits_of(int64_t T, int64_t T_other, int B, int H, int n_seqs, int slots) {
-  const int64_t blocks = (n_seqs > 0 ? T / 128 + n_seqs : (T + 127) / 128) * B * H;
+  const int64_t blocks = blocks_of(T, n_seqs) * B * H;
   if (blocks <= 0) return 1;
   const int64_t s = slots / blocks, most = (T_other + 127) / 128;   // shares of at least 128 rows
   return static_cast<int>(s < 1 || most <= 1 ? 1 : (s < most ? (s < 16 ? s : 16) : (most < 16 ? most : 16)));
 }
-// Workgroups at once on 256 CUs: two a CU where registers and LDS allow.
-constexpr int kSlots16 = 512, kSlots32 = 256, kSlotsKeys = 256;
-int q_slots(int dtype) { return dtype == KDA_DTYPE_F32 ? kSlots32 : kSlots16; }
+// One workgroup a CU; with two (bf16, T = 1333, 16 heads) the join costs what they gain.
+constexpr int kSlots = 256;
 
 struct FwdLayout { int splits; size_t ml, total; };
 FwdLayout fwd_layout(int B, int Tq, int Tk, int H, int dn, int n_seqs, int dtype) {
   FwdLayout L{};
-  L.splits = splits_of(Tq, Tk, B, H, n_seqs, q_slots(dtype));
+  L.splits = splits_of(Tq, Tk, B, H, n_seqs, kSlots);
   const size_t rows = L.splits > 1 ? static_cast<size_t>(L.splits) * B * H * Tq : 0;
   L.ml = align_up(rows * dn * 4);
   L.total = L.ml + align_up(rows * 8);
   return L;
 }
-struct BwdLayout { int splits, splits_k; size_t D, dmax, dkr, part, total; };
+struct BwdLayout { int splits, splits_k; int64_t blocks; size_t D, dmax, dkr, part, part_k, total; };
 BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dn, int dr, int n_seqs, int dtype) {
   BwdLayout L{};
   const size_t bh = static_cast<size_t>(B) * H;
-  L.splits = splits_of(Tq, Tk, B, H, n_seqs, q_slots(dtype));
-  L.splits_k = splits_of(Tk, Tq, B, H, n_seqs, kSlotsKeys);
+  L.splits = splits_of(Tq, Tk, B, H, n_seqs, kSlots);
+  L.splits_k = splits_of(Tk, Tq, B, H, n_seqs, kSlots);
   L.D = 0;
   L.dmax = align_up(bh * Tq * 4);
-  L.dkr = L.dmax + align_up(bh * ((Tq + 127) / 128) * 4);
+  L.blocks = blocks_of(Tq, n_seqs);
+  L.dkr = L.dmax + align_up(bh * L.blocks * 4);
   L.part = L.dkr + align_up(L.splits_k * bh * Tk * dr * 4);
-  const size_t pq = L.splits > 1 ? L.splits * bh * Tq * (dn + dr) * 4 : 0;        // used in turn
-  const size_t pk = L.splits_k > 1 ? L.splits_k * bh * Tk * 2 * dn * 4 : 0;
-  L.total = L.part + align_up(pq > pk ? pq : pk) + 256;
+  L.part_k = L.part + align_up(L.splits > 1 ? L.splits * bh * Tq * (dn + dr) * 4 : 0);
+  L.total = L.part_k + align_up(L.splits_k > 1 ? L.splits_k * bh * Tk * 2 * dn * 4 : 0) + 256;
   return L;
 }
 
@@ -196,9 +197,10 @@ int kda_latent_attn_bwd(hipStream_t stream, const void* q, const void* kv, const
   a.o_in = o; a.lse_in = lse; a.dout = d_o;
   a.D = reinterpret_cast<float*>(ws + L.D);
   a.dmax = reinterpret_cast<float*>(ws + L.dmax);
-  a.dmax_n = (Tq + 127) / 128;
+  a.dmax_n = static_cast<int>(L.blocks);
   a.dkr_part = reinterpret_cast<float*>(ws + L.dkr);
   a.part = reinterpret_cast<float*>(ws + L.part);
+  a.part_k = reinterpret_cast<float*>(ws + L.part_k);
   a.splits = L.splits;
   a.splits_k = L.splits_k;
   a.dq = dq; a.dkv = dkv; a.dkr = dk_rope;

@@ -5,18 +5,18 @@
 //   dq_i = scale sum_j g_ij k_j,  dk_j = scale sum_i g_ij q_i,  dv_j = sum_i p_ij do_i,
 // the rotary key's gradient summed over the heads.
 //
-// Three launches and one more for the sum over heads, no atomics, so a gradient
-// is the same bits in every run: the row pass (D, and for fp16 the largest
-// |do|), the query pass (a workgroup owns 128 queries and walks the keys; dq),
-// the key pass (a workgroup owns 128 keys and walks the queries; dk, dv, the
-// head's share of the rotary key's gradient in fp32), then that share's sum in
-// head order.  Both passes form p and g again: seven products instead of five,
+// Three launches, no atomics, so a gradient is the same bits in every run: the
+// query pass (a workgroup owns 128 queries and walks the keys; D, dq), the key
+// pass (a workgroup owns 128 keys and walks the queries; dk, dv, the head's share
+// of the rotary key's gradient in fp32), then the sums in fixed order: that
+// share's over the heads, and the parts of blocks that were shared out.  Both passes form p and g again: seven products instead of five,
 // against an fp32 dq kept in memory and added to by every key block.
 //
 // p and g are rounded to the inputs' type for the products they enter; sums
 // are fp32.  For fp16, whose smallest value is 6e-8, g is formed from do
-// scaled by a power of two that brings the head's largest |do| near 1, and the
-// sums are scaled back: p of a long row times a small do would vanish otherwise.
+// scaled by a power of two that brings the largest |do| (the query's, in the key
+// pass the head's) near 1, and the sums are scaled back: p of a long row times a
+// small do would vanish otherwise.
 
 #include "kda_internal.h"
 #include "kda_latent.h"
@@ -24,53 +24,18 @@
 namespace kda {
 namespace latent {
 
-// ---------------------------------------------------------------- row pass
-template <int DT, int DN>
-__global__ __launch_bounds__(256) void kda_latent_rows_kernel(LatentArgs a) {
-  constexpr int LPR = DN / 8;             // lanes of a row, eight elements each
-  constexpr int RPP = 256 / LPR;          // rows at a time
-  __shared__ float red[4];
-  const int bh = blockIdx.y, b = bh / a.H, head = bh - b * a.H;
-  const int e0 = (threadIdx.x % LPR) * 8;
-  float top = 0.f;
-#pragma unroll 2
-  for (int r = threadIdx.x / LPR; r < 128; r += RPP) {
-    const int row = blockIdx.x * 128 + r;
-    if (row >= a.Tq) break;
-    const int64_t i = ((static_cast<int64_t>(b) * a.Tq + row) * a.H + head) * DN + e0;
-    float d = 0.f;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const f4 x = ld4<DT>(a.dout, i + 4 * t), y = ld4<DT>(a.o_in, i + 4 * t);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        d = fmaf(x[e], y[e], d);
-        if constexpr (DT == 2) top = fmaxf(top, fabsf(x[e]));
-      }
-    }
-#pragma unroll
-    for (int s = 1; s < LPR; s <<= 1) d += __shfl_xor(d, s, 64);
-    if (e0 == 0) a.D[static_cast<int64_t>(bh) * a.Tq + row] = d;
-  }
-  if constexpr (DT == 2) {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-    __syncthreads();
-    if (threadIdx.x == 0)
-      a.dmax[static_cast<int64_t>(bh) * a.dmax_n + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  }
+// fp16: the power of two that brings t, the largest |do|, into [1, 2); 1 where
+// there is none (zeros, or a value that is not finite)
+__device__ __forceinline__ float to_one(float t) {
+  if (!(t > 0.f) || t > 65504.f) return 1.f;
+  return __uint_as_float((254u << 23) - (__float_as_uint(t) & 0x7F800000u));
 }
-
-// fp16: the power of two that brings the head's largest |do| into [1, 2);
-// 1 where there is none (zeros, or a value that is not finite)
 __device__ __forceinline__ float do_factor(const LatentArgs& a, int bh) {
   float t = 0.f;
   for (int i = __lane_id(); i < a.dmax_n; i += 64) t = fmaxf(t, a.dmax[static_cast<int64_t>(bh) * a.dmax_n + i]);
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) t = fmaxf(t, __shfl_xor(t, s, 64));
-  if (!(t > 0.f) || t > 65504.f) return 1.f;
-  return __uint_as_float((254u << 23) - (__float_as_uint(t) & 0x7F800000u));
+  return to_one(t);
 }
 
 template <int DT, int DN, int DR>
@@ -99,7 +64,10 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 31, h = lane >> 5;
   Where w;
-  if (!locate(a, nqb, C::BM, true, true, w)) return;
+  if (!locate(a, blockIdx.x, nqb, C::BM, true, true, w)) {
+    if (DT == 2 && blockIdx.y == 0 && threadIdx.x == 0) a.dmax[static_cast<int64_t>(w.bh) * nqb + w.blk] = 0.f;
+    return;
+  }
   const int nk = w.ke - w.k0;
   const int row = w.r0 + wave * 32 + m;
   const bool live = row < w.re;
@@ -110,7 +78,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   const int blk_hi = a.causal ? min(nk - 1, min(w.r0 + C::BM - 1, w.re - 1) + w.off) : nk - 1;
   const Share part(max(0, (blk_hi + BN) / BN), a.splits, blockIdx.y);
   const int nt = part.j1;
-  if (static_cast<int>(blockIdx.y) >= part.parts) return;
+  if (static_cast<int>(blockIdx.y) >= part.parts) return;   // never share 0, which also leaves D
 
   F qn[KN], qr[KR], dO[KN];
   {
@@ -125,8 +93,39 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
     for (int s = 0; s < KR; ++s) qr[s] = *reinterpret_cast<const F*>(qp + DN + 16 * s + 8 * h);
   }
   const int64_t ri = static_cast<int64_t>(w.bh) * a.Tq + crow;
-  const float lse2 = a.lse_in[ri] * kLog2e, D = a.D[ri];
-  const float gf = DT == 2 ? do_factor(a, w.bh) : 1.f;
+  const float lse2 = a.lse_in[ri] * kLog2e;
+  // D of this lane's query, for the key pass too, and the factor of its g
+  float D = 0.f, gf = 1.f;
+  {
+    const E* op = static_cast<const E*>(a.o_in) + ((static_cast<int64_t>(w.b) * a.Tq + crow) * a.H + w.head) * DN;
+    float top = 0.f;
+#pragma unroll
+    for (int s = 0; s < KN; ++s) {
+      const F o = *reinterpret_cast<const F*>(op + 16 * s + 8 * h);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        D = fmaf(static_cast<float>(dO[s][e]), static_cast<float>(o[e]), D);
+        if constexpr (DT == 2) top = fmaxf(top, fabsf(static_cast<float>(dO[s][e])));
+      }
+    }
+    D = half_sum(D);
+    if constexpr (DT == 2) {
+      top = half_max(top);
+      gf = to_one(top);
+    }
+    if (blockIdx.y == 0) {
+      if (live && h == 0) a.D[ri] = D;
+      if constexpr (DT == 2) {
+        __shared__ float tops[4];
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+        if (lane == 0) tops[wave] = top;
+        lds_barrier();
+        if (threadIdx.x == 0)
+          a.dmax[static_cast<int64_t>(w.bh) * nqb + w.blk] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      }
+    }
+  }
 
   const char* kvp = static_cast<const char*>(a.kv) + (w.b * a.kv_b + w.k0 * a.kv_t + w.head * a.kv_h) * ES;
   const char* krp = static_cast<const char*>(a.kr) + (w.b * a.kr_b + w.k0 * a.kr_t) * ES;
@@ -272,7 +271,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 31, h = lane >> 5, own = wave & 3, role = wave >> 2;
   Where w;
-  if (!locate(a, nkb, C::BM, false, false, w)) return;
+  if (!locate(a, blockIdx.x, nkb, C::BM, false, false, w)) return;
   const int nq = w.ke - w.k0;                   // queries of the sequence
   const int key = w.r0 + own * 32 + m;          // this lane's key (packed axis)
   const bool live = key < w.re;
@@ -374,7 +373,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   const bool parted = part.parts > 1;
   const int64_t prow = (static_cast<int64_t>(blockIdx.y) * a.B * a.H + w.bh) * a.Tk + key;
   auto put4 = [&](int col, float x, float y, float z, float u) {
-    if (parted) store4<0>(a.part, prow * (2 * DN) + 4 * h + col, x, y, z, u);
+    if (parted) store4<0>(a.part_k, prow * (2 * DN) + 4 * h + col, x, y, z, u);
     else store4<DT>(a.dkv, ob + col, x, y, z, u);
   };
   auto put_dv = [&](const f16v (&dv)[ND]) {
@@ -583,53 +582,53 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   }
 }
 
-// ------------------------------------- the rotary key's gradient: sum over heads
-template <int DT>
-__global__ __launch_bounds__(256) void kda_latent_dkr_kernel(LatentArgs a, int64_t per_b) {
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;   // element of [Tk, dr]
-  if (i >= per_b) return;
-  const float* p = a.dkr_part + static_cast<int64_t>(blockIdx.y) * a.H * per_b + i;
-  f4 s = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int hd = 0; hd < a.H; ++hd) s += *reinterpret_cast<const f4*>(p + hd * per_b);
-  store4<DT>(a.dkr, blockIdx.y * per_b + i, s[0], s[1], s[2], s[3]);
-}
-
-// Adds the parts of split blocks in part order; a quarter of a block a
-// workgroup.  Q: dq's blocks, else dkv's and (in place, in part 0) the rotary key's.
-template <int DT, int DN, int DR, bool Q>
-__global__ __launch_bounds__(256) void kda_latent_bwd_join_kernel(LatentArgs a, int nb) {
+// ------------------------------------------------------------------- sums
+// A quarter of a block of one head a workgroup, key blocks first, then (when the
+// query pass was shared out) query blocks: the parts of blocks that were shared
+// out, in part order, and the rotary key's gradient over the heads and parts,
+// whose rows the workgroups of a block's heads divide among themselves.
+template <int DT, int DN, int DR>
+__global__ __launch_bounds__(256) void kda_latent_sums_kernel(LatentArgs a, int nkb, int nqb) {
   typedef BwdCfg<DT, DN, DR> C;
-  constexpr int WID = Q ? DN + DR : 2 * DN;
+  const int keys = nkb * a.B * a.H;
+  const bool q_side = static_cast<int>(blockIdx.x) >= keys;
   Where w;
-  if (!locate(a, nb, C::BM, Q, Q, w)) return;
+  if (!locate(a, q_side ? blockIdx.x - keys : blockIdx.x, q_side ? nqb : nkb, C::BM, q_side, false, w)) return;
   const int n_o = w.ke - w.k0;
   int tiles;
-  if (Q) {
+  if (q_side) {
     const int hi = a.causal ? min(n_o - 1, min(w.r0 + C::BM - 1, w.re - 1) + w.off) : n_o - 1;
     tiles = max(0, (hi + C::BN) / C::BN);
   } else {
     tiles = max(0, (n_o + C::BN - 1) / C::BN - (a.causal ? max(0, w.r0 + w.off) : 0) / C::BN);
   }
-  const int parts = Share(tiles, Q ? a.splits : a.splits_k, 0).parts;
-  if (parts == 1) return;
-  const int T = Q ? a.Tq : a.Tk, ra = w.r0 + blockIdx.y * 32, n = min(32, w.re - ra);
+  const int parts = Share(tiles, q_side ? a.splits : a.splits_k, 0).parts;
+  const int T = q_side ? a.Tq : a.Tk, ra = w.r0 + blockIdx.y * 32, n = min(32, w.re - ra), WID4 = (q_side ? DN + DR : 2 * DN) / 4;
   const int64_t step = static_cast<int64_t>(a.B) * a.H * T, row0 = static_cast<int64_t>(w.bh) * T + ra;
+  if (parts > 1) {
+    const float* src = q_side ? a.part : a.part_k;
 #pragma unroll 2
-  for (int i = threadIdx.x; i < n * (WID / 4); i += 256) {
-    const int r = i / (WID / 4), col = i % (WID / 4) * 4;
-    f4 s = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int z = 0; z < parts; ++z) s += *reinterpret_cast<const f4*>(a.part + (z * step + row0 + r) * WID + col);
-    store4<DT>(Q ? a.dq : a.dkv, ((static_cast<int64_t>(w.b) * T + ra + r) * a.H + w.head) * WID + col, s[0], s[1], s[2], s[3]);
-  }
-  if constexpr (!Q)
-    for (int i = threadIdx.x; i < n * (DR / 4); i += 256) {
-      float* p = a.dkr_part + row0 * DR + i * 4;
+    for (int i = threadIdx.x; i < n * WID4; i += 256) {
+      const int r = i / WID4, col = i % WID4 * 4;
       f4 s = {0, 0, 0, 0};
-      for (int z = 0; z < parts; ++z) s += *reinterpret_cast<const f4*>(p + z * step * DR);
-      *reinterpret_cast<f4*>(p) = s;
+#pragma unroll 4
+      for (int z = 0; z < parts; ++z) s += *reinterpret_cast<const f4*>(src + (z * step + row0 + r) * (WID4 * 4) + col);
+      store4<DT>(q_side ? a.dq : a.dkv, ((static_cast<int64_t>(w.b) * T + ra + r) * a.H + w.head) * (WID4 * 4) + col, s[0], s[1],
+                 s[2], s[3]);
     }
+  }
+  if (q_side) return;
+  // rows ra + head, ra + head + H, ..
+  const int mine = n > w.head ? (n - w.head + a.H - 1) / a.H : 0;
+  for (int i = threadIdx.x; i < mine * (DR / 4); i += 256) {
+    const int row = ra + w.head + i / (DR / 4) * a.H, col = i % (DR / 4) * 4;
+    const float* p = a.dkr_part + (static_cast<int64_t>(w.b) * a.H * T + row) * DR + col;
+    f4 s = {0, 0, 0, 0};
+    for (int z = 0; z < parts; ++z)
+#pragma unroll 8
+      for (int hd = 0; hd < a.H; ++hd) s += *reinterpret_cast<const f4*>(p + (z * step + static_cast<int64_t>(hd) * T) * DR);
+    store4<DT>(a.dkr, (static_cast<int64_t>(w.b) * T + row) * DR + col, s[0], s[1], s[2], s[3]);
+  }
 }
 
 template <int DT, int DN, int DR>
@@ -639,19 +638,15 @@ hipError_t run_bwd(const LatentArgs& a, hipStream_t s) {
   const int64_t nqb = a.cu_q ? static_cast<int64_t>(a.Tq) / BM + a.n_seqs : (static_cast<int64_t>(a.Tq) + BM - 1) / BM;
   const int64_t nkb = a.cu_q ? static_cast<int64_t>(a.Tk) / BM + a.n_seqs : (static_cast<int64_t>(a.Tk) + BM - 1) / BM;
   if (bh <= 0) return hipSuccess;
-  if (a.Tq > 0) {
-    kda_latent_rows_kernel<DT, DN><<<dim3((a.Tq + 127) / 128, bh), dim3(256), 0, s>>>(a);
-    const unsigned gx = static_cast<unsigned>(nqb * bh);
-    kda_latent_dq_kernel<DT, DN, DR><<<dim3(gx, a.splits), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
-    if (a.splits > 1) kda_latent_bwd_join_kernel<DT, DN, DR, true><<<dim3(gx, 4), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
-  }
-  if (a.Tk > 0) {
-    const unsigned gx = static_cast<unsigned>(nkb * bh);
-    kda_latent_dkv_kernel<DT, DN, DR><<<dim3(gx, a.splits_k), dim3(KeyCfg<DT, DN, DR>::NT), 0, s>>>(a, static_cast<int>(nkb));
-    if (a.splits_k > 1) kda_latent_bwd_join_kernel<DT, DN, DR, false><<<dim3(gx, 4), dim3(256), 0, s>>>(a, static_cast<int>(nkb));
-    const int64_t per_b = static_cast<int64_t>(a.Tk) * DR;
-    kda_latent_dkr_kernel<DT><<<dim3(static_cast<unsigned>((per_b + 1023) / 1024), a.B), dim3(256), 0, s>>>(a, per_b);
-  }
+  if (a.Tq > 0)
+    kda_latent_dq_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(nqb * bh), a.splits), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
+  if (a.Tk > 0)
+    kda_latent_dkv_kernel<DT, DN, DR>
+        <<<dim3(static_cast<unsigned>(nkb * bh), a.splits_k), dim3(KeyCfg<DT, DN, DR>::NT), 0, s>>>(a, static_cast<int>(nkb));
+  const int64_t blocks = (nkb + (a.splits > 1 ? nqb : 0)) * bh;
+  if (blocks > 0)
+    kda_latent_sums_kernel<DT, DN, DR>
+        <<<dim3(static_cast<unsigned>(blocks), 4), dim3(256), 0, s>>>(a, static_cast<int>(nkb), static_cast<int>(nqb));
   return hipGetLastError();
 }
 

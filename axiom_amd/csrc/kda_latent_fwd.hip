@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
   const int m = lane & 31, h = lane >> 5;
 
   Where w;
-  if (!locate(a, nqb, C::BM, true, true, w)) return;
+  if (!locate(a, blockIdx.x, nqb, C::BM, true, true, w)) return;
   const int b = w.b, head = w.head, q0 = w.r0, qe = w.re, off = w.off, nk = w.ke - w.k0;
   const int row = q0 + wave * 32 + m;         // this lane's query
   const bool live = row < qe;
@@ -195,21 +195,21 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
   if (h == 0) a.lse[static_cast<int64_t>(w.bh) * a.Tq + row] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * kLn2;
 }
 
-// Joins the parts of split blocks, in part order; a quarter of a block a workgroup.
+// Joins the parts of split blocks, in part order; an eighth of a block a workgroup.
 template <int DT, int DN, int DR>
 __global__ __launch_bounds__(256) void kda_latent_fwd_join_kernel(LatentArgs a, int nqb) {
   typedef FwdCfg<DT, DN, DR> C;
   constexpr int LPR = DN / 4, RPP = 256 / LPR;
   Where w;
-  if (!locate(a, nqb, C::BM, true, true, w)) return;
+  if (!locate(a, blockIdx.x, nqb, C::BM, true, true, w)) return;
   const int nk = w.ke - w.k0, blk_hi = a.causal ? min(nk - 1, min(w.r0 + C::BM - 1, w.re - 1) + w.off) : nk - 1;
   const int parts = Share(max(0, (blk_hi + C::BN) / C::BN), a.splits, 0).parts;
   if (parts == 1) return;
   const int col = (threadIdx.x % LPR) * 4;
   const int64_t step = static_cast<int64_t>(a.B) * a.H * a.Tq;
 #pragma unroll 2
-  for (int r = threadIdx.x / LPR; r < 32; r += RPP) {
-    const int row = w.r0 + blockIdx.y * 32 + r;
+  for (int r = threadIdx.x / LPR; r < 16; r += RPP) {
+    const int row = w.r0 + blockIdx.y * 16 + r;
     if (row >= w.re) break;
     const int64_t pr = static_cast<int64_t>(w.bh) * a.Tq + row;
     float mx = kMaxInit, l = 0.f;
@@ -238,7 +238,7 @@ hipError_t run_fwd(const LatentArgs& a, hipStream_t s) {
   if (grid <= 0) return hipSuccess;
   const unsigned gx = static_cast<unsigned>(grid);
   kda_latent_fwd_kernel<DT, DN, DR><<<dim3(gx, a.splits), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
-  if (a.splits > 1) kda_latent_fwd_join_kernel<DT, DN, DR><<<dim3(gx, 4), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
+  if (a.splits > 1) kda_latent_fwd_join_kernel<DT, DN, DR><<<dim3(gx, 8), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
   return hipGetLastError();
 }
 

@@ -189,11 +189,13 @@ std::tuple<Tensor, Tensor, Tensor> attn_bwd(const Tensor& q, const Tensor& kv, c
 }
 
 struct LatentAttn : torch::autograd::Function<LatentAttn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& kv, const Tensor& kr, const Tensor& cu_q, const Tensor& cu_k,
-                        bool causal, double scale) {
-    const OptTensor cq = cu_q.defined() ? OptTensor(cu_q) : std::nullopt, ck = cu_k.defined() ? OptTensor(cu_k) : std::nullopt;
-    const auto [o, lse] = attn_fwd(q, kv, kr, cq, ck, causal, scale, std::nullopt, std::nullopt, std::nullopt);
-    ctx->save_for_backward({q, kv, kr, o, lse, cu_q, cu_k});
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& kv, const Tensor& kr, const OptTensor& cu_q,
+                        const OptTensor& cu_k, bool causal, double scale) {
+    const auto [o, lse] = attn_fwd(q, kv, kr, cu_q, cu_k, causal, scale, std::nullopt, std::nullopt, std::nullopt);
+    variable_list kept = {q, kv, kr, o, lse};
+    if (cu_q) kept.push_back(*cu_q);
+    if (cu_k) kept.push_back(*cu_k);
+    ctx->save_for_backward(std::move(kept));
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     return o;
@@ -202,8 +204,8 @@ struct LatentAttn : torch::autograd::Function<LatentAttn> {
     variable_list out(7);
     if (!grads[0].defined()) return out;
     const variable_list s = ctx->get_saved_variables();
-    const OptTensor cq = s[5].defined() ? OptTensor(s[5]) : std::nullopt, ck = s[6].defined() ? OptTensor(s[6]) : std::nullopt;
-    std::tie(out[0], out[1], out[2]) = attn_bwd(s[0], s[1], s[2], s[3], s[4], grads[0].contiguous(), cq, ck,
+    const OptTensor cu_q = s.size() > 5 ? OptTensor(s[5]) : std::nullopt, cu_k = s.size() > 6 ? OptTensor(s[6]) : std::nullopt;
+    std::tie(out[0], out[1], out[2]) = attn_bwd(s[0], s[1], s[2], s[3], s[4], grads[0].contiguous(), cu_q, cu_k,
                                                 ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), std::nullopt);
     return out;
   }
@@ -212,7 +214,7 @@ struct LatentAttn : torch::autograd::Function<LatentAttn> {
 Tensor attn(const Tensor& q, const Tensor& kv, const Tensor& kr, const OptTensor& cu_q, const OptTensor& cu_k, bool causal,
             std::optional<double> scale) {
   const Attn a = attn_check("latent_attn", q, kv, kr, cu_q, cu_k, scale);
-  return LatentAttn::apply(q, kv, kr, cu_q ? *cu_q : Tensor(), cu_k ? *cu_k : Tensor(), causal, a.scale);
+  return LatentAttn::apply(q, kv, kr, cu_q, cu_k, causal, a.scale);
 }
 
 OptTensor append(const Tensor& rows, const Tensor& positions, const Tensor& slots, const Tensor& cos_sin, Tensor cache,

@@ -78,13 +78,13 @@ def _splits(T, other, B, H, n, slots):
                                                (1, 700, 700, 2, 64, 32, 9), (1, 0, 50, 2, 64, 32, 0), (1, 50, 0, 2, 64, 32, 0)])
 @pytest.mark.parametrize("code", [0, 1, 2])
 def test_attention_workspaces(L, B, Tq, Tk, H, dn, dr, n, code):
-    s = _splits(Tq, Tk, B, H, n, 256 if code == 0 else 512)
+    s = _splits(Tq, Tk, B, H, n, 256)
     rows = s * B * H * Tq if s > 1 else 0
     assert L.kda_latent_attn_fwd_workspace(B, Tq, Tk, H, dn, dr, n, code) == _up(rows * dn * 4) + _up(rows * 8)
-    # D, the blocks' largest |do|, each head's (and part's) share of the rotary key's gradient, the parts of dq, then of dkv
+    # D, the blocks' largest |do|, each head's (and part's) share of the rotary key's gradient, the parts of dq and of dkv
     k = _splits(Tk, Tq, B, H, n, 256)
-    want = _up(B * H * Tq * 4) + _up(B * H * -(-Tq // 128) * 4) + _up(k * B * H * Tk * dr * 4)
-    want += _up(max(rows * (dn + dr) * 4, k * B * H * Tk * 2 * dn * 4 if k > 1 else 0)) + 256
+    want = _up(B * H * Tq * 4) + _up(B * H * (Tq // 128 + n if n else -(-Tq // 128)) * 4) + _up(k * B * H * Tk * dr * 4)
+    want += _up(rows * (dn + dr) * 4) + _up(k * B * H * Tk * 2 * dn * 4 if k > 1 else 0) + 256
     assert L.kda_latent_attn_bwd_workspace(B, Tq, Tk, H, dn, dr, n, code) == want
 
 
