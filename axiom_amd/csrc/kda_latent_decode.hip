@@ -195,9 +195,15 @@ __device__ __forceinline__ Run find_run(const LatentDecodeArgs& a, int w, int KT
     r.g1 = (r.len + KT - 1) / KT;
     return r;
   }
-  int n = lane < a.B ? seq_len(a, lane) : 0, nt = places(a, n, KT), sum = nt;
-  for (int i = lane + 64; i < a.B; i += 64) sum += places(a, seq_len(a, i), KT);
-  const int total = wave_sum(sum), per = max(a.least, (total + a.wgs - 1) / a.wgs);
+  int n = lane < a.B ? seq_len(a, lane) : 0, nt = places(a, n, KT);
+  const int first = wave_scan(nt);           // of the first 64 sequences
+  int total = __builtin_amdgcn_readlane(first, 63);
+  if (a.B > 64) {
+    int sum = 0;
+    for (int i = lane + 64; i < a.B; i += 64) sum += places(a, seq_len(a, i), KT);
+    total += wave_sum(sum);
+  }
+  const int per = max(a.least, (total + a.wgs - 1) / a.wgs);
   r.g = w * per;
   r.g1 = min(total, r.g + per);
   const bool tell = blockIdx.x == 0 && threadIdx.x < 64;   // the join kernel's starts of the sequences
@@ -209,7 +215,7 @@ __device__ __forceinline__ Run find_run(const LatentDecodeArgs& a, int w, int KT
       n = s0 + lane < a.B ? seq_len(a, s0 + lane) : 0;
       nt = places(a, n, KT);
     }
-    const int inc = wave_scan(nt);
+    const int inc = s0 > 0 ? wave_scan(nt) : first;
     if (tell && s0 + lane < a.B) a.line[1 + s0 + lane] = base + inc - nt;
     const unsigned long long hit = __ballot(base + inc > r.g);
     if (hit && !found) {
@@ -329,14 +335,29 @@ __global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decod
       wait_vmem_all();
       const int ln = fresh(lane), fm = ln & 15, fg = ln >> 4;
       f4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};     // two chains
+      // fragments in batches, the next batch's reads ahead of this one's products
+      constexpr int BT = ES == 2 ? 3 : 1;
+      F kf[2][BT];
+      auto read = [&](int k0, F (&dst)[BT]) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const F kf = k < KSN ? row_frag16<typename C::TN, F>(mine, fm, k, fg)
-                             : row_frag16<typename C::TR, F>(mine + C::OFF_R, fm, k - KSN, fg);
-        if (k & 1) s1 = mma_s(s1, kf, q[k]);
-        else s0 = mma_s(s0, kf, q[k]);
+        for (int x = 0; x < BT; ++x)
+          if (k0 + x < KS)
+            dst[x] = k0 + x < KSN ? row_frag16<typename C::TN, F>(mine, fm, k0 + x, fg)
+                                  : row_frag16<typename C::TR, F>(mine + C::OFF_R, fm, k0 + x - KSN, fg);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      read(0, kf[0]);
+#pragma unroll
+      for (int k = 0; k < KS; k += BT) {
+        if (k + BT < KS) read(k + BT, kf[(k / BT + 1) & 1]);
+#pragma unroll
+        for (int x = 0; x < BT; ++x)
+          if (k + x < KS) {
+            if ((k + x) & 1) s1 = mma_s(s1, kf[(k / BT) & 1][x], q[k + x]);
+            else s0 = mma_s(s0, kf[(k / BT) & 1][x], q[k + x]);
+          }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (ES == 2) pace<KS, 8, 1, 1>();
       const int key0 = j * KT + 4 * gq;
       f4 s = s0 + s1;
 #pragma unroll
@@ -357,9 +378,11 @@ __global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decod
         l += e[i];
       }
       const auto p = to_p4<DT>(e);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int v = 0; v < NV; ++v) acc[v] = mma_p(acc[v], v_frag<DT, typename C::TN>(mine, 16 * v, ln), p);
       if constexpr (ES == 2) pace<NV, 8, 1, 1>();
+      __builtin_amdgcn_sched_barrier(0);
       if (j + NW < tb) {
         lds_reads_done();                    // the buffer is read out
         fetch(slot_of(a, page, token(j + NW)));
@@ -369,21 +392,22 @@ __global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decod
 
     // the waves' sums: scaled to the common maximum, added in wave order by the wave that
     // owns a share of the columns, as many columns at a time as the buffers hold
+    const int el = fresh(lane), em = el & 15, eg = el >> 4, er = grp * 16 + em;   // formed here: the loop needs the registers
     l = group_sum(l);
-    if (gq == 0) {
-      red_m[wave][m] = mc;
-      red_l[wave][m] = l;
+    if (eg == 0) {
+      red_m[wave][em] = mc;
+      red_l[wave][em] = l;
     }
     lds_barrier();                           // also: every wave has left its buffer
     const bool whole = ta == 0 && tb == n_all;
-    float mt = red_m[0][m], ls = 0.f;
+    float mt = red_m[0][em], ls = 0.f;
 #pragma unroll
-    for (int x = 1; x < NW; ++x) mt = fmaxf(mt, red_m[x][m]);
+    for (int x = 1; x < NW; ++x) mt = fmaxf(mt, red_m[x][em]);
 #pragma unroll
-    for (int x = 0; x < NW; ++x) ls = fmaf(fast_exp2(red_m[x][m] - mt), red_l[x][m], ls);
+    for (int x = 0; x < NW; ++x) ls = fmaf(fast_exp2(red_m[x][em] - mt), red_l[x][em], ls);
     const float f = fast_exp2(mc - mt);
-    const int64_t row = static_cast<int64_t>(b) * rows + r;
-    const int64_t sr = (static_cast<int64_t>(2 * w + (ta > 0 ? 0 : 1)) * a.groups + grp) * 16 + m;
+    const int64_t row = static_cast<int64_t>(b) * rows + er;
+    const int64_t sr = (static_cast<int64_t>(2 * w + (ta > 0 ? 0 : 1)) * a.groups + grp) * 16 + em;
     const float inv = whole ? (ls > 0.f ? 1.f / ls : ls) : 1.f;   // nothing visible: zeros; NaN stays NaN
     constexpr int VR = C::NVR < NV ? (C::NVR >= NV / 2 ? NV / 2 : NV / 4) : NV;   // column blocks of a round
     static_assert(VR % NW == 0 && NV % VR == 0 && VR * NW * 1024 <= NW * C::WBUF, "rounds of columns");
@@ -392,23 +416,23 @@ __global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decod
       if (v0 > 0) lds_barrier();             // the round before has been read
 #pragma unroll
       for (int v = 0; v < VR; ++v)
-        *reinterpret_cast<f4*>(buf + (wave * VR + v) * 1024 + lane * 16) = acc[v0 + v] * f;
+        *reinterpret_cast<f4*>(buf + (wave * VR + v) * 1024 + el * 16) = acc[v0 + v] * f;
       lds_barrier();
 #pragma unroll
       for (int v = 0; v < VR / NW; ++v) {
         const int vb = wave * (VR / NW) + v;
         f4 o = {0, 0, 0, 0};
 #pragma unroll
-        for (int x = 0; x < NW; ++x) o += *reinterpret_cast<const f4*>(buf + (x * VR + vb) * 1024 + lane * 16);
+        for (int x = 0; x < NW; ++x) o += *reinterpret_cast<const f4*>(buf + (x * VR + vb) * 1024 + el * 16);
         o *= inv;
-        const int col = 16 * (v0 + vb) + 4 * gq;
-        if (r < rows) {
+        const int col = 16 * (v0 + vb) + 4 * eg;
+        if (er < rows) {
           if (whole) store4<DT>(a.o, row * R + col, o[0], o[1], o[2], o[3]);
           else *reinterpret_cast<f4*>(a.part_o + sr * R + col) = o;
         }
       }
     }
-    if (wave == 0 && gq == 0 && r < rows) {
+    if (wave == 0 && eg == 0 && er < rows) {
       if (whole) {
         a.lse[row] = ls == 0.f ? -INFINITY : (mt + __log2f(ls)) * kLn2;
       } else {
