@@ -163,6 +163,22 @@ __device__ __forceinline__ float group_sum(float x) {
 __device__ __forceinline__ void copy16(const char* src, char* dst) { __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0); }
 __device__ __forceinline__ void copy4(const void* src, char* dst) { __builtin_amdgcn_global_load_lds(src, dst, 4, 0, 0); }
 
+// The 16-byte copy as an instruction the compiler does not see as a memory access:
+// base + off (a lane's) to 1 KiB of LDS from byte address lds on.  The compiler
+// makes an LDS read wait for every copy it knows of unless it can tell their
+// arrays apart; code with a ring of buffers, indexed while it runs, copies with
+// this, waits with wait_vmem_but / wait_vmem_all and a barrier, and has no vector
+// loads of its own meanwhile (the compiler's wait for one would cover the copies).
+__device__ __forceinline__ void copy16_untracked(const char* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void copy16_untracked(const char* src, unsigned lds) {   // a lane's own address
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+
 // An LDS tile of rows of W elements of ES bytes.
 template <int W, int ES>
 struct Tile {

@@ -123,13 +123,14 @@ BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dn, int dr, int n_seqs, i
 // of each wave, or two of 32 keys).  Sequences whose table holds at most
 // kWholeTokens tokens get a workgroup each instead and no join launch.
 constexpr int kCUs = 256;
-constexpr int kWholeTokens = 256;
-struct DecodePlan { int rows, groups, wgs, whole, least; size_t part_ml, part_o, total; };
+constexpr int kWholeTokens = 128;
+struct DecodePlan { int rows, groups, wgs, whole, least, pad; size_t part_ml, part_o, total; };
 bool decode_plan(int B, int Tq, int H, int R, int page_size, int max_pages, int dtype, DecodePlan* P) {
   const int64_t rows = static_cast<int64_t>(Tq) * H, cap = static_cast<int64_t>(page_size) * max_pages;
   P->rows = rows <= 16 || dtype == KDA_DTYPE_F32 ? 16 : 64;
-  P->least = P->rows == 64 ? 2 : dtype == KDA_DTYPE_F32 ? 4 : 8;
-  const int64_t kt = kda::latent_decode_tile(P->rows), tiles = ((cap + kt - 1) / kt + 2 * P->least) * B;
+  P->least = 2;
+  P->pad = P->rows == 64 ? 4 : 8;
+  const int64_t kt = kda::latent_decode_tile(P->rows), tiles = ((cap + kt - 1) / kt + P->pad) * B;
   if (rows > (1 << 20) || cap >= (int64_t{1} << 31) || tiles >= (int64_t{1} << 30)) return false;
   P->groups = static_cast<int>((rows + P->rows - 1) / P->rows);
   P->whole = cap <= kWholeTokens;
@@ -272,7 +273,7 @@ int kda_latent_decode(hipStream_t stream, const void* q, const void* cache, cons
   a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + P.part_o);
   a.B = B; a.Tq = Tq; a.H = H; a.per = max_pages; a.n_pages = n_pages;
   for (a.page_shift = 0; (1 << a.page_shift) < page_size;) ++a.page_shift;
-  a.groups = P.groups; a.wgs = P.wgs; a.whole = P.whole; a.least = P.least; a.pad = 2 * P.least; a.scale = scale;
+  a.groups = P.groups; a.wgs = P.wgs; a.whole = P.whole; a.least = P.least; a.pad = P.pad; a.scale = scale;
   return launched(kda::launch_latent_decode(a, R, dr, dtype, P.rows, stream), "kda_latent_decode");
 }
 

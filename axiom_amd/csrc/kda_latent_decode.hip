@@ -7,6 +7,8 @@
 #include "kda_internal.h"
 #include "kda_latent.h"
 
+#include <type_traits>
+
 namespace kda {
 namespace latent {
 
@@ -85,24 +87,28 @@ __global__ __launch_bounds__(256) void kda_latent_append_kernel(LatentAppendArgs
 // row sum for the join kernel.  A workgroup holds 16 or 64 query rows (row =
 // token * H + head) in registers; the cache is read once for them.
 //
-// Up to 16 rows: bound by the cache's bytes (30 flop a byte), so the waves work
-// alone, without a barrier in the loop: each takes every NW-th group of 16 keys
-// of the run through an LDS buffer of its own, and a SIMD's second wave computes
-// while the first waits for its copies (147 KB a CU in buffers).  S^T = K Q^T
-// (16x16x32) leaves a lane four keys of one query, which is the second operand of
-// O^T += V^T P^T (16x16x16) as it stands, V^T being the same rows read
-// transposed.  The waves' sums meet once a run, in LDS.
+// Up to 16 rows: bound by the cache's bytes (30 flop a byte), so everything else
+// stays out of the copies' way.  Four waves score and four add: a score wave
+// holds the queries and takes every fourth tile of 16 keys (S^T = K Q^T,
+// 16x16x32), an output wave a quarter of the R columns for all tiles (O^T += V^T
+// P^T, 16x16x16, V^T being the tile's rows read transposed; the lane that made
+// a probability is the lane that needs it).  Tiles pass through a ring of eight
+// LDS buffers (147 KB): three on their way, four being scored over four
+// intervals, one added; an interval is one barrier.  The one score wave that
+// finishes in an interval raises the running maximum, if its tile asks for it,
+// so the waves agree on it without an exchange, and nothing is left to merge.
+// fp32, with operands twice as large: two score waves and a ring of four.
 template <int DT, int R, int DR>
 struct DecCfg {
   static constexpr int ES = El<DT>::ES;
-  static constexpr int NW = ES == 2 ? 8 : 4;               // a buffer a wave fills the LDS (R = 512)
   static constexpr int KT = 16;                            // keys of a tile
+  static constexpr int SP = ES == 2 ? 4 : 2;               // score waves, and intervals that a tile is scored over
+  static constexpr int RING = ES == 2 ? 8 : 4, AHEAD = RING - SP - 1;
   typedef Tile<R, ES> TN;
   typedef Tile<DR, ES> TR;
   static constexpr int OFF_R = TN::bytes(16);
-  static constexpr int WBUF = OFF_R + TR::bytes(16);       // one wave's buffer
+  static constexpr int BUF = OFF_R + TR::bytes(16);
   static constexpr int PN = 16 * TN::CPR / 64, PR = 16 * TR::CPR / 64;   // its 1 KiB pieces
-  static constexpr int NVR = NW * WBUF / (NW * 1024);      // 16-column blocks of all waves' sums that the LDS holds
 };
 
 // Row fragment of the 16 x 16 x 32 product: lane m = l & 15, group gq = l >> 4;
@@ -133,19 +139,20 @@ __device__ __forceinline__ typename P4<DT>::t to_p4(const float (&p)[4]) {
 __device__ __forceinline__ f4 mma_p(f4 c, const f4& a, const f4& b) { return mma16(c, a, b); }
 __device__ __forceinline__ f4 mma_p(f4 c, const h4& a, const h4& b) { return mma16(c, a, b); }
 __device__ __forceinline__ f4 mma_p(f4 c, const s4v& a, const s4v& b) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
-// First operand of O^T += V^T P^T: column col0 + m of V, keys 4 gq + j.
+// First operand of O^T += V^T P^T: column base + col0 + m of V, keys 4 gq + j; base a
+// multiple of 64 (128 in fp32 rows past 256 columns), col0 a constant below it.
 template <int DT, class TL>
-__device__ __forceinline__ typename P4<DT>::t v_frag(const char* base, int col0, int lane) {
+__device__ __forceinline__ typename P4<DT>::t v_frag(const char* tile, int base, int col0, int lane) {
   const int i = lane & 15, gq = lane >> 4;
   if constexpr (DT == 0) {
     f4 v;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      v[j] = *reinterpret_cast<const float*>(base + TL::off(4 * gq + j, col0 >> 2, i >> 2) + 4 * (i & 3));
+      v[j] = *reinterpret_cast<const float*>(tile + TL::off(4 * gq + j, (base + col0) >> 2, i >> 2) + 4 * (i & 3));
     return v;
   } else {
     return __builtin_bit_cast(typename P4<DT>::t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_s4)(base + TL::off(4 * gq + (i >> 2), col0 >> 3, (i & 3) >> 1) + 8 * (i & 1))));
+        (lds_s4)(tile + TL::off(4 * gq + (i >> 2), (base + col0) >> 3, (i & 3) >> 1) + 8 * (i & 1))));
   }
 }
 
@@ -253,194 +260,245 @@ __device__ __forceinline__ void empty_rows(const LatentDecodeArgs& a, int b, int
   }
 }
 
-// page of token tok, inside the cache; row of a token from it
+// Page of this lane's key x of tile j (KT keys): where a page holds a tile or more
+// it is the same for all, read by the scalar unit (the table does not change
+// under the kernel; a vector load's wait would cover the copies).
+template <int KT>
+__device__ __forceinline__ int page_of_tile(const LatentDecodeArgs& a, const int32_t* table, int len, int j, int x) {
+  if ((1 << a.page_shift) >= KT) {
+    const auto* t = (const __attribute__((address_space(4))) int32_t*)table;
+    return t[__builtin_amdgcn_readfirstlane(min(j * KT, len - 1) >> a.page_shift)];
+  }
+  return fresh(table[min(j * KT + x, len - 1) >> a.page_shift]);   // waited for here, not where the branches meet
+}
+// page of token tok by a vector load
 __device__ __forceinline__ int page_of(const LatentDecodeArgs& a, const int32_t* table, int tok) {
   return table[tok >> a.page_shift];
 }
+// whether tile j begins a page (or holds several)
+__device__ __forceinline__ bool new_page(const LatentDecodeArgs& a, int j, int KT) {
+  return ((j * KT) & ((1 << a.page_shift) - 1)) == 0 || (1 << a.page_shift) < KT;
+}
+// cache row of token tok, its page clamped into the cache
 __device__ __forceinline__ int slot_of(const LatentDecodeArgs& a, int page, int tok) {
   return (min(max(page, 0), static_cast<int>(a.n_pages - 1)) << a.page_shift) + (tok & ((1 << a.page_shift) - 1));
 }
 
-// One 1 KiB piece (number s / 64 of a buffer's tile) of cache rows to LDS: the
-// part of the rows from byte `from` on that tile TL holds.  slot: the cache row
-// of key `lane`.  A piece inside one row has its row in scalar registers.
-template <class TL>
-__device__ __forceinline__ void copy_piece(const char* cache, int row_bytes, int from, int slot, int piece, int lane, char* dst) {
+// One 1 KiB piece of a tile's cache rows to LDS: the part of the rows from byte
+// `from` on that tile TL holds, TL's first byte at dst.  slot: the cache row of
+// key `lane`.  A piece inside one row has its row in scalar registers.  dst: an
+// array (the compiler's own copy) or, for copy16_untracked, its LDS address.
+__device__ __forceinline__ void put_piece(const char* src, unsigned off, char* dst) { copy16(src + off, dst); }
+__device__ __forceinline__ void put_piece(const char* src, unsigned off, unsigned dst) { copy16_untracked(src, off, dst); }
+__device__ __forceinline__ void put_piece(const char* src, char* dst) { copy16(src, dst); }
+__device__ __forceinline__ void put_piece(const char* src, unsigned dst) { copy16_untracked(src, dst); }
+template <class TL, class DST>
+__device__ __forceinline__ void copy_piece(const char* cache, int row_bytes, int from, int slot, int piece, int lane, DST dst) {
   if constexpr (TL::CPR % 64 == 0) {
     constexpr int PPR = TL::CPR / 64;      // pieces of a row
     const int r = piece / PPR;
     const char* src = cache + static_cast<int64_t>(__builtin_amdgcn_readlane(slot, r)) * row_bytes + (from + piece % PPR * 1024);
-    copy16(src + static_cast<unsigned>((lane ^ TL::swz(r)) << 4), dst + piece * 1024);
+    put_piece(src, static_cast<unsigned>((lane ^ TL::swz(r)) << 4), dst + piece * 1024);
   } else {
     const int r = piece * (64 / TL::CPR) + lane / TL::CPR;
-    const unsigned off = static_cast<unsigned>(from + (((lane % TL::CPR) ^ TL::swz(r)) << 4));
-    copy16(cache + static_cast<int64_t>(__shfl(slot, r, 64)) * row_bytes + off, dst + piece * 1024);
+    const char* src = cache + static_cast<int64_t>(__shfl(slot, r, 64)) * row_bytes + (from + (((lane % TL::CPR) ^ TL::swz(r)) << 4));
+    put_piece(src, dst + piece * 1024);
   }
 }
 
 template <int DT, int R, int DR>
-__global__ __launch_bounds__((64 * DecCfg<DT, R, DR>::NW)) void kda_latent_decode16_kernel(LatentDecodeArgs a) {
+__global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeArgs a) {
   typedef DecCfg<DT, R, DR> C;
   typedef typename El<DT>::frag F;
   typedef typename El<DT>::t E;
-  constexpr int ES = C::ES, NW = C::NW, KT = C::KT, W = R + DR, KS = W / 32, KSN = R / 32, NV = R / 16;
-  __shared__ __attribute__((aligned(1024))) char buf[NW * C::WBUF];
-  __shared__ float red_m[NW][16], red_l[NW][16];
+  typedef typename P4<DT>::t PV;
+  constexpr int ES = C::ES, KT = C::KT, SP = C::SP, RING = C::RING, AHEAD = C::AHEAD;
+  constexpr int W = R + DR, KS = W / 32, KSN = R / 32, NV = R / 64;
+  constexpr int KP = (KS + (SP > 2 ? SP - 2 : 1)) / (SP > 2 ? SP - 1 : 2);   // products of an interval; SP = 4 keeps the last for the softmax
+  constexpr int PW = (C::PN + C::PR) / 8;                       // pieces of a tile that every wave copies at least
+  __shared__ __attribute__((aligned(1024))) char buf[RING * C::BUF];
+  __shared__ __attribute__((aligned(16))) PV sp[2][64];         // a tile's probabilities, by tile parity
+  __shared__ float top[16], fac[2][16], red[2][SP][16];
+  __shared__ int rose[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, gq = lane >> 4;
+  const bool scoring = wave < 4;
   int w, grp;
   run_group(a, w, grp);
   Run run = find_run(a, w, KT).uniform();
-  const int rows = a.Tq * a.H, r = grp * 16 + m;
-  if (a.whole && run.g1 == 0) empty_rows<DT, R>(a, w, grp * 16, min(rows, grp * 16 + 16), 64 * NW);
+  const int rows = a.Tq * a.H, r = grp * 16 + m, cr = min(r, rows - 1);
+  if (a.whole && run.g1 == 0) empty_rows<DT, R>(a, w, grp * 16, min(rows, grp * 16 + 16), 512);
 
   const float c = a.scale * kLog2e, lazy = kLazy / c;
   const char* cache = static_cast<const char*>(a.cache);
-  char* const mine = buf + wave * C::WBUF;
+  const unsigned lds0 = lds_address(buf);
 
   while (run.g < run.g1) {
     const int b = run.b, len = run.len, n_all = (len + KT - 1) / KT;
     const int ta = run.t, tb = min(n_all, ta + (run.g1 - run.g));   // this segment's tiles
     if (ta < tb) {
     const int32_t* table = a.table + static_cast<int64_t>(b) * a.per;
-
-    auto token = [&](int j) { return min(j * KT + m, len - 1); };   // key m of tile j
-    auto fetch = [&](int slot) {
-      const int ln = fresh(lane) & 63;
+    auto page_at = [&](int j) { return page_of_tile<KT>(a, table, len, j, m); };
+    auto fetch = [&](int j, int page) {
+      const int slot = slot_of(a, page, min(j * KT + m, len - 1)), ln = fresh(lane) & 63;
+      const unsigned dst = lds0 + (j & (RING - 1)) * C::BUF;
 #pragma unroll
-      for (int p = 0; p < C::PN; ++p) copy_piece<typename C::TN>(cache, W * ES, 0, slot, p, ln, mine);
-#pragma unroll
-      for (int p = 0; p < C::PR; ++p) copy_piece<typename C::TR>(cache, W * ES, R * ES, slot, p, ln, mine + C::OFF_R);
+      for (int p = wave; p < C::PN + C::PR; p += 8) {
+        if (p < C::PN) copy_piece<typename C::TN>(cache, W * ES, 0, slot, p, ln, dst);
+        else copy_piece<typename C::TR>(cache, W * ES, R * ES, slot, p - C::PN, ln, dst + C::OFF_R);
+      }
     };
-
-    int page = page_of(a, table, token(ta + wave));   // of the next tile to copy
-    if (ta + wave < tb) {
-      fetch(slot_of(a, page, token(ta + wave)));
-      page = page_of(a, table, token(ta + wave + NW));
-    }
+    int pages[AHEAD + 1];
+#pragma unroll
+    for (int x = 0; x <= AHEAD; ++x) pages[x] = page_at(ta + x);
     F q[KS];
-    {
-      const E* qp = static_cast<const E*>(a.q) + (static_cast<int64_t>(b) * rows + min(r, rows - 1)) * W;
+    if (wave < SP) {
+      const E* qp = static_cast<const E*>(a.q) + (static_cast<int64_t>(b) * rows + cr) * W;
 #pragma unroll
       for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const F*>(qp + 32 * s + 8 * gq);
     }
-    const int seen = len - (a.Tq - 1 - min(r, rows - 1) / a.H);
+    if (threadIdx.x < 16) top[threadIdx.x] = kMaxInit;
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x)
+      if (ta + x < tb) fetch(ta + x, pages[x]);
+    int page = pages[AHEAD];                 // of the next tile to copy
+    wait_vmem_all();                         // the queries' wait, which covers the first copies, is this one and no later one
 
-    f4 acc[NV];
-    float mx = kMaxInit, mc = kMaxInit * c, l = 0.f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) acc[v] = f4{0, 0, 0, 0};
-
-    for (int j = ta + wave; j < tb; j += NW) {
-      wait_vmem_all();
-      const int ln = fresh(lane), fm = ln & 15, fg = ln >> 4;
-      f4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};     // two chains
-      // fragments in batches, the next batch's reads ahead of this one's products
-      constexpr int BT = ES == 2 ? 3 : 1;
-      F kf[2][BT];
-      auto read = [&](int k0, F (&dst)[BT]) {
-#pragma unroll
-        for (int x = 0; x < BT; ++x)
-          if (k0 + x < KS)
-            dst[x] = k0 + x < KSN ? row_frag16<typename C::TN, F>(mine, fm, k0 + x, fg)
-                                  : row_frag16<typename C::TR, F>(mine + C::OFF_R, fm, k0 + x - KSN, fg);
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      read(0, kf[0]);
-#pragma unroll
-      for (int k = 0; k < KS; k += BT) {
-        if (k + BT < KS) read(k + BT, kf[(k / BT + 1) & 1]);
-#pragma unroll
-        for (int x = 0; x < BT; ++x)
-          if (k + x < KS) {
-            if ((k + x) & 1) s1 = mma_s(s1, kf[(k / BT) & 1][x], q[k + x]);
-            else s0 = mma_s(s0, kf[(k / BT) & 1][x], q[k + x]);
-          }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      const int key0 = j * KT + 4 * gq;
-      f4 s = s0 + s1;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = key0 + i < seen ? s[i] : -INFINITY;
-      const float tm = group_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-      if (__any(tm > mx + lazy)) {
-        const float nm = fmaxf(mx, tm), al = fast_exp2((mx - nm) * c);
-        mx = nm;
-        mc = nm * c;
-        l *= al;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) acc[v] *= al;
-      }
-      float e[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e[i] = fast_exp2(fmaf(s[i], c, -mc));
-        l += e[i];
-      }
-      const auto p = to_p4<DT>(e);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int v = 0; v < NV; ++v) acc[v] = mma_p(acc[v], v_frag<DT, typename C::TN>(mine, 16 * v, ln), p);
-      if constexpr (ES == 2) pace<NV, 8, 1, 1>();
-      __builtin_amdgcn_sched_barrier(0);
-      if (j + NW < tb) {
-        lds_reads_done();                    // the buffer is read out
-        fetch(slot_of(a, page, token(j + NW)));
-        page = page_of(a, table, token(j + 2 * NW));
-      }
-    }
-
-    // the waves' sums: scaled to the common maximum, added in wave order by the wave that
-    // owns a share of the columns, as many columns at a time as the buffers hold
-    const int el = fresh(lane), em = el & 15, eg = el >> 4, er = grp * 16 + em;   // formed here: the loop needs the registers
-    l = group_sum(l);
-    if (eg == 0) {
-      red_m[wave][em] = mc;
-      red_l[wave][em] = l;
-    }
-    lds_barrier();                           // also: every wave has left its buffer
-    const bool whole = ta == 0 && tb == n_all;
-    float mt = red_m[0][em], ls = 0.f;
-#pragma unroll
-    for (int x = 1; x < NW; ++x) mt = fmaxf(mt, red_m[x][em]);
-#pragma unroll
-    for (int x = 0; x < NW; ++x) ls = fmaf(fast_exp2(red_m[x][em] - mt), red_l[x][em], ls);
-    const float f = fast_exp2(mc - mt);
-    const int64_t row = static_cast<int64_t>(b) * rows + er;
-    const int64_t sr = (static_cast<int64_t>(2 * w + (ta > 0 ? 0 : 1)) * a.groups + grp) * 16 + em;
-    const float inv = whole ? (ls > 0.f ? 1.f / ls : ls) : 1.f;   // nothing visible: zeros; NaN stays NaN
-    constexpr int VR = C::NVR < NV ? (C::NVR >= NV / 2 ? NV / 2 : NV / 4) : NV;   // column blocks of a round
-    static_assert(VR % NW == 0 && NV % VR == 0 && VR * NW * 1024 <= NW * C::WBUF, "rounds of columns");
-#pragma unroll
-    for (int v0 = 0; v0 < NV; v0 += VR) {
-      if (v0 > 0) lds_barrier();             // the round before has been read
-#pragma unroll
-      for (int v = 0; v < VR; ++v)
-        *reinterpret_cast<f4*>(buf + (wave * VR + v) * 1024 + el * 16) = acc[v0 + v] * f;
+    // interval i: tile i begins to be scored, tile i - SP is added, tile i + AHEAD copied
+    auto turn = [&](int i) {
+      if (i + AHEAD - 1 < tb) wait_vmem_but<(AHEAD - 1) * PW>();
+      else wait_vmem_all();
       lds_barrier();
+      if (i + AHEAD < tb) {
+        fetch(i + AHEAD, page);
+        if (new_page(a, i + AHEAD + 1, KT)) page = page_at(i + AHEAD + 1);
+      }
+    };
+    const bool whole = ta == 0 && tb == n_all;
+    const int64_t srow = (static_cast<int64_t>(2 * w + (ta > 0 ? 0 : 1)) * a.groups + grp) * 16;
+
+    if (scoring) {
+      const int seen = len - (a.Tq - 1 - cr / a.H);
+      float mo = kMaxInit, l = 0.f;          // the maximum that l is against
+      f4 s0, s1;
+      int j = ta + wave;                     // the tile in hand
+      auto score = [&](auto phase) {
+        constexpr int ph = decltype(phase)::value;
+        const char* cur = buf + (j & (RING - 1)) * C::BUF;
+        const int ln = fresh(lane), fm = ln & 15, fg = ln >> 4;
+        if constexpr (ph == 0) s0 = s1 = f4{0, 0, 0, 0};
+        constexpr int k0 = ph * KP, k1 = k0 + KP < KS ? k0 + KP : KS;
+        if constexpr (k0 < k1) {
+          F kf[k1 - k0];
 #pragma unroll
-      for (int v = 0; v < VR / NW; ++v) {
-        const int vb = wave * (VR / NW) + v;
-        f4 o = {0, 0, 0, 0};
+          for (int k = k0; k < k1; ++k)
+            kf[k - k0] = k < KSN ? row_frag16<typename C::TN, F>(cur, fm, k, fg)
+                                 : row_frag16<typename C::TR, F>(cur + C::OFF_R, fm, k - KSN, fg);
 #pragma unroll
-        for (int x = 0; x < NW; ++x) o += *reinterpret_cast<const f4*>(buf + (x * VR + vb) * 1024 + el * 16);
-        o *= inv;
-        const int col = 16 * (v0 + vb) + 4 * eg;
-        if (er < rows) {
-          if (whole) store4<DT>(a.o, row * R + col, o[0], o[1], o[2], o[3]);
-          else *reinterpret_cast<f4*>(a.part_o + sr * R + col) = o;
+          for (int k = k0; k < k1; ++k) {
+            if (k & 1) s1 = mma_s(s1, kf[k - k0], q[k]);
+            else s0 = mma_s(s0, kf[k - k0], q[k]);
+          }
+        }
+        if constexpr (ph == SP - 1) {
+          const int key0 = j * KT + 4 * gq, par = j & 1;
+          f4 s = s0 + s1;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[e] = key0 + e < seen ? s[e] : -INFINITY;
+          const float tm = group_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+          float mx = top[m];
+          const bool up = __any(tm > mx + lazy);
+          if (up) {
+            const float nm = fmaxf(mx, tm);
+            if (gq == 0) {
+              fac[par][m] = fast_exp2((mx - nm) * c);
+              top[m] = nm;
+            }
+            mx = nm;
+          }
+          if (lane == 0) rose[par] = up;
+          l *= fast_exp2((mo - mx) * c);
+          mo = mx;
+          float e[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            e[x] = fast_exp2(fmaf(s[x], c, -mx * c));
+            l += e[x];
+          }
+          sp[par][lane] = to_p4<DT>(e);
+          j += SP;
+        }
+      };
+      for (int i = ta; i < tb + SP; ++i) {
+        turn(i);
+        const int ph = i - j;
+        if (wave >= SP || j >= tb || ph < 0) continue;
+        if (ph == 0) score(std::integral_constant<int, 0>());
+        else if (ph == 1) score(std::integral_constant<int, 1>());
+        else if constexpr (SP > 2) {
+          if (ph == 2) score(std::integral_constant<int, 2>());
+          else score(std::integral_constant<int, SP - 1>());
+        }
+      }
+      l = group_sum(l);
+      if (wave < SP && gq == 0) {
+        red[0][wave][m] = mo;
+        red[1][wave][m] = l;
+      }
+      lds_barrier();
+      if (wave == 0 && gq == 0 && r < rows) {
+        const float mx = top[m];
+        float ls = 0.f;
+#pragma unroll
+        for (int x = 0; x < SP; ++x) ls = fmaf(fast_exp2((red[0][x][m] - mx) * c), red[1][x][m], ls);
+        if (whole) {
+          a.lse[static_cast<int64_t>(b) * rows + r] = ls == 0.f ? -INFINITY : (mx * c + __log2f(ls)) * kLn2;
+        } else {
+          a.part_ml[2 * (srow + m)] = mx * c;
+          a.part_ml[2 * (srow + m) + 1] = ls;
+        }
+      }
+    } else {
+      const int col = (wave - 4) * (R / 4);
+      f4 acc[NV];
+#pragma unroll
+      for (int v = 0; v < NV; ++v) acc[v] = f4{0, 0, 0, 0};
+      for (int i = ta; i < tb + SP; ++i) {
+        turn(i);
+        const int j = i - SP;
+        if (j < ta) continue;
+        const int par = j & 1, up = rose[par];
+        const char* cur = buf + (j & (RING - 1)) * C::BUF;
+        const int ln = fresh(lane);
+        const PV p = sp[par][ln];
+        PV vf[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) vf[v] = v_frag<DT, typename C::TN>(cur, col, 16 * v, ln);
+        if (__builtin_amdgcn_readfirstlane(up)) {
+          const float al = fac[par][m];
+#pragma unroll
+          for (int v = 0; v < NV; ++v) acc[v] *= al;
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) acc[v] = mma_p(acc[v], vf[v], p);
+      }
+      lds_barrier();
+      float ls = 0.f;
+      const float mx = top[m];
+#pragma unroll
+      for (int x = 0; x < SP; ++x) ls = fmaf(fast_exp2((red[0][x][m] - mx) * c), red[1][x][m], ls);
+      if (r < rows) {
+        const float inv = ls > 0.f ? 1.f / ls : ls;   // nothing visible: zeros; NaN stays NaN
+        const int64_t row = static_cast<int64_t>(b) * rows + r;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int at = col + 16 * v + 4 * gq;
+          if (whole) store4<DT>(a.o, row * R + at, acc[v][0] * inv, acc[v][1] * inv, acc[v][2] * inv, acc[v][3] * inv);
+          else *reinterpret_cast<f4*>(a.part_o + (srow + m) * R + at) = acc[v];
         }
       }
     }
-    if (wave == 0 && eg == 0 && er < rows) {
-      if (whole) {
-        a.lse[row] = ls == 0.f ? -INFINITY : (mt + __log2f(ls)) * kLn2;
-      } else {
-        a.part_ml[2 * sr] = mt;
-        a.part_ml[2 * sr + 1] = ls;
-      }
-    }
-    lds_barrier();                           // the sums have been read: the buffers are free
+    lds_barrier();                           // the sums have been read
     }
     run.g += places(a, len, KT) - ta;
     ++run.b;
@@ -743,9 +801,8 @@ hipError_t run_append(const LatentAppendArgs& a, hipStream_t s) {
 
 template <int DT, int R, int DR>
 hipError_t run_decode(const LatentDecodeArgs& a, int m_rows, hipStream_t s) {
-  typedef DecCfg<DT, R, DR> C;
   if (m_rows == 16) {
-    kda_latent_decode16_kernel<DT, R, DR><<<dim3(a.wgs * a.groups), dim3(64 * C::NW), 0, s>>>(a);
+    kda_latent_decode16_kernel<DT, R, DR><<<dim3(a.wgs * a.groups), dim3(512), 0, s>>>(a);
   } else if constexpr (DT != 0) {
     kda_latent_decode64_kernel<DT, R, DR><<<dim3(a.wgs * a.groups), dim3(512), 0, s>>>(a);
   } else {
