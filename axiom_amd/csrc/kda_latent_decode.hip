@@ -743,44 +743,63 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
 }
 
 // Joins the parts of a split sequence in run order, one row a workgroup; writes
-// the rows of an empty sequence.  Two halves of the workgroup take every second part.
+// the rows of an empty sequence.  Bound by its chain of loads (places of the
+// sequence, then the parts): the first eight parts of a half are on their way
+// before their factors are known.  Two halves of the workgroup take every second
+// part.
 template <int DT, int R, int KT>
 __global__ __launch_bounds__(R / 2) void kda_latent_join_kernel(LatentDecodeArgs a, int M16) {
   __shared__ float fac[64];
   __shared__ f4 other[R / 4];
   const int rows = a.Tq * a.H, lane = threadIdx.x & 63;
   const int b = blockIdx.y, r = blockIdx.x, half = threadIdx.x / (R / 4), col = (threadIdx.x % (R / 4)) * 4;
-  const int n = (seq_len(a, b) + KT - 1) / KT;
+  const int per = a.line[0], g0 = a.line[1 + b], n = (seq_len(a, b) + KT - 1) / KT;
   const int64_t row = static_cast<int64_t>(b) * rows + r;
   if (n == 0) {
     if (half == 0) store4<DT>(a.o, row * R + col, 0.f, 0.f, 0.f, 0.f);
     if (threadIdx.x == 0) a.lse[row] = -INFINITY;
     return;
   }
-  const int per = a.line[0], g0 = a.line[1 + b];
-  const int w0 = g0 / per, w1 = (g0 + n - 1) / per;
-  if (w0 == w1) return;
+  const int w0 = g0 / per, cnt = (g0 + n - 1) / per - w0 + 1;
+  if (cnt == 1) return;
   const int grp = r / M16;
-  auto at = [&](int w) { return (static_cast<int64_t>(2 * w + (w == w0 ? 1 : 0)) * a.groups + grp) * M16 + (r - grp * M16); };
-  float mx = kMaxInit;
-  for (int w = w0 + lane; w <= w1; w += 64) mx = fmaxf(mx, a.part_ml[2 * at(w)]);
+  // part i: run w0 + i, whose first segment began inside the sequence but for part 0
+  auto at = [&](int i) {
+    return (static_cast<int64_t>(2 * (w0 + i) + (i == 0 ? 1 : 0)) * a.groups + grp) * M16 + (r - grp * M16);
+  };
+  constexpr int PRE = 8;
+  f4 pre[PRE];
+#pragma unroll
+  for (int x = 0; x < PRE; ++x)
+    pre[x] = half + 2 * x < cnt ? *reinterpret_cast<const f4*>(a.part_o + at(half + 2 * x) * R + col) : f4{0, 0, 0, 0};
+  float2 ml = lane < cnt ? *reinterpret_cast<const float2*>(a.part_ml + 2 * at(lane)) : make_float2(kMaxInit, 0.f);
+  float mx = ml.x;
+  for (int i = lane + 64; i < cnt; i += 64) mx = fmaxf(mx, a.part_ml[2 * at(i)]);
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) mx = fmaxf(mx, __shfl_xor(mx, s, 64));
   f4 o = {0, 0, 0, 0};
-  float l = 0.f;
-  for (int wb = w0; wb <= w1; wb += 64) {
-    const int cnt = min(64, w1 - wb + 1);
+  float l = 0.f;                             // this lane's parts
+  for (int i0 = 0; i0 < cnt; i0 += 64) {
+    if (i0 > 0) {
+      ml = i0 + lane < cnt ? *reinterpret_cast<const float2*>(a.part_ml + 2 * at(i0 + lane)) : make_float2(kMaxInit, 0.f);
+      __syncthreads();
+    }
+    const float f = i0 + lane < cnt ? fast_exp2(ml.x - mx) : 0.f;
+    l = fmaf(f, ml.y, l);
+    if (threadIdx.x < 64) fac[lane] = f;
     __syncthreads();
-    if (threadIdx.x < 64) fac[lane] = lane < cnt ? fast_exp2(a.part_ml[2 * at(wb + lane)] - mx) : 0.f;
-    const float pl = lane < cnt ? a.part_ml[2 * at(wb + lane) + 1] : 0.f;
-    __syncthreads();
-    float x = fac[lane] * pl;
+    const int m = min(64, cnt - i0);
+    if (i0 == 0) {
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) x += __shfl_xor(x, s, 64);
-    l += x;
+      for (int x = 0; x < PRE; ++x)
+        if (half + 2 * x < m) o += fac[half + 2 * x] * pre[x];
+    }
 #pragma unroll 8
-    for (int i = half; i < cnt; i += 2) o += fac[i] * *reinterpret_cast<const f4*>(a.part_o + at(wb + i) * R + col);
+    for (int i = half + (i0 == 0 ? 2 * PRE : 0); i < m; i += 2)
+      o += fac[i] * *reinterpret_cast<const f4*>(a.part_o + at(i0 + i) * R + col);
   }
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) l += __shfl_xor(l, s, 64);
   if (half == 1) other[col / 4] = o;
   __syncthreads();
   if (half == 1) return;
