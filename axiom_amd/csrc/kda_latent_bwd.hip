@@ -245,18 +245,23 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
 //
 // 16-bit types: a pair of waves owns 32 keys and splits the work by what it
 // holds.  The first wave holds the keys and dv (112 registers): s, p, dv += p
-// do.  The second holds the values and dk (128): do v^T, and with p from the
-// first, in fp32 through LDS, g and dk += g q.  Each has half of the products,
-// the two share a SIMD, and one wave's exponentials run under the other's
-// products; a wave that holds all of it (240 registers and the scores) is alone
-// on its SIMD and had the matrix cores busy 32 % of the time.
+// do.  The second holds the values and dk (128): do v^T, and, a tile behind, with
+// p from the first, g and dk += g q.  Each has half of the products, the two
+// share a SIMD, and one wave's exponentials run under the other's products; a
+// wave that holds all of it (240 registers and the scores) is alone on its SIMD
+// and had the matrix cores busy 32 % of the time.  A tile behind, because with p
+// handed over inside a tile's turn both waves wait twice for each other (40 %).
+// p crosses in fp16, times 2^12: within 2^-12 of itself down to 2^-26, less than
+// what g is rounded by next; dv and g take the factor out.  Three query tiles in
+// LDS: arriving, present, behind.
 // fp32: operands twice as large and products 16 times as slow, so one wave does it all.
 template <int DT, int DN, int DR>
 struct KeyCfg : BwdCfg<DT, DN, DR> {
   typedef BwdCfg<DT, DN, DR> B;
   static constexpr bool PAIR = B::ES == 2;
   static constexpr int NT = PAIR ? 512 : 256, NWV = NT / 64;
-  static constexpr int P_BYTES = PAIR ? 4 * 8192 : 16;    // p of a tile: 64 x 32 fp32 a pair
+  static constexpr int P_LOG2 = PAIR ? 12 : 0;            // p's factor
+  static constexpr int P_BYTES = PAIR ? 4 * 4096 : 16;    // p of a tile: 64 x 32 fp16 a pair
 };
 
 template <int DT, int DN, int DR>
@@ -267,7 +272,8 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   constexpr int ES = C::ES, BN = C::BN, KN = DN / 16, KR = DR / 16, ND = DN / 32, NR = DR / 32, NWV = C::NWV, NTL = BN / 32;
   __shared__ __attribute__((aligned(1024))) char buf0[C::BUF_K];
   __shared__ __attribute__((aligned(1024))) char buf1[C::BUF_K];
-  __shared__ __attribute__((aligned(1024))) char pbuf[C::P_BYTES];
+  __shared__ __attribute__((aligned(1024))) char buf2[C::PAIR ? C::BUF_K : 16];
+  __shared__ __attribute__((aligned(1024))) char pbuf[2][C::P_BYTES];   // by tile parity
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 31, h = lane >> 5, own = wave & 3, role = wave >> 2;
   Where w;
@@ -285,6 +291,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   const int j0 = jf + part.j0, nt = jf + part.j1;
   const float c = a.scale * kLog2e;
   const float gf = DT == 2 ? do_factor(a, w.bh) : 1.f;
+  constexpr float unp = 1.f / (1 << C::P_LOG2);
 
   const char* qp = static_cast<const char*>(a.q) + (w.b * a.q_b + w.k0 * a.q_t + w.head * a.q_h) * ES;
   const char* dp_ = static_cast<const char*>(a.dout) + ((static_cast<int64_t>(w.b) * a.Tq + w.k0) * a.H + w.head) * DN * ES;
@@ -324,7 +331,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   const E* kp = static_cast<const E*>(a.kv) + w.b * a.kv_b + static_cast<int64_t>(ckey) * a.kv_t + w.head * a.kv_h + 8 * h;
   const E* rp = static_cast<const E*>(a.kr) + w.b * a.kr_b + static_cast<int64_t>(ckey) * a.kr_t + 8 * h;
   const int64_t ob = ((static_cast<int64_t>(w.b) * a.Tk + key) * a.H + w.head) * (2 * DN) + 4 * h;
-  const float f = a.scale / gf;
+  const float f = a.scale * (DT == 1 ? unp : 1.f / gf);   // fp16: g holds gf and no factor of p
 
   // p of a score tile, from s; rows q0 .. of the sequence, rows 32 t .. of the tile
   auto probs = [&](const char* cur, int q0, int t, int fh, bool edge, f16v& s) {
@@ -332,7 +339,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
     for (int v = 0; v < 4; ++v) {
       const f4 ls = *reinterpret_cast<const f4*>(cur + C::OFF_L + (32 * t + 8 * v + 4 * fh) * 4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[4 * v + e] = fast_exp2(fmaf(s[4 * v + e], c, -ls[e] * kLog2e));
+      for (int e = 0; e < 4; ++e) s[4 * v + e] = fast_exp2(fmaf(s[4 * v + e], c, fmaf(-ls[e], kLog2e, C::P_LOG2)));
     }
     if (edge) {
 #pragma unroll
@@ -351,7 +358,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * v + e;
         float g = p[i] * (dp[i] - dd[e]);
-        if constexpr (DT == 2) g *= gf;
+        if constexpr (DT == 2) g *= gf * unp;
         dp[i] = edge && p[i] == 0.f ? 0.f : g;
       }
     }
@@ -380,7 +387,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
 #pragma unroll
     for (int n = 0; n < ND; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) put4(DN + 32 * n + 8 * i, dv[n][4 * i], dv[n][4 * i + 1], dv[n][4 * i + 2], dv[n][4 * i + 3]);
+      for (int i = 0; i < 4; ++i) put4(DN + 32 * n + 8 * i, dv[n][4 * i] * unp, dv[n][4 * i + 1] * unp, dv[n][4 * i + 2] * unp, dv[n][4 * i + 3] * unp);
   };
   auto put_dk = [&](const f16v (&dk)[ND + NR]) {
 #pragma unroll
@@ -398,7 +405,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
 
   if (j0 < nt) fetch(j0, buf0);
   if constexpr (C::PAIR) {
-    char* const mine = pbuf + own * 8192 + lane * 16;
+    const int mine = own * 4096 + lane * 16;
     if (role == 0) {
       F kn[KN], kr[KR];
 #pragma unroll
@@ -411,10 +418,9 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
       auto step = [&](int j, const char* cur, char* nxt) {
         turn(j, nxt);
         const int qt = j * BN;
-        const bool busy = qt + BN > wave_first;
         const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
-        F pf[2][2];
-        if (busy) {
+        if (j < nt) {
+          F pf[2][2];
           f16v s[2];
           zero(s[0]);
           zero(s[1]);
@@ -434,14 +440,19 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
           for (int t = 0; t < 2; ++t) {
             if (edge) probs(cur, qt + 32 * t, t, fh, true, s[t]);
             else probs(cur, qt + 32 * t, t, fh, false, s[t]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<f4*>(mine + (4 * t + i) * 1024) = f4{s[t][4 * i], s[t][4 * i + 1], s[t][4 * i + 2], s[t][4 * i + 3]};
             frags(s[t], pf[t]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              h8 x;
+              if constexpr (DT == 2) {
+                x = pf[t][u];
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = static_cast<_Float16>(s[t][8 * u + e]);
+              }
+              *reinterpret_cast<h8*>(pbuf[j & 1] + mine + (2 * t + u) * 1024) = x;
+            }
           }
-        }
-        lds_barrier();
-        if (busy) {
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int u = 0; u < 4; ++u)
@@ -452,10 +463,12 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
           __builtin_amdgcn_sched_barrier(0);
         }
       };
-      for (int j = j0; j < nt;) {
+      for (int j = j0; j < nt + 1 && j0 < nt;) {
         step(j, buf0, buf1);
-        if (++j >= nt) break;
-        step(j, buf1, buf0);
+        if (++j > nt) break;
+        step(j, buf1, buf2);
+        if (++j > nt) break;
+        step(j, buf2, buf0);
         ++j;
       }
       if (live) put_dv(dv);
@@ -466,13 +479,41 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
       f16v dk[ND + NR];
 #pragma unroll
       for (int n = 0; n < ND + NR; ++n) zero(dk[n]);
-      auto step = [&](int j, const char* cur, char* nxt) {
+      f16v dp[2];
+      auto step = [&](int j, const char* cur, const char* prev, char* nxt) {
         turn(j, nxt);
-        const int qt = j * BN;
-        const bool busy = qt + BN > wave_first;
         const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
-        f16v dp[2];
-        if (busy) {
+        const int qp = (j - 1) * BN;
+        if (j > j0) {
+          F gq[2][2];
+          const bool edge = qp < wave_full || qp + BN > nq;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            f16v p;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const h8 x = *reinterpret_cast<const h8*>(pbuf[(j - 1) & 1] + mine + (2 * t + u) * 1024);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) p[8 * u + e] = static_cast<float>(x[e]);
+            }
+            if (edge) adjoint(prev, t, fh, true, p, dp[t]);
+            else adjoint(prev, t, fh, false, p, dp[t]);
+            frags(dp[t], gq[t]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+              dk[n] = mma(dk[n], C::TN::template col_frag<F>(prev, 16 * u, 32 * n, ln), gq[u >> 1][u & 1]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+              dk[ND + n] = mma(dk[ND + n], C::TR::template col_frag<F>(prev + C::OFF_R, 16 * u, 32 * n, ln), gq[u >> 1][u & 1]);
+          }
+          pace<4 * (ND + NR), 4, 2, 1>();
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (j < nt) {
           zero(dp[0]);
           zero(dp[1]);
           __builtin_amdgcn_sched_barrier(0);
@@ -483,41 +524,13 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
           pace<2 * KN, 6, 1, 1>();
           __builtin_amdgcn_sched_barrier(0);
         }
-        lds_barrier();
-        if (busy) {
-          F gq[2][2];
-          const bool edge = qt < wave_full || qt + BN > nq;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            f16v p;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const f4 x = *reinterpret_cast<const f4*>(mine + (4 * t + i) * 1024);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) p[4 * i + e] = x[e];
-            }
-            if (edge) adjoint(cur, t, fh, true, p, dp[t]);
-            else adjoint(cur, t, fh, false, p, dp[t]);
-            frags(dp[t], gq[t]);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-#pragma unroll
-            for (int n = 0; n < ND; ++n)
-              dk[n] = mma(dk[n], C::TN::template col_frag<F>(cur, 16 * u, 32 * n, ln), gq[u >> 1][u & 1]);
-#pragma unroll
-            for (int n = 0; n < NR; ++n)
-              dk[ND + n] = mma(dk[ND + n], C::TR::template col_frag<F>(cur + C::OFF_R, 16 * u, 32 * n, ln), gq[u >> 1][u & 1]);
-          }
-          pace<4 * (ND + NR), 4, 2, 1>();
-          __builtin_amdgcn_sched_barrier(0);
-        }
       };
-      for (int j = j0; j < nt;) {
-        step(j, buf0, buf1);
-        if (++j >= nt) break;
-        step(j, buf1, buf0);
+      for (int j = j0; j < nt + 1 && j0 < nt;) {
+        step(j, buf0, buf2, buf1);
+        if (++j > nt) break;
+        step(j, buf1, buf0, buf2);
+        if (++j > nt) break;
+        step(j, buf2, buf1, buf0);
         ++j;
       }
       if (live) put_dk(dk);
