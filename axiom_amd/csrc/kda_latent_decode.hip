@@ -589,34 +589,39 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
         for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const F*>(qp + 32 * s + 8 * gq);
       }
       const int seen = len - (a.Tq - 1 - r / a.H);
+      const int clear = (len - (a.Tq - 1)) / KT;   // tiles before this one have no masked key
+      // the lane's places: of the fragments in a tile (a latent's repeat every four), of its probabilities
+      int at[4 + DR / 32], put[2];
+#pragma unroll
+      for (int k = 0; k < 4 + DR / 32; ++k) at[k] = k < 4 ? TN::off(m, 4 * k, gq) : TR::off(m, 4 * (k - 4), gq);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) put[t] = TP::off(m, 2 * t, gq & 1, 16 * own) + 8 * (gq >> 1);
       float mx = kMaxInit, mc = kMaxInit * c, l = 0.f;
       auto step = [&](int i, const char* cur, char* nxt) {
         turn(i, nxt);
-        if (i >= tb) return;
-        const int ln = fresh(lane), fm = ln & 15, fg = ln >> 4;
         f4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
-            s[t] = mma_s(s[t], k < KSN ? row_frag16<TN, F>(cur + TN::bytes(16 * t), fm, k, fg)
-                                       : row_frag16<TR, F>(cur + OFF_R + TR::bytes(16 * t), fm, k - KSN, fg), q[k]);
+            s[t] = mma_s(s[t], *reinterpret_cast<const F*>(cur + (k < KSN ? at[k & 3] + ((k >> 2) * 256 + TN::bytes(16 * t))
+                                                                           : at[4 + (k - KSN)] + (OFF_R + TR::bytes(16 * t)))), q[k]);
         pace<2 * KS, 8, 1, 1>();
         __builtin_amdgcn_sched_barrier(0);
-        const int key0 = i * KT + 4 * gq;
-        float tm = -INFINITY;
+        if (i >= clear) {
+          const int key0 = i * KT + 4 * gq;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[t][e] = key0 + 16 * t + e < seen ? s[t][e] : -INFINITY;
-            tm = fmaxf(tm, s[t][e]);
-          }
-        tm = group_max(tm);
+            for (int e = 0; e < 4; ++e) s[t][e] = key0 + 16 * t + e < seen ? s[t][e] : -INFINITY;
+        }
+        float tm = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) tm = fmaxf(tm, fmaxf(s[0][e], s[1][e]));
         const bool up = __any(tm > mx + lazy);
         if (up) {
-          const float nm = fmaxf(mx, tm), al = fast_exp2((mx - nm) * c);
+          const float nm = fmaxf(mx, group_max(tm)), al = fast_exp2((mx - nm) * c);
           mx = nm;
           mc = nm * c;
           l *= al;
@@ -632,19 +637,20 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
             l += p[e];
           }
           // the output waves' fragment order: chunk 2 t + half, first or second four keys
-          store4<DT>(sp[i & 1] + TP::off(fm, 2 * t, fg & 1, 16 * own) + 8 * (fg >> 1), 0, p[0], p[1], p[2], p[3]);
+          store4<DT>(sp[i & 1] + put[t], 0, p[0], p[1], p[2], p[3]);
         }
       };
-      for (int i = ta; i <= tb;) {
+      for (int i = ta; i < tb;) {
         step(i, buf0, buf2);
-        if (++i > tb) break;
+        if (++i >= tb) break;
         step(i, buf1, buf3);
-        if (++i > tb) break;
+        if (++i >= tb) break;
         step(i, buf2, buf0);
-        if (++i > tb) break;
+        if (++i >= tb) break;
         step(i, buf3, buf1);
         ++i;
       }
+      turn(tb, buf0);                        // the last tile is added; nothing to copy
       l = group_sum(l);
       if (gq == 0) {
         ml[0][16 * own + m] = mc;
@@ -668,9 +674,17 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[v][n][e] = 0.f;
+      // the lane's places: of its columns in a tile, of the probabilities
+      int at[NV][2], pat[2];
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          at[v][y] = TN::off(4 * h + (m >> 2 & 3) + 8 * y, (own * (R / 4) + 32 * v) >> 3, 2 * (m >> 4) + ((m & 3) >> 1)) + 8 * (m & 1);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) pat[k] = TP::off(m, 2 * k, h);
       auto step = [&](int i, const char* prev, char* nxt) {
         turn(i, nxt);
-        if (i == ta) return;
         const int par = (i - 1) & 1;
         const int4 up = rose[par];
         if (__builtin_amdgcn_readfirstlane(up.x | up.y | up.z | up.w)) {
@@ -684,14 +698,17 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
               for (int e = 0; e < 16; ++e) acc[v][n][e] *= al;
           }
         }
-        const int ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const F p0 = TP::template row_frag<F>(sp[par], fm, k, fh), p1 = TP::template row_frag<F>(sp[par], fm, k, fh, 32);
+          const F p0 = *reinterpret_cast<const F*>(sp[par] + pat[k]), p1 = *reinterpret_cast<const F*>(sp[par] + pat[k] + TP::bytes(32));
 #pragma unroll
           for (int v = 0; v < NV; ++v) {
-            const F vf = TN::template col_frag<F>(prev, 16 * k, own * (R / 4) + 32 * v, ln);
+            union { s4v s[2]; F f; } u;
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              u.s[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(prev + at[v][y] + TN::bytes(16 * k)));
+            const F vf = u.f;
             acc[v][0] = mma(acc[v][0], vf, p0);
             acc[v][1] = mma(acc[v][1], vf, p1);
           }
@@ -704,14 +721,15 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
         }
         __builtin_amdgcn_sched_barrier(0);
       };
-      for (int i = ta; i <= tb;) {
-        step(i, buf3, buf2);
-        if (++i > tb) break;
+      turn(ta, buf2);
+      for (int i = ta + 1; i <= tb;) {
         step(i, buf0, buf3);
         if (++i > tb) break;
         step(i, buf1, buf0);
         if (++i > tb) break;
         step(i, buf2, buf1);
+        if (++i > tb) break;
+        step(i, buf3, buf2);
         ++i;
       }
       lds_barrier();
