@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
     if (blockIdx.y == 0) {
       if (live && h == 0) a.D[ri] = D;
       if constexpr (DT == 2) {
-        __shared__ float tops[4];
+        float* const tops = reinterpret_cast<float*>(buf1);   // two workgroups' LDS leave no byte of a CU's
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
         if (lane == 0) tops[wave] = top;
