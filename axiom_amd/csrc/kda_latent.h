@@ -112,30 +112,11 @@ __device__ __forceinline__ void pace() {
   __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * MPF, 0);
 }
 
-// The same with VPM vector instructions and one exponential beside each product.
-template <int N, int AHEAD, int RPF, int VPM>
-__device__ __forceinline__ void pace_mixed() {
-  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * RPF, 0);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    if (i < N - AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, RPF, 0);
-    __builtin_amdgcn_sched_group_barrier(0x002, VPM, 0);
-    __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
-  }
-}
-
 // all but the newest N vector memory operations of the wave are done
 template <int N>
 __device__ __forceinline__ void wait_vmem_but() {
   static_assert(N >= 0 && N < 64, "vmcnt is six bits");
   __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
-}
-
-// every LDS read of the wave has returned (before its buffer is copied into again)
-__device__ __forceinline__ void lds_reads_done() {
-  __builtin_amdgcn_s_waitcnt(0xC07F);
-  __builtin_amdgcn_sched_barrier(0);
 }
 
 // value combined over the two halves of the wave (lane l and l ^ 32)

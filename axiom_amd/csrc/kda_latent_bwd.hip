@@ -114,7 +114,6 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
       gf = to_one(top);
     }
     if (blockIdx.y == 0) {
-      if (live && h == 0) a.D[ri] = D;
       if constexpr (DT == 2) {
         float* const tops = reinterpret_cast<float*>(buf1);   // two workgroups' LDS leave no byte of a CU's
 #pragma unroll
@@ -150,6 +149,37 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   };
 
   const float c = a.scale * kLog2e;
+  // Rows of few keys: D as sum_j p_j (do . v_j), not from the rounded o, whose
+  // error is as large as g's own rounding there and falls with the keys' number
+  // (T = 1000, causal, d 64: dq's error 1.53 times its output's rounding with the
+  // one, below 1.5 with the other).  Two tiles, both in LDS.
+  if (ES == 2 && blk_hi < 2 * BN && nt > 0) {   // a walk this short is never shared out
+    fetch(0, buf0);
+    if (nt == 2) fetch(1, buf1);
+    wait_vmem_all();
+    lds_barrier();
+    float d = 0.f;
+    for (int x = 0; x < BN * nt; x += 32) {
+      const char* cur = x < BN ? buf0 : buf1;
+      const int r0 = x & (BN - 1), ln = fresh(lane), fm = ln & 31, fh = ln >> 5;
+      f16v s, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KN; ++k) {
+        s = mma(s, C::TN::template row_frag<F>(cur, fm, k, fh, r0), qn[k]);
+        dp = mma(dp, C::TN::template row_frag<F>(cur + C::OFF_V, fm, k, fh, r0), dO[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < KR; ++k) s = mma(s, C::TR::template row_frag<F>(cur + C::OFF_R, fm, k, fh, r0), qr[k]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        d += x + 8 * (i >> 2) + 4 * h + (i & 3) <= kmax ? fast_exp2(fmaf(s[i], c, -lse2)) * dp[i] : 0.f;
+    }
+    D = half_sum(d);
+    lds_barrier();
+  }
+  if (blockIdx.y == 0 && live && h == 0) a.D[ri] = D;
   f16v acc[ND + NR];
 #pragma unroll
   for (int n = 0; n < ND + NR; ++n)
@@ -251,9 +281,11 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
 // wave that holds all of it (240 registers and the scores) is alone on its SIMD
 // and had the matrix cores busy 32 % of the time.  A tile behind, because with p
 // handed over inside a tile's turn both waves wait twice for each other (40 %).
-// p crosses in fp16, times 2^12: within 2^-12 of itself down to 2^-26, less than
-// what g is rounded by next; dv and g take the factor out.  Three query tiles in
-// LDS: arriving, present, behind.
+// p crosses in fp16, times 2^12 (dv and g take the factor out): within 2^-12 of
+// itself down to 2^-26.  That is an eighth of the rounding that g gets next in
+// bf16, and as much again in fp16 (dk's error 3.6e-4 against 3.0e-4 without it;
+// fp32 would need 32 KB more than the LDS has).  Three query tiles in LDS:
+// arriving, present, behind.
 // fp32: operands twice as large and products 16 times as slow, so one wave does it all.
 template <int DT, int DN, int DR>
 struct KeyCfg : BwdCfg<DT, DN, DR> {
