@@ -283,9 +283,9 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
 // handed over inside a tile's turn both waves wait twice for each other (40 %).
 // p crosses in fp16, times 2^12 (dv and g take the factor out): within 2^-12 of
 // itself down to 2^-26.  That is an eighth of the rounding that g gets next in
-// bf16, and as much again in fp16 (dk's error 3.6e-4 against 3.0e-4 without it;
-// fp32 would need 32 KB more than the LDS has).  Three query tiles in LDS:
-// arriving, present, behind.
+// bf16, and as much again in fp16 (dk's error 3.6e-4, where g's and the output's
+// roundings alone make 3.0e-4; p in fp32 would need more LDS than a CU has).
+// Three query tiles in LDS: arriving, present, behind.
 // fp32: operands twice as large and products 16 times as slow, so one wave does it all.
 template <int DT, int DN, int DR>
 struct KeyCfg : BwdCfg<DT, DN, DR> {
