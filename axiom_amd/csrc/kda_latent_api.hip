@@ -119,9 +119,9 @@ BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dn, int dr, int n_seqs, i
 // Decode: query rows of a workgroup (16, or 64 where there are more than 16;
 // fp32 16, whose operands take twice the registers and LDS), the row groups
 // of a sequence, and the workgroups along the cache: one a CU (its buffers take
-// the LDS), and no more than there can be runs of `least` tiles (a tile
-// of each wave, or two of 32 keys).  Sequences whose table holds at most
-// kWholeTokens tokens get a workgroup each instead and no join launch.
+// the LDS), and no more than there can be runs of `least` tiles.  Sequences whose
+// table holds at most kWholeTokens tokens get a workgroup each instead and no join
+// launch.
 constexpr int kCUs = 256;
 constexpr int kWholeTokens = 128;
 struct DecodePlan { int rows, groups, wgs, whole, least, pad; size_t part_ml, part_o, total; };

@@ -10,6 +10,12 @@
 // the tensor all heads share; no broadcast copy of it exists anywhere.
 // P is rounded to the inputs' type for the second product (the matrix cores'
 // operand); the row sum adds the unrounded values.
+//
+// Bound by the products: B1 H16 T16384, d 128 + 64, bf16, causal takes 1.23 ms,
+// 1.12 PFLOP/s over the pairs it has to form (an 8192^3 product reaches 1.19);
+// B4 H16 T4096 340 us, 1.01.  128 queries a workgroup and two workgroups a CU,
+// because a wave's 32 queries, their output and a score tile are 256 registers.
+// fp32 (products 16 times as slow, one workgroup a CU): B1 H8 T1024 53 us.
 
 #include "kda_internal.h"
 #include "kda_latent.h"
@@ -196,6 +202,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
 }
 
 // Joins the parts of split blocks, in part order; an eighth of a block a workgroup.
+// Bound by its launch and one round of loads: 4 to 7 us.
 template <int DT, int DN, int DR>
 __global__ __launch_bounds__(256) void kda_latent_fwd_join_kernel(LatentArgs a, int nqb) {
   typedef FwdCfg<DT, DN, DR> C;
