@@ -311,7 +311,7 @@ struct LatentArgs {
   // Few blocks: up to `splits` workgroups a block, each with a share of the
   // other axis, leave fp32 parts that a join adds (forward: also the maxima
   // and sums); part index z, then [B*H][rows][width].
-  int splits;
+  int splits, share, live; // share: its tiles, live: the shares of a head; 0: `splits` equal shares of a block
   float* part;
   float* part_ml;
   // backward
@@ -322,7 +322,7 @@ struct LatentArgs {
   float* dmax;             // fp16: largest |do| of each query block, [B*H][dmax_n]
   int dmax_n;
   float* dkr_part;         // [splits][B,H,Tk,dr]: each head's share of the rotary key's gradient
-  int splits_k;            // the key pass' splits and parts (`splits`, `part` are the query pass')
+  int splits_k, share_k, live_k;   // the key pass' (those above and `part` are the query pass')
   float* part_k;
   void* dq;
   void* dkv;

@@ -262,11 +262,11 @@ struct Copy {
 };
 
 // A block's share z of its n tiles along the other axis: [j0, j1) of `parts`
-// shares of at least two tiles each.
+// shares of `len` tiles, or (len 0) of `splits` equal ones of at least two.
 struct Share {
   int j0, j1, parts;
-  __device__ __forceinline__ Share(int n, int splits, int z) {
-    const int c = splits > 1 ? max(2, (n + splits - 1) / splits) : max(n, 1);
+  __device__ __forceinline__ Share(int n, int splits, int len, int z) {
+    const int c = len > 0 ? len : splits > 1 ? max(2, (n + splits - 1) / splits) : max(n, 1);
     parts = max(1, (n + c - 1) / c);
     j0 = z * c;
     j1 = min(n, j0 + c);
@@ -321,20 +321,53 @@ struct Where { int b, head, bh, blk, r0, re, k0, ke, off; };   // rows owned fro
 // the last head's longest blocks began when the other heads' were done (B4 H16
 // T4096: forward 368 -> 341 us, query pass 658 -> 597, key pass 813 -> 802).  A
 // head of 256 blocks is long enough alone.
-__device__ __forceinline__ bool locate(const LatentArgs& a, int id, int nb, int BM, bool q_side, bool reverse, Where& w) {
+__device__ __forceinline__ void order(const LatentArgs& a, int id, int nb, bool reverse, int& bh, int& blk) {
   const int bh_n = a.B * a.H;
-  int blk;
   if (bh_n % 8 == 0) {
     const int slot = id >> 3, group = a.causal ? max(1, min(4, 256 / nb)) : 1;
     const int g = slot / (nb * group), in = min(group, (bh_n >> 3) - g * group);
     const int i = slot - g * nb * group;
-    w.bh = (id & 7) + 8 * (g * group + i % in);
+    bh = (id & 7) + 8 * (g * group + i % in);
     blk = i / in;
   } else {
-    w.bh = id % bh_n;
+    bh = id % bh_n;
     blk = id / bh_n;
   }
   if (reverse) blk = nb - 1 - blk;
+}
+// Share `id` of a grid of live shares: heads go round the XCDs, a head's blocks
+// follow each other with all their shares.  BN: rows of a tile.
+__device__ __forceinline__ void live_share(const LatentArgs& a, int id, int nb, int BN, bool q_side, int len, int& bh, int& blk, int& z) {
+  const int bh_n = a.B * a.H, lane = __lane_id(), all = ((q_side ? a.Tk : a.Tq) + BN - 1) / BN, u = id / bh_n;
+  bh = id - u * bh_n;
+  blk = z = 0;
+  for (int b0 = 0, base = 0; b0 < nb; b0 += 64) {
+    const int i = b0 + lane;
+    int n = all;
+    if (a.causal) {
+      n = q_side ? max(0, min(a.Tk - 1, min(128 * i + 127, a.Tq - 1) + a.Tk - a.Tq) + BN) / BN
+                 : max(0, all - max(0, 128 * i + a.Tq - a.Tk) / BN);
+    }
+    n = i < nb ? max(1, (n + len - 1) / len) : 0;
+    int inc = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(inc, d, 64);
+      inc += lane >= d ? up : 0;
+    }
+    const unsigned long long hit = __ballot(base + inc > u);
+    if (hit) {
+      const int x = __ffsll(static_cast<long long>(hit)) - 1;
+      blk = b0 + x;
+      z = u - base - (__builtin_amdgcn_readlane(inc, x) - __builtin_amdgcn_readlane(n, x));
+      return;
+    }
+    base += __builtin_amdgcn_readlane(inc, 63);
+  }
+}
+// Where block blk of head bh stands; false: a packed call's surplus block.
+__device__ __forceinline__ bool place(const LatentArgs& a, int bh, int blk, int BM, bool q_side, Where& w) {
+  w.bh = bh;
   w.blk = blk;
   w.b = w.bh / a.H;
   w.head = w.bh - w.b * a.H;
@@ -357,6 +390,21 @@ __device__ __forceinline__ bool locate(const LatentArgs& a, int id, int nb, int 
     w.off = q_side ? a.Tk - a.Tq : a.Tq - a.Tk;
   }
   return true;
+}
+
+__device__ __forceinline__ bool locate(const LatentArgs& a, int id, int nb, int BM, bool q_side, bool reverse, Where& w) {
+  int bh, blk;
+  order(a, id, nb, reverse, bh, blk);
+  return place(a, bh, blk, BM, q_side, w);
+}
+// ... of this workgroup of a pass, and its share z
+__device__ __forceinline__ bool locate_share(const LatentArgs& a, int nb, int BM, int BN, bool q_side, bool reverse, Where& w, int& z) {
+  const int len = q_side ? a.share : a.share_k;
+  int bh, blk;
+  z = blockIdx.y;
+  if (len > 0) live_share(a, blockIdx.x, nb, BN, q_side, len, bh, blk, z);
+  else order(a, blockIdx.x, nb, reverse, bh, blk);
+  return place(a, bh, blk, BM, q_side, w);
 }
 
 }  // namespace latent

@@ -76,43 +76,74 @@ kda::LatentArgs attn_args(const void* q, const void* kv, const void* kr, const i
   return a;
 }
 
-// Workgroups of a block of 128 rows along the other axis.  A launch of fewer
-// blocks than the chip runs at once leaves CUs idle while each block walks its
-// whole row of tiles, so the walk is shared out, up to 16 ways, until there are
-// `slots` workgroups; a join adds their fp32 parts.
+// Shares of a block of 128 rows along the other axis.  A launch of fewer blocks
+// than the chip runs at once leaves CUs idle while each block walks its whole
+// row of tiles, so the walks are cut into shares of `len` tiles (up to 16 a
+// block, 128 rows each at least), as short as kSlots workgroups allow; a join
+// adds their fp32 parts.  Equal lengths, not equal numbers: a causal call's walks
+// differ, and its longest share is what it waits for (fp32 B1 H8 T1024
+// forward and backward 256 us with equal numbers, 195 with these; bf16 1 x 1000 of
+// d 64 the five kernels 72 us, 65).  `live`:
+// the shares of a head's blocks, one a workgroup of the grid (a grid of blocks by
+// the most shares, its empty workgroups leaving at once, put two of the others on
+// some CUs: 1.3 times as long).  Not where the longest walk falls by less than a
+// quarter.  Packed lengths are on the device: there `parts` equal shares of each
+// block (len 0).
+constexpr int kSlots = 256;   // one workgroup a CU; with two (bf16, T = 1333, 16 heads) the join costs what they gain
+struct Shares { int len, parts, live; };
 // blocks of 128 rows of one head; packed: every sequence ends in at most one partial block
 int64_t blocks_of(int64_t T, int n_seqs) { return n_seqs > 0 ? T / 128 + n_seqs : (T + 127) / 128; }
-int splits_of(int64_t T, int64_t T_other, int B, int H, int n_seqs, int slots) {
-  const int64_t blocks = blocks_of(T, n_seqs) * B * H;
-  if (blocks <= 0) return 1;
-  const int64_t s = slots / blocks, most = (T_other + 127) / 128;   // shares of at least 128 rows
-  return static_cast<int>(s < 1 || most <= 1 ? 1 : (s < most ? (s < 16 ? s : 16) : (most < 16 ? most : 16)));
+// q_side: blocks of queries that walk keys, else keys that walk queries
+Shares shares_of(bool q_side, int64_t Tq, int64_t Tk, int64_t heads, int n_seqs, bool causal, int dtype) {
+  const int64_t T = q_side ? Tq : Tk, other = q_side ? Tk : Tq, blocks = blocks_of(T, n_seqs);
+  const int64_t most = std::min<int64_t>(16, (other + 127) / 128);
+  if (blocks <= 0 || blocks * heads > kSlots || most <= 1) return {0, 1, 0};
+  if (n_seqs > 0) return {0, static_cast<int>(std::max<int64_t>(1, std::min(kSlots / (blocks * heads), most))), 0};
+  const int64_t tile = dtype == KDA_DTYPE_F32 ? 32 : 64, all = (other + tile - 1) / tile;
+  auto walk = [&](int64_t i) {
+    if (!causal) return all;
+    if (q_side) return std::max<int64_t>(0, std::min(Tk - 1, std::min(128 * i + 127, Tq - 1) + Tk - Tq) + tile) / tile;
+    return std::max<int64_t>(0, all - std::max<int64_t>(0, 128 * i + Tq - Tk) / tile);
+  };
+  const int64_t longest = walk(q_side ? blocks - 1 : 0);
+  auto live = [&](int64_t len) {
+    int64_t n = 0;
+    for (int64_t i = 0; i < blocks; ++i) n += std::max<int64_t>(1, (walk(i) + len - 1) / len);
+    return n;
+  };
+  int64_t lo = std::max<int64_t>(128 / tile, (longest + most - 1) / most), hi = longest;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if (live(mid) * heads <= kSlots) hi = mid;
+    else lo = mid + 1;
+  }
+  if (4 * lo > 3 * longest) return {0, 1, 0};
+  return {static_cast<int>(lo), static_cast<int>((longest + lo - 1) / lo), static_cast<int>(live(lo))};
 }
-// One workgroup a CU; with two (bf16, T = 1333, 16 heads) the join costs what they gain.
-constexpr int kSlots = 256;
 
-struct FwdLayout { int splits; size_t ml, total; };
-FwdLayout fwd_layout(int B, int Tq, int Tk, int H, int dn, int n_seqs, int dtype) {
+struct FwdLayout { Shares q; size_t ml, total; };
+FwdLayout fwd_layout(int B, int Tq, int Tk, int H, int dn, int n_seqs, bool causal, int dtype) {
   FwdLayout L{};
-  L.splits = splits_of(Tq, Tk, B, H, n_seqs, kSlots);
-  const size_t rows = L.splits > 1 ? static_cast<size_t>(L.splits) * B * H * Tq : 0;
+  const int64_t bh = static_cast<int64_t>(B) * H;
+  L.q = shares_of(true, Tq, Tk, bh, n_seqs, causal, dtype);
+  const size_t rows = L.q.parts > 1 ? static_cast<size_t>(L.q.parts) * bh * Tq : 0;
   L.ml = align_up(rows * dn * 4);
   L.total = L.ml + align_up(rows * 8);
   return L;
 }
-struct BwdLayout { int splits, splits_k; int64_t blocks; size_t D, dmax, dkr, part, part_k, total; };
-BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dn, int dr, int n_seqs, int dtype) {
+struct BwdLayout { Shares q, k; int64_t blocks; size_t D, dmax, dkr, part, part_k, total; };
+BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dn, int dr, int n_seqs, bool causal, int dtype) {
   BwdLayout L{};
   const size_t bh = static_cast<size_t>(B) * H;
-  L.splits = splits_of(Tq, Tk, B, H, n_seqs, kSlots);
-  L.splits_k = splits_of(Tk, Tq, B, H, n_seqs, kSlots);
+  L.q = shares_of(true, Tq, Tk, static_cast<int64_t>(bh), n_seqs, causal, dtype);
+  L.k = shares_of(false, Tq, Tk, static_cast<int64_t>(bh), n_seqs, causal, dtype);
   L.D = 0;
   L.dmax = align_up(bh * Tq * 4);
   L.blocks = blocks_of(Tq, n_seqs);
   L.dkr = L.dmax + align_up(bh * L.blocks * 4);
-  L.part = L.dkr + align_up(L.splits_k * bh * Tk * dr * 4);
-  L.part_k = L.part + align_up(L.splits > 1 ? L.splits * bh * Tq * (dn + dr) * 4 : 0);
-  L.total = L.part_k + align_up(L.splits_k > 1 ? L.splits_k * bh * Tk * 2 * dn * 4 : 0) + 256;
+  L.part = L.dkr + align_up(L.k.parts * bh * Tk * dr * 4);
+  L.part_k = L.part + align_up(L.q.parts > 1 ? L.q.parts * bh * Tq * (dn + dr) * 4 : 0);
+  L.total = L.part_k + align_up(L.k.parts > 1 ? L.k.parts * bh * Tk * 2 * dn * 4 : 0) + 256;
   return L;
 }
 
@@ -155,14 +186,14 @@ int kda_latent_attn_fwd(hipStream_t stream, const void* q, const void* kv, const
   if (static_cast<int64_t>(B) * Tq == 0) return KDA_OK;
   if (!o || !lse) return fail(KDA_ERR_INVALID_ARGUMENT, "null o or lse");
   if (!aligned(o, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "o must be aligned to 16 bytes");
-  const FwdLayout L = fwd_layout(B, Tq, Tk, H, dn, cu_q ? n_seqs : 0, dtype);
+  const FwdLayout L = fwd_layout(B, Tq, Tk, H, dn, cu_q ? n_seqs : 0, causal != 0, dtype);
   if (L.total > 0 && (!workspace || workspace_bytes < L.total))
     return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0}, L.total);
   if (!aligned(workspace, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "workspace must be aligned to 16 bytes");
   kda::LatentArgs a = attn_args(q, kv, k_rope, strides, cu_q, cu_k, n_seqs, B, Tq, Tk, H, causal, scale);
   a.o = o;
   a.lse = lse;
-  a.splits = L.splits;
+  a.splits = L.q.parts; a.share = L.q.len; a.live = L.q.live;
   a.part = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + L.ml);
   return launched(kda::launch_latent_fwd(a, dn, dr, dtype, stream), "kda_latent_attn_fwd");
@@ -170,12 +201,13 @@ int kda_latent_attn_fwd(hipStream_t stream, const void* q, const void* kv, const
 
 size_t kda_latent_attn_fwd_workspace(int B, int Tq, int Tk, int H, int dn, int dr, int32_t n_seqs, int dtype) {
   if (!sizes_ok(B, Tq, Tk, H, dn, dr, n_seqs, dtype)) return 0;
-  return fwd_layout(B, Tq, Tk, H, dn, n_seqs, dtype).total;
+  return std::max(fwd_layout(B, Tq, Tk, H, dn, n_seqs, false, dtype).total, fwd_layout(B, Tq, Tk, H, dn, n_seqs, true, dtype).total);
 }
 
 size_t kda_latent_attn_bwd_workspace(int B, int Tq, int Tk, int H, int dn, int dr, int32_t n_seqs, int dtype) {
   if (!sizes_ok(B, Tq, Tk, H, dn, dr, n_seqs, dtype)) return 0;
-  return bwd_layout(B, Tq, Tk, H, dn, dr, n_seqs, dtype).total;
+  return std::max(bwd_layout(B, Tq, Tk, H, dn, dr, n_seqs, false, dtype).total,
+                  bwd_layout(B, Tq, Tk, H, dn, dr, n_seqs, true, dtype).total);
 }
 
 int kda_latent_attn_bwd(hipStream_t stream, const void* q, const void* kv, const void* k_rope, const int64_t* strides,
@@ -189,7 +221,7 @@ int kda_latent_attn_bwd(hipStream_t stream, const void* q, const void* kv, const
   for (const void* p : {o, d_o, static_cast<const void*>(dq), static_cast<const void*>(dkv), static_cast<const void*>(dk_rope)})
     if (!aligned(p, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "o, d_o, dq, dkv and dk_rope must be aligned to 16 bytes");
   if (static_cast<int64_t>(H) * dn * elem(dtype) >= kMaxRowBytes) return fail(KDA_ERR_UNSUPPORTED, "H * dn too large");
-  const BwdLayout L = bwd_layout(B, Tq, Tk, H, dn, dr, cu_q ? n_seqs : 0, dtype);
+  const BwdLayout L = bwd_layout(B, Tq, Tk, H, dn, dr, cu_q ? n_seqs : 0, causal != 0, dtype);
   if (!workspace || workspace_bytes < L.total)
     return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0}, L.total);
   if (!aligned(workspace, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "workspace must be aligned to 16 bytes");
@@ -202,8 +234,8 @@ int kda_latent_attn_bwd(hipStream_t stream, const void* q, const void* kv, const
   a.dkr_part = reinterpret_cast<float*>(ws + L.dkr);
   a.part = reinterpret_cast<float*>(ws + L.part);
   a.part_k = reinterpret_cast<float*>(ws + L.part_k);
-  a.splits = L.splits;
-  a.splits_k = L.splits_k;
+  a.splits = L.q.parts; a.share = L.q.len; a.live = L.q.live;
+  a.splits_k = L.k.parts; a.share_k = L.k.len; a.live_k = L.k.live;
   a.dq = dq; a.dkv = dkv; a.dkr = dk_rope;
   return launched(kda::launch_latent_bwd(a, dn, dr, dtype, stream), "kda_latent_attn_bwd");
 }

@@ -67,8 +67,9 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 31, h = lane >> 5;
   Where w;
-  if (!locate(a, blockIdx.x, nqb, C::BM, true, true, w)) {
-    if (DT == 2 && blockIdx.y == 0 && threadIdx.x == 0) a.dmax[static_cast<int64_t>(w.bh) * nqb + w.blk] = 0.f;
+  int z;
+  if (!locate_share(a, nqb, C::BM, BN, true, true, w, z)) {
+    if (DT == 2 && z == 0 && threadIdx.x == 0) a.dmax[static_cast<int64_t>(w.bh) * nqb + w.blk] = 0.f;
     return;
   }
   const int nk = w.ke - w.k0;
@@ -79,9 +80,9 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   const int wave_lo = a.causal ? min(nk - 1, w.r0 + wave * 32 + w.off) : nk - 1;
   const int wave_hi = a.causal ? min(nk - 1, min(w.r0 + wave * 32 + 31, w.re - 1) + w.off) : nk - 1;
   const int blk_hi = a.causal ? min(nk - 1, min(w.r0 + C::BM - 1, w.re - 1) + w.off) : nk - 1;
-  const Share part(max(0, (blk_hi + BN) / BN), a.splits, blockIdx.y);
+  const Share part(max(0, (blk_hi + BN) / BN), a.splits, a.share, z);
   const int nt = part.j1;
-  if (static_cast<int>(blockIdx.y) >= part.parts) return;   // never share 0, which also leaves D
+  if (z >= part.parts) return;   // never share 0, which also leaves D
 
   F qn[KN], qr[KR], dO[KN];
   {
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
       top = half_max(top);
       gf = to_one(top);
     }
-    if (blockIdx.y == 0) {
+    if (z == 0) {
       if constexpr (DT == 2) {
         float* const tops = reinterpret_cast<float*>(buf1);   // two workgroups' LDS leave no byte of a CU's
 #pragma unroll
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
     D = half_sum(d);
     lds_barrier();
   }
-  if (blockIdx.y == 0 && live && h == 0) a.D[ri] = D;
+  if (z == 0 && live && h == 0) a.D[ri] = D;
   f16v acc[ND + NR];
 #pragma unroll
   for (int n = 0; n < ND + NR; ++n)
@@ -253,7 +254,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   if (!live) return;
   const float f = a.scale / gf;
   if (part.parts > 1) {
-    const int64_t pb = ((static_cast<int64_t>(blockIdx.y) * a.B * a.H + w.bh) * a.Tq + row) * (DN + DR) + 4 * h;
+    const int64_t pb = ((static_cast<int64_t>(z) * a.B * a.H + w.bh) * a.Tq + row) * (DN + DR) + 4 * h;
 #pragma unroll
     for (int n = 0; n < ND + NR; ++n)
 #pragma unroll
@@ -313,7 +314,8 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 31, h = lane >> 5, own = wave & 3, role = wave >> 2;
   Where w;
-  if (!locate(a, blockIdx.x, nkb, C::BM, false, false, w)) return;
+  int z;
+  if (!locate_share(a, nkb, C::BM, BN, false, false, w, z)) return;
   const int nq = w.ke - w.k0;                   // queries of the sequence
   const int key = w.r0 + own * 32 + m;          // this lane's key (packed axis)
   const bool live = key < w.re;
@@ -322,8 +324,8 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   const int wave_first = a.causal ? max(0, w.r0 + own * 32 + w.off) : 0;    // ... any of the wave's keys
   const int wave_full = a.causal ? max(0, min(w.r0 + own * 32 + 31, w.re - 1) + w.off) : 0;   // ... all of them
   const int jf = (a.causal ? max(0, w.r0 + w.off) : 0) / BN;                // the block's first query tile
-  const Share part(max(0, (nq + BN - 1) / BN - jf), a.splits_k, blockIdx.y);
-  if (static_cast<int>(blockIdx.y) >= part.parts) return;
+  const Share part(max(0, (nq + BN - 1) / BN - jf), a.splits_k, a.share_k, z);
+  if (z >= part.parts) return;
   const int j0 = jf + part.j0, nt = jf + part.j1;
   const float c = a.scale * kLog2e;
   const float gf = DT == 2 ? do_factor(a, w.bh) : 1.f;
@@ -414,7 +416,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   };
   // dv, dk and the rotary part of this lane's key, or this share's parts of them
   const bool parted = part.parts > 1;
-  const int64_t prow = (static_cast<int64_t>(blockIdx.y) * a.B * a.H + w.bh) * a.Tk + key;
+  const int64_t prow = (static_cast<int64_t>(z) * a.B * a.H + w.bh) * a.Tk + key;
   auto put4 = [&](int col, float x, float y, float z, float u) {
     if (parted) store4<0>(a.part_k, prow * (2 * DN) + 4 * h + col, x, y, z, u);
     else store4<DT>(a.dkv, ob + col, x, y, z, u);
@@ -652,7 +654,7 @@ __global__ __launch_bounds__(256) void kda_latent_sums_kernel(LatentArgs a, int 
   } else {
     tiles = max(0, (n_o + C::BN - 1) / C::BN - (a.causal ? max(0, w.r0 + w.off) : 0) / C::BN);
   }
-  const int parts = Share(tiles, q_side ? a.splits : a.splits_k, 0).parts;
+  const int parts = Share(tiles, q_side ? a.splits : a.splits_k, q_side ? a.share : a.share_k, 0).parts;
   const int T = q_side ? a.Tq : a.Tk, ra = w.r0 + blockIdx.y * 32, n = min(32, w.re - ra), WID4 = (q_side ? DN + DR : 2 * DN) / 4;
   const int64_t step = static_cast<int64_t>(a.B) * a.H * T, row0 = static_cast<int64_t>(w.bh) * T + ra;
   if (parts > 1) {
@@ -689,10 +691,10 @@ hipError_t run_bwd(const LatentArgs& a, hipStream_t s) {
   const int64_t nkb = a.cu_q ? static_cast<int64_t>(a.Tk) / BM + a.n_seqs : (static_cast<int64_t>(a.Tk) + BM - 1) / BM;
   if (bh <= 0) return hipSuccess;
   if (a.Tq > 0)
-    kda_latent_dq_kernel<DT, DN, DR><<<dim3(static_cast<unsigned>(nqb * bh), a.splits), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
+    kda_latent_dq_kernel<DT, DN, DR><<<a.share > 0 ? dim3(static_cast<unsigned>(a.live * bh)) : dim3(static_cast<unsigned>(nqb * bh), a.splits), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
   if (a.Tk > 0)
     kda_latent_dkv_kernel<DT, DN, DR>
-        <<<dim3(static_cast<unsigned>(nkb * bh), a.splits_k), dim3(KeyCfg<DT, DN, DR>::NT), 0, s>>>(a, static_cast<int>(nkb));
+        <<<a.share_k > 0 ? dim3(static_cast<unsigned>(a.live_k * bh)) : dim3(static_cast<unsigned>(nkb * bh), a.splits_k), dim3(KeyCfg<DT, DN, DR>::NT), 0, s>>>(a, static_cast<int>(nkb));
   const int64_t blocks = (nkb + (a.splits > 1 ? nqb : 0)) * bh;
   if (blocks > 0)
     kda_latent_sums_kernel<DT, DN, DR>

@@ -47,7 +47,8 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
   const int m = lane & 31, h = lane >> 5;
 
   Where w;
-  if (!locate(a, blockIdx.x, nqb, C::BM, true, true, w)) return;
+  int z;
+  if (!locate_share(a, nqb, C::BM, BN, true, true, w, z)) return;
   const int b = w.b, head = w.head, q0 = w.r0, qe = w.re, off = w.off, nk = w.ke - w.k0;
   const int row = q0 + wave * 32 + m;         // this lane's query
   const bool live = row < qe;
@@ -56,9 +57,9 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
   const int wave_hi = a.causal ? min(nk - 1, min(q0 + wave * 32 + 31, qe - 1) + off) : nk - 1;
   const int blk_hi = a.causal ? min(nk - 1, min(q0 + C::BM - 1, qe - 1) + off) : nk - 1;
   // key tiles of the block (none when no query sees a key) and this workgroup's
-  const Share part(max(0, (blk_hi + BN) / BN), a.splits, blockIdx.y);
+  const Share part(max(0, (blk_hi + BN) / BN), a.splits, a.share, z);
   const int nt = part.j1;
-  if (static_cast<int>(blockIdx.y) >= part.parts) return;
+  if (z >= part.parts) return;
 
   F qn[KN], qr[KR];
   {
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
   l = half_sum(l);
   if (!live) return;
   if (part.parts > 1) {
-    const int64_t pr = (static_cast<int64_t>(blockIdx.y) * a.B * a.H + w.bh) * a.Tq + row;
+    const int64_t pr = (static_cast<int64_t>(z) * a.B * a.H + w.bh) * a.Tq + row;
 #pragma unroll
     for (int n = 0; n < ND; ++n)
 #pragma unroll
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(256) void kda_latent_fwd_join_kernel(LatentArgs a, 
   Where w;
   if (!locate(a, blockIdx.x, nqb, C::BM, true, true, w)) return;
   const int nk = w.ke - w.k0, blk_hi = a.causal ? min(nk - 1, min(w.r0 + C::BM - 1, w.re - 1) + w.off) : nk - 1;
-  const int parts = Share(max(0, (blk_hi + C::BN) / C::BN), a.splits, 0).parts;
+  const int parts = Share(max(0, (blk_hi + C::BN) / C::BN), a.splits, a.share, 0).parts;
   if (parts == 1) return;
   const int col = (threadIdx.x % LPR) * 4;
   const int64_t step = static_cast<int64_t>(a.B) * a.H * a.Tq;
@@ -244,7 +245,7 @@ hipError_t run_fwd(const LatentArgs& a, hipStream_t s) {
   const int64_t grid = nqb * a.B * a.H;
   if (grid <= 0) return hipSuccess;
   const unsigned gx = static_cast<unsigned>(grid);
-  kda_latent_fwd_kernel<DT, DN, DR><<<dim3(gx, a.splits), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
+  kda_latent_fwd_kernel<DT, DN, DR><<<a.share > 0 ? dim3(static_cast<unsigned>(a.live * a.B * a.H)) : dim3(gx, a.splits), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
   if (a.splits > 1) kda_latent_fwd_join_kernel<DT, DN, DR><<<dim3(gx, 8), dim3(256), 0, s>>>(a, static_cast<int>(nqb));
   return hipGetLastError();
 }

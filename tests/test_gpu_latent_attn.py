@@ -63,6 +63,13 @@ def test_strided_inputs(cuda, dtype):
     _compare(q, kv, kr, do, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("Tq,Tk,H", [(700, 1100, 2), (900, 500, 3), (1000, 1000, 8), (8400, 8400, 1)])
+def test_uneven_causal_walks(cuda, dtype, Tq, Tk, H):
+    """Few blocks with walks of different lengths, shared out in equal pieces; 8400 rows: more blocks than lanes."""
+    _compare(*attn_inputs(1, Tq, Tk, H, 64, 32, dtype, cuda, seed=Tq + H), dtype)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_queries_without_keys(cuda, dtype):
     """Causal with more queries than keys: the first rows see none."""
