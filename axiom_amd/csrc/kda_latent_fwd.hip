@@ -15,7 +15,7 @@
 // 1.12 PFLOP/s over the pairs it has to form (an 8192^3 product reaches 1.19);
 // B4 H16 T4096 340 us, 1.01.  128 queries a workgroup and two workgroups a CU,
 // because a wave's 32 queries, their output and a score tile are 256 registers.
-// fp32 (products 16 times as slow, one workgroup a CU): B1 H8 T1024 53 us.
+// fp32 (products 16 times as slow, one workgroup a CU): B1 H8 T1024 39 us.
 
 #include "kda_internal.h"
 #include "kda_latent.h"
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
 }
 
 // Joins the parts of split blocks, in part order; an eighth of a block a workgroup.
-// Bound by its launch and one round of loads: 4 to 7 us.
+// Bound by its launch and one round of loads: 4 to 9 us.
 template <int DT, int DN, int DR>
 __global__ __launch_bounds__(256) void kda_latent_fwd_join_kernel(LatentArgs a, int nqb) {
   typedef FwdCfg<DT, DN, DR> C;
