@@ -158,6 +158,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   // (T = 1000, causal, d 64: dq's error 1.53 times its output's rounding with the
   // one, below 1.5 with the other).  Two tiles, both in LDS.
   if (ES == 2 && blk_hi < 2 * BN && nt > 0) {   // a walk this short is never shared out
+    if constexpr (DT == 2) lds_barrier();         // buf1 held the |do|: read by now
     fetch(0, buf0);
     if (nt == 2) fetch(1, buf1);
     wait_vmem_all();
