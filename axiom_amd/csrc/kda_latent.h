@@ -119,6 +119,11 @@ __device__ __forceinline__ void wait_vmem_but() {
   __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
+// A barrier between LDS reads whose values have been used and writes to their
+// places: it waits for nothing.  lds_barrier would wait for the copies on their way
+// too, which are LDS writes to the compiler.
+__device__ __forceinline__ void reuse_barrier() { asm volatile("s_barrier" : : : "memory"); }
+
 // value combined over the two halves of the wave (lane l and l ^ 32)
 __device__ __forceinline__ float half_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

@@ -287,10 +287,14 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
 // wave that holds all of it (240 registers and the scores) is alone on its SIMD
 // and had the matrix cores busy 32 % of the time.  A tile behind, because with p
 // handed over inside a tile's turn both waves wait twice for each other (40 %).
-// p crosses in fp16, times 2^12 (dv and g take the factor out): within 2^-12 of
-// itself down to 2^-26.  That is an eighth of the rounding that g gets next in
-// bf16, and as much again in fp16 (dk's error 3.6e-4, where g's and the output's
-// roundings alone make 3.0e-4; p in fp32 would need more LDS than a CU has).
+// p carries a factor of 2^12 (dv and g take it out).  bf16: it crosses in fp16,
+// within 2^-11 of itself down to 2^-26, an eighth of the rounding that g gets
+// next.  fp16: it crosses in fp32, since another rounding of g's own size made
+// dk's error 1.2 times what it has to be.  Its two tiles by parity do not fit
+// beside d = 128's buffers: there one place serves both, and a second barrier in
+// the middle of a turn parts the second wave's reads, before its dk products,
+// from the first wave's writes, after its score products (B4 H16 T4096 fp16, both
+// passes: 1494 us with p in fp16, 1525 with this).
 // Three query tiles in LDS: arriving, present, behind.
 // fp32: operands twice as large and products 16 times as slow, so one wave does it all.
 template <int DT, int DN, int DR>
@@ -299,7 +303,9 @@ struct KeyCfg : BwdCfg<DT, DN, DR> {
   static constexpr bool PAIR = B::ES == 2;
   static constexpr int NT = PAIR ? 512 : 256, NWV = NT / 64;
   static constexpr int P_LOG2 = PAIR ? 12 : 0;            // p's factor
-  static constexpr int P_BYTES = PAIR ? 4 * 4096 : 16;    // p of a tile: 64 x 32 fp16 a pair
+  static constexpr int P_ES = DT == 2 ? 4 : 2, P_PAIR = 64 * 32 * P_ES;   // p of a tile, a pair's: in fp32 or fp16
+  static constexpr int P_BUFS = DT == 2 && DN == 128 ? 1 : 2;             // by tile parity, or one place and a barrier more
+  static constexpr int P_BYTES = PAIR ? 4 * P_PAIR : 16;
 };
 
 template <int DT, int DN, int DR>
@@ -311,7 +317,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   __shared__ __attribute__((aligned(1024))) char buf0[C::BUF_K];
   __shared__ __attribute__((aligned(1024))) char buf1[C::BUF_K];
   __shared__ __attribute__((aligned(1024))) char buf2[C::PAIR ? C::BUF_K : 16];
-  __shared__ __attribute__((aligned(1024))) char pbuf[2][C::P_BYTES];   // by tile parity
+  __shared__ __attribute__((aligned(1024))) char pbuf[C::P_BUFS][C::P_BYTES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 31, h = lane >> 5, own = wave & 3, role = wave >> 2;
   Where w;
@@ -444,7 +450,9 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
 
   if (j0 < nt) fetch(j0, buf0);
   if constexpr (C::PAIR) {
-    const int mine = own * 4096 + lane * 16;
+    const int mine = own * C::P_PAIR + lane * 16;
+    constexpr bool MID = C::P_BUFS == 1;
+    auto place_of = [&](int j) -> char* { return pbuf[MID ? 0 : j & 1] + mine; };
     if (role == 0) {
       F kn[KN], kr[KR];
 #pragma unroll
@@ -474,6 +482,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
             for (int t = 0; t < 2; ++t) s[t] = mma(s[t], C::TR::template row_frag<F>(cur + C::OFF_R, fm, k, fh, 32 * t), kr[k]);
           pace<2 * (KN + KR), 6, 1, 1>();
           __builtin_amdgcn_sched_barrier(0);
+          if constexpr (MID) reuse_barrier();     // the second wave has read the last tile's p
           const bool edge = qt < wave_full || qt + BN > nq;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
@@ -482,14 +491,17 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
             frags(s[t], pf[t]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              h8 x;
+              char* const to = place_of(j) + (2 * t + u) * (512 * C::P_ES);
               if constexpr (DT == 2) {
-                x = pf[t][u];
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+                  *reinterpret_cast<f4*>(to + 1024 * v) = f4{s[t][8 * u + 4 * v], s[t][8 * u + 4 * v + 1], s[t][8 * u + 4 * v + 2], s[t][8 * u + 4 * v + 3]};
               } else {
+                h8 x;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = static_cast<_Float16>(s[t][8 * u + e]);
+                *reinterpret_cast<h8*>(to) = x;
               }
-              *reinterpret_cast<h8*>(pbuf[j & 1] + mine + (2 * t + u) * 1024) = x;
             }
           }
           __builtin_amdgcn_sched_barrier(0);
@@ -500,6 +512,8 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
               dv[n] = mma(dv[n], C::TN::template col_frag<F>(cur + C::OFF_V, 16 * u, 32 * n, ln), pf[u >> 1][u & 1]);
           pace<4 * ND, 4, 2, 1>();
           __builtin_amdgcn_sched_barrier(0);
+        } else if constexpr (MID) {
+          reuse_barrier();
         }
       };
       for (int j = j0; j < nt + 1 && j0 < nt;) {
@@ -531,9 +545,19 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
             f16v p;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const h8 x = *reinterpret_cast<const h8*>(pbuf[(j - 1) & 1] + mine + (2 * t + u) * 1024);
+              const char* const from = place_of(j - 1) + (2 * t + u) * (512 * C::P_ES);
+              if constexpr (DT == 2) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) p[8 * u + e] = static_cast<float>(x[e]);
+                for (int v = 0; v < 2; ++v) {
+                  const f4 x = *reinterpret_cast<const f4*>(from + 1024 * v);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) p[8 * u + 4 * v + e] = x[e];
+                }
+              } else {
+                const h8 x = *reinterpret_cast<const h8*>(from);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[8 * u + e] = static_cast<float>(x[e]);
+              }
             }
             if (edge) adjoint(prev, t, fh, true, p, dp[t]);
             else adjoint(prev, t, fh, false, p, dp[t]);
@@ -552,6 +576,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
           pace<4 * (ND + NR), 4, 2, 1>();
           __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (MID) reuse_barrier();     // the last tile's p has been read
         if (j < nt) {
           zero(dp[0]);
           zero(dp[1]);
