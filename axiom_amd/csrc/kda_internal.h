@@ -319,8 +319,6 @@ struct LatentArgs {
   const void* dout;
   const float* lse_in;
   float* D;                // sum over dn of do * o
-  float* dmax;             // fp16: largest |do| of each query block, [B*H][dmax_n]
-  int dmax_n;
   float* dkr_part;         // [splits][B,H,Tk,dr]: each head's share of the rotary key's gradient
   int splits_k, share_k, live_k;   // the key pass' (those above and `part` are the query pass')
   float* part_k;

@@ -131,16 +131,16 @@ FwdLayout fwd_layout(int B, int Tq, int Tk, int H, int dn, int n_seqs, bool caus
   L.total = L.ml + align_up(rows * 8);
   return L;
 }
-struct BwdLayout { Shares q, k; int64_t blocks; size_t D, dmax, dkr, part, part_k, total; };
+struct BwdLayout { Shares q, k; size_t D, dkr, part, part_k, total; };
 BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dn, int dr, int n_seqs, bool causal, int dtype) {
   BwdLayout L{};
   const size_t bh = static_cast<size_t>(B) * H;
   L.q = shares_of(true, Tq, Tk, static_cast<int64_t>(bh), n_seqs, causal, dtype);
   L.k = shares_of(false, Tq, Tk, static_cast<int64_t>(bh), n_seqs, causal, dtype);
   L.D = 0;
-  L.dmax = align_up(bh * Tq * 4);
-  L.blocks = blocks_of(Tq, n_seqs);
-  L.dkr = L.dmax + align_up(bh * L.blocks * 4);
+  // after D, room for 4 bytes a query block that no kernel uses: the size of a
+  // workspace stays what it was while one did
+  L.dkr = align_up(bh * Tq * 4) + align_up(bh * blocks_of(Tq, n_seqs) * 4);
   L.part = L.dkr + align_up(L.k.parts * bh * Tk * dr * 4);
   L.part_k = L.part + align_up(L.q.parts > 1 ? L.q.parts * bh * Tq * (dn + dr) * 4 : 0);
   L.total = L.part_k + align_up(L.k.parts > 1 ? L.k.parts * bh * Tk * 2 * dn * 4 : 0) + 256;
@@ -229,8 +229,6 @@ int kda_latent_attn_bwd(hipStream_t stream, const void* q, const void* kv, const
   char* ws = static_cast<char*>(workspace);
   a.o_in = o; a.lse_in = lse; a.dout = d_o;
   a.D = reinterpret_cast<float*>(ws + L.D);
-  a.dmax = reinterpret_cast<float*>(ws + L.dmax);
-  a.dmax_n = static_cast<int>(L.blocks);
   a.dkr_part = reinterpret_cast<float*>(ws + L.dkr);
   a.part = reinterpret_cast<float*>(ws + L.part);
   a.part_k = reinterpret_cast<float*>(ws + L.part_k);

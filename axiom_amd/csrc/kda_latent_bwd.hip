@@ -13,10 +13,12 @@
 // against an fp32 dq kept in memory and added to by every key block.
 //
 // p and g are rounded to the inputs' type for the products they enter; sums
-// are fp32.  For fp16, whose smallest value is 6e-8, g is formed from do
-// scaled by a power of two that brings the largest |do| (the query's, in the key
-// pass the head's) near 1, and the sums are scaled back: p of a long row times a
-// small do would vanish otherwise.
+// are fp32.  fp16, whose values lie between 6e-8 and 65504, takes g times a power
+// of two of its own for every column of g, that is for every query in the query
+// pass and every key in the key pass: as a running maximum, it follows the
+// column's largest |g| so far, and the column's sum is rescaled where it falls.
+// What a query's do or another sequence holds is then nothing to a key that does
+// not see it, and neither a small do nor large values cost the operand its range.
 
 #include "kda_internal.h"
 #include "kda_latent.h"
@@ -24,19 +26,15 @@
 namespace kda {
 namespace latent {
 
-// fp16: the power of two that brings t, the largest |do|, into [1, 2); 1 where
-// there is none (zeros, or a value that is not finite)
-__device__ __forceinline__ float to_one(float t) {
-  if (!(t > 0.f) || t > 65504.f) return 1.f;
-  return __uint_as_float((254u << 23) - (__float_as_uint(t) & 0x7F800000u));
+// fp16: a column's factor.  It starts high, and where the largest |g| times it
+// passes 2^15 it becomes the power of two that brings that |g| into [2^10, 2^11),
+// five powers below, so that it seldom changes.  A |g| that is not finite leaves it.
+constexpr float kFactor0 = 0x1p100f;
+__device__ __forceinline__ bool past(float top, float f) { return top * f > 0x1p15f; }
+__device__ __forceinline__ float factor(float top, float f) {
+  return past(top, f) && top <= 3.4028234e38f ? __uint_as_float((264u << 23) - (__float_as_uint(top) & 0x7F800000u)) : f;
 }
-__device__ __forceinline__ float do_factor(const LatentArgs& a, int bh) {
-  float t = 0.f;
-  for (int i = __lane_id(); i < a.dmax_n; i += 64) t = fmaxf(t, a.dmax[static_cast<int64_t>(bh) * a.dmax_n + i]);
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) t = fmaxf(t, __shfl_xor(t, s, 64));
-  return to_one(t);
-}
+__device__ __forceinline__ float inverse(float f) { return __uint_as_float((254u << 23) - __float_as_uint(f)); }   // of a power of two
 
 template <int DT, int DN, int DR>
 struct BwdCfg {
@@ -68,10 +66,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   const int m = lane & 31, h = lane >> 5;
   Where w;
   int z;
-  if (!locate_share(a, nqb, C::BM, BN, true, true, w, z)) {
-    if (DT == 2 && z == 0 && threadIdx.x == 0) a.dmax[static_cast<int64_t>(w.bh) * nqb + w.blk] = 0.f;
-    return;
-  }
+  if (!locate_share(a, nqb, C::BM, BN, true, true, w, z)) return;
   const int nk = w.ke - w.k0;
   const int row = w.r0 + wave * 32 + m;
   const bool live = row < w.re;
@@ -98,36 +93,16 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   }
   const int64_t ri = static_cast<int64_t>(w.bh) * a.Tq + crow;
   const float lse2 = a.lse_in[ri] * kLog2e;
-  // D of this lane's query, for the key pass too, and the factor of its g
-  float D = 0.f, gf = 1.f;
+  float D = 0.f, gf = kFactor0;   // D of this lane's query, for the key pass too, and the factor of its g
   {
     const E* op = static_cast<const E*>(a.o_in) + ((static_cast<int64_t>(w.b) * a.Tq + crow) * a.H + w.head) * DN;
-    float top = 0.f;
 #pragma unroll
     for (int s = 0; s < KN; ++s) {
       const F o = *reinterpret_cast<const F*>(op + 16 * s + 8 * h);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        D = fmaf(static_cast<float>(dO[s][e]), static_cast<float>(o[e]), D);
-        if constexpr (DT == 2) top = fmaxf(top, fabsf(static_cast<float>(dO[s][e])));
-      }
+      for (int e = 0; e < 8; ++e) D = fmaf(static_cast<float>(dO[s][e]), static_cast<float>(o[e]), D);
     }
     D = half_sum(D);
-    if constexpr (DT == 2) {
-      top = half_max(top);
-      gf = to_one(top);
-    }
-    if (z == 0) {
-      if constexpr (DT == 2) {
-        float* const tops = reinterpret_cast<float*>(buf1);   // two workgroups' LDS leave no byte of a CU's
-#pragma unroll
-        for (int s = 1; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
-        if (lane == 0) tops[wave] = top;
-        lds_barrier();
-        if (threadIdx.x == 0)
-          a.dmax[static_cast<int64_t>(w.bh) * nqb + w.blk] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      }
-    }
   }
 
   const char* kvp = static_cast<const char*>(a.kv) + (w.b * a.kv_b + w.k0 * a.kv_t + w.head * a.kv_h) * ES;
@@ -158,7 +133,6 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
   // (T = 1000, causal, d 64: dq's error 1.53 times its output's rounding with the
   // one, below 1.5 with the other).  Two tiles, both in LDS.
   if (ES == 2 && blk_hi < 2 * BN && nt > 0) {   // a walk this short is never shared out
-    if constexpr (DT == 2) lds_barrier();         // buf1 held the |do|: read by now
     fetch(0, buf0);
     if (nt == 2) fetch(1, buf1);
     wait_vmem_all();
@@ -214,14 +188,27 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
       if constexpr (ES == 2) pace<2 * KN + KR, 4, 1, 1>();
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = fast_exp2(fmaf(s[i], c, -lse2)) * (dp[i] - D);
-        if constexpr (DT == 2) s[i] *= gf;
-      }
+      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], c, -lse2)) * (dp[i] - D);
       if (kt + 32 * t + 31 > wave_lo) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (kt + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) > kmax) s[i] = 0.f;
+      }
+      if constexpr (DT == 2) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(s[i]));
+        top = half_max(top);
+        if (__any(past(top, gf))) {
+          const float nf = factor(top, gf), al = nf * inverse(gf);
+          gf = nf;
+#pragma unroll
+          for (int n = 0; n < ND + NR; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[n][i] *= al;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] *= gf;
       }
       F gq[2];
 #pragma unroll
@@ -253,7 +240,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
     ++j;
   }
   if (!live) return;
-  const float f = a.scale / gf;
+  const float f = DT == 2 ? a.scale * inverse(gf) : a.scale;
   if (part.parts > 1) {
     const int64_t pb = ((static_cast<int64_t>(z) * a.B * a.H + w.bh) * a.Tq + row) * (DN + DR) + 4 * h;
 #pragma unroll
@@ -335,7 +322,6 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   if (z >= part.parts) return;
   const int j0 = jf + part.j0, nt = jf + part.j1;
   const float c = a.scale * kLog2e;
-  const float gf = DT == 2 ? do_factor(a, w.bh) : 1.f;
   constexpr float unp = 1.f / (1 << C::P_LOG2);
 
   const char* qp = static_cast<const char*>(a.q) + (w.b * a.q_b + w.k0 * a.q_t + w.head * a.q_h) * ES;
@@ -376,7 +362,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
   const E* kp = static_cast<const E*>(a.kv) + w.b * a.kv_b + static_cast<int64_t>(ckey) * a.kv_t + w.head * a.kv_h + 8 * h;
   const E* rp = static_cast<const E*>(a.kr) + w.b * a.kr_b + static_cast<int64_t>(ckey) * a.kr_t + 8 * h;
   const int64_t ob = ((static_cast<int64_t>(w.b) * a.Tk + key) * a.H + w.head) * (2 * DN) + 4 * h;
-  const float f = a.scale * (DT == 1 ? unp : 1.f / gf);   // fp16: g holds gf and no factor of p
+  float gf = kFactor0;                                    // fp16: factor of this lane's key, above p's
 
   // p of a score tile, from s; rows q0 .. of the sequence, rows 32 t .. of the tile
   auto probs = [&](const char* cur, int q0, int t, int fh, bool edge, f16v& s) {
@@ -402,8 +388,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * v + e;
-        float g = p[i] * (dp[i] - dd[e]);
-        if constexpr (DT == 2) g *= gf * unp;
+        const float g = p[i] * (dp[i] - dd[e]);
         dp[i] = edge && p[i] == 0.f ? 0.f : g;
       }
     }
@@ -435,6 +420,7 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
       for (int i = 0; i < 4; ++i) put4(DN + 32 * n + 8 * i, dv[n][4 * i] * unp, dv[n][4 * i + 1] * unp, dv[n][4 * i + 2] * unp, dv[n][4 * i + 3] * unp);
   };
   auto put_dk = [&](const f16v (&dk)[ND + NR]) {
+    const float f = DT == 2 ? a.scale * unp * inverse(gf) : a.scale * unp;
 #pragma unroll
     for (int n = 0; n < ND; ++n)
 #pragma unroll
@@ -561,7 +547,27 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
             }
             if (edge) adjoint(prev, t, fh, true, p, dp[t]);
             else adjoint(prev, t, fh, false, p, dp[t]);
-            frags(dp[t], gq[t]);
+            if constexpr (DT != 2) frags(dp[t], gq[t]);
+          }
+          if constexpr (DT == 2) {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(dp[i >> 4][i & 15]));
+            top = half_max(top);
+            if (__any(past(top, gf))) {
+              const float nf = factor(top, gf), al = nf * inverse(gf);
+              gf = nf;
+#pragma unroll
+              for (int n = 0; n < ND + NR; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dk[n][i] *= al;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) dp[t][i] *= gf;
+              frags(dp[t], gq[t]);
+            }
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
