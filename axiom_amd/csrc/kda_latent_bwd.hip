@@ -240,6 +240,12 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
     ++j;
   }
   if (!live) return;
+  if (kmax < part.j0 * BN) {   // no visible key: zeros, whatever 0 times the others' values made
+#pragma unroll
+    for (int n = 0; n < ND + NR; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
+  }
   const float f = DT == 2 ? a.scale * inverse(gf) : a.scale;
   if (part.parts > 1) {
     const int64_t pb = ((static_cast<int64_t>(z) * a.B * a.H + w.bh) * a.Tq + row) * (DN + DR) + 4 * h;

@@ -493,10 +493,11 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
 #pragma unroll
       for (int x = 0; x < SP; ++x) ls = fmaf(fast_exp2((red[0][x][m] - mx) * c), red[1][x][m], ls);
       if (r < rows) {
-        const float inv = ls > 0.f ? 1.f / ls : ls;   // nothing visible: zeros; NaN stays NaN
+        const float inv = ls > 0.f ? 1.f / ls : ls;   // NaN stays NaN
         const int64_t row = static_cast<int64_t>(b) * rows + r;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
+          if (ls == 0.f) acc[v] = f4{0, 0, 0, 0};     // nothing visible: zeros, whatever 0 times the others' rows made
           const int at = col + 16 * v + 4 * gq;
           if (whole) store4<DT>(a.o, row * R + at, acc[v][0] * inv, acc[v][1] * inv, acc[v][2] * inv, acc[v][3] * inv);
           else *reinterpret_cast<f4*>(a.part_o + (srow + m) * R + at) = acc[v];
@@ -750,12 +751,13 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
         const float ls = ml[1][32 * n + m];
         const int64_t row = static_cast<int64_t>(b) * rows + r;
         const int col = own * (R / 4) + 4 * h;
-        const float inv = ls > 0.f ? 1.f / ls : ls;   // nothing visible: zeros; NaN stays NaN
+        const float inv = ls > 0.f ? 1.f / ls : ls;   // NaN stays NaN
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const f4 o = {acc[v][n][4 * e], acc[v][n][4 * e + 1], acc[v][n][4 * e + 2], acc[v][n][4 * e + 3]};
+            f4 o = {acc[v][n][4 * e], acc[v][n][4 * e + 1], acc[v][n][4 * e + 2], acc[v][n][4 * e + 3]};
+            if (ls == 0.f) o = f4{0, 0, 0, 0};         // nothing visible: zeros, whatever 0 times the others' rows made
             if (whole) store4<DT>(a.o, row * R + col + 32 * v + 8 * e, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
             else *reinterpret_cast<f4*>(a.part_o + (srow + 32 * n + m) * R + col + 32 * v + 8 * e) = o;
           }

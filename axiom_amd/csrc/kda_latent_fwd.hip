@@ -181,6 +181,12 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
 
   l = half_sum(l);
   if (!live) return;
+  if (l == 0.f) {   // no visible key: zeros, whatever 0 times the others' values made
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
+  }
   if (part.parts > 1) {
     const int64_t pr = (static_cast<int64_t>(z) * a.B * a.H + w.bh) * a.Tq + row;
 #pragma unroll
@@ -191,7 +197,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
     if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(mc, l);
     return;
   }
-  const float inv = l > 0.f ? 1.f / l : l;      // no visible key: zeros; NaN stays NaN
+  const float inv = l > 0.f ? 1.f / l : l;      // NaN stays NaN
   const int64_t ob = ((static_cast<int64_t>(b) * a.Tq + row) * a.H + head) * DN + 4 * h;
 #pragma unroll
   for (int n = 0; n < ND; ++n)

@@ -54,7 +54,8 @@ def latent_attn_fwd(q, kv, k_rope, cu_seqlens=None, cu_seqlens_k=None, causal: b
     last axis contiguous, other strides free (multiples of 16 bytes).  ``o
     [B,Tq,H,dn]`` in that dtype; ``lse [B,H,Tq]`` fp32, natural logarithm.
     ``causal``: query i sees keys ``j <= i + Tk - Tq``.  A query that sees no key
-    gets zeros and ``-inf``.  ``cu_seqlens`` (int32 ``[N+1]`` on the device, B ==
+    gets zeros and ``-inf``, whatever the keys hold; else values that are not finite
+    may reach rows of the same sequence that do not see them.  ``cu_seqlens`` (int32 ``[N+1]`` on the device, B ==
     1) packs N sequences; ``cu_seqlens_k`` its key offsets where they differ.
     ``scale``: default ``(dn + dr) ** -0.5``.  dn in {64, 128}, dr in {32, 64}.
     ``out`` / ``lse``: optional preallocated outputs; ``workspace``: an optional

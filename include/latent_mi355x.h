@@ -29,7 +29,11 @@ extern "C" {
  * of eight element strides: q's (batch, token, head), kv's (batch, token,
  * head), k_rope's (batch, token).  o [B,Tq,H,dn] in dtype, contiguous; lse
  * [B,H,Tq] fp32.  causal != 0: query i sees keys j <= i + Tk - Tq (the last
- * query sees all).  A query that sees no key gets o = 0 and lse = -inf.
+ * query sees all).  A query that sees no key gets o = 0 and lse = -inf (dq = 0),
+ * whatever the keys hold.  Else a masked pair enters the products of its tile
+ * with weight 0: values that are not finite in a key, query or cotangent may
+ * reach rows of the same sequence that do not see them, never those of another
+ * batch element or packed sequence.
  * cu_q, cu_k (both or neither; int32 [n_seqs+1] on the device, B == 1) pack
  * n_seqs sequences, sequence i being rows cu[i] .. cu[i+1] of its axis; the
  * first offset is 0 and the last the axis' length.  Offsets are clamped so
@@ -97,7 +101,8 @@ KDA_API int kda_latent_append(hipStream_t stream, const void* rows, int64_t rows
  * ones among them):
  *   s_j = scale q . row_j,  o = sum_j softmax_j(s) row_j[:R],  lse as above.
  * Token t sees the first seq_len - (Tq - 1 - t) rows; with none, o = 0 and
- * lse = -inf.  o [B,Tq,H,R] in dtype, lse [B,Tq,H] fp32; all contiguous.
+ * lse = -inf, whatever the rows hold (else a row of the newest Tq that is not
+ * finite may reach the earlier tokens of its sequence).  o [B,Tq,H,R] in dtype, lse [B,Tq,H] fp32; all contiguous.
  * Lengths are clamped into [0, max_pages * page_size] and page numbers into
  * [0, n_pages), so no access leaves the tensors.  R in {256, 512}, dr in {32,
  * 64}, page_size a power of two, n_pages * page_size < 2^31, scale > 0 and
