@@ -11,6 +11,7 @@
 
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/python.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <optional>
@@ -76,6 +77,8 @@ at::Device one_gpu(const char* what, const Tensor& first, const T&... rest) {
   return d;
 }
 
+// A call launches on the device that is current, and the default stream's handle
+// names none: every entry point makes the tensors' device current while it runs.
 hipStream_t stream_of(at::Device d) { return c10::hip::getCurrentHIPStream(d.index()).stream(); }
 
 Tensor output(const char* what, const char* name, const OptTensor& t, at::IntArrayRef shape, at::ScalarType dt, at::Device d) {
@@ -149,6 +152,7 @@ std::tuple<Tensor, Tensor> attn_fwd(const Tensor& q, const Tensor& kv, const Ten
   const char* what = "latent_attn_fwd";
   const Attn a = attn_check(what, q, kv, kr, cu_q, cu_k, scale);
   const at::Device d = one_gpu(what, q, kv, kr, a.cu_q, a.cu_k);
+  const c10::DeviceGuard on(d);
   Tensor o = output(what, "out", out, {a.B, a.Tq, a.H, a.dn}, q.scalar_type(), d);
   Tensor lse = output(what, "lse", lse_out, {a.B, a.H, a.Tq}, at::kFloat, d);
   const size_t bytes = kda_latent_attn_fwd_workspace(a.B, a.Tq, a.Tk, a.H, a.dn, a.dr, a.n_seqs, a.code);
@@ -175,6 +179,7 @@ std::tuple<Tensor, Tensor, Tensor> attn_bwd(const Tensor& q, const Tensor& kv, c
   if (lse.sizes() != at::IntArrayRef(rows, 3) || lse.scalar_type() != at::kFloat) refuse(what, "lse must be fp32 ", at::IntArrayRef(rows, 3));
   contiguous("lse", lse);
   const at::Device d = one_gpu(what, q, kv, kr, o, lse, d_o, a.cu_q, a.cu_k);
+  const c10::DeviceGuard on(d);
   const size_t bytes = kda_latent_attn_bwd_workspace(a.B, a.Tq, a.Tk, a.H, a.dn, a.dr, a.n_seqs, a.code);
   const Tensor ws = work(workspace, bytes, d);
   const auto opt = q.options().requires_grad(false);
@@ -253,6 +258,7 @@ OptTensor append(const Tensor& rows, const Tensor& positions, const Tensor& slot
     refuse(what, "q_out requires q_rope");
   }
   const at::Device d = one_gpu(what, rows, positions, slots, cos_sin, cache, weight, q, q_out);
+  const c10::DeviceGuard on(d);
   checked(kda_latent_append(stream_of(d), ptr(rows), rows.stride(0), static_cast<const int64_t*>(ptr(positions)),
                             static_cast<const int64_t*>(ptr(slots)), static_cast<const float*>(ptr(cos_sin)), cos_sin.size(0),
                             static_cast<const float*>(ptr(weight)), static_cast<float>(eps), ptr(cache), cache.size(0) * cache.size(1),
@@ -278,6 +284,7 @@ std::tuple<Tensor, Tensor> decode(const Tensor& q, const Tensor& cache, const Te
   contiguous("block_table", table);
   contiguous("seq_lens", lens);
   const at::Device d = one_gpu(what, q, cache, table, lens);
+  const c10::DeviceGuard on(d);
   const int page = static_cast<int>(cache.size(1)), per = static_cast<int>(table.size(1));
   const size_t bytes = kda_latent_decode_workspace(B, Tq, H, R, W - R, page, per, code);
   const Tensor ws = work(workspace, bytes, d);
