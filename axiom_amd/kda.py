@@ -58,6 +58,18 @@ def _stream(device):
     return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _call(entry, device, *args):
+    """An entry point of the library on the device's current stream, with that device current: a launch
+    goes to the current device, and the default stream's handle names none."""
+    if _current_device() == device.index:
+        return entry(_stream(device), *args)
+    with torch.cuda.device(device):
+        return entry(_stream(device), *args)
+
+
 def _require_gpu(tensors, what: str) -> torch.device:
     """The one GPU all tensors are on; raises as :func:`_wrong_device` otherwise."""
     index = dev = None
@@ -208,15 +220,15 @@ def kda_chunk_fwd(q, k, v, g, beta, initial_state=None, cu_seqlens=None, chunk_s
         ht = final_state
     else:
         ht = torch.empty((N, H, dk, dv), dtype=torch.float32, device=dev)
-    rc = L.kda_chunk_fwd(_stream(dev), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta),
-                         _ptr(initial_state), _ptr(cu_seqlens), n_seqs, _ptr(o), _ptr(ht),
-                         B, T, H, dk, dv, CHUNK, float(scale), in_code, _OUT_CODES[out_dtype],
-                         _ptr(workspace), ws_bytes)
+    rc = _call(L.kda_chunk_fwd, dev, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta),
+               _ptr(initial_state), _ptr(cu_seqlens), n_seqs, _ptr(o), _ptr(ht),
+               B, T, H, dk, dv, CHUNK, float(scale), in_code, _OUT_CODES[out_dtype],
+               _ptr(workspace), ws_bytes)
     _lib.check(rc, what)
     if check_finite:
         flags = ctypes.c_int32(0)
-        rc = L.kda_chunk_fwd_status(_stream(dev), _ptr(workspace), ws_bytes, B, T, H, dk, dv, CHUNK,
-                                    n_seqs, in_code, ctypes.byref(flags))
+        rc = _call(L.kda_chunk_fwd_status, dev, _ptr(workspace), ws_bytes, B, T, H, dk, dv, CHUNK,
+                   n_seqs, in_code, ctypes.byref(flags))
         _lib.check(rc, "kda_chunk_fwd_status")
         if flags.value & _lib.KDA_STATUS_NONFINITE:
             raise ValueError(f"{what}: non-finite result: an fp16 operand left its range (16-bit inputs "
@@ -288,11 +300,11 @@ def _chunk_bwd(q, k, v, g, beta, do, dht, initial_state, scale, chunk_size, need
     dg = torch.empty((B, T, H, dk), dtype=gate_dtype, device=dev)
     dbeta = torch.empty((B, T, H), dtype=gate_dtype, device=dev)
     dh0 = torch.empty((B, H, dk, dv), dtype=torch.float32, device=dev) if need_dh0 else None
-    rc = L.axiom_chunk_bwd(_stream(dev), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta),
-                         _ptr(initial_state), _ptr(do), _ptr(dht),
-                         _ptr(dq), _ptr(dk_), _ptr(dv_), _ptr(dg), _ptr(dbeta), _ptr(dh0),
-                         B, T, H, dk, dv, CHUNK, float(scale), in_code, _OUT_CODES[do.dtype],
-                         _IN_CODES[qkv_dtype], _IN_CODES[gate_dtype], _ptr(workspace), ws_bytes)
+    rc = _call(L.axiom_chunk_bwd, dev, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta),
+               _ptr(initial_state), _ptr(do), _ptr(dht),
+               _ptr(dq), _ptr(dk_), _ptr(dv_), _ptr(dg), _ptr(dbeta), _ptr(dh0),
+               B, T, H, dk, dv, CHUNK, float(scale), in_code, _OUT_CODES[do.dtype],
+               _IN_CODES[qkv_dtype], _IN_CODES[gate_dtype], _ptr(workspace), ws_bytes)
     _lib.check(rc, what)
     return dq, dk_, dv_, dg, dbeta, dh0
 
@@ -361,8 +373,8 @@ def ut_solve(a, b, transpose: bool = False):
     H, C, N = _ut_check(a, b, what)
     dev = _require_gpu([a, b], what)
     x = torch.empty_like(b)
-    rc = _lib.lib().kda_ut_solve(_stream(dev), _ptr(a), _ptr(b), _ptr(x), H, C, N, _UT_CODES[a.dtype],
-                                 1 if transpose else 0)
+    rc = _call(_lib.lib().kda_ut_solve, dev, _ptr(a), _ptr(b), _ptr(x), H, C, N, _UT_CODES[a.dtype],
+               1 if transpose else 0)
     _lib.check(rc, what)
     return x
 
@@ -377,8 +389,8 @@ def ut_solve_bwd(a, x, dx, transpose: bool = False):
     dev = _require_gpu([a, x, dx], what)
     da = torch.empty_like(a)
     db = torch.empty_like(dx)
-    rc = _lib.lib().kda_ut_solve_bwd(_stream(dev), _ptr(a), _ptr(x), _ptr(dx), _ptr(da), _ptr(db),
-                                     H, C, N, _UT_CODES[a.dtype], 1 if transpose else 0)
+    rc = _call(_lib.lib().kda_ut_solve_bwd, dev, _ptr(a), _ptr(x), _ptr(dx), _ptr(da), _ptr(db),
+               H, C, N, _UT_CODES[a.dtype], 1 if transpose else 0)
     _lib.check(rc, what)
     return da, db
 
@@ -448,9 +460,9 @@ def kda_prologue(qp, kp, vp, wq, wk, wv, num_heads: int, conv_state=None, return
     new = tuple(torch.empty((B, K - 1, HD), dtype=torch.float32, device=dev) for _ in range(3)) \
         if return_state else (None, None, None)
     bin_ = conv_state if conv_state is not None else (None, None, None)
-    rc = _lib.lib().kda_prologue(_stream(dev), _ptr(qp), _ptr(kp), _ptr(vp), _ptr(wq), _ptr(wk), _ptr(wv),
-                                 *(_ptr(b) for b in bin_), *(_ptr(b) for b in new), _ptr(q), _ptr(k), _ptr(v),
-                                 B, T, H, d, K, _UT_CODES[qp.dtype], _UT_CODES[out_dtype])
+    rc = _call(_lib.lib().kda_prologue, dev, _ptr(qp), _ptr(kp), _ptr(vp), _ptr(wq), _ptr(wk), _ptr(wv),
+               *(_ptr(b) for b in bin_), *(_ptr(b) for b in new), _ptr(q), _ptr(k), _ptr(v),
+               B, T, H, d, K, _UT_CODES[qp.dtype], _UT_CODES[out_dtype])
     _lib.check(rc, what)
     return q, k, v, (new if return_state else None)
 
@@ -475,8 +487,8 @@ def kda_epilogue(o, gate, eps: float = 1e-6, out_dtype=torch.bfloat16):
     _contig("gate", gate)
     dev = _require_gpu([o, gate], what)
     y = torch.empty((B, T, H * dv), dtype=out_dtype, device=dev)
-    rc = _lib.lib().kda_epilogue(_stream(dev), _ptr(o), _ptr(gate), _ptr(y), B, T, H, dv, float(eps),
-                                 _UT_CODES[o.dtype], _UT_CODES[gate.dtype], _UT_CODES[out_dtype])
+    rc = _call(_lib.lib().kda_epilogue, dev, _ptr(o), _ptr(gate), _ptr(y), B, T, H, dv, float(eps),
+               _UT_CODES[o.dtype], _UT_CODES[gate.dtype], _UT_CODES[out_dtype])
     _lib.check(rc, what)
     return y
 
@@ -511,8 +523,8 @@ def kda_decode_layer_step(qp, kp, vp, g, beta, gate, wq, wk, wv, conv_state, sta
     if workspace is None or workspace.numel() * workspace.element_size() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     y = torch.empty((B, H * d), dtype=out_dtype, device=dev)
-    rc = L.kda_decode_layer_step(_stream(dev), *(_ptr(t) for t in tensors), _ptr(y), B, H, d, K, float(scale),
-                                 float(eps), _UT_CODES[dt], _UT_CODES[out_dtype], _ptr(workspace), need)
+    rc = _call(L.kda_decode_layer_step, dev, *(_ptr(t) for t in tensors), _ptr(y), B, H, d, K, float(scale),
+               float(eps), _UT_CODES[dt], _UT_CODES[out_dtype], _ptr(workspace), need)
     _lib.check(rc, what)
     return y
 
@@ -587,10 +599,10 @@ def kda_layer_fwd(qp, kp, vp, g, beta, gate, wq, wk, wv, conv_state=None, initia
     new = tuple(torch.empty((B, K - 1, H * d), dtype=torch.float32, device=dev) for _ in range(3)) \
         if return_conv_state else (None, None, None)
     bin_ = conv_state if conv_state is not None else (None, None, None)
-    rc = L.kda_layer_fwd(_stream(dev), _ptr(qp), _ptr(kp), _ptr(vp), _ptr(g), _ptr(beta), _ptr(gate),
-                         _ptr(wq), _ptr(wk), _ptr(wv), *(_ptr(b) for b in bin_), *(_ptr(b) for b in new),
-                         _ptr(initial_state), _ptr(ht), _ptr(y), _ptr(o_out), B, T, H, d, K, float(scale), float(eps),
-                         code, _OUT_CODES[gate.dtype], _OUT_CODES[out_dtype], _ptr(workspace), need)
+    rc = _call(L.kda_layer_fwd, dev, _ptr(qp), _ptr(kp), _ptr(vp), _ptr(g), _ptr(beta), _ptr(gate),
+               _ptr(wq), _ptr(wk), _ptr(wv), *(_ptr(b) for b in bin_), *(_ptr(b) for b in new),
+               _ptr(initial_state), _ptr(ht), _ptr(y), _ptr(o_out), B, T, H, d, K, float(scale), float(eps),
+               code, _OUT_CODES[gate.dtype], _OUT_CODES[out_dtype], _ptr(workspace), need)
     _lib.check(rc, what)
     return y, ht, (new if return_conv_state else None)
 
@@ -654,10 +666,10 @@ def _prologue_bwd(qp, kp, vp, wq, wk, wv, dq, dk, dv, conv_state, workspace, dx_
     db = tuple(torch.empty((B, K - 1, HD), dtype=f32, device=dev) for _ in range(3)) if want_db \
         else (None, None, None)
     bin_ = conv_state if conv_state is not None else (None, None, None)
-    rc = L.axiom_prologue_bwd(_stream(dev), _ptr(qp), _ptr(kp), _ptr(vp), _ptr(wq), _ptr(wk), _ptr(wv),
-                            *(_ptr(b) for b in bin_), _ptr(dq), _ptr(dk), _ptr(dv),
-                            *(_ptr(t) for t in dx), *(_ptr(t) for t in dw), *(_ptr(t) for t in db),
-                            B, T, H, d, K, _UT_CODES[qp.dtype], _UT_CODES[dx_dtype], _ptr(workspace), need)
+    rc = _call(L.axiom_prologue_bwd, dev, _ptr(qp), _ptr(kp), _ptr(vp), _ptr(wq), _ptr(wk), _ptr(wv),
+               *(_ptr(b) for b in bin_), _ptr(dq), _ptr(dk), _ptr(dv),
+               *(_ptr(t) for t in dx), *(_ptr(t) for t in dw), *(_ptr(t) for t in db),
+               B, T, H, d, K, _UT_CODES[qp.dtype], _UT_CODES[dx_dtype], _ptr(workspace), need)
     _lib.check(rc, what)
     return dx, dw, (db if want_db else None)
 
@@ -683,9 +695,9 @@ def kda_epilogue_bwd(o, gate, dy, eps: float = 1e-6, dgate_dtype=None):
     dev = _require_gpu([o, gate, dy], what)
     do = torch.empty((B, T, H, dv), dtype=torch.float32, device=dev)
     dgate = torch.empty((B, T, H * dv), dtype=dgate_dtype, device=dev)
-    rc = _lib.lib().kda_epilogue_bwd(_stream(dev), _ptr(o), _ptr(gate), _ptr(dy), _ptr(do), _ptr(dgate),
-                                     B, T, H, dv, float(eps), _UT_CODES[o.dtype], _UT_CODES[gate.dtype],
-                                     _UT_CODES[dy.dtype], _UT_CODES[dgate_dtype])
+    rc = _call(_lib.lib().kda_epilogue_bwd, dev, _ptr(o), _ptr(gate), _ptr(dy), _ptr(do), _ptr(dgate),
+               B, T, H, dv, float(eps), _UT_CODES[o.dtype], _UT_CODES[gate.dtype],
+               _UT_CODES[dy.dtype], _UT_CODES[dgate_dtype])
     _lib.check(rc, what)
     return do, dgate
 
@@ -746,9 +758,9 @@ def kda_layer(qp, kp, vp, g, beta, gate, wq, wk, wv, conv_state=None, initial_st
 def varlen_status(workspace, B, T, H, dk, dv, n_seqs, in_code=_lib.KDA_DTYPE_BF16) -> int:
     """Validation bits of the last varlen call that used ``workspace`` (synchronises)."""
     flags = ctypes.c_int32(0)
-    rc = _lib.lib().kda_varlen_status(_stream(workspace.device), _ptr(workspace),
-                                      workspace.numel() * workspace.element_size(),
-                                      B, T, H, dk, dv, CHUNK, n_seqs, in_code, ctypes.byref(flags))
+    rc = _call(_lib.lib().kda_varlen_status, workspace.device, _ptr(workspace),
+               workspace.numel() * workspace.element_size(),
+               B, T, H, dk, dv, CHUNK, n_seqs, in_code, ctypes.byref(flags))
     _lib.check(rc, "kda_varlen_status")
     return int(flags.value)
 
@@ -779,9 +791,9 @@ def kda_recurrent_step(q, k, v, g, beta, state, scale: float = 1.0, out_dtype=to
         _contig(name, t)
     dev = _require_gpu([q, k, v, g, beta, state], what)
     o = torch.empty((B, H, dv), dtype=out_dtype, device=dev)
-    rc = _lib.lib().kda_recurrent_step(_stream(dev), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta),
-                                       _ptr(state), _ptr(o), B, H, dk, dv, float(scale),
-                                       _IN_CODES[q.dtype], _OUT_CODES[out_dtype])
+    rc = _call(_lib.lib().kda_recurrent_step, dev, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta),
+               _ptr(state), _ptr(o), B, H, dk, dv, float(scale),
+               _IN_CODES[q.dtype], _OUT_CODES[out_dtype])
     _lib.check(rc, what)
     return o
 
@@ -834,8 +846,8 @@ def _cc_scan_fwd(q, k, v, alpha, beta32, S, tile, chunk):
     workspace = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
     o = torch.empty(q.shape[:-1] + (H * dv,), dtype=torch.float32, device=dev)
     S_new = torch.empty_like(S)
-    rc = L.kda_cc_scan_batched(_stream(dev), _ptr(q), _ptr(k), _ptr(v), _ptr(alpha), _ptr(beta32), _ptr(S),
-                               _ptr(o), _ptr(S_new), nb, T, H, dk, dv, int(tile), C, _ptr(workspace), ws_bytes)
+    rc = _call(L.kda_cc_scan_batched, dev, _ptr(q), _ptr(k), _ptr(v), _ptr(alpha), _ptr(beta32), _ptr(S),
+               _ptr(o), _ptr(S_new), nb, T, H, dk, dv, int(tile), C, _ptr(workspace), ws_bytes)
     _lib.check(rc, "cc_scan")
     return o, S_new
 
@@ -877,10 +889,10 @@ def cc_scan_bwd(q, k, v, alpha, beta32, S, do, dS=None, tile: int = 16, chunk: i
     dalpha = torch.empty_like(alpha)
     dbeta32 = torch.empty_like(beta32)
     dS_in = torch.empty_like(S)
-    rc = L.axiom_cc_scan_bwd(_stream(dev), _ptr(q), _ptr(k), _ptr(v), _ptr(alpha), _ptr(beta32), _ptr(S),
-                             _ptr(do), _ptr(dS), _ptr(dq), _ptr(dk_), _ptr(dv_), _ptr(dalpha),
-                             _ptr(dbeta32), _ptr(dS_in), nb, T, H, dk, dv, int(tile), C,
-                             _ptr(workspace), ws_bytes)
+    rc = _call(L.axiom_cc_scan_bwd, dev, _ptr(q), _ptr(k), _ptr(v), _ptr(alpha), _ptr(beta32), _ptr(S),
+               _ptr(do), _ptr(dS), _ptr(dq), _ptr(dk_), _ptr(dv_), _ptr(dalpha),
+               _ptr(dbeta32), _ptr(dS_in), nb, T, H, dk, dv, int(tile), C,
+               _ptr(workspace), ws_bytes)
     _lib.check(rc, what)
     return dq, dk_, dv_, dalpha, dbeta32, dS_in
 
