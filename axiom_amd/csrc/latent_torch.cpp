@@ -10,6 +10,7 @@
 // failures RuntimeError, as in the package's other calls.
 
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/python.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -212,6 +213,14 @@ struct LatentAttn : torch::autograd::Function<LatentAttn> {
     const OptTensor cu_q = s.size() > 5 ? OptTensor(s[5]) : std::nullopt, cu_k = s.size() > 6 ? OptTensor(s[6]) : std::nullopt;
     std::tie(out[0], out[1], out[2]) = attn_bwd(s[0], s[1], s[2], s[3], s[4], grads[0].contiguous(), cu_q, cu_k,
                                                 ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), std::nullopt);
+    // create_graph: the gradients are the kernels' and have no derivative of their
+    // own; differentiating them by what they were made from raises instead of
+    // leaving terms out
+    if (at::GradMode::is_enabled()) {
+      const auto once = std::make_shared<torch::autograd::Error>("latent_attn is not differentiable twice",
+                                                                 torch::autograd::collect_next_edges(s[0], s[1], s[2], grads[0]));
+      for (int i = 0; i < 3; ++i) torch::autograd::create_gradient_edge(out[i], once);
+    }
     return out;
   }
 };
