@@ -98,6 +98,11 @@ Tensor work(const OptTensor& t, size_t bytes, at::Device d) {
 }
 void* work_ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// a caller's tensor has been written: autograd notices where it is needed as it was
+void written(const OptTensor& t) {
+  if (t && !t->is_inference()) torch::autograd::impl::bump_version(*t);
+}
+
 // sizes, strides and packed offsets of an expanded-form call
 struct Attn {
   int B, Tq, Tk, H, dn, dr, n_seqs = 0, code;
@@ -162,6 +167,8 @@ std::tuple<Tensor, Tensor> attn_fwd(const Tensor& q, const Tensor& kv, const Ten
                               static_cast<const int32_t*>(ptr(a.cu_k)), a.n_seqs, ptr(o), static_cast<float*>(ptr(lse)), a.B, a.Tq,
                               a.Tk, a.H, a.dn, a.dr, causal, static_cast<float>(a.scale), a.code, work_ptr(ws), bytes),
           what);
+  written(out);
+  written(lse_out);
   return {o, lse};
 }
 
@@ -274,6 +281,8 @@ OptTensor append(const Tensor& rows, const Tensor& positions, const Tensor& slot
                             ptr(q), st[0], st[1], ptr(q_out), st[2], st[3], static_cast<int>(N), static_cast<int>(H),
                             static_cast<int>(R), static_cast<int>(dr), interleaved, code),
           what);
+  written(cache);
+  written(q_out);
   return q_out;
 }
 
@@ -303,6 +312,8 @@ std::tuple<Tensor, Tensor> decode(const Tensor& q, const Tensor& cache, const Te
                             ptr(o), static_cast<float*>(ptr(lse)), B, Tq, H, R, W - R, cache.size(0), page, per,
                             static_cast<float>(scale), code, work_ptr(ws), bytes),
           what);
+  written(out);
+  written(lse_out);
   return {o, lse};
 }
 
