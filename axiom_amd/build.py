@@ -10,6 +10,7 @@ that library.  Run ``python -m axiom_amd.build`` or call :func:`build`.
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -80,22 +81,30 @@ def _link_binding(obj: Path) -> None:
 
 
 def build(verbose: bool = False) -> Path:
-    """Compile all sources, link ``libkda_mi355x.so`` and its torch binding; returns the library's path."""
+    """Compile all sources, link ``libkda_mi355x.so``, then its torch binding; returns the library's path.
+
+    The library needs nothing of torch: it is in place before the binding is
+    linked, and where torch is not importable the binding is left out.
+    """
     hipcc = _hipcc()
     BUILD.mkdir(exist_ok=True)
     binding_obj = BUILD / "latent_torch.o"
     objs = [BUILD / (s.replace(".hip", ".o")) for s in SOURCES]
+    with_torch = importlib.util.find_spec("torch") is not None
     with ThreadPoolExecutor(max_workers=min(len(SOURCES) + 1, os.cpu_count() or 1)) as ex:
-        binding = ex.submit(_compile_binding, binding_obj, hipcc)
+        binding = ex.submit(_compile_binding, binding_obj, hipcc) if with_torch else None
         list(ex.map(lambda so: _compile(CSRC / so[0], so[1], hipcc), zip(SOURCES, objs)))
-        binding.result()
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     p = subprocess.run(cmd, capture_output=True, text=True)
     if p.returncode != 0:
         raise RuntimeError(f"link failed:\n{p.stderr}")
     os.replace(tmp, LIB)
-    _link_binding(binding_obj)
+    if binding is None:
+        print(f"torch is not importable: {BINDING.name} (the torch binding of the latent attention) is not built", file=sys.stderr)
+    else:
+        binding.result()
+        _link_binding(binding_obj)
     if verbose:
         print(f"built {LIB}")
     return LIB
