@@ -842,8 +842,9 @@ __global__ __launch_bounds__(R / 2) void kda_latent_join_kernel(LatentDecodeArgs
 template <int DT, int R, int DR>
 hipError_t run_append(const LatentAppendArgs& a, hipStream_t s) {
   // few tokens: a workgroup each, so a call of one token is one round of loads;
-  // many: a wave each
-  if (a.N < 1024) kda_latent_append_kernel<DT, R, DR, 4><<<dim3(a.N), dim3(256), 0, s>>>(a);
+  // many: a wave each (H16 R512 dr64 bf16 from cold memory, workgroup and wave a
+  // token: 1024 tokens 5.8 and 6.7 us, 2048 7.2 and 7.9, 4096 11.7 and 10.8)
+  if (a.N <= 2048) kda_latent_append_kernel<DT, R, DR, 4><<<dim3(a.N), dim3(256), 0, s>>>(a);
   else kda_latent_append_kernel<DT, R, DR, 1><<<dim3((a.N + 3) / 4), dim3(256), 0, s>>>(a);
   return hipGetLastError();
 }

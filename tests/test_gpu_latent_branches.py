@@ -9,7 +9,7 @@ import torch
 import axiom_amd
 from latent_testutil import attn_inputs, bar, check, check_lse, terms
 from oracle import latent as O
-from test_gpu_latent_cache import _decode_case, _decode_compare
+from test_gpu_latent_cache import _append_bar, _append_case, _decode_case, _decode_compare, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,16 @@ def test_64_row_decode_many_sequences(cuda):
 def test_decode_in_small_pages_and_tables(cuda, H):
     """A workgroup a sequence with pages of one token."""
     _decode_compare(_decode_case([17, 0, 1, 60], 2, H // 2, 512, 64, 1, "bf16", cuda, seed=H), 512, "bf16")
+
+
+@pytest.mark.parametrize("N", [2047, 2048, 2049, 2051, 5000])
+@pytest.mark.parametrize("R,dr,dtype,inter", [(512, 64, "bf16", False), (512, 64, "fp32", True), (256, 32, "fp16", True)])
+def test_append_of_many_tokens(cuda, N, R, dr, dtype, inter):
+    """Both ways to split tokens over waves, a last workgroup of one to four tokens among them."""
+    d, cs = _append_case(N, 3, R, dr, 16, dtype, cuda, seed=N), _table(500, dr, cuda)
+    d["slots"][1] = -1
+    ref, q_ref = O.append(d["rows"], d["positions"], d["slots"], cs, d["cache"], d["w"], 1e-5, d["q"], inter)
+    q_out = axiom_amd.latent_append(d["rows"], d["positions"], d["slots"], cs, d["cache"], norm_weight=d["w"], eps=1e-5,
+                                    q_rope=d["q"], interleaved=inter)
+    check("cache", d["cache"], ref, _append_bar(dtype), ())
+    check("q", q_out, q_ref, _append_bar(dtype), ())
