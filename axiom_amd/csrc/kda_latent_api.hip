@@ -89,7 +89,13 @@ kda::LatentArgs attn_args(const void* q, const void* kv, const void* kr, const i
 // some CUs: 1.3 times as long).  Not where the longest walk falls by less than a
 // quarter.  Packed lengths are on the device: there `parts` equal shares of each
 // block (len 0).
-constexpr int kSlots = 256;   // one workgroup a CU; with two (bf16, T = 1333, 16 heads) the join costs what they gain
+// kSlots: one workgroup a CU, and no shares past as many blocks.  Against 512 (bf16,
+// forward / backward): T = 1000 H8 d 64, 64 blocks, 13.9 / 38.5 us and 14.4 / 48.7; T =
+// 2048 H8, 128 blocks, 31.1 / 95.0 and 34.6 / 108; but T = 2560 H12, 240 blocks, 58 / 212
+// and 48 / 176, and T = 4096 H8, 256 blocks, 89 / 322 and 67 / 241: from some 200
+// causal blocks up the longest walk is twice the mean, and 256 workgroups leave
+// nothing to even it out with.  At 512 blocks neither shares any.
+constexpr int kSlots = 256;
 struct Shares { int len, parts, live; };
 // blocks of 128 rows of one head; packed: every sequence ends in at most one partial block
 int64_t blocks_of(int64_t T, int n_seqs) { return n_seqs > 0 ? T / 128 + n_seqs : (T + 127) / 128; }
@@ -152,7 +158,14 @@ BwdLayout bwd_layout(int B, int Tq, int Tk, int H, int dn, int dr, int n_seqs, b
 // of a sequence, and the workgroups along the cache: one a CU (its buffers take
 // the LDS), and no more than there can be runs of `least` tiles.  Sequences whose
 // table holds at most kWholeTokens tokens get a workgroup each instead and no join
-// launch.
+// launch: R512 bf16, 16 rows, tables of 128 tokens 11.8 us for one sequence and 14.0
+// for 256, in runs 12.6 and 20.4; of 192 tokens 13.8 and 16.5, in runs 12.7 and 23.0, so
+// from there on it is the number of sequences that decides, and runs are taken.
+// pad, the places of a sequence beside its tiles (16 rows; 64 sequences of 1 to
+// 8192 tokens and 256 of 1 to 1024): 0 62 and 65 us, 4 40 and 33, 8 34 and 30, 16 34 and
+// 34; 64 rows: 0 83 and 70, 2 55 and 54, 4 46 and 49, 8 46 and 50.
+// least: 2 and 1 are alike but for 64 rows of one sequence of 4096 tokens (22 and
+// 28 us); 4 takes 17.1 for 19.4 with 16 rows there, and 14.2 for 13.4 at 512 tokens.
 constexpr int kCUs = 256;
 constexpr int kWholeTokens = 128;
 struct DecodePlan { int rows, groups, wgs, whole, least, pad; size_t part_ml, part_o, total; };

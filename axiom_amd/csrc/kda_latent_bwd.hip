@@ -129,9 +129,12 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
 
   const float c = a.scale * kLog2e;
   // Rows of few keys: D as sum_j p_j (do . v_j), not from the rounded o, whose
-  // error is as large as g's own rounding there and falls with the keys' number
-  // (T = 1000, causal, d 64: dq's error 1.53 times its output's rounding with the
-  // one, below 1.5 with the other).  Two tiles, both in LDS.
+  // error is as large as g's own rounding there and falls with the keys' number.
+  // dq's error over that of its result's rounding, d 64, causal, where g's rounding
+  // alone makes it sqrt 2: rows 0 to 31 1.47 with this and 1.87 (fp16 1.43 and 1.75)
+  // with o's D, 32 to 63 1.44 and 1.57, 64 to 127 1.43 and 1.52; 128 to 255 1.48 with o's.
+  // So it ends there, with two tiles, both in LDS.  It costs 8 us of 150 where every
+  // row is such a one (B64 H16 T128) and nothing measurable at T = 1000.
   if (ES == 2 && blk_hi < 2 * BN && nt > 0) {   // a walk this short is never shared out
     fetch(0, buf0);
     if (nt == 2) fetch(1, buf1);
@@ -288,7 +291,8 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
 // the middle of a turn parts the second wave's reads, before its dk products,
 // from the first wave's writes, after its score products (B4 H16 T4096 fp16, both
 // passes: 1494 us with p in fp16, 1525 with this).
-// Three query tiles in LDS: arriving, present, behind.
+// Three query tiles in LDS: arriving, present, behind.  A pair takes every tile of
+// its block's walk, also the one at the diagonal that none of its keys are seen by.
 // fp32: operands twice as large and products 16 times as slow, so one wave does it all.
 template <int DT, int DN, int DR>
 struct KeyCfg : BwdCfg<DT, DN, DR> {

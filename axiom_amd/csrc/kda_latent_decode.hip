@@ -36,9 +36,10 @@ __device__ __forceinline__ void rotate_unit(const void* src, int64_t si, void* d
 // One token by TPW threads' worth of waves: wave 0 of the token norms and stores
 // its latent, all of them share the rotations (the row's own and H heads').
 // Bound by memory: every element is read and written once, 16 (norm) or 8 bytes a
-// lane.  16384 tokens, H16 R512 dr64 bf16: 32.7 us, 3.3 TB/s (a large copy reaches
-// 5.1; the heads' rotary parts are pieces of 128 bytes); one token 2.5 us of
-// kernel.  Loading two or three rounds of rotations ahead changed nothing.
+// lane.  16384 tokens, H16 R512 dr64 bf16: 22 us from a warm cache, 29 to 33 from
+// cold memory, 3.3 TB/s (a large copy reaches 5.1; the heads' rotary parts are
+// pieces of 128 bytes); one token 2.5 us of kernel.  Loading two or three rounds of
+// rotations ahead took 23.2 for 22.4 warm; it was not measured cold.
 template <int DT, int R, int DR, int WPT>
 __global__ __launch_bounds__(256) void kda_latent_append_kernel(LatentAppendArgs a) {
   constexpr int V = R / 64;               // latent elements of a lane
