@@ -289,8 +289,9 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
 // dk's error 1.2 times what it has to be.  Its two tiles by parity do not fit
 // beside d = 128's buffers: there one place serves both, and a second barrier in
 // the middle of a turn parts the second wave's reads, before its dk products,
-// from the first wave's writes, after its score products (B4 H16 T4096 fp16, both
-// passes: 1494 us with p in fp16, 1525 with this).
+// from the first wave's writes, after its exponentials (both passes, fp16: B4 H16
+// T4096 1468 us with p in fp16 and 1513 with this; 24 packed sequences of 17 to
+// 1024 tokens, H8, 135 and 143).
 // Three query tiles in LDS: arriving, present, behind.  A pair takes every tile of
 // its block's walk, also the one at the diagonal that none of its keys are seen by.
 // fp32: operands twice as large and products 16 times as slow, so one wave does it all.
@@ -478,13 +479,8 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
             for (int t = 0; t < 2; ++t) s[t] = mma(s[t], C::TR::template row_frag<F>(cur + C::OFF_R, fm, k, fh, 32 * t), kr[k]);
           pace<2 * (KN + KR), 6, 1, 1>();
           __builtin_amdgcn_sched_barrier(0);
-          if constexpr (MID) reuse_barrier();     // the second wave has read the last tile's p
           const bool edge = qt < wave_full || qt + BN > nq;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (edge) probs(cur, qt + 32 * t, t, fh, true, s[t]);
-            else probs(cur, qt + 32 * t, t, fh, false, s[t]);
-            frags(s[t], pf[t]);
+          auto hand_over = [&](int t) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               char* const to = place_of(j) + (2 * t + u) * (512 * C::P_ES);
@@ -499,6 +495,19 @@ __global__ __launch_bounds__((KeyCfg<DT, DN, DR>::NT)) void kda_latent_dkv_kerne
                 *reinterpret_cast<h8*>(to) = x;
               }
             }
+          };
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (edge) probs(cur, qt + 32 * t, t, fh, true, s[t]);
+            else probs(cur, qt + 32 * t, t, fh, false, s[t]);
+            frags(s[t], pf[t]);
+            if constexpr (!MID) hand_over(t);
+          }
+          if constexpr (MID) {
+            __builtin_amdgcn_sched_barrier(0);
+            reuse_barrier();                      // the second wave has read the last tile's p
+            hand_over(0);
+            hand_over(1);
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
