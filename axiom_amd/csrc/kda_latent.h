@@ -37,6 +37,8 @@ typedef __attribute__((address_space(3))) s4v* lds_s4;
 constexpr float kLn2 = 0.6931471805599453f;
 // finite start of the running maximum: exp2 of a masked (-inf) score minus it is 0
 constexpr float kMaxInit = -1e30f;
+// ... in raw score units, where c is the scale times log2 e: times c it has to stay finite too
+__device__ __forceinline__ float max_init(float c) { return fmaxf(kMaxInit, -1e37f / c); }
 // The running maximum is raised (and the accumulators rescaled) only when a
 // tile exceeds it by more than 2^kLazy: probabilities then reach at most
 // 2^8, in range for the 16-bit operands and without loss, since the row sum is

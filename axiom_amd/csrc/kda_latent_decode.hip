@@ -363,7 +363,7 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
 #pragma unroll
       for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const F*>(qp + 32 * s + 8 * gq);
     }
-    if (threadIdx.x < 16) top[threadIdx.x] = kMaxInit;
+    if (threadIdx.x < 16) top[threadIdx.x] = max_init(c);
 #pragma unroll
     for (int x = 0; x < AHEAD; ++x)
       if (ta + x < tb) fetch(ta + x, pages[x]);
@@ -385,7 +385,7 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
 
     if (scoring) {
       const int seen = len - (a.Tq - 1 - cr / a.H);
-      float mo = kMaxInit, l = 0.f;          // the maximum that l is against
+      float mo = max_init(c), l = 0.f;       // the maximum that l is against
       f4 s0, s1;
       int j = ta + wave;                     // the tile in hand
       auto score = [&](auto phase) {
@@ -608,7 +608,7 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
       for (int k = 0; k < 4 + DR / 32; ++k) at[k] = k < 4 ? TN::off(m, 4 * k, gq) : TR::off(m, 4 * (k - 4), gq);
 #pragma unroll
       for (int t = 0; t < 2; ++t) put[t] = TP::off(m, 2 * t, gq & 1, 16 * own) + 8 * (gq >> 1);
-      float mx = kMaxInit, mc = kMaxInit * c, l = 0.f;
+      float mx = max_init(c), mc = mx * c, l = 0.f;
       auto step = [&](int i, const char* cur, char* nxt) {
         turn(i, nxt);
         f4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};

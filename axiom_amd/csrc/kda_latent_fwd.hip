@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
   };
 
   const float c = a.scale * kLog2e;
-  float mx = kMaxInit, mc = kMaxInit * c, l = 0.f;   // running maximum (raw score units, and times c) and sum
+  float mx = max_init(c), mc = mx * c, l = 0.f;   // running maximum (raw score units, and times c) and sum
   const float lazy = kLazy / c;
   f16v acc[ND];
 #pragma unroll
