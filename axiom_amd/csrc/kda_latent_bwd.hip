@@ -9,8 +9,9 @@
 // query pass (a workgroup owns 128 queries and walks the keys; D, dq), the key
 // pass (a workgroup owns 128 keys and walks the queries; dk, dv, the head's share
 // of the rotary key's gradient in fp32), then the sums in fixed order: that
-// share's over the heads, and the parts of blocks that were shared out.  Both passes form p and g again: seven products instead of five,
-// against an fp32 dq kept in memory and added to by every key block.
+// share's over the heads, and the parts of blocks that were shared out.  Both
+// passes form p and g again: seven products instead of five, against an fp32 dq
+// kept in memory and added to by every key block.
 //
 // p and g are rounded to the inputs' type for the products they enter; sums
 // are fp32.  fp16, whose values lie between 6e-8 and 65504, takes g times a power
@@ -52,7 +53,7 @@ struct BwdCfg {
 // As the forward: scores transposed, one query a lane column.  g^T is the second
 // operand of dq^T += K^T g^T, whose first operand is the key tile read transposed.
 // Bound by the products and the waits between them: B4 H16 T4096, d 128 + 64, bf16,
-// causal 595 us, 920 TFLOP/s of its three products.  s and do v^T of 32 keys at a time:
+// causal 604 us, 910 TFLOP/s of its three products.  s and do v^T of 32 keys at a time:
 // with queries, do and the sums in registers (256 in all) 64 would spill.
 template <int DT, int DN, int DR>
 __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_kernel(LatentArgs a, int nqb) {
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_dq_ke
 // Scores untransposed: a lane column is one key; the query tile (nope, rotary,
 // do) is in LDS, read by rows for the two score products and transposed for
 // dk^T and dv^T.  Bound as the query pass: B4 H16 T4096, d 128 + 64, bf16, causal
-// 790 us, 870 TFLOP/s of its four products; the clock falls to 2.0 GHz under them.
+// 838 us, 820 TFLOP/s of its four products (804 at the least).
 //
 // 16-bit types: a pair of waves owns 32 keys and splits the work by what it
 // holds.  The first wave holds the keys and dv (112 registers): s, p, dv += p

@@ -102,8 +102,8 @@ __global__ __launch_bounds__(256) void kda_latent_append_kernel(LatentAppendArgs
 // finishes in an interval raises the running maximum, if its tile asks for it,
 // so the waves agree on it without an exchange, and nothing is left to merge.
 // fp32, with operands twice as large: two score waves and a ring of four.
-// 64 sequences of 1 to 8192 tokens, H16 R512 dr64 bf16: 28.6 us with the join, 3.0
-// TB/s of the cache's bytes; one of 512 tokens 12.8 us, a chain of loads.
+// 64 sequences of 1 to 8192 tokens, H16 R512 dr64 bf16: 28.8 us with the join, 3.0
+// TB/s of the cache's bytes, in fp32 66; one of 512 tokens 12.9 us, a chain of loads.
 template <int DT, int R, int DR>
 struct DecCfg {
   static constexpr int ES = El<DT>::ES;
@@ -524,8 +524,8 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
 // so its maximum needs no exchange; where it rises (by 2^8, seldom) the factor
 // goes to the output waves beside the probabilities.  Four buffers: one each
 // is written to, arrived, scored and added.
-// 8 sequences of 20000 to 32768 tokens, two queries each, H64 R512 dr64 fp16: 82 us
-// and 9 of join, 690 TFLOP/s; the score waves' LDS reads (each of four reads every
+// 8 sequences of 20000 to 32768 tokens, two queries each, H64 R512 dr64 fp16: 86 us
+// and 9 of join, 650 TFLOP/s; the score waves' LDS reads (each of four reads every
 // key) and their chain of reads, products and softmax bound it.  Two waves a tile
 // with 32 rows each and 16 keys at a time, which reads LDS half as often, took 112:
 // the chain is per tile, not per key.
