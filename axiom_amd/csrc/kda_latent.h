@@ -44,6 +44,10 @@ __device__ __forceinline__ float max_init(float c) { return fmaxf(kMaxInit, -1e3
 // 2^8, in range for the 16-bit operands and without loss, since the row sum is
 // kept in fp32 and both are divided at the end.
 constexpr float kLazy = 8.f;
+// fp16 probabilities are held 2^7 times as large, up to 2^15: its smallest step, 6e-8, is
+// then 5e-10 of the row's maximum, and a hundred thousand keys that are each far below
+// it keep what they add up to.  The reference of the exponents is lower by as much.
+template <int DT> constexpr float kLift = DT == 2 ? 7.f : 0.f;
 
 template <int DT> struct El;
 template <> struct El<0> { typedef float t; typedef f8 frag; static constexpr int ES = 4; };

@@ -427,10 +427,8 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
           mo = mx;
           float e[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            e[x] = fast_exp2(fmaf(s[x], c, -mx * c));
-            l += e[x];
-          }
+          for (int x = 0; x < 4; ++x) e[x] = fast_exp2(fmaf(s[x], c, kLift<DT> - mx * c));
+          l += (e[0] + e[1]) + (e[2] + e[3]);
           sp[par][lane] = to_p4<DT>(e);
           j += SP;
         }
@@ -458,9 +456,9 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
 #pragma unroll
         for (int x = 0; x < SP; ++x) ls = fmaf(fast_exp2((red[0][x][m] - mx) * c), red[1][x][m], ls);
         if (whole) {
-          a.lse[static_cast<int64_t>(b) * rows + r] = ls == 0.f ? -INFINITY : (mx * c + __log2f(ls)) * kLn2;
+          a.lse[static_cast<int64_t>(b) * rows + r] = ls == 0.f ? -INFINITY : (mx * c - kLift<DT> + __log2f(ls)) * kLn2;
         } else {
-          a.part_ml[2 * (srow + m)] = mx * c;
+          a.part_ml[2 * (srow + m)] = mx * c - kLift<DT>;
           a.part_ml[2 * (srow + m) + 1] = ls;
         }
       }
@@ -608,7 +606,7 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
       for (int k = 0; k < 4 + DR / 32; ++k) at[k] = k < 4 ? TN::off(m, 4 * k, gq) : TR::off(m, 4 * (k - 4), gq);
 #pragma unroll
       for (int t = 0; t < 2; ++t) put[t] = TP::off(m, 2 * t, gq & 1, 16 * own) + 8 * (gq >> 1);
-      float mx = max_init(c), mc = mx * c, l = 0.f;
+      float mx = max_init(c), mc = mx * c - kLift<DT>, l = 0.f;
       auto step = [&](int i, const char* cur, char* nxt) {
         turn(i, nxt);
         f4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -635,22 +633,22 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
         if (up) {
           const float nm = fmaxf(mx, group_max(tm)), al = fast_exp2((mx - nm) * c);
           mx = nm;
-          mc = nm * c;
+          mc = nm * c - kLift<DT>;
           l *= al;
           if (gq == 0) fac[i & 1][16 * own + m] = al;
         }
         if (lane == 0) reinterpret_cast<int*>(&rose[i & 1])[own] = up;
+        float sum[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           float p[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            p[e] = fast_exp2(fmaf(s[t][e], c, -mc));
-            l += p[e];
-          }
+          for (int e = 0; e < 4; ++e) p[e] = fast_exp2(fmaf(s[t][e], c, -mc));
+          sum[t] = (p[0] + p[1]) + (p[2] + p[3]);
           // the output waves' fragment order: chunk 2 t + half, first or second four keys
           store4<DT>(sp[i & 1] + put[t], 0, p[0], p[1], p[2], p[3]);
         }
+        l += sum[0] + sum[1];
       };
       for (int i = ta; i < tb;) {
         step(i, buf0, buf2);

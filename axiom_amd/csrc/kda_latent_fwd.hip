@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
   };
 
   const float c = a.scale * kLog2e;
-  float mx = max_init(c), mc = mx * c, l = 0.f;   // running maximum (raw score units, and times c) and sum
+  float mx = max_init(c), mc = mx * c - kLift<DT>, l = 0.f;   // running maximum (raw score units), the exponents' reference, sum
   const float lazy = kLazy / c;
   f16v acc[ND];
 #pragma unroll
@@ -144,24 +144,27 @@ __global__ __launch_bounds__(256, El<DT>::ES == 2 ? 2 : 1) void kda_latent_fwd_k
       const float nm = fmaxf(mx, tm);
       const float al = fast_exp2((mx - nm) * c);
       mx = nm;
-      mc = nm * c;
+      mc = nm * c - kLift<DT>;
       l *= al;
 #pragma unroll
       for (int n = 0; n < ND; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[n][i] *= al;
     }
+    // the tile's sum first: one by one, values below 2^-24 of l would be lost in it
     F pf[2 * NB];
+    float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < 2 * NB; ++u) {
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         p[e] = fast_exp2(fmaf(s[u >> 1][8 * (u & 1) + e], c, -mc));
-        l += p[e];
+        sum += p[e];
       }
       pf[u] = to_frag<DT>(p);
     }
+    l += sum;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < 2 * NB; ++u)
