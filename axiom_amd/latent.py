@@ -81,6 +81,7 @@ def latent_attn(q, kv, k_rope, cu_seqlens=None, cu_seqlens_k=None, causal: bool 
     """Differentiable latent attention, expanded form: ``o`` of :func:`latent_attn_fwd` with the HIP backward.
 
     Gradients flow to ``q``, ``kv`` and ``k_rope`` (the heads' sum), in their dtype.
+    Differentiable once: differentiating the gradients themselves raises RuntimeError.
     """
     return _ext().attn(q, kv, k_rope, cu_seqlens, cu_seqlens_k, causal, scale)
 
