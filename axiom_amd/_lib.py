@@ -14,6 +14,7 @@ PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libkda_mi355x.so"
 HEADER = PKG.parent / "include" / "kda_mi355x.h"
 LATENT_HEADER = PKG.parent / "include" / "latent_mi355x.h"
+TREE_HEADER = PKG.parent / "include" / "tree_mi355x.h"
 
 KDA_OK = 0
 KDA_ERR_INVALID_ARGUMENT = -1
@@ -89,13 +90,25 @@ _LATENT = {
     "kda_latent_decode_workspace": (_sz, [_i] * 8),
 }
 
-# Entry points outside the C ABI of kda_mi355x.h: those of latent_mi355x.h, and
+# The C ABI of include/tree_mi355x.h
+_TREE = {
+    "kda_tree_step": (_i, [_vp] * 10 + [_i] * 5 + [_f, _i, _i]),
+    "kda_tree_commit": (_i, [_vp] * 7 + [_i] * 6),
+    "kda_latent_tree_decode": (_i, [_vp] * 8 + [_i] * 5 + [_i64, _i, _i, _f, _i, _vp, _sz]),
+    "kda_latent_tree_decode_workspace": (_sz, [_i] * 8),
+    "kda_latent_tree_commit": (_i, [_vp] * 7 + [_i] * 5 + [_i64, _i, _i, _i]),
+    "kda_tree_verify": (_i, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz]),
+    "kda_tree_verify_workspace": (_sz, [_i] * 3),
+}
+
+# Entry points outside the C ABI of kda_mi355x.h: those of latent_mi355x.h and tree_mi355x.h, and
 # the binding's own (neither header's): the two
 # backward calls whose outputs may be rounded to the primals' 16-bit types by
 # the kernels that form them, and the seam's backward with the workspace its
 # direct form needs (axiom_amd/csrc/kda_internal.h)
 _PRIVATE = {
     **_LATENT,
+    **_TREE,
     "axiom_chunk_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                              _vp, _vp, _vp, _vp, _vp, _vp,
                              _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _i, _vp, _sz]),

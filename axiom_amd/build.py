@@ -2,10 +2,10 @@
 
 Every HIP source under ``axiom_amd/csrc`` is compiled with hipcc for gfx950
 only, then linked into one shared library whose exported functions are the C
-ABI of ``include/kda_mi355x.h`` and ``include/latent_mi355x.h`` and the package's
-own entry points (``_lib._PRIVATE``, declared in ``csrc/kda_internal.h``); the
-torch binding of the latent attention, ``_latent_torch.so``, is host C++ over
-that library.  Run ``python -m axiom_amd.build`` or call :func:`build`.
+ABI of ``include/kda_mi355x.h``, ``include/latent_mi355x.h`` and
+``include/tree_mi355x.h`` and the package's own entry points (``_lib._PRIVATE``,
+declared in ``csrc/kda_internal.h``); the torch binding of the latent attention
+and the tree calls, ``_latent_torch.so``, is host C++ over that library.  Run ``python -m axiom_amd.build`` or call :func:`build`.
 """
 
 from __future__ import annotations
@@ -38,7 +38,9 @@ HIPCC_FLAGS = [
     "-Wno-unused-command-line-argument",
 ]
 SOURCES = ["kda_chunk.hip", "kda_varlen.hip", "kda_decode.hip", "kda_bwd.hip", "kda_ut.hip", "kda_prologue.hip",
-           "kda_latent_fwd.hip", "kda_latent_bwd.hip", "kda_latent_decode.hip", "kda_latent_api.hip", "kda_api.hip"]
+           "kda_latent_fwd.hip", "kda_latent_bwd.hip", "kda_latent_decode.hip", "kda_latent_api.hip", "kda_tree.hip",
+           "kda_tree_verify.hip", "kda_tree_api.hip", "kda_api.hip"]
+BINDING_SOURCES = ["latent_torch.cpp", "tree_torch.cpp"]
 
 
 def _hipcc() -> str:
@@ -55,24 +57,24 @@ def _compile(src: Path, obj: Path, hipcc: str) -> None:
         raise RuntimeError(f"hipcc failed for {src.name}:\n{p.stderr}")
 
 
-def _compile_binding(obj: Path, hipcc: str) -> None:
+def _compile_binding(src: Path, obj: Path, hipcc: str) -> None:
     """Host C++ against torch's headers (no kernel in it)."""
     import torch
     from torch.utils.cpp_extension import include_paths
     inc = [f"-I{p}" for p in (*include_paths(), sysconfig.get_paths()["include"], INCLUDE, Path(hipcc).resolve().parents[1] / "include")]
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            "-DTORCH_EXTENSION_NAME=_latent_torch", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *inc,
-           "-c", str(CSRC / "latent_torch.cpp"), "-o", str(obj)]
+           "-c", str(src), "-o", str(obj)]
     p = subprocess.run(cmd, capture_output=True, text=True)
     if p.returncode != 0:
-        raise RuntimeError(f"g++ failed for latent_torch.cpp:\n{p.stderr}")
+        raise RuntimeError(f"g++ failed for {src.name}:\n{p.stderr}")
 
 
-def _link_binding(obj: Path) -> None:
+def _link_binding(objs: list[Path]) -> None:
     import torch
     libs = Path(torch.__file__).parent / "lib"
     tmp = BINDING.with_suffix(".so.tmp")
-    cmd = [shutil.which("g++") or "g++", "-shared", "-o", str(tmp), str(obj), f"-L{PKG}", "-lkda_mi355x", f"-L{libs}", "-lc10",
+    cmd = [shutil.which("g++") or "g++", "-shared", "-o", str(tmp), *map(str, objs), f"-L{PKG}", "-lkda_mi355x", f"-L{libs}", "-lc10",
            "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     p = subprocess.run(cmd, capture_output=True, text=True)
     if p.returncode != 0:
@@ -88,11 +90,11 @@ def build(verbose: bool = False) -> Path:
     """
     hipcc = _hipcc()
     BUILD.mkdir(exist_ok=True)
-    binding_obj = BUILD / "latent_torch.o"
+    binding_objs = [BUILD / s.replace(".cpp", ".o") for s in BINDING_SOURCES]
     objs = [BUILD / (s.replace(".hip", ".o")) for s in SOURCES]
     with_torch = importlib.util.find_spec("torch") is not None
-    with ThreadPoolExecutor(max_workers=min(len(SOURCES) + 1, os.cpu_count() or 1)) as ex:
-        binding = ex.submit(_compile_binding, binding_obj, hipcc) if with_torch else None
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES) + len(BINDING_SOURCES), os.cpu_count() or 1)) as ex:
+        bindings = [ex.submit(_compile_binding, CSRC / s, o, hipcc) for s, o in zip(BINDING_SOURCES, binding_objs)] if with_torch else []
         list(ex.map(lambda so: _compile(CSRC / so[0], so[1], hipcc), zip(SOURCES, objs)))
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
@@ -100,11 +102,13 @@ def build(verbose: bool = False) -> Path:
     if p.returncode != 0:
         raise RuntimeError(f"link failed:\n{p.stderr}")
     os.replace(tmp, LIB)
-    if binding is None:
-        print(f"torch is not importable: {BINDING.name} (the torch binding of the latent attention) is not built", file=sys.stderr)
+    if not with_torch:
+        print(f"torch is not importable: {BINDING.name} (the torch binding of the latent attention and the tree calls) is not built",
+              file=sys.stderr)
     else:
-        binding.result()
-        _link_binding(binding_obj)
+        for b in bindings:
+            b.result()
+        _link_binding(binding_objs)
     if verbose:
         print(f"built {LIB}")
     return LIB

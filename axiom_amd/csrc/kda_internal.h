@@ -365,9 +365,69 @@ struct LatentDecodeArgs {
   int64_t n_pages;
   int groups, wgs;         // row groups of a sequence; workgroups along the cache
   float scale;
+  // a tree of drafts (N = Tq places): [B, Tq] in tree calls, which the last field is for too
+  const int32_t* parents;
+  int items;               // 0: wgs a multiple of eight or one group; else the workgroups in use, of a multiple of eight
 };
 int latent_decode_tile(int m_rows);   // keys of a tile, by the query rows of a workgroup
 hipError_t launch_latent_decode(const LatentDecodeArgs& a, int R, int dr, int dt, int m_rows, hipStream_t s);
+hipError_t launch_latent_tree_decode(const LatentDecodeArgs& a, int R, int dr, int dt, int m_rows, hipStream_t s);
+
+// The latent cache after an accepted path (include/tree_mi355x.h).
+struct LatentTreeCommitArgs {
+  char* cache;             // [layers, n_pages, page, row_bytes]
+  const int32_t* table;    // [B, per]
+  const int32_t* lens;     // [B]
+  const int32_t* parents;  // [B, N]
+  const int32_t* last;     // [B]
+  int32_t* new_lens;       // [B]
+  int layers, B, N, per, page_shift, row_bytes;
+  int64_t n_pages;
+};
+hipError_t launch_latent_tree_commit(const LatentTreeCommitArgs& a, hipStream_t s);
+
+// A tree of N places over the state: o, u [B,N,H,d] and the state as it was.
+struct TreeStepArgs {
+  const void* q;           // [B,N,H,d]
+  const void* k;
+  const void* v;
+  const void* g;
+  const void* beta;        // [B,N,H]
+  const int32_t* parents;  // [B,N]
+  const float* state;      // [B,H,d,d]
+  void* o;
+  float* u;
+  int B, N, H;
+  float scale;
+};
+hipError_t launch_tree_step(const TreeStepArgs& a, int d, int dt, int out_dt, hipStream_t s);
+
+struct TreeCommitArgs {
+  const void* k;           // [B,N,H,d]
+  const void* g;
+  const float* u;
+  const int32_t* parents;  // [B,N]
+  const int32_t* last;     // [B]
+  float* state;            // [B,H,d,d], in place
+  int B, N, H;
+};
+hipError_t launch_tree_commit(const TreeCommitArgs& a, int d, int dt, hipStream_t s);
+
+// Verification: a row is cut into `slices` of `per` entries, a workgroup each.
+struct TreeVerifyArgs {
+  const void* target;      // [B,N+1,V] with strides
+  const void* draft;       // [B,N,V] with strides, or null
+  const int64_t* tokens;   // [B,N]
+  const int32_t* parents;  // [B,N]
+  const float* uniforms;   // [B,N+1]; null: greedy
+  int32_t* last;
+  int64_t* next;
+  int32_t* accepted;
+  int64_t t_b, t_row, d_b, d_row;
+  int B, N, V, slices, per;
+  void* ws;
+};
+hipError_t launch_tree_verify(const TreeVerifyArgs& a, int dt, hipStream_t s);
 
 }  // namespace kda
 

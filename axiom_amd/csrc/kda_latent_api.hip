@@ -1,5 +1,6 @@
-// C ABI of the latent attention: argument validation, workspace layout, dispatch.
+// C ABI of the latent attention, and of its calls on trees of drafts: argument validation, workspace layout, dispatch.
 #include "latent_mi355x.h"
+#include "tree_mi355x.h"
 
 #include <cmath>
 #include <cstdarg>
@@ -188,6 +189,65 @@ bool decode_plan(int B, int Tq, int H, int R, int page_size, int max_pages, int 
 }
 bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
 
+// A tree of drafts: the same, but that a tree has many row groups, so the runs a
+// sequence is cut into are no longer multiples of eight: as many as give each CU a
+// workgroup, dealt out so that the groups of a run meet in one XCD's L2.  25 groups:
+// 250 workgroups, 200 otherwise.
+bool tree_plan(int B, int N, int H, int R, int page_size, int max_pages, int dtype, DecodePlan* P, int* items) {
+  if (!decode_plan(B, N, H, R, page_size, max_pages, dtype, P)) return false;
+  *items = 0;
+  if (P->whole || P->groups == 1) return true;
+  const int64_t kt = kda::latent_decode_tile(P->rows), cap = static_cast<int64_t>(page_size) * max_pages;
+  const int64_t runs = (((cap + kt - 1) / kt + P->pad) * B + P->least - 1) / P->least;
+  const int64_t wgs = kCUs / P->groups > 0 ? kCUs / P->groups : 1;
+  P->wgs = static_cast<int>(wgs < runs ? wgs : runs > 0 ? runs : 1);
+  *items = P->wgs * P->groups;
+  const size_t slots = 2 * static_cast<size_t>(P->wgs) * P->groups * P->rows;
+  P->part_o = P->part_ml + align_up(slots * 8);
+  P->total = P->part_o + align_up(slots * R * 4);
+  return true;
+}
+
+// kda_latent_decode, or (parents) kda_latent_tree_decode
+int decode_call(hipStream_t stream, const char* what, const void* q, const void* cache, const int32_t* block_table,
+                const int32_t* seq_lens, const int32_t* parents, bool tree, void* o, float* lse, int B, int Tq, int H, int R,
+                int dr, int64_t n_pages, int page_size, int max_pages, float scale, int dtype, void* workspace,
+                size_t workspace_bytes) {
+  if (!dtype_ok(dtype)) return fail(KDA_ERR_INVALID_ARGUMENT, "dtype=%d must be F32, BF16 or F16", dtype);
+  if ((R != 256 && R != 512) || (dr != 32 && dr != 64))
+    return fail(KDA_ERR_UNSUPPORTED, "R=%d, dr=%d unsupported (R in {256, 512}, dr in {32, 64})", R, dr);
+  if (B < 0 || Tq < 1 || H < 1 || max_pages < 0 || n_pages < 0) return fail(KDA_ERR_INVALID_ARGUMENT, "sizes out of range");
+  if (tree && Tq > 64) return fail(KDA_ERR_UNSUPPORTED, "N=%d places, 64 at most", Tq);
+  if (!pow2(page_size)) return fail(KDA_ERR_INVALID_ARGUMENT, "page_size=%d must be a power of two", page_size);
+  if (n_pages >= (int64_t{1} << 31) / page_size) return fail(KDA_ERR_UNSUPPORTED, "n_pages * page_size must be below 2^31");
+  if (B > 65535) return fail(KDA_ERR_UNSUPPORTED, "B=%d over 65535", B);
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(KDA_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  if (B == 0) return KDA_OK;
+  if (n_pages == 0) max_pages = 0;      // no page: every length is 0
+  if (tree && !parents) return fail(KDA_ERR_INVALID_ARGUMENT, "null parents");
+  if (!q || !seq_lens || !o || !lse || (max_pages > 0 && (!cache || !block_table)))
+    return fail(KDA_ERR_INVALID_ARGUMENT, "null q, cache, block_table, seq_lens, o or lse");
+  for (const void* p : {q, cache, static_cast<const void*>(o), static_cast<const void*>(workspace)})
+    if (!aligned(p, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "q, cache, o and workspace must be aligned to 16 bytes");
+  DecodePlan P;
+  int items = 0;
+  if (!(tree ? tree_plan(B, Tq, H, R, page_size, max_pages, dtype, &P, &items) : decode_plan(B, Tq, H, R, page_size, max_pages, dtype, &P)))
+    return fail(KDA_ERR_UNSUPPORTED, "Tq * H = %lld rows or B * max_pages * page_size too large", static_cast<long long>(Tq) * H);
+  if (!workspace || workspace_bytes < P.total)
+    return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0}, P.total);
+  kda::LatentDecodeArgs a{};
+  a.q = q; a.cache = cache; a.table = block_table; a.lens = seq_lens; a.o = o; a.lse = lse;
+  a.line = static_cast<int*>(workspace);
+  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + P.part_ml);
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + P.part_o);
+  a.B = B; a.Tq = Tq; a.H = H; a.per = max_pages; a.n_pages = n_pages;
+  for (a.page_shift = 0; (1 << a.page_shift) < page_size;) ++a.page_shift;
+  a.groups = P.groups; a.wgs = P.wgs; a.whole = P.whole; a.least = P.least; a.pad = P.pad; a.scale = scale;
+  a.parents = parents; a.items = items;
+  return launched(tree ? kda::launch_latent_tree_decode(a, R, dr, dtype, P.rows, stream)
+                       : kda::launch_latent_decode(a, R, dr, dtype, P.rows, stream), what);
+}
+
 }  // namespace
 
 extern "C" {
@@ -290,34 +350,51 @@ size_t kda_latent_decode_workspace(int B, int Tq, int H, int R, int dr, int page
 int kda_latent_decode(hipStream_t stream, const void* q, const void* cache, const int32_t* block_table, const int32_t* seq_lens,
                       void* o, float* lse, int B, int Tq, int H, int R, int dr, int64_t n_pages, int page_size, int max_pages,
                       float scale, int dtype, void* workspace, size_t workspace_bytes) {
+  return decode_call(stream, "kda_latent_decode", q, cache, block_table, seq_lens, nullptr, false, o, lse, B, Tq, H, R, dr, n_pages,
+                     page_size, max_pages, scale, dtype, workspace, workspace_bytes);
+}
+
+size_t kda_latent_tree_decode_workspace(int B, int N, int H, int R, int dr, int page_size, int max_pages, int dtype) {
+  DecodePlan P;
+  int items;
+  if (B < 0 || N < 1 || N > 64 || H < 1 || (R != 256 && R != 512) || (dr != 32 && dr != 64) || !pow2(page_size) || max_pages < 0 ||
+      !dtype_ok(dtype) || !tree_plan(B, N, H, R, page_size, max_pages, dtype, &P, &items))
+    return 0;
+  return P.total;
+}
+
+int kda_latent_tree_decode(hipStream_t stream, const void* q, const void* cache, const int32_t* block_table,
+                           const int32_t* seq_lens, const int32_t* parents, void* o, float* lse, int B, int N, int H, int R,
+                           int dr, int64_t n_pages, int page_size, int max_pages, float scale, int dtype, void* workspace,
+                           size_t workspace_bytes) {
+  return decode_call(stream, "kda_latent_tree_decode", q, cache, block_table, seq_lens, parents, true, o, lse, B, N, H, R, dr, n_pages,
+                     page_size, max_pages, scale, dtype, workspace, workspace_bytes);
+}
+
+int kda_latent_tree_commit(hipStream_t stream, void* cache, const int32_t* block_table, const int32_t* seq_lens,
+                           const int32_t* parents, const int32_t* last, int32_t* new_lens, int layers, int B, int N, int R,
+                           int dr, int64_t n_pages, int page_size, int max_pages, int dtype) {
   if (!dtype_ok(dtype)) return fail(KDA_ERR_INVALID_ARGUMENT, "dtype=%d must be F32, BF16 or F16", dtype);
   if ((R != 256 && R != 512) || (dr != 32 && dr != 64))
     return fail(KDA_ERR_UNSUPPORTED, "R=%d, dr=%d unsupported (R in {256, 512}, dr in {32, 64})", R, dr);
-  if (B < 0 || Tq < 1 || H < 1 || max_pages < 0 || n_pages < 0) return fail(KDA_ERR_INVALID_ARGUMENT, "sizes out of range");
+  if (B < 0 || N < 1 || layers < 1 || max_pages < 0 || n_pages < 0) return fail(KDA_ERR_INVALID_ARGUMENT, "sizes out of range");
+  if (N > 64) return fail(KDA_ERR_UNSUPPORTED, "N=%d places, 64 at most", N);
   if (!pow2(page_size)) return fail(KDA_ERR_INVALID_ARGUMENT, "page_size=%d must be a power of two", page_size);
-  if (n_pages >= (int64_t{1} << 31) / page_size) return fail(KDA_ERR_UNSUPPORTED, "n_pages * page_size must be below 2^31");
-  if (B > 65535) return fail(KDA_ERR_UNSUPPORTED, "B=%d over 65535", B);
-  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(KDA_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  if (n_pages >= (int64_t{1} << 31) / page_size || static_cast<int64_t>(max_pages) * page_size >= (int64_t{1} << 31))
+    return fail(KDA_ERR_UNSUPPORTED, "n_pages * page_size and max_pages * page_size must be below 2^31");
+  if (layers > 65535 || B > kMaxBlocks) return fail(KDA_ERR_UNSUPPORTED, "layers=%d or B=%d too large", layers, B);
   if (B == 0) return KDA_OK;
   if (n_pages == 0) max_pages = 0;      // no page: every length is 0
-  if (!q || !seq_lens || !o || !lse || (max_pages > 0 && (!cache || !block_table)))
-    return fail(KDA_ERR_INVALID_ARGUMENT, "null q, cache, block_table, seq_lens, o or lse");
-  for (const void* p : {q, cache, static_cast<const void*>(o), static_cast<const void*>(workspace)})
-    if (!aligned(p, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "q, cache, o and workspace must be aligned to 16 bytes");
-  DecodePlan P;
-  if (!decode_plan(B, Tq, H, R, page_size, max_pages, dtype, &P))
-    return fail(KDA_ERR_UNSUPPORTED, "Tq * H = %lld rows or B * max_pages * page_size too large", static_cast<long long>(Tq) * H);
-  if (!workspace || workspace_bytes < P.total)
-    return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0}, P.total);
-  kda::LatentDecodeArgs a{};
-  a.q = q; a.cache = cache; a.table = block_table; a.lens = seq_lens; a.o = o; a.lse = lse;
-  a.line = static_cast<int*>(workspace);
-  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + P.part_ml);
-  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + P.part_o);
-  a.B = B; a.Tq = Tq; a.H = H; a.per = max_pages; a.n_pages = n_pages;
+  if (!seq_lens || !parents || !last || !new_lens || (max_pages > 0 && (!cache || !block_table)))
+    return fail(KDA_ERR_INVALID_ARGUMENT, "null cache, block_table, seq_lens, parents, last or new_lens");
+  if (new_lens == seq_lens) return fail(KDA_ERR_INVALID_ARGUMENT, "new_lens must not be seq_lens");
+  if (!aligned(cache, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "cache must be aligned to 16 bytes");
+  kda::LatentTreeCommitArgs a{};
+  a.cache = static_cast<char*>(cache); a.table = block_table; a.lens = seq_lens; a.parents = parents; a.last = last;
+  a.new_lens = new_lens; a.layers = layers; a.B = B; a.N = N; a.per = max_pages; a.n_pages = n_pages;
+  a.row_bytes = static_cast<int>((R + dr) * elem(dtype));
   for (a.page_shift = 0; (1 << a.page_shift) < page_size;) ++a.page_shift;
-  a.groups = P.groups; a.wgs = P.wgs; a.whole = P.whole; a.least = P.least; a.pad = P.pad; a.scale = scale;
-  return launched(kda::launch_latent_decode(a, R, dr, dtype, P.rows, stream), "kda_latent_decode");
+  return launched(kda::launch_latent_tree_commit(a, stream), "kda_latent_tree_commit");
 }
 
 }  // extern "C"

@@ -6,6 +6,7 @@
 
 #include "kda_internal.h"
 #include "kda_latent.h"
+#include "kda_tree.h"
 
 #include <type_traits>
 
@@ -246,8 +247,13 @@ __device__ __forceinline__ Run find_run(const LatentDecodeArgs& a, int w, int KT
 
 // workgroup -> run and row group; the groups of one run are eight workgroups
 // apart, on one XCD, whose L2 then serves all but the first
+template <bool TREE>
 __device__ __forceinline__ void run_group(const LatentDecodeArgs& a, int& w, int& grp) {
-  if (a.wgs % 8 == 0) {
+  if (TREE && a.items) {             // an eighth of the items an XCD, one run's groups behind each other
+    const int item = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    grp = item % a.groups;
+    w = item / a.groups;             // from a.wgs on: nothing to do
+  } else if (a.wgs % 8 == 0) {
     grp = (blockIdx.x >> 3) % a.groups;
     w = (blockIdx.x / (8 * a.groups)) * 8 + (blockIdx.x & 7);
   } else {
@@ -255,6 +261,26 @@ __device__ __forceinline__ void run_group(const LatentDecodeArgs& a, int& w, int
     w = blockIdx.x / a.groups;
   }
 }
+
+// A tree of drafts: the places' rows are the newest Tq of the sequence.  A row
+// without a draft is not read (it may hold anything, and 0 times it would not be
+// 0): the copies take the newest row before the places for it, or a draft's.
+struct Tree {
+  u64 paths, live;                   // of place `lane`; which places hold a draft
+  int base;                          // the first place's row
+  __device__ __forceinline__ void load(const LatentDecodeArgs& a, int b, int len) {
+    paths = tree_paths(a.parents[static_cast<int64_t>(b) * a.Tq + min(static_cast<int>(__lane_id()), a.Tq - 1)], a.Tq);
+    live = __ballot(paths != 0);
+    base = len - a.Tq;
+  }
+  __device__ __forceinline__ int token(int t) const {
+    if (t < base || (live >> (t - base)) & 1) return t;
+    if (base > 0) return base - 1;
+    const u64 rest = live >> -base;
+    return rest ? __ffsll(static_cast<long long>(rest)) - 1 : t;
+  }
+  static __device__ __forceinline__ bool sees(u64 path, int place) { return place < 0 || (place < 64 && (path >> (place & 63) & 1)); }
+};
 
 // zeros for the rows of an empty sequence
 template <int DT, int R>
@@ -312,7 +338,7 @@ __device__ __forceinline__ void copy_piece(const char* cache, int row_bytes, int
   }
 }
 
-template <int DT, int R, int DR>
+template <int DT, int R, int DR, bool TREE = false>
 __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeArgs a) {
   typedef DecCfg<DT, R, DR> C;
   typedef typename El<DT>::frag F;
@@ -330,7 +356,8 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
   const int m = lane & 15, gq = lane >> 4;
   const bool scoring = wave < 4;
   int w, grp;
-  run_group(a, w, grp);
+  run_group<TREE>(a, w, grp);
+  if (TREE && w >= a.wgs) return;
   Run run = find_run(a, w, KT).uniform();
   const int rows = a.Tq * a.H, r = grp * 16 + m, cr = min(r, rows - 1);
   if (a.whole && run.g1 == 0) empty_rows<DT, R>(a, w, grp * 16, min(rows, grp * 16 + 16), 512);
@@ -344,9 +371,16 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
     const int ta = run.t, tb = min(n_all, ta + (run.g1 - run.g));   // this segment's tiles
     if (ta < tb) {
     const int32_t* table = a.table + static_cast<int64_t>(b) * a.per;
-    auto page_at = [&](int j) { return page_of_tile<KT>(a, table, len, j, m); };
+    Tree tree;
+    if constexpr (TREE) tree.load(a, b, len);
+    const int clear = TREE ? max(tree.base, 0) / KT : 0;   // a tree: tiles before this one hold no place
+    auto token = [&](int j) { return TREE ? tree.token(min(j * KT + m, len - 1)) : min(j * KT + m, len - 1); };
+    auto page_at = [&](int j) {
+      if (TREE && j >= clear) return fresh(page_of(a, table, token(j)));
+      return page_of_tile<KT>(a, table, len, j, m);
+    };
     auto fetch = [&](int j, int page) {
-      const int slot = slot_of(a, page, min(j * KT + m, len - 1)), ln = fresh(lane) & 63;
+      const int slot = slot_of(a, page, token(j)), ln = fresh(lane) & 63;
       const unsigned dst = lds0 + (j & (RING - 1)) * C::BUF;
 #pragma unroll
       for (int p = wave; p < C::PN + C::PR; p += 8) {
@@ -363,6 +397,13 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
 #pragma unroll
       for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const F*>(qp + 32 * s + 8 * gq);
     }
+    u64 mine = 0;
+    if constexpr (TREE) {
+      mine = shfl_u64(tree.paths, cr / a.H);
+      if (wave < SP && mine == 0)            // no draft: a score of nothing, whatever its query holds
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = F{};
+    }
     if (threadIdx.x < 16) top[threadIdx.x] = max_init(c);
 #pragma unroll
     for (int x = 0; x < AHEAD; ++x)
@@ -377,7 +418,7 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
       lds_barrier();
       if (i + AHEAD < tb) {
         fetch(i + AHEAD, page);
-        if (new_page(a, i + AHEAD + 1, KT)) page = page_at(i + AHEAD + 1);
+        if (new_page(a, i + AHEAD + 1, KT) || (TREE && i + AHEAD + 1 >= clear)) page = page_at(i + AHEAD + 1);
       }
     };
     const bool whole = ta == 0 && tb == n_all;
@@ -410,7 +451,7 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
           const int key0 = j * KT + 4 * gq, par = j & 1;
           f4 s = s0 + s1;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[e] = key0 + e < seen ? s[e] : -INFINITY;
+          for (int e = 0; e < 4; ++e) s[e] = (TREE ? Tree::sees(mine, key0 + e - tree.base) : key0 + e < seen) ? s[e] : -INFINITY;
           const float tm = group_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
           float mx = top[m];
           const bool up = __any(tm > mx + lazy);
@@ -444,7 +485,7 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
           else score(std::integral_constant<int, SP - 1>());
         }
       }
-      l = group_sum(l);
+      l = TREE && mine == 0 ? 0.f : group_sum(l);
       if (wave < SP && gq == 0) {
         red[0][wave][m] = mo;
         red[1][wave][m] = l;
@@ -527,7 +568,7 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
 // key) and their chain of reads, products and softmax bound it.  Two waves a tile
 // with 32 rows each and 16 keys at a time, which reads LDS half as often, took 112:
 // the chain is per tile, not per key.
-template <int DT, int R, int DR>
+template <int DT, int R, int DR, bool TREE = false>
 __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeArgs a) {
   typedef typename El<DT>::frag F;
   typedef typename El<DT>::t E;
@@ -550,7 +591,8 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
   const int own = wave & 3;
   const bool scoring = wave < 4;
   int w, grp;
-  run_group(a, w, grp);
+  run_group<TREE>(a, w, grp);
+  if (TREE && w >= a.wgs) return;
   Run run = find_run(a, w, KT).uniform();
   const int rows = a.Tq * a.H, r0 = grp * 64;
   if (a.whole && run.g1 == 0) empty_rows<DT, R>(a, w, r0, min(rows, r0 + 64), 512);
@@ -563,7 +605,12 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
     const int ta = run.t, tb = min(n_all, ta + (run.g1 - run.g));
     if (ta < tb) {
     const int32_t* table = a.table + static_cast<int64_t>(b) * a.per;
-    auto token = [&](int j) { return min(j * KT + (lane & 31), len - 1); };   // a key a lane
+    Tree tree;
+    if constexpr (TREE) tree.load(a, b, len);
+    auto token = [&](int j) {                // a key a lane
+      const int t = min(j * KT + (lane & 31), len - 1);
+      return TREE ? tree.token(t) : t;
+    };
     auto fetch = [&](int slot, char* dst) {
       const int ln = fresh(lane) & 63;
 #pragma unroll
@@ -599,7 +646,14 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
         for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const F*>(qp + 32 * s + 8 * gq);
       }
       const int seen = len - (a.Tq - 1 - r / a.H);
-      const int clear = (len - (a.Tq - 1)) / KT;   // tiles before this one have no masked key
+      const int clear = TREE ? max(tree.base, 0) / KT : (len - (a.Tq - 1)) / KT;   // tiles before this one have no masked key
+      u64 mine = 0;
+      if constexpr (TREE) {
+        mine = shfl_u64(tree.paths, r / a.H);
+        if (mine == 0)                       // no draft: a score of nothing, whatever its query holds
+#pragma unroll
+          for (int s = 0; s < KS; ++s) q[s] = F{};
+      }
       // the lane's places: of the fragments in a tile (a latent's repeat every four), of its probabilities
       int at[4 + DR / 32], put[2];
 #pragma unroll
@@ -624,7 +678,10 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][e] = key0 + 16 * t + e < seen ? s[t][e] : -INFINITY;
+            for (int e = 0; e < 4; ++e) {
+              const int key = key0 + 16 * t + e;
+              s[t][e] = (TREE ? Tree::sees(mine, key - tree.base) : key < seen) ? s[t][e] : -INFINITY;
+            }
         }
         float tm = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
@@ -661,7 +718,7 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
         ++i;
       }
       turn(tb, buf0);                        // the last tile is added; nothing to copy
-      l = group_sum(l);
+      l = TREE && mine == 0 ? 0.f : group_sum(l);
       if (gq == 0) {
         ml[0][16 * own + m] = mc;
         ml[1][16 * own + m] = l;
@@ -838,6 +895,53 @@ __global__ __launch_bounds__(R / 2) void kda_latent_join_kernel(LatentDecodeArgs
   if (threadIdx.x == 0) a.lse[row] = l == 0.f ? -INFINITY : (mx + __log2f(l)) * kLn2;
 }
 
+// The cache after an accepted path: its rows move to the front of the places'.  A
+// thread takes the same 16 bytes of every row; rows move down only, so eight
+// rows read and then written clobber none that a later eight read, and threads
+// need not wait for each other.  Bound by the moved rows' bytes.
+__global__ __launch_bounds__(192) void kda_latent_tree_commit_kernel(LatentTreeCommitArgs a) {
+  const int lane = threadIdx.x & 63, b = blockIdx.x, N = a.N;
+  const int64_t cap = static_cast<int64_t>(a.per) << a.page_shift;
+  const int parent = a.parents[static_cast<int64_t>(b) * N + min(lane, N - 1)], last = a.last[b], given = a.lens[b];
+  const int len = given < 0 ? 0 : (given > cap ? static_cast<int>(cap) : given), base = len - N;
+  const u64 paths = tree_paths(parent, N);
+  const u64 path = last >= 0 && last < N && base >= 0 ? uniform_u64(shfl_u64(paths, last)) : 0;
+  if (blockIdx.y == 0 && threadIdx.x == 0) a.new_lens[b] = base < 0 ? given : base + __popcll(path);
+  // lane: place `lane`; from row `src` to row `dst` of a layer's cache
+  const int rank = __popcll(path & ((u64{1} << lane) - 1));
+  const bool moves = (path >> lane & 1) && rank != lane;
+  int src = 0, dst = 0;
+  if (moves) {
+    auto slot = [&](int tok) {
+      const int page = a.table[static_cast<int64_t>(b) * a.per + (tok >> a.page_shift)];
+      return (min(max(page, 0), static_cast<int>(a.n_pages - 1)) << a.page_shift) + (tok & ((1 << a.page_shift) - 1));
+    };
+    src = slot(base + lane);
+    dst = slot(base + rank);
+  }
+  u64 rest = __ballot(moves);
+  const bool mine = threadIdx.x * 16 < a.row_bytes;
+  char* cache = a.cache + blockIdx.y * (a.n_pages << a.page_shift) * a.row_bytes + threadIdx.x * 16;
+  while (rest) {
+    u32x4 row[8];
+    int to[8];
+    int n = 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (rest) {
+        const int i = __ffsll(static_cast<long long>(rest)) - 1;
+        rest &= rest - 1;
+        const int from = __builtin_amdgcn_readlane(src, i);
+        to[x] = __builtin_amdgcn_readlane(dst, i);
+        if (mine) row[x] = *reinterpret_cast<const u32x4*>(cache + static_cast<int64_t>(from) * a.row_bytes);
+        n = x + 1;
+      }
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (x < n && mine) *reinterpret_cast<u32x4*>(cache + static_cast<int64_t>(to[x]) * a.row_bytes) = row[x];
+  }
+}
+
 template <int DT, int R, int DR>
 hipError_t run_append(const LatentAppendArgs& a, hipStream_t s) {
   // few tokens: a workgroup each, so a call of one token is one round of loads;
@@ -848,26 +952,27 @@ hipError_t run_append(const LatentAppendArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int DT, int R, int DR>
+template <int DT, int R, int DR, bool TREE>
 hipError_t run_decode(const LatentDecodeArgs& a, int m_rows, hipStream_t s) {
+  const dim3 grid(TREE && a.items ? (a.items + 7) / 8 * 8 : a.wgs * a.groups);
   if (m_rows == 16) {
-    kda_latent_decode16_kernel<DT, R, DR><<<dim3(a.wgs * a.groups), dim3(512), 0, s>>>(a);
+    kda_latent_decode16_kernel<DT, R, DR, TREE><<<grid, dim3(512), 0, s>>>(a);
   } else if constexpr (DT != 0) {
-    kda_latent_decode64_kernel<DT, R, DR><<<dim3(a.wgs * a.groups), dim3(512), 0, s>>>(a);
+    kda_latent_decode64_kernel<DT, R, DR, TREE><<<grid, dim3(512), 0, s>>>(a);
   } else {
     return hipErrorInvalidValue;
   }
   if (a.whole) return hipGetLastError();
-  const dim3 grid(a.Tq * a.H, a.B), block(R / 2);
-  if (m_rows == 16) kda_latent_join_kernel<DT, R, 16><<<grid, block, 0, s>>>(a, 16);
-  else kda_latent_join_kernel<DT, R, 32><<<grid, block, 0, s>>>(a, 64);
+  const dim3 rows(a.Tq * a.H, a.B), block(R / 2);
+  if (m_rows == 16) kda_latent_join_kernel<DT, R, 16><<<rows, block, 0, s>>>(a, 16);
+  else kda_latent_join_kernel<DT, R, 32><<<rows, block, 0, s>>>(a, 64);
   return hipGetLastError();
 }
 
-template <int DT>
+template <int DT, bool TREE>
 hipError_t decode_by_dims(const LatentDecodeArgs& a, int R, int dr, int m_rows, hipStream_t s) {
-  if (R == 512) return dr == 64 ? run_decode<DT, 512, 64>(a, m_rows, s) : run_decode<DT, 512, 32>(a, m_rows, s);
-  return dr == 64 ? run_decode<DT, 256, 64>(a, m_rows, s) : run_decode<DT, 256, 32>(a, m_rows, s);
+  if (R == 512) return dr == 64 ? run_decode<DT, 512, 64, TREE>(a, m_rows, s) : run_decode<DT, 512, 32, TREE>(a, m_rows, s);
+  return dr == 64 ? run_decode<DT, 256, 64, TREE>(a, m_rows, s) : run_decode<DT, 256, 32, TREE>(a, m_rows, s);
 }
 template <int DT>
 hipError_t append_by_dims(const LatentAppendArgs& a, int R, int dr, hipStream_t s) {
@@ -883,8 +988,17 @@ hipError_t launch_latent_append(const LatentAppendArgs& a, int R, int dr, int dt
 }
 int latent_decode_tile(int m_rows) { return m_rows == 16 ? 16 : 32; }
 hipError_t launch_latent_decode(const LatentDecodeArgs& a, int R, int dr, int dt, int m_rows, hipStream_t s) {
-  return dt == 0 ? latent::decode_by_dims<0>(a, R, dr, m_rows, s) : dt == 1 ? latent::decode_by_dims<1>(a, R, dr, m_rows, s)
-                                                                        : latent::decode_by_dims<2>(a, R, dr, m_rows, s);
+  return dt == 0 ? latent::decode_by_dims<0, false>(a, R, dr, m_rows, s) : dt == 1 ? latent::decode_by_dims<1, false>(a, R, dr, m_rows, s)
+                                                                               : latent::decode_by_dims<2, false>(a, R, dr, m_rows, s);
+}
+hipError_t launch_latent_tree_decode(const LatentDecodeArgs& a, int R, int dr, int dt, int m_rows, hipStream_t s) {
+  return dt == 0 ? latent::decode_by_dims<0, true>(a, R, dr, m_rows, s) : dt == 1 ? latent::decode_by_dims<1, true>(a, R, dr, m_rows, s)
+                                                                              : latent::decode_by_dims<2, true>(a, R, dr, m_rows, s);
+}
+hipError_t launch_latent_tree_commit(const LatentTreeCommitArgs& a, hipStream_t s) {
+  const int chunks = a.row_bytes / 16;
+  latent::kda_latent_tree_commit_kernel<<<dim3(a.B, a.layers), dim3((chunks + 63) / 64 * 64), 0, s>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace kda

@@ -1,0 +1,335 @@
+// KDA states and a tree of drafted tokens: the read-out of every place of a tree
+// in one pass over the state, and the state after the path that was accepted.
+//
+// With gamma_i the product of a = exp(g) over the path of place i and u_j what
+// place j writes,
+//   S_i = diag(gamma_i) S + sum over j on the path of (gamma_i / gamma_j) k_j u_j^T,
+// so the delta rule over a tree is a unit lower triangular system:
+//   u_i + beta_i sum_{j above i} L_ij u_j = beta_i (v_i - (gamma_i k_i)^T S),
+//   L_ij = k_i . (gamma_i / gamma_j) k_j,
+//   o_i = (gamma_i q_i)^T S + sum_{j on the path} A_ij u_j,  A_ij = q_i . (gamma_i / gamma_j) k_j.
+// The quotient is never formed: it is the product of a over the places between,
+// taken while walking up the path, so nothing overflows however strong the decay.
+
+#include "kda_common.h"
+#include "kda_internal.h"
+#include "kda_tree.h"
+
+namespace kda {
+namespace {
+
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+template <int N>
+__device__ __forceinline__ float row_ror(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xF, 0xF, false));
+}
+// sum over the 16 lanes of a DPP row, in all of them
+__device__ __forceinline__ float row_sum16(float x) {
+  x += row_ror<8>(x);
+  x += row_ror<4>(x);
+  x += row_ror<2>(x);
+  x += row_ror<1>(x);
+  return x;
+}
+__device__ __forceinline__ float dot4(f4 a, f4 b, float c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = fmaf(a[e], b[e], c);
+  return c;
+}
+
+// One workgroup a (sequence, head): D / 32 waves of 32 value columns each, whose
+// slice of the state waits in registers while the scores are made.
+//   1. 16 lanes a place walk up its path: A and L to LDS, gamma_i in hand at the end.
+//   2. (gamma q)^T S and (gamma k)^T S by 16x16x4 fp32 products, the state read once.
+//   3. u tile of 16 places by tile: inverses of the diagonal tiles (I + beta L)^-1 times what the
+//      tiles before leave, o from A u.  A tile's result is the next product's operand in
+//      the registers it was made in (row 4 gq + e of its four is step e's).
+// All in fp32: the operations (4 N d^2 a head) take less than the state's and the
+// tokens' bytes.
+template <int D, int DT, int NT, int OUT>
+__global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
+  constexpr int NW = D / 32, NP = 16 * NT, G = 4 * NW, NPG = NP / G > 0 ? NP / G : 1;   // places of a group of 16 lanes
+  constexpr int C4 = D / 64, LK = D + 4, LA = NP + 4, LT = 20;
+  __shared__ __attribute__((aligned(16))) float rk[NP * LK];   // k, then gamma k
+  __shared__ __attribute__((aligned(16))) float rq[NP * LK];   // a, then gamma q
+  __shared__ __attribute__((aligned(16))) float As[NP * LA], Ls[NP * LA];
+  __shared__ __attribute__((aligned(16))) float Ts[NT * 16 * LT];
+  __shared__ float bet[NP];
+  __shared__ int above[NP];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 15, gq = lane >> 4, grp = tid >> 4;
+  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, N = a.N;
+  auto place = [&](int x) { return x * G + ((x & 1) ? G - 1 - grp : grp); };   // deep and shallow ones in turn
+  auto token = [&](int i) { return (static_cast<int64_t>(b) * N + min(i, N - 1)) * a.H + h; };
+
+  // the tokens' rows first, then the state: loads return in order
+  const int parent = a.parents[static_cast<int64_t>(b) * N + min(lane, N - 1)];
+  f4 kv[NPG][C4], qv[NPG][C4], av[NPG][C4];
+  float bt[NPG];
+#pragma unroll
+  for (int x = 0; x < NPG; ++x) {
+    const int64_t t = token(place(x));
+#pragma unroll
+    for (int c = 0; c < C4; ++c) {
+      kv[x][c] = ld4<DT>(a.k, t * D + 64 * c + 4 * m);
+      qv[x][c] = ld4<DT>(a.q, t * D + 64 * c + 4 * m);
+      av[x][c] = ld4<DT>(a.g, t * D + 64 * c + 4 * m);
+    }
+    bt[x] = ld1<DT>(a.beta, t);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  const int col = 32 * wave + 2 * m;     // and col + 1: columns m of the wave's two tiles
+  const float* Sp = a.state + static_cast<int64_t>(blockIdx.x) * D * D + col;
+  f2 S[D / 16][4];
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) S[s][e] = *reinterpret_cast<const f2*>(Sp + (16 * s + 4 * gq + e) * D);
+  __builtin_amdgcn_sched_barrier(0);
+
+  const u64 path = tree_paths(parent, N), live = __ballot(path != 0);
+  if (wave == 0 && lane < NP) above[lane] = path != 0 ? parent : -1;
+  for (int i = tid; i < NP * LA / 4; i += 64 * NW) {
+    reinterpret_cast<f4*>(As)[i] = f4{0, 0, 0, 0};
+    reinterpret_cast<f4*>(Ls)[i] = f4{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int x = 0; x < NPG; ++x) {
+    const int i = place(x);
+    if (i >= NP) continue;
+    const bool on = (live >> i) & 1;
+    if (!on) bt[x] = 0.f;
+#pragma unroll
+    for (int c = 0; c < C4; ++c) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        kv[x][c][e] = on ? kv[x][c][e] : 0.f;
+        qv[x][c][e] = on ? qv[x][c][e] * a.scale : 0.f;
+        av[x][c][e] = on ? fast_exp2(av[x][c][e] * kLog2e) : 0.f;
+      }
+      *reinterpret_cast<f4*>(rk + i * LK + 64 * c + 4 * m) = kv[x][c];
+      *reinterpret_cast<f4*>(rq + i * LK + 64 * c + 4 * m) = av[x][c];
+    }
+    if (m == 0) bet[i] = bt[x];
+  }
+  lds_barrier();
+
+#pragma unroll
+  for (int x = 0; x < NPG; ++x) {
+    const int i = place(x);
+    if (i >= NP) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < C4; ++c) s = dot4(qv[x][c], kv[x][c], s);
+    s = row_sum16(s);
+    if (m == 0) As[i * LA + i] = s;
+    int j = above[i];                    // -1 too where there is no draft
+    while (__any(j >= 0)) {
+      const int jj = max(j, 0);
+      float sq = 0.f, sk = 0.f;
+      f4 aj[C4];
+#pragma unroll
+      for (int c = 0; c < C4; ++c) {
+        const f4 t = av[x][c] * *reinterpret_cast<const f4*>(rk + jj * LK + 64 * c + 4 * m);
+        aj[c] = *reinterpret_cast<const f4*>(rq + jj * LK + 64 * c + 4 * m);
+        sq = dot4(qv[x][c], t, sq);
+        sk = dot4(kv[x][c], t, sk);
+      }
+      sq = row_sum16(sq);
+      sk = row_sum16(sk) * bt[x];
+      if (j >= 0) {
+        if (m < 2) (m == 0 ? As : Ls)[i * LA + j] = m == 0 ? sq : sk;
+#pragma unroll
+        for (int c = 0; c < C4; ++c) av[x][c] *= aj[c];
+        j = above[j];
+      }
+    }
+  }
+  lds_barrier();
+#pragma unroll
+  for (int x = 0; x < NPG; ++x) {
+    const int i = place(x);
+    if (i >= NP) continue;
+#pragma unroll
+    for (int c = 0; c < C4; ++c) {
+      *reinterpret_cast<f4*>(rk + i * LK + 64 * c + 4 * m) = av[x][c] * kv[x][c];
+      *reinterpret_cast<f4*>(rq + i * LK + 64 * c + 4 * m) = av[x][c] * qv[x][c];
+    }
+  }
+  // (I + beta L)^-1 of the diagonal tiles: tile gq, a column a lane, row after row
+  if (wave == 0 && gq < NT) {
+    float t[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == m ? 1.f : 0.f;
+#pragma unroll
+      for (int k = 0; k < i; ++k) s = fmaf(-Ls[(16 * gq + i) * LA + 16 * gq + k], t[k], s);
+      t[i] = s;
+      Ts[(gq * 16 + i) * LT + m] = s;
+    }
+  }
+  lds_barrier();
+
+  f4 pk[NT][2], pq[NT][2];
+#pragma unroll
+  for (int r = 0; r < NT; ++r)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) pk[r][c] = pq[r][c] = f4{0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+    for (int r = 0; r < NT; ++r) {
+      const f4 fk = *reinterpret_cast<const f4*>(rk + (16 * r + m) * LK + 16 * s + 4 * gq);
+      const f4 fq = *reinterpret_cast<const f4*>(rq + (16 * r + m) * LK + 16 * s + 4 * gq);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          pk[r][c] = mfma4(fk[e], S[s][e][c], pk[r][c]);
+          pq[r][c] = mfma4(fq[e], S[s][e][c], pq[r][c]);
+        }
+    }
+  f4 u[NT][2];
+#pragma unroll
+  for (int r = 0; r < NT; ++r) {
+    f4 w[2];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 16 * r + 4 * gq + e;
+      const int64_t t = token(i) * D + col;
+      const float be = bet[i];
+      const bool on = (live >> i) & 1;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) w[c][e] = on ? be * (ld1<DT>(a.v, t + c) - pk[r][c][e]) : 0.f;
+    }
+#pragma unroll
+    for (int y = 0; y < r; ++y) {
+      const f4 l = *reinterpret_cast<const f4*>(Ls + (16 * r + m) * LA + 16 * y + 4 * gq);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) w[c] = mfma4(-l[e], u[y][c][e], w[c]);
+    }
+    const f4 ti = *reinterpret_cast<const f4*>(Ts + (16 * r + m) * LT + 4 * gq);
+    u[r][0] = u[r][1] = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) u[r][c] = mfma4(ti[e], w[c][e], u[r][c]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (!((live >> (16 * r + 4 * gq + e)) & 1)) u[r][0][e] = u[r][1][e] = 0.f;
+#pragma unroll
+    for (int y = 0; y <= r; ++y) {
+      const f4 p = *reinterpret_cast<const f4*>(As + (16 * r + m) * LA + 16 * y + 4 * gq);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) pq[r][c] = mfma4(p[e], u[y][c][e], pq[r][c]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 16 * r + 4 * gq + e;
+      if (i >= N) continue;
+      const int64_t t = token(i) * D + col;
+      const bool on = (live >> i) & 1;
+      *reinterpret_cast<f2*>(a.u + t) = f2{u[r][0][e], u[r][1][e]};
+      const float x = on ? pq[r][0][e] : 0.f, y = on ? pq[r][1][e] : 0.f;
+      if constexpr (OUT == 0) *reinterpret_cast<f2*>(static_cast<float*>(a.o) + t) = f2{x, y};
+      else *reinterpret_cast<unsigned*>(static_cast<u16*>(a.o) + t) = pack_bf16x2(x, y);
+    }
+  }
+}
+
+// The state after the path of place last[b], in place: two workgroups a (sequence,
+// head), each half of the value columns.  A thread holds four columns of D / 16
+// channels; the path's decayed keys go through LDS, the newest 16 places first,
+// while the state is on its way.  Bound by the state's bytes, read and written once.
+template <int D, int DT>
+__global__ __launch_bounds__(2 * D) void kda_tree_commit_kernel(TreeCommitArgs a) {
+  constexpr int W = D / 2, NCQ = W / 4, RPT = D / 16, PIECE = 16;
+  static_assert(2 * D / NCQ * RPT == D && RPT % 4 == 0, "four channels a read");
+  __shared__ __attribute__((aligned(16))) float lk[PIECE][D];
+  __shared__ __attribute__((aligned(16))) float gam[D];
+  const int tid = threadIdx.x, lane = tid & 63, N = a.N;
+  const int bh = blockIdx.x >> 1, b = bh / a.H, h = bh - b * a.H, c0 = (blockIdx.x & 1) * W;
+  const int last = a.last[b], parent = a.parents[static_cast<int64_t>(b) * N + min(lane, N - 1)];
+  if (last < 0 || last >= N) return;
+  u64 path = uniform_u64(shfl_u64(tree_paths(parent, N), last));
+  if (path == 0) return;
+  const int cq = tid % NCQ, d0 = tid / NCQ * RPT;
+  float* S = a.state + static_cast<int64_t>(bh) * D * D + c0 + 4 * cq;
+  f4 sv[RPT], acc[RPT];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    sv[i] = *reinterpret_cast<const f4*>(S + (d0 + i) * D);
+    acc[i] = f4{0, 0, 0, 0};
+  }
+  float fade = 1.f;                      // of channel tid: the product of a over the places behind
+  while (path) {
+    u64 rest = path;
+    int n = 0;
+    for (; n < PIECE && rest; ++n) {
+      const int j = 63 - __clzll(static_cast<long long>(rest));
+      rest &= ~(u64{1} << j);
+      if (tid < D) {
+        const int64_t t = ((static_cast<int64_t>(b) * N + j) * a.H + h) * D + tid;
+        lk[n][tid] = fade * ld1<DT>(a.k, t);
+        fade *= fast_exp2(ld1<DT>(a.g, t) * kLog2e);
+      }
+    }
+    if (tid < D && rest == 0) gam[tid] = fade;
+    lds_barrier();
+    for (int x = 0; x < n; ++x) {
+      const int j = 63 - __clzll(static_cast<long long>(path));
+      path &= ~(u64{1} << j);
+      const f4 uj = *reinterpret_cast<const f4*>(a.u + ((static_cast<int64_t>(b) * N + j) * a.H + h) * D + c0 + 4 * cq);
+#pragma unroll
+      for (int i = 0; i < RPT; i += 4) {
+        const f4 w = *reinterpret_cast<const f4*>(&lk[x][d0 + i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i + e] += w[e] * uj;
+      }
+    }
+    if (path) lds_barrier();             // the piece has been read
+  }
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) *reinterpret_cast<f4*>(S + (d0 + i) * D) = gam[d0 + i] * sv[i] + acc[i];
+}
+
+template <int D, int DT, int NT>
+hipError_t step_out(const TreeStepArgs& a, int out, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(a.B * a.H)), block(2 * D);
+  if (out == 0) kda_tree_step_kernel<D, DT, NT, 0><<<grid, block, 0, s>>>(a);
+  else kda_tree_step_kernel<D, DT, NT, 1><<<grid, block, 0, s>>>(a);
+  return hipGetLastError();
+}
+template <int D, int DT>
+hipError_t step_places(const TreeStepArgs& a, int out, hipStream_t s) {
+  return a.N <= 16 ? step_out<D, DT, 1>(a, out, s) : a.N <= 32 ? step_out<D, DT, 2>(a, out, s) : step_out<D, DT, 4>(a, out, s);
+}
+template <int D>
+hipError_t step_types(const TreeStepArgs& a, int dt, int out, hipStream_t s) {
+  return dt == 0 ? step_places<D, 0>(a, out, s) : dt == 1 ? step_places<D, 1>(a, out, s) : step_places<D, 2>(a, out, s);
+}
+template <int D>
+hipError_t commit_types(const TreeCommitArgs& a, int dt, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(2 * a.B * a.H));
+  if (dt == 0) kda_tree_commit_kernel<D, 0><<<grid, dim3(2 * D), 0, s>>>(a);
+  else if (dt == 1) kda_tree_commit_kernel<D, 1><<<grid, dim3(2 * D), 0, s>>>(a);
+  else kda_tree_commit_kernel<D, 2><<<grid, dim3(2 * D), 0, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_tree_step(const TreeStepArgs& a, int d, int dt, int out_dt, hipStream_t s) {
+  return d == 128 ? step_types<128>(a, dt, out_dt, s) : step_types<64>(a, dt, out_dt, s);
+}
+hipError_t launch_tree_commit(const TreeCommitArgs& a, int d, int dt, hipStream_t s) {
+  return d == 128 ? commit_types<128>(a, dt, s) : commit_types<64>(a, dt, s);
+}
+
+}  // namespace kda
