@@ -279,7 +279,12 @@ struct Tree {
     const u64 rest = live >> -base;
     return rest ? __ffsll(static_cast<long long>(rest)) - 1 : t;
   }
-  static __device__ __forceinline__ bool sees(u64 path, int place) { return place < 0 || (place < 64 && (path >> (place & 63) & 1)); }
+  // whether a row with this path sees the row of a place (negative: one before the places')
+  static __device__ __forceinline__ bool sees_one(u64 path, int place) { return place < 0 || (place < 64 && (path >> (place & 63) & 1)); }
+  // which of a tile's rows, from place `first` on (uniform; above -64), a row with this path sees: bits
+  static __device__ __forceinline__ unsigned sees(u64 path, int first) {
+    return static_cast<unsigned>(first >= 64 ? 0 : first >= 0 ? path >> first : path << -first | ((u64{1} << -first) - 1));
+  }
 };
 
 // zeros for the rows of an empty sequence
@@ -374,7 +379,10 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
     Tree tree;
     if constexpr (TREE) tree.load(a, b, len);
     const int clear = TREE ? max(tree.base, 0) / KT : 0;   // a tree: tiles before this one hold no place
-    auto token = [&](int j) { return TREE ? tree.token(min(j * KT + m, len - 1)) : min(j * KT + m, len - 1); };
+    auto token = [&](int j) {
+      const int t = min(j * KT + m, len - 1);
+      return TREE && j >= clear ? tree.token(t) : t;
+    };
     auto page_at = [&](int j) {
       if (TREE && j >= clear) return fresh(page_of(a, table, token(j)));
       return page_of_tile<KT>(a, table, len, j, m);
@@ -389,8 +397,15 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
       }
     };
     int pages[AHEAD + 1];
+    if constexpr (TREE) {                    // all on their way before the first is waited for
 #pragma unroll
-    for (int x = 0; x <= AHEAD; ++x) pages[x] = page_at(ta + x);
+      for (int x = 0; x <= AHEAD; ++x) pages[x] = page_of(a, table, token(ta + x));
+#pragma unroll
+      for (int x = 0; x <= AHEAD; ++x) pages[x] = fresh(pages[x]);
+    } else {
+#pragma unroll
+      for (int x = 0; x <= AHEAD; ++x) pages[x] = page_at(ta + x);
+    }
     F q[KS];
     if (wave < SP) {
       const E* qp = static_cast<const E*>(a.q) + (static_cast<int64_t>(b) * rows + cr) * W;
@@ -449,9 +464,10 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
         }
         if constexpr (ph == SP - 1) {
           const int key0 = j * KT + 4 * gq, par = j & 1;
+          const unsigned bits = !TREE ? 0 : j < clear ? 15 : Tree::sees(mine, j * KT - tree.base) >> (4 * gq);
           f4 s = s0 + s1;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[e] = (TREE ? Tree::sees(mine, key0 + e - tree.base) : key0 + e < seen) ? s[e] : -INFINITY;
+          for (int e = 0; e < 4; ++e) s[e] = (TREE ? bits >> e & 1 : key0 + e < seen) ? s[e] : -INFINITY;
           const float tm = group_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
           float mx = top[m];
           const bool up = __any(tm > mx + lazy);
@@ -568,6 +584,12 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
 // key) and their chain of reads, products and softmax bound it.  Two waves a tile
 // with 32 rows each and 16 keys at a time, which reads LDS half as often, took 112:
 // the chain is per tile, not per key.
+// A tree of drafts (TREE) has many groups of 64 rows against the same cache.  25 drafts,
+// 64 heads, 4 sequences of 20000 to 32768 tokens, fp16: 380 to 400 us, 930 TFLOP/s over all
+// rows (780 over those that hold a draft).  What bounds it there is the copies: 36 KB a tile and CU go to
+// LDS at 21 to 28 bytes a clock, 1300 to 1750 of a tile's 2500 clocks, and nothing hides them whole.
+// Score waves of 32 rows (half the LDS reads of keys) took as long or longer in four
+// arrangements, 16 or 32 keys a tile, alternating or sharing tiles: 395 to 745 us.
 template <int DT, int R, int DR, bool TREE = false>
 __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeArgs a) {
   typedef typename El<DT>::frag F;
@@ -607,9 +629,10 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
     const int32_t* table = a.table + static_cast<int64_t>(b) * a.per;
     Tree tree;
     if constexpr (TREE) tree.load(a, b, len);
+    const int first = TREE ? max(tree.base, 0) / KT : 0;   // a tree: tiles before this one hold no place
     auto token = [&](int j) {                // a key a lane
       const int t = min(j * KT + (lane & 31), len - 1);
-      return TREE ? tree.token(t) : t;
+      return TREE && j >= first ? tree.token(t) : t;
     };
     auto fetch = [&](int slot, char* dst) {
       const int ln = fresh(lane) & 63;
@@ -624,15 +647,22 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
     if (ta + 1 < tb) fetch(slot_of(a, page1, tok1), buf1);
 
     // interval i: tile i is scored, tile i - 1 added, tile i + 2 copied
-    auto turn = [&](int i, char* nxt) {
+    auto arrive = [&](int i) {
       if (i + 1 < tb) wait_vmem_but<PN>();
       else wait_vmem_all();
       lds_barrier();
+    };
+    auto copy = [&](auto plain, int i, char* nxt) {
       if (i + 2 < tb) {
-        const int slot = slot_of(a, page, token(i + 2));
-        page = page_of(a, table, token(i + 3));
+        auto tok = [&](int j) { return decltype(plain)::value ? j * KT + (lane & 31) : token(j); };
+        const int slot = slot_of(a, page, tok(i + 2));
+        page = page_of(a, table, tok(i + 3));
         fetch(slot, nxt);
       }
+    };
+    auto turn = [&](int i, char* nxt) {
+      arrive(i);
+      copy(std::false_type(), i, nxt);
     };
     const bool whole = ta == 0 && tb == n_all;
     const int64_t srow = (static_cast<int64_t>(2 * w + (ta > 0 ? 0 : 1)) * a.groups + grp) * 64;
@@ -661,8 +691,9 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
 #pragma unroll
       for (int t = 0; t < 2; ++t) put[t] = TP::off(m, 2 * t, gq & 1, 16 * own) + 8 * (gq >> 1);
       float mx = max_init(c), mc = mx * c - kLift<DT>, l = 0.f;
-      auto step = [&](int i, const char* cur, char* nxt) {
-        turn(i, nxt);
+      auto step = [&](auto masked, int i, const char* cur, char* nxt) {
+        arrive(i);
+        copy(std::bool_constant<TREE && !decltype(masked)::value>(), i, nxt);
         f4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -673,15 +704,16 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
                                                                            : at[4 + (k - KSN)] + (OFF_R + TR::bytes(16 * t)))), q[k]);
         pace<2 * KS, 8, 1, 1>();
         __builtin_amdgcn_sched_barrier(0);
-        if (i >= clear) {
+        if (decltype(masked)::value && i >= clear) {
           const int key0 = i * KT + 4 * gq;
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 4; ++e)
+{
               const int key = key0 + 16 * t + e;
-              s[t][e] = (TREE ? Tree::sees(mine, key - tree.base) : key < seen) ? s[t][e] : -INFINITY;
-            }
+              s[t][e] = (TREE ? Tree::sees_one(mine, key - tree.base) : key < seen) ? s[t][e] : -INFINITY;
+}
         }
         float tm = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
@@ -707,14 +739,28 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
         }
         l += sum[0] + sum[1];
       };
-      for (int i = ta; i < tb;) {
-        step(i, buf0, buf2);
+      int i = ta;
+      constexpr std::false_type none;
+      constexpr std::true_type masked;
+      if constexpr (TREE) {
+        // Without the mask, whose branches keep the scheduler from the products around them: 25
+        // drafts, 64 heads, four sequences of 20000 to 32768 tokens 394 us for 430 (fp16, cold
+        // cache; warm 389 and 393), 32 sequences of up to 8192 with 256 rows 85 for 96.
+        for (const int most = min(clear, tb); i + 7 <= most; i += 4) {
+          step(none, i, buf0, buf2);
+          step(none, i + 1, buf1, buf3);
+          step(none, i + 2, buf2, buf0);
+          step(none, i + 3, buf3, buf1);
+        }
+      }
+      while (i < tb) {
+        step(masked, i, buf0, buf2);
         if (++i >= tb) break;
-        step(i, buf1, buf3);
+        step(masked, i, buf1, buf3);
         if (++i >= tb) break;
-        step(i, buf2, buf0);
+        step(masked, i, buf2, buf0);
         if (++i >= tb) break;
-        step(i, buf3, buf1);
+        step(masked, i, buf3, buf1);
         ++i;
       }
       turn(tb, buf0);                        // the last tile is added; nothing to copy
@@ -750,8 +796,9 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
           at[v][y] = TN::off(4 * h + (m >> 2 & 3) + 8 * y, (own * (R / 4) + 32 * v) >> 3, 2 * (m >> 4) + ((m & 3) >> 1)) + 8 * (m & 1);
 #pragma unroll
       for (int k = 0; k < 2; ++k) pat[k] = TP::off(m, 2 * k, h);
-      auto step = [&](int i, const char* prev, char* nxt) {
-        turn(i, nxt);
+      auto step = [&](auto plain, int i, const char* prev, char* nxt) {
+        arrive(i);
+        copy(plain, i, nxt);
         const int par = (i - 1) & 1;
         const int4 up = rose[par];
         if (__builtin_amdgcn_readfirstlane(up.x | up.y | up.z | up.w)) {
@@ -789,21 +836,32 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
         __builtin_amdgcn_sched_barrier(0);
       };
       turn(ta, buf2);
-      for (int i = ta + 1; i <= tb;) {
-        step(i, buf0, buf3);
+      int i = ta + 1;
+      constexpr std::true_type plain;
+      constexpr std::false_type any;
+      if constexpr (TREE) {
+        for (const int most = min(max(tree.base, 0) / KT, tb); i + 7 <= most; i += 4) {
+          step(plain, i, buf0, buf3);
+          step(plain, i + 1, buf1, buf0);
+          step(plain, i + 2, buf2, buf1);
+          step(plain, i + 3, buf3, buf2);
+        }
+      }
+      while (i <= tb) {
+        step(any, i, buf0, buf3);
         if (++i > tb) break;
-        step(i, buf1, buf0);
+        step(any, i, buf1, buf0);
         if (++i > tb) break;
-        step(i, buf2, buf1);
+        step(any, i, buf2, buf1);
         if (++i > tb) break;
-        step(i, buf3, buf2);
+        step(any, i, buf3, buf2);
         ++i;
       }
       lds_barrier();
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const int r = r0 + 32 * n + m;
-        if (r >= rows) continue;
+        if (r >= rows) continue;             // a tree's join reads no such row either
         const float ls = ml[1][32 * n + m];
         const int64_t row = static_cast<int64_t>(b) * rows + r;
         const int col = own * (R / 4) + 4 * h;
@@ -815,6 +873,7 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
             f4 o = {acc[v][n][4 * e], acc[v][n][4 * e + 1], acc[v][n][4 * e + 2], acc[v][n][4 * e + 3]};
             if (ls == 0.f) o = f4{0, 0, 0, 0};         // nothing visible: zeros, whatever 0 times the others' rows made
             if (whole) store4<DT>(a.o, row * R + col + 32 * v + 8 * e, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+            else if constexpr (TREE) reinterpret_cast<f4*>(a.part_o + (srow + 32 * n) * R)[(own * (R / 32) + 4 * v + e) * 64 + lane] = o;
             else *reinterpret_cast<f4*>(a.part_o + (srow + 32 * n + m) * R + col + 32 * v + 8 * e) = o;
           }
       }
@@ -895,10 +954,54 @@ __global__ __launch_bounds__(R / 2) void kda_latent_join_kernel(LatentDecodeArgs
   if (threadIdx.x == 0) a.lse[row] = l == 0.f ? -INFINITY : (mx + __log2f(l)) * kLn2;
 }
 
+// The same for a tree's 64 rows a workgroup, whose parts lie as the output waves held
+// them, 32 rows by R: every read and write is 1 KiB in a row (a row's own 2 KiB between
+// rows take twice as long: 16 and 10 us with 256 rows of 32 sequences).  A wave
+// takes PW groups of eight columns of 32 rows.
+template <int DT, int R, int PW>
+__global__ __launch_bounds__(256) void kda_latent_tree_join_kernel(LatentDecodeArgs a) {
+  constexpr int KT = 32, NC = R / 8, CH = NC / PW / 4;   // groups of columns; workgroups of 32 rows
+  const int rows = a.Tq * a.H, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.y, blk = blockIdx.x / CH, e0 = (blockIdx.x % CH * 4 + wave) * PW;
+  const int m = lane & 31, h = lane >> 5, r = 32 * blk + m;
+  const int per = a.line[0], g0 = a.line[1 + b], n = (seq_len(a, b) + KT - 1) / KT;
+  const int64_t row = static_cast<int64_t>(b) * rows + r;
+  f4 o[PW];
+#pragma unroll
+  for (int e = 0; e < PW; ++e) o[e] = f4{0, 0, 0, 0};
+  float l = 0.f, mx = 0.f;
+  if (n > 0) {
+    const int w0 = g0 / per, cnt = (g0 + n - 1) / per - w0 + 1;
+    if (cnt == 1) return;
+    // part i: run w0 + i, whose first segment began inside the sequence but for part 0
+    auto at = [&](int i) { return ((static_cast<int64_t>(2 * (w0 + i) + (i == 0 ? 1 : 0)) * a.groups + blk / 2) * 2 + blk % 2) * 32; };
+    auto stat = [&](int i) { return *reinterpret_cast<const float2*>(a.part_ml + 2 * (at(i) + m)); };
+    mx = stat(0).x;
+#pragma unroll 8
+    for (int i = 1; i < cnt; ++i) mx = fmaxf(mx, stat(i).x);
+#pragma unroll 4
+    for (int i = 0; i < cnt; ++i) {
+      const float2 s = stat(i);
+      const float f = fast_exp2(s.x - mx);
+      l = fmaf(f, s.y, l);
+      const f4* part = reinterpret_cast<const f4*>(a.part_o + at(i) * R) + e0 * 64 + lane;
+#pragma unroll
+      for (int e = 0; e < PW; ++e) o[e] += f * part[e * 64];
+    }
+  }
+  if (r >= rows) return;
+  const float inv = l > 0.f ? 1.f / l : l;
+#pragma unroll
+  for (int e = 0; e < PW; ++e)
+    store4<DT>(a.o, row * R + 8 * (e0 + e) + 4 * h, o[e][0] * inv, o[e][1] * inv, o[e][2] * inv, o[e][3] * inv);
+  if (e0 == 0 && h == 0) a.lse[row] = l == 0.f ? -INFINITY : (mx + __log2f(l)) * kLn2;
+}
+
 // The cache after an accepted path: its rows move to the front of the places'.  A
-// thread takes the same 16 bytes of every row; rows move down only, so eight
-// rows read and then written clobber none that a later eight read, and threads
+// thread takes the same 16 bytes of every row; rows move down only, so kMoves
+// rows read and then written clobber none that the next ones read, and threads
 // need not wait for each other.  Bound by the moved rows' bytes.
+constexpr int kMoves = 16;
 __global__ __launch_bounds__(192) void kda_latent_tree_commit_kernel(LatentTreeCommitArgs a) {
   const int lane = threadIdx.x & 63, b = blockIdx.x, N = a.N;
   const int64_t cap = static_cast<int64_t>(a.per) << a.page_shift;
@@ -923,11 +1026,11 @@ __global__ __launch_bounds__(192) void kda_latent_tree_commit_kernel(LatentTreeC
   const bool mine = threadIdx.x * 16 < a.row_bytes;
   char* cache = a.cache + blockIdx.y * (a.n_pages << a.page_shift) * a.row_bytes + threadIdx.x * 16;
   while (rest) {
-    u32x4 row[8];
-    int to[8];
+    u32x4 row[kMoves];
+    int to[kMoves];
     int n = 0;
 #pragma unroll
-    for (int x = 0; x < 8; ++x)
+    for (int x = 0; x < kMoves; ++x)
       if (rest) {
         const int i = __ffsll(static_cast<long long>(rest)) - 1;
         rest &= rest - 1;
@@ -937,7 +1040,7 @@ __global__ __launch_bounds__(192) void kda_latent_tree_commit_kernel(LatentTreeC
         n = x + 1;
       }
 #pragma unroll
-    for (int x = 0; x < 8; ++x)
+    for (int x = 0; x < kMoves; ++x)
       if (x < n && mine) *reinterpret_cast<u32x4*>(cache + static_cast<int64_t>(to[x]) * a.row_bytes) = row[x];
   }
 }
@@ -964,6 +1067,15 @@ hipError_t run_decode(const LatentDecodeArgs& a, int m_rows, hipStream_t s) {
   }
   if (a.whole) return hipGetLastError();
   const dim3 rows(a.Tq * a.H, a.B), block(R / 2);
+  if constexpr (TREE) {
+    if (m_rows == 64) {
+      // few rows: a wave a group of columns, so that the chip has more of them
+      const int blocks = (a.Tq * a.H + 31) / 32;
+      if (blocks * a.B <= 64) kda_latent_tree_join_kernel<DT, R, 1><<<dim3(blocks * (R / 32), a.B), dim3(256), 0, s>>>(a);
+      else kda_latent_tree_join_kernel<DT, R, R / 128><<<dim3(blocks * 4, a.B), dim3(256), 0, s>>>(a);
+      return hipGetLastError();
+    }
+  }
   if (m_rows == 16) kda_latent_join_kernel<DT, R, 16><<<rows, block, 0, s>>>(a, 16);
   else kda_latent_join_kernel<DT, R, 32><<<rows, block, 0, s>>>(a, 64);
   return hipGetLastError();
