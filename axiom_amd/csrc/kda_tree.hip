@@ -8,8 +8,6 @@
 //   u_i + beta_i sum_{j above i} L_ij u_j = beta_i (v_i - (gamma_i k_i)^T S),
 //   L_ij = k_i . (gamma_i / gamma_j) k_j,
 //   o_i = (gamma_i q_i)^T S + sum_{j on the path} A_ij u_j,  A_ij = q_i . (gamma_i / gamma_j) k_j.
-// The quotient is never formed: it is the product of a over the places between,
-// taken while walking up the path, so nothing overflows however strong the decay.
 
 #include "kda_common.h"
 #include "kda_internal.h"
@@ -39,9 +37,25 @@ __device__ __forceinline__ float dot4(f4 a, f4 b, float c) {
   return c;
 }
 
+// two neighbouring elements, as they lie in memory
+template <int DT> struct Two {
+  typedef unsigned t;
+  static __device__ __forceinline__ f2 floats(unsigned x) {
+    if constexpr (DT == 1) return f2{__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u)};
+    else return f2{f16bits_to_f32(static_cast<u16>(x)), f16bits_to_f32(static_cast<u16>(x >> 16))};
+  }
+};
+template <> struct Two<0> {
+  typedef f2 t;
+  static __device__ __forceinline__ f2 floats(f2 x) { return x; }
+};
+
 // One workgroup a (sequence, head): D / 32 waves of 32 value columns each, whose
 // slice of the state waits in registers while the scores are made.
-//   1. 16 lanes a place walk up its path: A and L to LDS, gamma_i in hand at the end.
+//   1. 16 lanes a place: log2 gamma by doubling along the paths; A and L as products of tiles
+//      of gamma_i q_i and k_j / gamma_j.  Where a path decays by more than 2^-100 its pairs are taken one by
+//      one instead, the quotient being the product of a over the places between, so that nothing
+//      overflows however strong the decay.
 //   2. (gamma q)^T S and (gamma k)^T S by 16x16x4 fp32 products, the state read once.
 //   3. u tile of 16 places by tile: inverses of the diagonal tiles (I + beta L)^-1 times what the
 //      tiles before leave, o from A u.  A tile's result is the next product's operand in
@@ -53,11 +67,12 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
   constexpr int NW = D / 32, NP = 16 * NT, G = 4 * NW, NPG = NP / G > 0 ? NP / G : 1;   // places of a group of 16 lanes
   constexpr int C4 = D / 64, LK = D + 4, LA = NP + 4, LT = 20;
   __shared__ __attribute__((aligned(16))) float rk[NP * LK];   // k, then gamma k
-  __shared__ __attribute__((aligned(16))) float rq[NP * LK];   // a, then gamma q
+  __shared__ __attribute__((aligned(16))) float rq[NP * LK];   // log2 gamma (or a), then gamma q
+  __shared__ __attribute__((aligned(16))) float rn[NT > 1 ? NP * LK : 4];   // k / gamma
   __shared__ __attribute__((aligned(16))) float As[NP * LA], Ls[NP * LA];
   __shared__ __attribute__((aligned(16))) float Ts[NT * 16 * LT];
   __shared__ float bet[NP];
-  __shared__ int above[NP];
+  __shared__ int wide;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, gq = lane >> 4, grp = tid >> 4;
   const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, N = a.N;
@@ -87,18 +102,20 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
   for (int s = 0; s < D / 16; ++s)
 #pragma unroll
     for (int e = 0; e < 4; ++e) S[s][e] = *reinterpret_cast<const f2*>(Sp + (16 * s + 4 * gq + e) * D);
+  typedef typename Two<DT>::t V2;
+  V2 vv[NT][4];                          // v of the lane's rows, its two columns
+#pragma unroll
+  for (int r = 0; r < NT; ++r)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vv[r][e] = static_cast<const V2*>(a.v)[(token(16 * r + 4 * gq + e) * D + col) / 2];
   __builtin_amdgcn_sched_barrier(0);
 
   const u64 path = tree_paths(parent, N), live = __ballot(path != 0);
-  if (wave == 0 && lane < NP) above[lane] = path != 0 ? parent : -1;
-  for (int i = tid; i < NP * LA / 4; i += 64 * NW) {
-    reinterpret_cast<f4*>(As)[i] = f4{0, 0, 0, 0};
-    reinterpret_cast<f4*>(Ls)[i] = f4{0, 0, 0, 0};
-  }
+  if (tid == 0) wide = 0;
+  f4 lv[NPG][C4];                        // log2 gamma of the places in hand
 #pragma unroll
   for (int x = 0; x < NPG; ++x) {
     const int i = place(x);
-    if (i >= NP) continue;
     const bool on = (live >> i) & 1;
     if (!on) bt[x] = 0.f;
 #pragma unroll
@@ -107,57 +124,152 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
       for (int e = 0; e < 4; ++e) {
         kv[x][c][e] = on ? kv[x][c][e] : 0.f;
         qv[x][c][e] = on ? qv[x][c][e] * a.scale : 0.f;
-        av[x][c][e] = on ? fast_exp2(av[x][c][e] * kLog2e) : 0.f;
+        av[x][c][e] = on ? av[x][c][e] * kLog2e : 0.f;
       }
-      *reinterpret_cast<f4*>(rk + i * LK + 64 * c + 4 * m) = kv[x][c];
-      *reinterpret_cast<f4*>(rq + i * LK + 64 * c + 4 * m) = av[x][c];
+      lv[x][c] = av[x][c];
+      if constexpr (NT > 1) *reinterpret_cast<f4*>(rq + i * LK + 64 * c + 4 * m) = lv[x][c];
     }
     if (m == 0) bet[i] = bt[x];
   }
-  lds_barrier();
-
+  // sums along the paths, their lengths doubling: what a place has plus what the place above its own has
+  int up = NT > 1 && path != 0 ? parent : -1;
+  while (__any(up >= 0)) {
+    f4 more[NPG][C4];
+    int ui[NPG];
+    lds_barrier();
 #pragma unroll
-  for (int x = 0; x < NPG; ++x) {
-    const int i = place(x);
-    if (i >= NP) continue;
-    float s = 0.f;
+    for (int x = 0; x < NPG; ++x) {
+      ui[x] = __shfl(up, place(x), 64);
 #pragma unroll
-    for (int c = 0; c < C4; ++c) s = dot4(qv[x][c], kv[x][c], s);
-    s = row_sum16(s);
-    if (m == 0) As[i * LA + i] = s;
-    int j = above[i];                    // -1 too where there is no draft
-    while (__any(j >= 0)) {
-      const int jj = max(j, 0);
-      float sq = 0.f, sk = 0.f;
-      f4 aj[C4];
+      for (int c = 0; c < C4; ++c) more[x][c] = *reinterpret_cast<const f4*>(rq + max(ui[x], 0) * LK + 64 * c + 4 * m);
+    }
+    lds_barrier();
+#pragma unroll
+    for (int x = 0; x < NPG; ++x) {
+      if (ui[x] < 0) continue;
 #pragma unroll
       for (int c = 0; c < C4; ++c) {
-        const f4 t = av[x][c] * *reinterpret_cast<const f4*>(rk + jj * LK + 64 * c + 4 * m);
-        aj[c] = *reinterpret_cast<const f4*>(rq + jj * LK + 64 * c + 4 * m);
-        sq = dot4(qv[x][c], t, sq);
-        sk = dot4(kv[x][c], t, sk);
+        lv[x][c] += more[x][c];
+        *reinterpret_cast<f4*>(rq + place(x) * LK + 64 * c + 4 * m) = lv[x][c];
       }
-      sq = row_sum16(sq);
-      sk = row_sum16(sk) * bt[x];
-      if (j >= 0) {
-        if (m < 2) (m == 0 ? As : Ls)[i * LA + j] = m == 0 ? sq : sk;
+    }
+    const int next = __shfl(up, max(up, 0), 64);
+    up = up >= 0 ? next : up;
+  }
+  // Within 2^kWide the quotient may be two factors: gamma_i q_i times k_j / gamma_j, and
+  // the scores are products of tiles.  The logarithms' sums are then rounded by 2^-18, 2.6e-6 of a
+  // factor, at most; past it (or where one is not a number) the paths are walked.  So are
+  // those of up to 16 places, which are short: B8 N6 8.3 us and 8.8, B64 N16 24.9 and 26.3;
+  // 32 places 48.2 and 47.1 (64 of d = 64 in fp32 28.3 and 25.4), 64 75.8 and 61.7.
+  constexpr float kWide = 100.f;
+  bool far = NT == 1;
 #pragma unroll
-        for (int c = 0; c < C4; ++c) av[x][c] *= aj[c];
-        j = above[j];
+  for (int x = 0; x < NPG; ++x)
+#pragma unroll
+    for (int c = 0; c < C4; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) far |= !(fabsf(lv[x][c][e]) <= kWide);
+  if (NT > 1) {
+    if (__any(far) && lane == 0) wide = 1;
+    lds_barrier();
+  }
+  if (NT > 1 && __builtin_amdgcn_readfirstlane(wide) == 0) {
+#pragma unroll
+    for (int x = 0; x < NPG; ++x) {
+      const int at = place(x) * LK + 4 * m;
+#pragma unroll
+      for (int c = 0; c < C4; ++c) {
+        f4 gm, in;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          gm[e] = fast_exp2(lv[x][c][e]);
+          in[e] = fast_exp2(-lv[x][c][e]);
+        }
+        *reinterpret_cast<f4*>(rk + at + 64 * c) = gm * kv[x][c];
+        *reinterpret_cast<f4*>(rq + at + 64 * c) = gm * qv[x][c];
+        *reinterpret_cast<f4*>(rn + at + 64 * c) = in * kv[x][c];
+      }
+    }
+    lds_barrier();
+    // tiles (r, y <= r) of A and of beta L, dealt out to the waves
+    for (int it = wave; it < NT * (NT + 1); it += NW) {
+      const int t = it >> 1, r = t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0, y = t - r * (r + 1) / 2;
+      const float* rows = it & 1 ? rk : rq;
+      f4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        const f4 x = *reinterpret_cast<const f4*>(rows + (16 * r + m) * LK + 16 * s + 4 * gq);
+        const f4 z = *reinterpret_cast<const f4*>(rn + (16 * y + m) * LK + 16 * s + 4 * gq);
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          s0 = mfma4(x[e], z[e], s0);
+          s1 = mfma4(x[e + 1], z[e + 1], s1);
+        }
+      }
+      s0 += s1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 16 * r + 4 * gq + e, j = 16 * y + m;
+        const bool on = shfl_u64(path, i) >> j & 1;
+        if (it & 1) Ls[i * LA + j] = on && j != i ? bet[i] * s0[e] : 0.f;
+        else As[i * LA + j] = on ? s0[e] : 0.f;
+      }
+    }
+  } else {
+    for (int i = tid; i < NP * LA / 4; i += 64 * NW) {
+      reinterpret_cast<f4*>(As)[i] = f4{0, 0, 0, 0};
+      reinterpret_cast<f4*>(Ls)[i] = f4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int x = 0; x < NPG; ++x)
+#pragma unroll
+      for (int c = 0; c < C4; ++c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) av[x][c][e] = fast_exp2(av[x][c][e]);
+        *reinterpret_cast<f4*>(rk + place(x) * LK + 64 * c + 4 * m) = kv[x][c];
+        *reinterpret_cast<f4*>(rq + place(x) * LK + 64 * c + 4 * m) = av[x][c];
+      }
+    lds_barrier();
+#pragma unroll
+    for (int x = 0; x < NPG; ++x) {
+      const int i = place(x);
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < C4; ++c) s = dot4(qv[x][c], kv[x][c], s);
+      s = row_sum16(s);
+      if (m == 0) As[i * LA + i] = s;
+      u64 rest = shfl_u64(path, i) & ((u64{1} << i) - 1);   // the places above, the nearest first
+      while (__any(rest != 0)) {
+        const int j = rest ? 63 - __clzll(static_cast<long long>(rest)) : -1;
+        float sq = 0.f, sk = 0.f;
+#pragma unroll
+        for (int c = 0; c < C4; ++c) {
+          const f4 t = av[x][c] * *reinterpret_cast<const f4*>(rk + max(j, 0) * LK + 64 * c + 4 * m);
+          const f4 aj = *reinterpret_cast<const f4*>(rq + max(j, 0) * LK + 64 * c + 4 * m);
+          sq = dot4(qv[x][c], t, sq);
+          sk = dot4(kv[x][c], t, sk);
+          if (j >= 0) av[x][c] *= aj;
+        }
+        sq = row_sum16(sq);
+        sk = row_sum16(sk) * bt[x];
+        if (j >= 0) {
+          if (m < 2) (m == 0 ? As : Ls)[i * LA + j] = m == 0 ? sq : sk;
+          rest &= ~(u64{1} << j);
+        }
+      }
+    }
+    lds_barrier();
+#pragma unroll
+    for (int x = 0; x < NPG; ++x) {
+      const int i = place(x);
+#pragma unroll
+      for (int c = 0; c < C4; ++c) {
+        *reinterpret_cast<f4*>(rk + i * LK + 64 * c + 4 * m) = av[x][c] * kv[x][c];
+        *reinterpret_cast<f4*>(rq + i * LK + 64 * c + 4 * m) = av[x][c] * qv[x][c];
       }
     }
   }
   lds_barrier();
-#pragma unroll
-  for (int x = 0; x < NPG; ++x) {
-    const int i = place(x);
-    if (i >= NP) continue;
-#pragma unroll
-    for (int c = 0; c < C4; ++c) {
-      *reinterpret_cast<f4*>(rk + i * LK + 64 * c + 4 * m) = av[x][c] * kv[x][c];
-      *reinterpret_cast<f4*>(rq + i * LK + 64 * c + 4 * m) = av[x][c] * qv[x][c];
-    }
-  }
   // (I + beta L)^-1 of the diagonal tiles: tile gq, a column a lane, row after row
   if (wave == 0 && gq < NT) {
     float t[16];
@@ -170,7 +282,6 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
       Ts[(gq * 16 + i) * LT + m] = s;
     }
   }
-  lds_barrier();
 
   f4 pk[NT][2], pq[NT][2];
 #pragma unroll
@@ -191,6 +302,7 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
           pq[r][c] = mfma4(fq[e], S[s][e][c], pq[r][c]);
         }
     }
+  lds_barrier();                         // the inverses are there
   f4 u[NT][2];
 #pragma unroll
   for (int r = 0; r < NT; ++r) {
@@ -198,11 +310,11 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = 16 * r + 4 * gq + e;
-      const int64_t t = token(i) * D + col;
       const float be = bet[i];
       const bool on = (live >> i) & 1;
+      const f2 v = Two<DT>::floats(vv[r][e]);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) w[c][e] = on ? be * (ld1<DT>(a.v, t + c) - pk[r][c][e]) : 0.f;
+      for (int c = 0; c < 2; ++c) w[c][e] = on ? be * (v[c] - pk[r][c][e]) : 0.f;
     }
 #pragma unroll
     for (int y = 0; y < r; ++y) {
