@@ -40,12 +40,12 @@ int check_states(int B, int N, int H, int dk, int dv, int dtype) {
 
 // Slices of a row, a workgroup each.  Drawing: one workgroup a CU over all
 // sequences, none under 4096 entries (a wave's share is then one round of loads); greedy, where all
-// rows of all sequences are looked at: two, none under 2048.
+// rows of all sequences are looked at: four, none under 2048.
 int draw_slices(int64_t B, int64_t V) {
   return static_cast<int>(std::max<int64_t>(1, std::min({int64_t{64}, 256 / std::max<int64_t>(B, 1), V / 4096})));
 }
 int greedy_slices(int64_t rows, int64_t V) {
-  return static_cast<int>(std::max<int64_t>(1, std::min({int64_t{64}, 512 / std::max<int64_t>(rows, 1), V / 2048})));
+  return static_cast<int>(std::max<int64_t>(1, std::min({int64_t{64}, 1024 / std::max<int64_t>(rows, 1), V / 2048})));
 }
 constexpr size_t kWalkBytes = 16 + 8 * kPlaces, kPieceBytes = 16 * 16;   // a sequence's walk; a slice's sums
 

@@ -21,15 +21,16 @@ constexpr int kWaves = 16, kThreads = 64 * kWaves;
 // EPL elements of a row at any alignment: one 16-byte load
 template <int DT> struct Pack { static constexpr int EPL = DT == 0 ? 4 : 8; };
 template <int DT>
-__device__ __forceinline__ void load_pack(const void* row, int64_t at, float (&x)[Pack<DT>::EPL]) {
-  if constexpr (DT == 0) {
-    __builtin_memcpy(x, static_cast<const float*>(row) + at, 16);
-  } else {
-    u16 h[8];
-    __builtin_memcpy(h, static_cast<const u16*>(row) + at, 16);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = DT == 1 ? bf16_to_f32(h[e]) : f16bits_to_f32(h[e]);
-  }
+__device__ __forceinline__ u32x4 load_pack(const void* row, int64_t at) {
+  u32x4 x;
+  __builtin_memcpy(&x, static_cast<const char*>(row) + at * (DT == 0 ? 4 : 2), 16);
+  return x;
+}
+template <int DT>
+__device__ __forceinline__ float element(const u32x4& x, int e) {
+  if constexpr (DT == 0) return __uint_as_float(x[e]);
+  else if constexpr (DT == 1) return __uint_as_float(e & 1 ? x[e >> 1] & 0xFFFF0000u : x[e >> 1] << 16);
+  else return f16bits_to_f32(static_cast<u16>(e & 1 ? x[e >> 1] >> 16 : x[e >> 1]));
 }
 __device__ __forceinline__ double readlane_f64(double x, int lane) {
   const u64 b = __builtin_bit_cast(u64, x);
@@ -71,39 +72,44 @@ __device__ __forceinline__ double weight(const Weights& w, double z, int x, int 
   }
   return r;
 }
-// The wave's sums of R and of the row itself over entries [lo, hi), a lane's share.
-template <int DT, bool DRAFT>
+// The wave's sums of R and (PLAIN) of the row itself over entries [lo, hi), a lane's share.
+template <int DT, bool DRAFT, bool PLAIN>
 __device__ __forceinline__ void sum_range(const Weights& w, double z, int x, int lo, int hi, double& sum, double& plain) {
   constexpr int EPL = Pack<DT>::EPL, U = 16 / EPL, STEP = 64 * EPL;   // 16 entries in hand
   const int lane = __lane_id();
   sum = plain = 0.0;
+  const int i0 = w.rej ? __ffsll(static_cast<long long>(w.rej)) - 1 : 0;
+  const double z0 = w.rej ? readlane_f64(z, i0) : 0.0;
   for (int v0 = lo; v0 + EPL <= hi; v0 += U * STEP) {
+    u32x4 p[U], q[U];
     double r[U][EPL];
     bool in[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int v = v0 + k * STEP + lane * EPL;
       in[k] = v + EPL <= hi;
-      float t[EPL];
-      load_pack<DT>(w.p, in[k] ? v : lo, t);
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) r[k][e] = t[e] > 0.f ? t[e] : 0.0;
+      p[k] = load_pack<DT>(w.p, in[k] ? v : lo);
+      // the first rejected draft's row together with it (where there is none: the same row once more)
+      if constexpr (DRAFT) q[k] = load_pack<DT>(w.rej ? w.draft : w.p, (w.rej ? i0 * w.d_row : 0) + (in[k] ? v : lo));
     }
 #pragma unroll
     for (int k = 0; k < U; ++k)
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) plain += in[k] ? r[k][e] : 0.0;
-    for (u64 rest = w.rej; rest; rest &= rest - 1) {
+      for (int e = 0; e < EPL; ++e) {
+        const float t = element<DT>(p[k], e);
+        r[k][e] = in[k] && t > 0.f ? t : 0.f;
+        if (PLAIN) plain += r[k][e];
+        if constexpr (DRAFT) r[k][e] = fmax(r[k][e] - z0 * static_cast<double>(element<DT>(q[k], e)), 0.0);
+      }
+    for (u64 rest = DRAFT ? w.rej & (w.rej - 1) : w.rej; rest; rest &= rest - 1) {
       const int i = __ffsll(static_cast<long long>(rest)) - 1;
       if constexpr (DRAFT) {
         const double zi = readlane_f64(z, i);
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-          const int v = v0 + k * STEP + lane * EPL;
-          float t[EPL];
-          load_pack<DT>(w.draft, i * w.d_row + (in[k] ? v : lo), t);
+          const u32x4 y = load_pack<DT>(w.draft, i * w.d_row + (in[k] ? v0 + k * STEP + lane * EPL : lo));
 #pragma unroll
-          for (int e = 0; e < EPL; ++e) r[k][e] = fmax(r[k][e] - zi * static_cast<double>(t[e]), 0.0);
+          for (int e = 0; e < EPL; ++e) r[k][e] = fmax(r[k][e] - zi * static_cast<double>(element<DT>(y, e)), 0.0);
         }
       } else {
         const int xi = __builtin_amdgcn_readlane(x, i);
@@ -116,17 +122,16 @@ __device__ __forceinline__ void sum_range(const Weights& w, double z, int x, int
 #pragma unroll
     for (int k = 0; k < U; ++k)
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) sum += in[k] ? r[k][e] : 0.0;
+      for (int e = 0; e < EPL; ++e) sum += r[k][e];
   }
   // a last pack that the range's end cuts
-  const int tail = lo + (hi - lo) / EPL * EPL + lane;
-  if (hi > lo && tail < hi) {
-    const float p = ld1<DT>(w.p, tail);
-    plain += p > 0.f ? p : 0.0;
+  const int tail = lo + max(hi - lo, 0) / EPL * EPL + lane;
+  if (__any(tail < hi)) {
+    const double r = weight<DT, DRAFT>(w, z, x, tail < hi ? tail : lo);
+    const float t = ld1<DT>(w.p, tail < hi ? tail : lo);
+    sum += tail < hi ? r : 0.0;
+    if (PLAIN) plain += tail < hi && t > 0.f ? t : 0.0;
   }
-  double r = 0.0;
-  if (hi > lo && __any(tail < hi)) r = weight<DT, DRAFT>(w, z, x, tail < hi ? tail : lo);
-  sum += hi > lo && tail < hi ? r : 0.0;
 }
 
 // ws of a sequence: the walk's end, then the sums of the row's pieces (R, row), one a wave of each slice
@@ -146,70 +151,97 @@ __device__ __forceinline__ void piece(const TreeVerifyArgs& a, int j, int& lo, i
   hi = min(s1, lo + len);
 }
 
-// One wave: the lowest v whose running sum of R passes u times the sum.
+// Running sum over the workgroup's threads, and the whole (the same bits in every thread).
+__device__ __forceinline__ double block_scan(double x, double* lds, double& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double s = wave_scan(x);
+  if (lane == 63) lds[wave] = s;
+  __syncthreads();
+  double before = 0.0;
+  total = 0.0;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) {
+    before += k < wave ? lds[k] : 0.0;
+    total += lds[k];
+  }
+  __syncthreads();
+  return s + before;
+}
+// The first thread that says `hit`, else the last that says `has` (one does), in all threads.
+__device__ __forceinline__ int block_pick(bool hit, bool has, int* lds) {
+  if (threadIdx.x == 0) {
+    lds[0] = kThreads;
+    lds[1] = -1;
+  }
+  __syncthreads();
+  const u64 h = __ballot(hit), l = __ballot(has);
+  const int first = threadIdx.x & ~63;
+  if ((threadIdx.x & 63) == 0) {
+    if (h) atomicMin(&lds[0], first + __ffsll(static_cast<long long>(h)) - 1);
+    if (l) atomicMax(&lds[1], first + 63 - __clzll(static_cast<long long>(l)));
+  }
+  __syncthreads();
+  const int r = lds[0] < kThreads ? lds[0] : lds[1];
+  __syncthreads();
+  return r;
+}
+
+// The lowest v whose running sum of R passes u times the sum: the piece of the row, then
+// the thread whose few entries of it, then the entry.  sums: of the pieces, R and the row.
 template <int DT, bool DRAFT>
-__device__ __forceinline__ int pick(const TreeVerifyArgs& a, const double* sums, const Weights& given, double z, int x, double u) {
-  const int lane = __lane_id(), n = a.slices * kWaves, per = (n + 63) / 64;
+__device__ __forceinline__ void pick(const TreeVerifyArgs& a, int b, const double* sums, const Weights& given, double z, int x, double u) {
+  __shared__ double lds[kWaves];
+  __shared__ int which[2];
+  const int n = a.slices * kWaves;       // at most as many as threads
   Weights w = given;
-  double mine[2] = {0.0, 0.0};
-  for (int e = 0; e < per; ++e) {
-    const int j = lane * per + e;
-    if (j < n) {
-      mine[0] += sums[2 * j];
-      mine[1] += sums[2 * j + 1];
+  const int tid = threadIdx.x;
+  double own = tid < n ? sums[2 * tid] : 0.0, total;
+  double scan = block_scan(own, lds, total);
+  if (!(total > 0.0)) {                  // nothing left: the row as it was
+    w.rej = 0;
+    own = tid < n ? sums[2 * tid + 1] : 0.0;
+    scan = block_scan(own, lds, total);
+    if (!(total > 0.0)) {
+      if (tid == 0) a.next[b] = -1;
+      return;
     }
   }
-  double scan = wave_scan(mine[0]), total = readlane_f64(scan, 63);
-  int which = 0;
-  if (!(total > 0.0)) {                  // nothing left: the row as it was
-    which = 1;
-    w.rej = 0;
-    scan = wave_scan(mine[1]);
-    total = readlane_f64(scan, 63);
-    if (!(total > 0.0)) return -1;
-  }
-  const double t = u * total, own = which ? mine[1] : mine[0];
-  const u64 over = __ballot(own > 0.0 && scan > t), some = __ballot(own > 0.0);
-  // past every sum (u not below 1): the last entry that has a weight
-  const int at = over ? __ffsll(static_cast<long long>(over)) - 1 : 63 - __clzll(static_cast<long long>(some));
-  double sum = readlane_f64(scan, at) - readlane_f64(own, at), before = sum;
-  int j = at * per;
-  for (int e = 0; e < per && at * per + e < n; ++e) {
-    const double next = sums[2 * (at * per + e) + which];
-    if (!(next > 0.0)) continue;
-    j = at * per + e;
-    before = sum;
-    sum += next;
-    if (sum > t) break;
-  }
-  // the piece in 64 chunks, a lane each, and the chunk found entry by entry
+  // past every sum (u not below 1): the last that has a weight
+  const double t = u * total;
+  const int j = block_pick(own > 0.0 && scan > t, own > 0.0, which);
+  if (tid == j) lds[0] = scan - own;
+  __syncthreads();
+  const double before = lds[0];
+  __syncthreads();
   int lo, hi;
   piece(a, j, lo, hi);
-  const int len = (hi - lo + 63) / 64;
+  const int len = (hi - lo + kThreads - 1) / kThreads, v0 = lo + tid * len;
   double c = 0.0;
   for (int e = 0; e < len; ++e) {
-    const int v = lo + lane * len + e;
-    const double r = weight<DT, DRAFT>(w, z, x, v < hi ? v : lo);
-    c += v < hi ? r : 0.0;
+    const double r = weight<DT, DRAFT>(w, z, x, v0 + e < hi ? v0 + e : lo);
+    c += v0 + e < hi ? r : 0.0;
   }
-  const double cs = wave_scan(c);
-  const u64 hit = __ballot(c > 0.0 && before + cs > t), has = __ballot(c > 0.0);
-  if (!has) return lo;                   // not reached: the piece's sum is of these entries
-  const int chunk = hit ? __ffsll(static_cast<long long>(hit)) - 1 : 63 - __clzll(static_cast<long long>(has));
-  before += readlane_f64(cs, chunk) - readlane_f64(c, chunk);
-  lo += chunk * len;
-  hi = min(hi, lo + len);
-  int found = -1;
-  for (int v0 = lo; v0 < hi; v0 += 64) {
-    const int v = v0 + lane;
-    const double r = weight<DT, DRAFT>(w, z, x, v < hi ? v : lo), e = v < hi ? r : 0.0;
-    const double es = wave_scan(e);
-    const u64 first = __ballot(e > 0.0 && before + es > t), any = __ballot(e > 0.0);
-    if (any) found = v0 + 63 - __clzll(static_cast<long long>(any));
-    if (first) return v0 + __ffsll(static_cast<long long>(first)) - 1;
-    before += readlane_f64(es, 63);
+  const double cs = block_scan(c, lds, total);
+  const int at = block_pick(c > 0.0 && before + cs > t, c > 0.0, which);
+  // no entry has a weight only if the piece's sum has none
+  if (at < 0) {
+    if (tid == 0) a.next[b] = lo;
+    return;
   }
-  return found;
+  if ((tid & ~63) == (at & ~63)) {       // the wave of that thread: weight() reads over its lanes
+    double acc = before + cs - c;
+    int found = -1;
+    bool done = false;
+    for (int e = 0; e < len; ++e) {
+      const double r = weight<DT, DRAFT>(w, z, x, v0 + e < hi ? v0 + e : lo);
+      if (v0 + e < hi && r > 0.0 && !done) {
+        found = v0 + e;
+        acc += r;
+        done = acc > t;
+      }
+    }
+    if (tid == at) a.next[b] = found;
+  }
 }
 
 // A workgroup a (slice, sequence).  Every wave walks the tree (the same numbers, the
@@ -254,7 +286,7 @@ __global__ __launch_bounds__(kThreads) void kda_tree_sample_kernel(TreeVerifyArg
     if constexpr (DRAFT) {
       const int len = ((a.V + kWaves - 1) / kWaves + 63) & ~63;
       double sum, plain;
-      sum_range<DT, DRAFT>(w, z, x, min(a.V, wave * len), min(a.V, (wave + 1) * len), sum, plain);
+      sum_range<DT, DRAFT, false>(w, z, x, min(a.V, wave * len), min(a.V, (wave + 1) * len), sum, plain);
       sum = wave_sum(sum);
       if (lane == 0) red[turn][wave] = sum;
       const double qx = real ? ld1<DT>(w.draft, i * a.d_row + x) : 0.0;
@@ -273,7 +305,7 @@ __global__ __launch_bounds__(kThreads) void kda_tree_sample_kernel(TreeVerifyArg
   int lo, hi;
   piece(a, s * kWaves + wave, lo, hi);
   double sum, plain;
-  sum_range<DT, DRAFT>(w, z, x, lo, hi, sum, plain);
+  sum_range<DT, DRAFT, true>(w, z, x, lo, hi, sum, plain);
   sum = wave_sum(sum);
   plain = wave_sum(plain);
   double* out = a.slices == 1 ? sums : pieces_of(a, b) + 2 * s * kWaves;
@@ -296,26 +328,22 @@ __global__ __launch_bounds__(kThreads) void kda_tree_sample_kernel(TreeVerifyArg
     }
   }
   if (a.slices == 1) {
-    lds_barrier();
-    if (wave == 0) {
-      const int v = pick<DT, DRAFT>(a, sums, w, z, x, u_next);
-      if (lane == 0) a.next[b] = v;
-    }
+    __syncthreads();
+    pick<DT, DRAFT>(a, b, sums, w, z, x, u_next);
   }
 }
 
 // The next token of a sequence whose row was summed in slices.
 template <int DT, bool DRAFT>
-__global__ __launch_bounds__(64) void kda_tree_pick_kernel(TreeVerifyArgs a) {
+__global__ __launch_bounds__(kThreads) void kda_tree_pick_kernel(TreeVerifyArgs a) {
   constexpr int ES = DT == 0 ? 4 : 2;
-  const int b = blockIdx.x, lane = threadIdx.x;
+  const int b = blockIdx.x, lane = threadIdx.x & 63;
   const WalkEnd* e = walk_end(a, b);
   const int64_t x64 = a.tokens[static_cast<int64_t>(b) * a.N + min(lane, a.N - 1)];
   const Weights w{static_cast<const char*>(a.target) + (b * a.t_b + (__builtin_amdgcn_readfirstlane(e->cur) + 1) * a.t_row) * ES,
                   DRAFT ? static_cast<const char*>(a.draft) + b * a.d_b * ES : nullptr, a.d_row, uniform_u64(e->rej)};
   const int x = x64 >= 0 && x64 < a.V ? static_cast<int>(x64) : -1;
-  const int v = pick<DT, DRAFT>(a, pieces_of(a, b), w, e->z[lane], x, a.uniforms[static_cast<int64_t>(b) * (a.N + 1) + a.N]);
-  if (lane == 0) a.next[b] = v;
+  pick<DT, DRAFT>(a, b, pieces_of(a, b), w, e->z[lane], x, a.uniforms[static_cast<int64_t>(b) * (a.N + 1) + a.N]);
 }
 
 // ------------------------------------------------------------------ greedy
@@ -347,18 +375,18 @@ __device__ __forceinline__ u64 best_of(const void* row, int lo, int hi) {
     }
   };
   for (int v0 = lo; v0 + EPL <= hi; v0 += U * STEP) {
-    float t[U][EPL];
+    u32x4 t[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int v = v0 + k * STEP + lane * EPL;
-      load_pack<DT>(row, v + EPL <= hi ? v : lo, t[k]);
+      t[k] = load_pack<DT>(row, v + EPL <= hi ? v : lo);
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int v = v0 + k * STEP + lane * EPL;
       if (v + EPL <= hi)
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) see(t[k][e], v + e);
+        for (int e = 0; e < EPL; ++e) see(element<DT>(t[k], e), v + e);
     }
   }
   const int tail = lo + (hi - lo) / EPL * EPL + lane;
@@ -428,8 +456,8 @@ hipError_t verify(const TreeVerifyArgs& a, hipStream_t s) {
   if (a.draft) kda_tree_sample_kernel<DT, true><<<grid, block, 0, s>>>(a);
   else kda_tree_sample_kernel<DT, false><<<grid, block, 0, s>>>(a);
   if (a.slices > 1) {
-    if (a.draft) kda_tree_pick_kernel<DT, true><<<dim3(a.B), dim3(64), 0, s>>>(a);
-    else kda_tree_pick_kernel<DT, false><<<dim3(a.B), dim3(64), 0, s>>>(a);
+    if (a.draft) kda_tree_pick_kernel<DT, true><<<dim3(a.B), block, 0, s>>>(a);
+    else kda_tree_pick_kernel<DT, false><<<dim3(a.B), block, 0, s>>>(a);
   }
   return hipGetLastError();
 }

@@ -142,7 +142,7 @@ def test_verify_workspace(L):
     assert [L.kda_tree_verify_workspace(*a) for a in ((-1, 4, 9), (1, 0, 9), (1, 65, 9), (1, 4, 0))] == [0] * 4
     for B, N, V in ((1, 1, 1), (1, 64, 10 ** 6), (64, 16, 128000), (300, 3, 50021), (0, 4, 100)):
         draw, rows = max(1, min(64, 256 // max(B, 1), V // 4096)), B * (N + 1)
-        greedy = max(1, min(64, 512 // max(rows, 1), V // 2048))
+        greedy = max(1, min(64, 1024 // max(rows, 1), V // 2048))
         assert L.kda_tree_verify_workspace(B, N, V) == max(B * (528 + 256 * draw), 8 * rows * greedy, 16)
 
 
