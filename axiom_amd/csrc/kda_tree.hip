@@ -72,7 +72,7 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
   __shared__ __attribute__((aligned(16))) float As[NP * LA], Ls[NP * LA];
   __shared__ __attribute__((aligned(16))) float Ts[NT * 16 * LT];
   __shared__ float bet[NP];
-  __shared__ int wide;
+  __shared__ int wide[NW];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, gq = lane >> 4, grp = tid >> 4;
   const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, N = a.N;
@@ -111,7 +111,6 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
   __builtin_amdgcn_sched_barrier(0);
 
   const u64 path = tree_paths(parent, N), live = __ballot(path != 0);
-  if (tid == 0) wide = 0;
   f4 lv[NPG][C4];                        // log2 gamma of the places in hand
 #pragma unroll
   for (int x = 0; x < NPG; ++x) {
@@ -157,8 +156,8 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
     up = up >= 0 ? next : up;
   }
   // Within 2^kWide the quotient may be two factors: gamma_i q_i times k_j / gamma_j, and
-  // the scores are products of tiles.  The logarithms' sums are then rounded by 2^-18, 2.6e-6 of a
-  // factor, at most; past it (or where one is not a number) the paths are walked.  So are
+  // the scores are products of tiles.  An addition of logarithms then rounds by 2^-18, 2.6e-6 of a
+  // factor, at most, and each has six; past it (or where one is not a number) the paths are walked.  So are
   // those of up to 16 places, which are short: B8 N6 8.3 us and 8.8, B64 N16 24.9 and 26.3;
   // 32 places 48.2 and 47.1 (64 of d = 64 in fp32 28.3 and 25.4), 64 75.8 and 61.7.
   constexpr float kWide = 100.f;
@@ -170,10 +169,14 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) far |= !(fabsf(lv[x][c][e]) <= kWide);
   if (NT > 1) {
-    if (__any(far) && lane == 0) wide = 1;
+    const bool any = __any(far);
+    if (lane == 0) wide[wave] = any;
     lds_barrier();
+    far = false;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) far |= wide[x] != 0;
   }
-  if (NT > 1 && __builtin_amdgcn_readfirstlane(wide) == 0) {
+  if (NT > 1 && __builtin_amdgcn_readfirstlane(far) == 0) {
 #pragma unroll
     for (int x = 0; x < NPG; ++x) {
       const int at = place(x) * LK + 4 * m;

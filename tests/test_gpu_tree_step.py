@@ -45,6 +45,19 @@ def test_decays(cuda, decay):
     compare(step_inputs(3, 40, 3, 128, "fp32", cuda, seed=3, decay=decay), p)
 
 
+@pytest.mark.parametrize("decay", [60.0, 300.0, float("inf")])
+@pytest.mark.parametrize("kind", ["star", "chain"])
+@pytest.mark.parametrize("N,d", [(17, 128), (33, 64), (64, 128), (64, 64)])
+def test_one_place_of_strong_decay(cuda, N, d, kind, decay):
+    """A sequence a place: whichever wave holds it, no quotient overflows.  exp(60) = 2^87 is still
+    carried by two factors: twice six additions of logarithms, each off by 2^-18 / sqrt(3) rms,
+    are sqrt(12) 2^-18 / sqrt(3) ln 2 = 5.3e-6 of a pair's share, and the bar holds the rest."""
+    x = step_inputs(N, N, 1, d, "fp32", cuda, seed=N, decay=0.02)
+    for b in range(N):
+        x["g"][b, b, :, 1::2] -= decay
+    compare(x, trees([kind] * N, N, cuda))
+
+
 def test_growing_gates(cuda):
     d = step_inputs(2, 12, 2, 64, "fp32", cuda, seed=4, decay=-0.1)     # g > 0
     compare(d, trees(["random", "chain"], 12, cuda))
