@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 namespace kda {
 
 // Geometry of one chunked call.  Dense: B sequences of T tokens (cu == null).
@@ -290,6 +292,25 @@ hipError_t launch_cc_finish(const CcFinishArgs& a, hipStream_t s);
 
 // Sets the calling thread's error message and returns `code` (kda_last_error).
 int api_fail(int code, const char* msg);
+
+// Whether something a call writes shares memory with another of its arguments.
+struct Bytes {
+  const void* p;
+  size_t n;
+};
+inline bool overlap(std::initializer_list<Bytes> written, std::initializer_list<Bytes> read) {
+  auto meet = [](const Bytes& x, const Bytes& y) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x.p), b = reinterpret_cast<uintptr_t>(y.p);
+    return x.p && y.p && x.n && y.n && (a < b ? b - a < x.n : a - b < y.n);
+  };
+  for (const Bytes* x = written.begin(); x != written.end(); ++x) {
+    for (const Bytes& y : read)
+      if (meet(*x, y)) return true;
+    for (const Bytes* y = x + 1; y != written.end(); ++y)
+      if (meet(*x, *y)) return true;
+  }
+  return false;
+}
 
 // Latent attention, expanded form.  Strides in elements; the last axis of every
 // tensor is contiguous.  o, dout, dq are [B,Tq,H,*] and dkv [B,Tk,H,2 dn],

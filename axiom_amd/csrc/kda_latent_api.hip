@@ -235,6 +235,13 @@ int decode_call(hipStream_t stream, const char* what, const void* q, const void*
     return fail(KDA_ERR_UNSUPPORTED, "Tq * H = %lld rows or B * max_pages * page_size too large", static_cast<long long>(Tq) * H);
   if (!workspace || workspace_bytes < P.total)
     return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0}, P.total);
+  if (tree) {
+    const size_t rows = static_cast<size_t>(B) * Tq * H, W = (R + dr) * elem(dtype), b4 = static_cast<size_t>(B) * 4;
+    if (kda::overlap({{o, rows * R * elem(dtype)}, {lse, rows * 4}, {workspace, P.total}},
+                     {{q, rows * W}, {cache, static_cast<size_t>(n_pages) * page_size * W}, {block_table, b4 * max_pages},
+                      {seq_lens, b4}, {parents, b4 * Tq}}))
+      return fail(KDA_ERR_INVALID_ARGUMENT, "o, lse and workspace must not overlap each other or the inputs");
+  }
   kda::LatentDecodeArgs a{};
   a.q = q; a.cache = cache; a.table = block_table; a.lens = seq_lens; a.o = o; a.lse = lse;
   a.line = static_cast<int*>(workspace);
@@ -387,8 +394,11 @@ int kda_latent_tree_commit(hipStream_t stream, void* cache, const int32_t* block
   if (n_pages == 0) max_pages = 0;      // no page: every length is 0
   if (!seq_lens || !parents || !last || !new_lens || (max_pages > 0 && (!cache || !block_table)))
     return fail(KDA_ERR_INVALID_ARGUMENT, "null cache, block_table, seq_lens, parents, last or new_lens");
-  if (new_lens == seq_lens) return fail(KDA_ERR_INVALID_ARGUMENT, "new_lens must not be seq_lens");
   if (!aligned(cache, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "cache must be aligned to 16 bytes");
+  const size_t b4 = static_cast<size_t>(B) * 4;
+  if (kda::overlap({{cache, static_cast<size_t>(layers) * n_pages * page_size * (R + dr) * elem(dtype)}, {new_lens, b4}},
+                   {{block_table, b4 * max_pages}, {seq_lens, b4}, {parents, b4 * N}, {last, b4}}))
+    return fail(KDA_ERR_INVALID_ARGUMENT, "cache and new_lens must not overlap each other or the inputs");
   kda::LatentTreeCommitArgs a{};
   a.cache = static_cast<char*>(cache); a.table = block_table; a.lens = seq_lens; a.parents = parents; a.last = last;
   a.new_lens = new_lens; a.layers = layers; a.B = B; a.N = N; a.per = max_pages; a.n_pages = n_pages;

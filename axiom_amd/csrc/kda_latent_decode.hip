@@ -709,11 +709,10 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-{
+            for (int e = 0; e < 4; ++e) {
               const int key = key0 + 16 * t + e;
               s[t][e] = (TREE ? Tree::sees_one(mine, key - tree.base) : key < seen) ? s[t][e] : -INFINITY;
-}
+            }
         }
         float tm = fmaxf(s[0][0], s[1][0]);
 #pragma unroll

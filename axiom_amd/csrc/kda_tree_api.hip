@@ -24,6 +24,7 @@ int launched(hipError_t e, const char* what) {
   return e == hipSuccess ? KDA_OK : fail(KDA_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+size_t elem(int dtype) { return dtype == KDA_DTYPE_F32 ? 4 : 2; }
 bool dtype_ok(int dtype) { return dtype == KDA_DTYPE_F32 || dtype == KDA_DTYPE_BF16 || dtype == KDA_DTYPE_F16; }
 
 constexpr int kPlaces = 64;
@@ -64,6 +65,11 @@ int kda_tree_step(hipStream_t stream, const void* q, const void* k, const void* 
   if (!q || !k || !v || !g || !beta || !parents || !state || !o || !u) return fail(KDA_ERR_INVALID_ARGUMENT, "null pointer");
   for (const void* p : {q, k, v, g, static_cast<const void*>(state), static_cast<const void*>(o), static_cast<const void*>(u)})
     if (!aligned(p, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "q, k, v, g, state, o and u must be aligned to 16 bytes");
+  const size_t bn = static_cast<size_t>(B) * N, rows = bn * H, in = rows * dk * elem(in_dtype);
+  if (kda::overlap({{o, rows * dv * elem(out_dtype)}, {u, rows * dv * 4}},
+                   {{q, in}, {k, in}, {v, in}, {g, in}, {beta, rows * elem(in_dtype)}, {parents, bn * 4},
+                    {state, static_cast<size_t>(B) * H * dk * dv * 4}}))
+    return fail(KDA_ERR_INVALID_ARGUMENT, "o and u must not overlap each other or the inputs");
   kda::TreeStepArgs a{};
   a.q = q; a.k = k; a.v = v; a.g = g; a.beta = beta; a.parents = parents; a.state = state; a.o = o; a.u = u;
   a.B = B; a.N = N; a.H = H; a.scale = scale;
@@ -77,6 +83,10 @@ int kda_tree_commit(hipStream_t stream, const void* k, const void* g, const floa
   if (!k || !g || !u || !parents || !last || !state) return fail(KDA_ERR_INVALID_ARGUMENT, "null pointer");
   for (const void* p : {k, g, static_cast<const void*>(u), static_cast<const void*>(state)})
     if (!aligned(p, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "k, g, u and state must be aligned to 16 bytes");
+  const size_t bn = static_cast<size_t>(B) * N, rows = bn * H, in = rows * dk * elem(in_dtype);
+  if (kda::overlap({{state, static_cast<size_t>(B) * H * dk * dv * 4}},
+                   {{k, in}, {g, in}, {u, rows * dv * 4}, {parents, bn * 4}, {last, static_cast<size_t>(B) * 4}}))
+    return fail(KDA_ERR_INVALID_ARGUMENT, "state must not overlap the other arguments");
   kda::TreeCommitArgs a{};
   a.k = k; a.g = g; a.u = u; a.parents = parents; a.last = last; a.state = state;
   a.B = B; a.N = N; a.H = H;
@@ -108,6 +118,14 @@ int kda_tree_verify(hipStream_t stream, const void* target, int64_t target_b, in
     return fail(KDA_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : size_t{0},
                 kda_tree_verify_workspace(B, N, V));
   if (!aligned(workspace, 16)) return fail(KDA_ERR_INVALID_ARGUMENT, "workspace must be aligned to 16 bytes");
+  auto extent = [&](int64_t s_b, int64_t s_row, int n) {   // of n rows a sequence
+    return static_cast<size_t>((B - 1) * s_b + (n - 1) * s_row + V) * elem(dtype);
+  };
+  const size_t b4 = static_cast<size_t>(B) * 4, bn = static_cast<size_t>(B) * N;
+  if (kda::overlap({{last, b4}, {next, 2 * b4}, {accepted, b4}, {workspace, kda_tree_verify_workspace(B, N, V)}},
+                   {{target, extent(target_b, target_row, N + 1)}, {tokens, bn * 8}, {parents, bn * 4}, {uniforms, (bn + B) * 4},
+                    {draft, extent(draft_b, draft_row, N)}}))
+    return fail(KDA_ERR_INVALID_ARGUMENT, "last, next, accepted and workspace must not overlap each other or the inputs");
   kda::TreeVerifyArgs a{};
   a.target = target; a.draft = draft; a.tokens = tokens; a.parents = parents; a.uniforms = uniforms;
   a.last = last; a.next = next; a.accepted = accepted;

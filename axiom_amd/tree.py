@@ -19,6 +19,8 @@ for the host, so a step of a serving loop can be captured into a HIP graph.  A
 place without a draft gets zeros, and what its inputs hold reaches nothing; a
 draft whose own values are not finite may reach the other drafts of its sequence.
 
+What a call writes must not overlap its other arguments.
+
 Every function calls the HIP library through its C ABI (``include/tree_mi355x.h``)
 on torch's current stream, by the C++ binding that also checks the arguments;
 nothing here computes on the CPU.  None is differentiable.

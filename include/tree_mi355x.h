@@ -13,7 +13,8 @@
  * read on the device; every value of parents is safe.  Places without a
  * draft get zeros, and what their inputs hold reaches nothing.  A draft
  * whose own values are not finite may reach other drafts of its sequence and
- * head, on its path or not.
+ * head, on its path or not.  What a call writes must not overlap its other
+ * arguments.
  */
 #ifndef TREE_MI355X_H_
 #define TREE_MI355X_H_
@@ -55,11 +56,11 @@ KDA_API int kda_tree_commit(hipStream_t stream, const void* k, const void* g, co
  * sees the rows before those of the places, and those of its path:
  *   s_j = scale q . row_j,  o = sum_j softmax_j(s) row_j[:R],  lse natural.
  * Places without a draft, and those whose row would lie before the sequence's
- * first (seq_len < N), get o = 0 and lse = -inf.  as kda_latent_decode: o
- * [B,N,H,R] in dtype, lse [B,N,H] fp32, page numbers and lengths clamped, R in {256, 512}, dr in {32, 64},
- * page_size a power of two, caller workspace of
- * kda_latent_tree_decode_workspace bytes, pointers aligned to 16 bytes
- * (tables to their elements).
+ * first (seq_len < N), get o = 0 and lse = -inf.  The rest as
+ * kda_latent_decode: o [B,N,H,R] in dtype, lse [B,N,H] fp32, page numbers and
+ * lengths clamped, R in {256, 512}, dr in {32, 64}, page_size a power of two,
+ * caller workspace of kda_latent_tree_decode_workspace bytes, pointers aligned
+ * to 16 bytes (tables to their elements).
  */
 KDA_API int kda_latent_tree_decode(hipStream_t stream, const void* q, const void* cache, const int32_t* block_table,
                 const int32_t* seq_lens, const int32_t* parents, void* o, float* lse, int B, int N, int H, int R, int dr,
@@ -76,8 +77,8 @@ KDA_API size_t kda_latent_tree_decode_workspace(int B, int N, int H, int R, int 
  * caches [n_pages, page_size, R+dr] that lie one behind the other and share
  * the block table; new_lens[b] = seq_len - N + the path's length.  last[b]
  * outside [0, N), or a place without a draft: the path is empty.  A sequence
- * of fewer than N rows is left as it is, its length too.  new_lens must not
- * be seq_lens.  Page numbers and lengths are clamped as in
+ * of fewer than N rows is left as it is, its length too.  new_lens is not
+ * seq_lens, which calls for further layers still read.  Page numbers and lengths are clamped as in
  * kda_latent_tree_decode.  cache aligned to 16 bytes.
  */
 KDA_API int kda_latent_tree_commit(hipStream_t stream, void* cache, const int32_t* block_table, const int32_t* seq_lens,

@@ -101,6 +101,29 @@ def test_verify_refuses(L, kw, code):
     assert _lib.last_error()
 
 
+@pytest.mark.parametrize("call,kw", [
+    ("step", dict(o="q")), ("step", dict(u="q")), ("step", dict(u="S")), ("step", dict(o="u")), ("step", dict(o="beta")), ("step", dict(u="par")),
+    ("commit", dict(S="u")), ("commit", dict(S="last")), ("commit", dict(S="k")), ("decode", dict(o="q")), ("decode", dict(lse="lens")),
+    ("decode", dict(ws="cache")), ("decode", dict(ws="o")), ("decode", dict(o="par")), ("keep", dict(new="lens")), ("keep", dict(new="last")),
+    ("keep", dict(new="par")), ("keep", dict(new="table")), ("keep", dict(new="cache")), ("verify", dict(nxt="tok")), ("verify", dict(last="par")),
+    ("verify", dict(acc="last")), ("verify", dict(ws="t")), ("verify", dict(nxt="u")), ("verify", dict(acc="ws"))])
+def test_overlaps_are_refused(L, call, kw):
+    """What a call writes in the last bytes of another argument; every other one far from the rest."""
+    names, sizes, f = {
+        "step": (("q", "k", "v", "g", "beta", "par", "S", "o", "u"), dict(q=2048, beta=16, par=16, S=131072, u=4096), _step),
+        "commit": (("k", "g", "u", "par", "last", "S"), dict(u=4096, last=4, k=2048), _commit),
+        "decode": (("q", "cache", "table", "lens", "par", "o", "lse", "ws"), dict(q=9216, lens=4, cache=165888, o=8192, par=16), _decode),
+        "keep": (("cache", "table", "lens", "par", "last", "new"), dict(lens=4, last=4, par=16, table=16, cache=165888), _keep),
+        "verify": (("t", "tok", "par", "u", "last", "nxt", "acc", "ws"), dict(tok=32, par=16, last=4, t=2000, u=20, ws=784), _verify)}[call]
+    at = {n: OK + (i << 24) for i, n in enumerate(names)}
+    (n, other), = kw.items()
+    big = n in ("o", "u", "S", "ws") and call != "verify"
+    step = 16 if big or n == "ws" else 8 if n == "nxt" else 4
+    for p in {at[other], at[other] + (sizes[other] - 1) // step * step}:
+        assert f(L, **{**at, n: p}) == -1, hex(p)
+        assert "overlap" in _lib.last_error()
+
+
 def test_empty_calls_do_nothing(L):
     z = dict(B=0)
     assert _step(L, q=None, **z) == 0 and _commit(L, k=None, **z) == 0 and _decode(L, q=None, **z) == 0
