@@ -4,8 +4,10 @@ Chunked Kimi-Delta-Attention forward in WY/UT form, the single-token recurrent
 decode step, varlen scheduling, the chunked backward and the layer's prologue/epilogue
 (forward and backward), and the latent attention that stands between KDA layers
 (:mod:`axiom_amd.latent`: expanded form with its backward, paged cache, absorbed
-form), and the step over a tree of drafted tokens on both (:mod:`axiom_amd.tree`), as hand-written HIP kernels behind the C ABI of ``include/kda_mi355x.h``.  The Python layer (:mod:`axiom_amd.kda`) only
-validates arguments and hands device pointers to that library.
+form), and the step over a tree of drafted tokens on both (:mod:`axiom_amd.tree`),
+as hand-written HIP kernels behind the C ABI of ``include/kda_mi355x.h``.  The Python
+layer (:mod:`axiom_amd.kda`) only validates arguments and hands device pointers to
+that library.
 """
 
 from .kda import (cc_scan, cc_scan_bwd, kda_chunk, kda_chunk_bwd, kda_chunk_fwd, kda_decode_layer_step,  # noqa: F401

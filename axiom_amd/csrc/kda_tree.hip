@@ -50,27 +50,78 @@ template <> struct Two<0> {
   static __device__ __forceinline__ f2 floats(f2 x) { return x; }
 };
 
+// A float is the sum of three bf16, eight bits each cut off its end: the parts of two floats,
+// p0's the largest.  Six of the nine products of two such sums (without the three below 2^-22 of the
+// factors' powers of two) are the fp32 product to some 2^-24, at 96 clocks for 256.
+struct Parts {
+  unsigned p[3];
+};
+__device__ __forceinline__ Parts parts(float x, float y) {
+  Parts r;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const unsigned a = __float_as_uint(x), b = __float_as_uint(y);
+    r.p[k] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    x -= __uint_as_float(a & 0xFFFF0000u);
+    y -= __uint_as_float(b & 0xFFFF0000u);
+  }
+  return r;
+}
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+// Rows of D fp32 values as planes of NP rows of parts: channel 16 s + 4 g + e at place
+// 32 (s / 2) + 8 g + 4 (s % 2) + e, so that the eight of one lane's 16x16x32 operand lie together and a
+// float's channels are those the lanes hold of the state.
+template <int NP, int LP>
+__device__ __forceinline__ void put_parts(u16* planes, int row, int c, int m, f4 v) {
+  const Parts a = parts(v[0], v[1]), b = parts(v[2], v[3]);
+  u16* at = planes + row * LP + 32 * (2 * c + (m >> 3)) + 8 * (m & 3) + 4 * ((m >> 2) & 1);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(at + k * NP * LP) = u32x2{a.p[k], b.p[k]};
+}
+struct Split {
+  b8 p[3];
+};
+template <int NP, int LP>
+__device__ __forceinline__ Split get_parts(const u16* planes, int row, int at) {
+  Split r;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) r.p[k] = *reinterpret_cast<const b8*>(planes + (k * NP + row) * LP + at);
+  return r;
+}
+constexpr int kPa[6] = {0, 2, 1, 0, 1, 0}, kPb[6] = {2, 0, 1, 1, 0, 0};   // the small products first
+
 // One workgroup a (sequence, head): D / 32 waves of 32 value columns each, whose
 // slice of the state waits in registers while the scores are made.
 //   1. 16 lanes a place: log2 gamma by doubling along the paths; A and L as products of tiles
-//      of gamma_i q_i and k_j / gamma_j.  Where a path decays by more than 2^-100 its pairs are taken one by
-//      one instead, the quotient being the product of a over the places between, so that nothing
-//      overflows however strong the decay.
-//   2. (gamma q)^T S and (gamma k)^T S by 16x16x4 fp32 products, the state read once.
+//      of gamma_i q_i and k_j / gamma_j (TILES).  Where a path decays by more than 2^-80 its pairs are
+//      taken one by one instead, the quotient being the product of a over the places between, so that
+//      nothing overflows however strong the decay.
+//   2. (gamma q)^T S and (gamma k)^T S, the state read once.  Both kinds of products are of
+//      fp32 factors in three bf16 parts; as 16x16x4 fp32 products they were 24 us of matrix
+//      time for 64 sequences of 32 places and 16 heads, beside 26 of bytes, and the call took 48.
 //   3. u tile of 16 places by tile: inverses of the diagonal tiles (I + beta L)^-1 times what the
-//      tiles before leave, o from A u.  A tile's result is the next product's operand in
+//      tiles before leave, o from A u, in fp32.  A tile's result is the next product's operand in
 //      the registers it was made in (row 4 gq + e of its four is step e's).
-// All in fp32: the operations (4 N d^2 a head) take less than the state's and the
-// tokens' bytes.
-template <int D, int DT, int NT, int OUT>
+// That call takes 40 us warm: the bytes, and phases of the two workgroups of a CU that overlap in part
+// (a third does not fit the LDS).  Few sequences: a chain of loads, walk, products, 8.4 us for B8 N6 H16.
+template <int D, int DT, int NT, bool TILES, int OUT>
 __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
   constexpr int NW = D / 32, NP = 16 * NT, G = 4 * NW, NPG = NP / G > 0 ? NP / G : 1;   // places of a group of 16 lanes
-  constexpr int C4 = D / 64, LK = D + 4, LA = NP + 4, LT = 20;
-  __shared__ __attribute__((aligned(16))) float rk[NP * LK];   // k, then gamma k
-  __shared__ __attribute__((aligned(16))) float rq[NP * LK];   // log2 gamma (or a), then gamma q
-  __shared__ __attribute__((aligned(16))) float rn[NT > 1 ? NP * LK : 4];   // k / gamma
-  __shared__ __attribute__((aligned(16))) float As[NP * LA], Ls[NP * LA];
-  __shared__ __attribute__((aligned(16))) float Ts[NT * 16 * LT];
+  constexpr int C4 = D / 64, LK = D + 4, LA = NP + 4, LT = 20, LP = D + 8, PL = 3 * NP * LP;
+  constexpr int SMALL = 2 * NP * LA + NT * 16 * LT;
+  static_assert(2 * PL >= 4 * NP * LK, "what shares a place fits");
+  constexpr int THIRD = !TILES ? 0 : PL > 2 * SMALL ? PL : 2 * SMALL;
+  __shared__ __attribute__((aligned(16))) u16 pieces[2 * PL + THIRD];
+  __shared__ __attribute__((aligned(16))) float small[TILES ? 4 : SMALL];
+  u16* const rk = pieces;                // gamma k in parts; on a walk k before
+  u16* const rq = pieces + PL;           // gamma q; on a walk a before
+  u16* const rn = pieces + 2 * PL;       // log2 gamma; then k / gamma; then A, L, T
+  float* const fk = reinterpret_cast<float*>(rk);
+  float* const fq = reinterpret_cast<float*>(rq);
+  float* const fl = reinterpret_cast<float*>(TILES ? rn : rq);
+  float* const As = TILES ? fl : small;
+  float* const Ls = As + NP * LA;
+  float* const Ts = Ls + NP * LA;
   __shared__ float bet[NP];
   __shared__ int wide[NW];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -126,12 +177,12 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
         av[x][c][e] = on ? av[x][c][e] * kLog2e : 0.f;
       }
       lv[x][c] = av[x][c];
-      if constexpr (NT > 1) *reinterpret_cast<f4*>(rq + i * LK + 64 * c + 4 * m) = lv[x][c];
+      if constexpr (TILES) *reinterpret_cast<f4*>(fl + i * LK + 64 * c + 4 * m) = lv[x][c];
     }
     if (m == 0) bet[i] = bt[x];
   }
   // sums along the paths, their lengths doubling: what a place has plus what the place above its own has
-  int up = NT > 1 && path != 0 ? parent : -1;
+  int up = TILES && path != 0 ? parent : -1;
   while (__any(up >= 0)) {
     f4 more[NPG][C4];
     int ui[NPG];
@@ -140,7 +191,7 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
     for (int x = 0; x < NPG; ++x) {
       ui[x] = __shfl(up, place(x), 64);
 #pragma unroll
-      for (int c = 0; c < C4; ++c) more[x][c] = *reinterpret_cast<const f4*>(rq + max(ui[x], 0) * LK + 64 * c + 4 * m);
+      for (int c = 0; c < C4; ++c) more[x][c] = *reinterpret_cast<const f4*>(fl + max(ui[x], 0) * LK + 64 * c + 4 * m);
     }
     lds_barrier();
 #pragma unroll
@@ -149,7 +200,7 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
 #pragma unroll
       for (int c = 0; c < C4; ++c) {
         lv[x][c] += more[x][c];
-        *reinterpret_cast<f4*>(rq + place(x) * LK + 64 * c + 4 * m) = lv[x][c];
+        *reinterpret_cast<f4*>(fl + place(x) * LK + 64 * c + 4 * m) = lv[x][c];
       }
     }
     const int next = __shfl(up, max(up, 0), 64);
@@ -157,18 +208,16 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
   }
   // Within 2^kWide the quotient may be two factors: gamma_i q_i times k_j / gamma_j, and
   // the scores are products of tiles.  An addition of logarithms then rounds by 2^-18, 2.6e-6 of a
-  // factor, at most, and each has six; past it (or where one is not a number) the paths are walked.  So are
-  // those of up to 16 places, which are short: B8 N6 8.3 us and 8.8, B64 N16 24.9 and 26.3;
-  // 32 places 48.2 and 47.1 (64 of d = 64 in fp32 28.3 and 25.4), 64 75.8 and 61.7.
-  constexpr float kWide = 100.f;
-  bool far = NT == 1;
+  // factor, at most, and each has six; past it (or where one is not a number) the paths are walked.
+  constexpr float kWide = 80.f;
+  bool far = !TILES;
 #pragma unroll
   for (int x = 0; x < NPG; ++x)
 #pragma unroll
     for (int c = 0; c < C4; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) far |= !(fabsf(lv[x][c][e]) <= kWide);
-  if (NT > 1) {
+  if (TILES) {
     const bool any = __any(far);
     if (lane == 0) wide[wave] = any;
     lds_barrier();
@@ -176,10 +225,9 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
 #pragma unroll
     for (int x = 0; x < NW; ++x) far |= wide[x] != 0;
   }
-  if (NT > 1 && __builtin_amdgcn_readfirstlane(far) == 0) {
+  if (TILES && __builtin_amdgcn_readfirstlane(far) == 0) {
 #pragma unroll
     for (int x = 0; x < NPG; ++x) {
-      const int at = place(x) * LK + 4 * m;
 #pragma unroll
       for (int c = 0; c < C4; ++c) {
         f4 gm, in;
@@ -188,34 +236,50 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
           gm[e] = fast_exp2(lv[x][c][e]);
           in[e] = fast_exp2(-lv[x][c][e]);
         }
-        *reinterpret_cast<f4*>(rk + at + 64 * c) = gm * kv[x][c];
-        *reinterpret_cast<f4*>(rq + at + 64 * c) = gm * qv[x][c];
-        *reinterpret_cast<f4*>(rn + at + 64 * c) = in * kv[x][c];
+        put_parts<NP, LP>(rk, place(x), c, m, gm * kv[x][c]);
+        put_parts<NP, LP>(rq, place(x), c, m, gm * qv[x][c]);
+        put_parts<NP, LP>(rn, place(x), c, m, in * kv[x][c]);
       }
     }
     lds_barrier();
     // tiles (r, y <= r) of A and of beta L, dealt out to the waves
-    for (int it = wave; it < NT * (NT + 1); it += NW) {
-      const int t = it >> 1, r = t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0, y = t - r * (r + 1) / 2;
-      const float* rows = it & 1 ? rk : rq;
+    constexpr int ITEMS = NT * (NT + 1), MINE = (ITEMS + NW - 1) / NW;
+    auto tile = [](int it, int& r, int& y) {
+      const int t = it >> 1;
+      r = t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0;
+      y = t - r * (r + 1) / 2;
+    };
+    f4 sc[MINE];
+#pragma unroll
+    for (int n = 0; n < MINE; ++n) {
+      const int it = wave + n * NW;
+      sc[n] = f4{0, 0, 0, 0};
+      if (it >= ITEMS) continue;
+      int r, y;
+      tile(it, r, y);
       f4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        const f4 x = *reinterpret_cast<const f4*>(rows + (16 * r + m) * LK + 16 * s + 4 * gq);
-        const f4 z = *reinterpret_cast<const f4*>(rn + (16 * y + m) * LK + 16 * s + 4 * gq);
+      for (int p = 0; p < D / 32; ++p) {
+        const Split x = get_parts<NP, LP>(it & 1 ? rk : rq, 16 * r + m, 32 * p + 8 * gq);
+        const Split z = get_parts<NP, LP>(rn, 16 * y + m, 32 * p + 8 * gq);
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          s0 = mfma4(x[e], z[e], s0);
-          s1 = mfma4(x[e + 1], z[e + 1], s1);
-        }
+        for (int k = 0; k < 6; ++k) (p & 1 ? s1 : s0) = mma32_bf16(p & 1 ? s1 : s0, x.p[kPa[k]], z.p[kPb[k]]);
       }
-      s0 += s1;
+      sc[n] = s0 + s1;
+    }
+    lds_barrier();                       // k / gamma has been read; the scores go there
+#pragma unroll
+    for (int n = 0; n < MINE; ++n) {
+      const int it = wave + n * NW;
+      if (it >= ITEMS) continue;
+      int r, y;
+      tile(it, r, y);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 16 * r + 4 * gq + e, j = 16 * y + m;
         const bool on = shfl_u64(path, i) >> j & 1;
-        if (it & 1) Ls[i * LA + j] = on && j != i ? bet[i] * s0[e] : 0.f;
-        else As[i * LA + j] = on ? s0[e] : 0.f;
+        if (it & 1) Ls[i * LA + j] = on && j != i ? bet[i] * sc[n][e] : 0.f;
+        else As[i * LA + j] = on ? sc[n][e] : 0.f;
       }
     }
   } else {
@@ -229,8 +293,8 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
       for (int c = 0; c < C4; ++c) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) av[x][c][e] = fast_exp2(av[x][c][e]);
-        *reinterpret_cast<f4*>(rk + place(x) * LK + 64 * c + 4 * m) = kv[x][c];
-        *reinterpret_cast<f4*>(rq + place(x) * LK + 64 * c + 4 * m) = av[x][c];
+        *reinterpret_cast<f4*>(fk + place(x) * LK + 64 * c + 4 * m) = kv[x][c];
+        *reinterpret_cast<f4*>(fq + place(x) * LK + 64 * c + 4 * m) = av[x][c];
       }
     lds_barrier();
 #pragma unroll
@@ -247,8 +311,8 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
         float sq = 0.f, sk = 0.f;
 #pragma unroll
         for (int c = 0; c < C4; ++c) {
-          const f4 t = av[x][c] * *reinterpret_cast<const f4*>(rk + max(j, 0) * LK + 64 * c + 4 * m);
-          const f4 aj = *reinterpret_cast<const f4*>(rq + max(j, 0) * LK + 64 * c + 4 * m);
+          const f4 t = av[x][c] * *reinterpret_cast<const f4*>(fk + max(j, 0) * LK + 64 * c + 4 * m);
+          const f4 aj = *reinterpret_cast<const f4*>(fq + max(j, 0) * LK + 64 * c + 4 * m);
           sq = dot4(qv[x][c], t, sq);
           sk = dot4(kv[x][c], t, sk);
           if (j >= 0) av[x][c] *= aj;
@@ -264,11 +328,10 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
     lds_barrier();
 #pragma unroll
     for (int x = 0; x < NPG; ++x) {
-      const int i = place(x);
 #pragma unroll
       for (int c = 0; c < C4; ++c) {
-        *reinterpret_cast<f4*>(rk + i * LK + 64 * c + 4 * m) = av[x][c] * kv[x][c];
-        *reinterpret_cast<f4*>(rq + i * LK + 64 * c + 4 * m) = av[x][c] * qv[x][c];
+        put_parts<NP, LP>(rk, place(x), c, m, av[x][c] * kv[x][c]);
+        put_parts<NP, LP>(rq, place(x), c, m, av[x][c] * qv[x][c]);
       }
     }
   }
@@ -292,19 +355,33 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) pk[r][c] = pq[r][c] = f4{0, 0, 0, 0};
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s)
+  for (int p = 0; p < D / 32; ++p) {
+    Split st[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      u32x4 w[3];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const f2* s = &S[2 * p + (x >> 1)][2 * (x & 1)];
+        const Parts two = parts(s[0][c], s[1][c]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) w[k][x] = two.p[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) st[c].p[k] = __builtin_bit_cast(b8, w[k]);
+    }
 #pragma unroll
     for (int r = 0; r < NT; ++r) {
-      const f4 fk = *reinterpret_cast<const f4*>(rk + (16 * r + m) * LK + 16 * s + 4 * gq);
-      const f4 fq = *reinterpret_cast<const f4*>(rq + (16 * r + m) * LK + 16 * s + 4 * gq);
+      const Split xk = get_parts<NP, LP>(rk, 16 * r + m, 32 * p + 8 * gq), xq = get_parts<NP, LP>(rq, 16 * r + m, 32 * p + 8 * gq);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int k = 0; k < 6; ++k)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          pk[r][c] = mfma4(fk[e], S[s][e][c], pk[r][c]);
-          pq[r][c] = mfma4(fq[e], S[s][e][c], pq[r][c]);
+          pk[r][c] = mma32_bf16(pk[r][c], xk.p[kPa[k]], st[c].p[kPb[k]]);
+          pq[r][c] = mma32_bf16(pq[r][c], xq.p[kPa[k]], st[c].p[kPb[k]]);
         }
     }
+  }
   lds_barrier();                         // the inverses are there
   f4 u[NT][2];
 #pragma unroll
@@ -414,16 +491,20 @@ __global__ __launch_bounds__(2 * D) void kda_tree_commit_kernel(TreeCommitArgs a
   for (int i = 0; i < RPT; ++i) *reinterpret_cast<f4*>(S + (d0 + i) * D) = gam[d0 + i] * sv[i] + acc[i];
 }
 
-template <int D, int DT, int NT>
+template <int D, int DT, int NT, bool TILES>
 hipError_t step_out(const TreeStepArgs& a, int out, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(a.B * a.H)), block(2 * D);
-  if (out == 0) kda_tree_step_kernel<D, DT, NT, 0><<<grid, block, 0, s>>>(a);
-  else kda_tree_step_kernel<D, DT, NT, 1><<<grid, block, 0, s>>>(a);
+  if (out == 0) kda_tree_step_kernel<D, DT, NT, TILES, 0><<<grid, block, 0, s>>>(a);
+  else kda_tree_step_kernel<D, DT, NT, TILES, 1><<<grid, block, 0, s>>>(a);
   return hipGetLastError();
 }
 template <int D, int DT>
 hipError_t step_places(const TreeStepArgs& a, int out, hipStream_t s) {
-  return a.N <= 16 ? step_out<D, DT, 1>(a, out, s) : a.N <= 32 ? step_out<D, DT, 2>(a, out, s) : step_out<D, DT, 4>(a, out, s);
+  // Paths of up to eight places are walked: B8 N6 8.4 us and 8.7 with products, B2 N7 6.1 and 6.5; a
+  // chain of 16 (B4) 11.1 and 9.1, B32 N12 14.5 and 14.0, 32 places (B64) 47.4 and 39.7.
+  if (a.N <= 8) return step_out<D, DT, 1, false>(a, out, s);
+  if (a.N <= 16) return step_out<D, DT, 1, true>(a, out, s);
+  return a.N <= 32 ? step_out<D, DT, 2, true>(a, out, s) : step_out<D, DT, 4, true>(a, out, s);
 }
 template <int D>
 hipError_t step_types(const TreeStepArgs& a, int dt, int out, hipStream_t s) {

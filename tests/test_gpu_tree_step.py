@@ -38,6 +38,24 @@ def test_sizes(cuda, N, d, dtype):
     compare(step_inputs(len(kinds), N, 2, d, dtype, cuda, seed=N, decay=0.2), p, scale=0.5)
 
 
+@pytest.mark.parametrize("N", [8, 9, 12])
+@pytest.mark.parametrize("d,dtype", [(128, "fp32"), (64, "bf16")])
+def test_sizes_where_products_replace_the_walk(cuda, N, d, dtype):
+    p = trees(["random", "chain", "star", "broken"], N, cuda, seed=N)
+    compare(step_inputs(4, N, 3, d, dtype, cuda, seed=N, decay=0.2), p, scale=2.0)
+
+
+@pytest.mark.parametrize("N", [5, 14, 30, 50])
+def test_states_of_any_size(cuda, N):
+    """fp32 factors are split for the products: no size of a state's entry costs them precision."""
+    x = step_inputs(3, N, 2, 128, "fp32", cuda, seed=N, decay=0.1)
+    gen = torch.Generator(device=cuda).manual_seed(N)
+    x["state"][0] *= 1e-20
+    x["state"][1] *= 1e20
+    x["state"][2] *= 10.0 ** (30 * torch.rand(2, 128, 1, device=cuda, generator=gen) - 15)
+    compare(x, trees(["random", "chain", "deep"], N, cuda, seed=N))
+
+
 @pytest.mark.parametrize("decay", [0.0, 1.0, 30.0, 150.0])
 def test_decays(cuda, decay):
     """No decay at all, and decays under which a product of a few underflows."""
