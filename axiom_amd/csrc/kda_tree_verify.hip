@@ -285,10 +285,22 @@ __global__ __launch_bounds__(kThreads) void kda_tree_sample_kernel(TreeVerifyArg
     w.rej |= u64{1} << i;
     if (!kids) break;
     if constexpr (DRAFT) {
-      const int len = ((a.V + kWaves - 1) / kWaves + 63) & ~63;
-      double sum, plain;
-      sum_range<DT, DRAFT, false>(w, z, x, min(a.V, wave * len), min(a.V, (wave + 1) * len), sum, plain);
-      sum = wave_sum(sum);
+      // A wave's entries in four parts, which the slices take in turns: what one fetches another finds in
+      // its L2.  The parts' sums are added in one order.
+      constexpr int ROUND = 1024;
+      const int len = ((a.V + kWaves - 1) / kWaves + 63) & ~63, cut = len < 4 * ROUND ? len : (len / 4 + ROUND - 1) / ROUND * ROUND;
+      const int end = min(a.V, (wave + 1) * len);
+      double quarter[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 1
+      for (int t = 0; t < 4; ++t) {
+        const int k = (t + s) & 3, from = wave * len + k * cut;
+        if (from >= end) continue;
+        double part, plain;
+        sum_range<DT, DRAFT, false>(w, z, x, from, min(end, from + cut), part, plain);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) quarter[y] = y == k ? part : quarter[y];
+      }
+      double sum = wave_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]));
       if (lane == 0) red[turn][wave] = sum;
       const double qx = real ? ld1<DT>(w.draft, i * a.d_row + x) : 0.0;
       if ((kids >> lane) & 1) r = fmax(r - Z * qx, 0.0);   // of the children still to ask
