@@ -147,9 +147,10 @@ def _up(x):
 def test_decode_workspace(L, B, N, H, R, page, per, code):
     """Starts of the sequences on the line, and two parts a workgroup of every run where there are runs."""
     m = 16 if N * H <= 16 or code == 0 else 64
-    kt, pad, cap = (16, 8, page * per) if m == 16 else (32, 4, page * per)
     groups = -(-N * H // m)
-    runs = ((-(-cap // kt) + pad) * B + 1) // 2
+    kt, pad, cap = (16, 8, page * per) if m == 16 else (32, 4 if groups == 1 else 8, page * per)
+    least = 2 if groups == 1 else 4
+    runs = ((-(-cap // kt) + pad) * B + least - 1) // least
     if cap <= 128:
         slots = 0
     elif groups == 1:
