@@ -955,7 +955,7 @@ __global__ __launch_bounds__(R / 2) void kda_latent_join_kernel(LatentDecodeArgs
 
 // The same for a tree's 64 rows a workgroup, whose parts lie as the output waves held
 // them, 32 rows by R: every read and write is 1 KiB in a row (a row's own 2 KiB between
-// rows take twice as long: 16 and 10 us with 256 rows of 32 sequences).  A wave
+// rows take twice as long: 16 and 10 us with 256 rows of 32 sequences; with fewer cuts now 9).  A wave
 // takes PW groups of eight columns of 32 rows.
 template <int DT, int R, int PW>
 __global__ __launch_bounds__(256) void kda_latent_tree_join_kernel(LatentDecodeArgs a) {
@@ -999,7 +999,9 @@ __global__ __launch_bounds__(256) void kda_latent_tree_join_kernel(LatentDecodeA
 // The cache after an accepted path: its rows move to the front of the places'.  A
 // thread takes the same 16 bytes of every row; rows move down only, so kMoves
 // rows read and then written clobber none that the next ones read, and threads
-// need not wait for each other.  Bound by the moved rows' bytes.
+// need not wait for each other.  Bound by the moved rows, single ones of 1152 bytes all over a
+// cache of 1.3 GB behind a chain of loads (parents, pages, rows): eight layers, 256 sequences of 64
+// places 20.7 us, 12 of bytes; one sequence 4.2, its launch.
 constexpr int kMoves = 16;
 __global__ __launch_bounds__(192) void kda_latent_tree_commit_kernel(LatentTreeCommitArgs a) {
   const int lane = threadIdx.x & 63, b = blockIdx.x, N = a.N;

@@ -438,7 +438,8 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
 // The state after the path of place last[b], in place: two workgroups a (sequence,
 // head), each half of the value columns.  A thread holds four columns of D / 16
 // channels; the path's decayed keys go through LDS, the newest 16 places first,
-// while the state is on its way.  Bound by the state's bytes, read and written once.
+// while the state is on its way.  Bound by the state's bytes, read and written once: 64
+// sequences of 16 heads, trees of 32 places, 31.2 us, 4.5 TB/s; one sequence 3.5, its launch.
 template <int D, int DT>
 __global__ __launch_bounds__(2 * D) void kda_tree_commit_kernel(TreeCommitArgs a) {
   constexpr int W = D / 2, NCQ = W / 4, RPT = D / 16, PIECE = 16;

@@ -4,8 +4,11 @@
 //
 // A decision compares 24-bit numbers' products and sums over a vocabulary; all of
 // that is in 64 bits, so another order of the same sums decides alike but for one
-// case in 2^40 or so.  Bound by the one or two rows that the next token is drawn
-// from; the walk itself needs a few entries of the rows, a lane a place.
+// case in 2^40 or so.  Bound by rows: one of the target and of each draft refused for the next
+// token, and the same for every sibling asked after a refusal, since Z is a sum over the
+// vocabulary; the walk itself needs a few entries of the rows, a lane a place.  64 sequences
+// of 16 places and 128000 fp32 entries: 51 us, of which a pass over one pair of rows of all
+// is 13 of bytes, two to three are needed in turn, and 7 are the second launch.
 
 #include "kda_internal.h"
 #include "kda_tree.h"
@@ -286,7 +289,7 @@ __global__ __launch_bounds__(kThreads) void kda_tree_sample_kernel(TreeVerifyArg
     if (!kids) break;
     if constexpr (DRAFT) {
       // A wave's entries in four parts, which the slices take in turns: what one fetches another finds in
-      // its L2.  The parts' sums are added in one order.
+      // its L2 (cold 47.2 us for 49.6).  The parts' sums are added in one order, so all see one Z.
       constexpr int ROUND = 1024;
       const int len = ((a.V + kWaves - 1) / kWaves + 63) & ~63, cut = len < 4 * ROUND ? len : (len / 4 + ROUND - 1) / ROUND * ROUND;
       const int end = min(a.V, (wave + 1) * len);
@@ -407,7 +410,10 @@ __device__ __forceinline__ u64 best_of(const void* row, int lo, int hi) {
   return wave_max(at < 0 ? 0 : best_key(top, at));
 }
 
-// The largest entry of a slice of a row: a workgroup each, of every row that a walk can reach.
+// The largest entry of a slice of a row: a workgroup each, of every row that a walk can reach (which
+// one it does is known only after the rows before it).  Bound by their bytes where
+// there are many, 54 sequences of 2 places and 129186 entries 18 us; 16 of 8 places and 50021 bf16 7, and 3
+// of the walk's launch.
 template <int DT>
 __global__ __launch_bounds__(256) void kda_tree_best_kernel(TreeVerifyArgs a) {
   constexpr int ES = DT == 0 ? 4 : 2;
@@ -466,7 +472,7 @@ hipError_t verify(const TreeVerifyArgs& a, hipStream_t s) {
     return hipGetLastError();
   }
   // A sequence's slices eight workgroups apart, on one XCD, whose L2 then serves the rows that
-  // all of them sum: 64 sequences of 128000 bf16 entries, warm, 30.1 us for 32.9; fewer than
+  // all of them sum: 64 sequences of 128000 fp32 entries, warm, 30.1 us for 32.9; fewer than
   // eight would leave XCDs idle.
   const unsigned wide = a.slices > 1 ? (a.B >= 8 ? 8 : 1) : a.B;
   const dim3 grid(wide, a.slices, (a.B + wide - 1) / wide), block(kThreads);
