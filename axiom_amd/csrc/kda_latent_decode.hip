@@ -585,8 +585,8 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
 // with 32 rows each and 16 keys at a time, which reads LDS half as often, took 112:
 // the chain is per tile, not per key.
 // A tree of drafts (TREE) has many groups of 64 rows against the same cache.  25 drafts,
-// 64 heads, 4 sequences of 20000 to 32768 tokens, fp16: 380 to 400 us, 930 TFLOP/s over all
-// rows (780 over those that hold a draft).  What bounds it there is the copies: 36 KB a tile and CU go to
+// 64 heads, 4 sequences of 20000 to 32768 tokens, fp16: 370 to 400 us, 950 TFLOP/s over all
+// rows (800 over those that hold a draft).  What bounds it there is the copies: 36 KB a tile and CU go to
 // LDS at 21 to 28 bytes a clock, 1300 to 1750 of a tile's 2500 clocks, and nothing hides them whole.
 // Score waves of 32 rows (half the LDS reads of keys) took as long or longer in four
 // arrangements, 16 or 32 keys a tile, alternating or sharing tiles: 395 to 745 us.
@@ -744,7 +744,8 @@ __global__ __launch_bounds__(512) void kda_latent_decode64_kernel(LatentDecodeAr
       if constexpr (TREE) {
         // Without the mask, whose branches keep the scheduler from the products around them: 25
         // drafts, 64 heads, four sequences of 20000 to 32768 tokens 394 us for 430 (fp16, cold
-        // cache; warm 389 and 393), 32 sequences of up to 8192 with 256 rows 85 for 96.
+        // cache; warm 389 and 393), 32 sequences of up to 8192 with 256 rows 85 for 96
+        // (77 since a start counts as eight tiles).
         for (const int most = min(clear, tb); i + 7 <= most; i += 4) {
           step(none, i, buf0, buf2);
           step(none, i + 1, buf1, buf3);
