@@ -90,6 +90,28 @@ __device__ __forceinline__ Split get_parts(const u16* planes, int row, int at) {
 }
 constexpr int kPa[6] = {0, 2, 1, 0, 1, 0}, kPb[6] = {2, 0, 1, 1, 0, 0};   // the small products first
 
+// Logarithms along a path are whole numbers of 2^-24: their sums are exact, so gamma_i / gamma_j of two
+// places far down a path is as good as their own few decays (a float of 64 or more has steps
+// of 2^-17, and a pair's decay would err by those of the whole path before it).  A gate's own
+// logarithm is off by 2^-25 whatever its size: what the product with log2 e rounds away is added.
+constexpr float kUnits = 16777216.f, kWideGate = 55.f;
+constexpr unsigned kWide = 80u << 24;
+__device__ __forceinline__ unsigned log2_units(float g) {
+  constexpr float low = 1.925963e-8f * kUnits;   // of log2 e, what the float lacks
+  g = fminf(fmaxf(g, -64.f), 64.f);              // past kWideGate, and a whole number holds it
+  const float t = g * (kLog2e * kUnits), rest = fmaf(g, low, fmaf(g, kLog2e * kUnits, -t));
+  return static_cast<unsigned>(static_cast<int>(rintf(t)) + static_cast<int>(rintf(rest)));
+}
+// 2^x and 2^-x of such a number: only the fraction's powers round
+__device__ __forceinline__ void exp2_units(unsigned x, float& up, float& down) {
+  const int whole = static_cast<int>(x) >> 24;
+  const float part = static_cast<float>(x & 0xFFFFFFu) * (1.f / kUnits);
+  up = ldexpf(fast_exp2(part), whole);
+  down = ldexpf(fast_exp2(-part), -whole);
+}
+// bits of |x|: in the order of the values, with infinity and what is no number last
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
 // One workgroup a (sequence, head): D / 32 waves of 32 value columns each, whose
 // slice of the state waits in registers while the scores are made.
 //   1. 16 lanes a place: log2 gamma by doubling along the paths; A and L as products of tiles
@@ -162,7 +184,8 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
   __builtin_amdgcn_sched_barrier(0);
 
   const u64 path = tree_paths(parent, N), live = __ballot(path != 0);
-  f4 lv[NPG][C4];                        // log2 gamma of the places in hand
+  u32x4 lv[NPG][C4];                     // log2 gamma of the places in hand, in units
+  unsigned gates = 0;
 #pragma unroll
   for (int x = 0; x < NPG; ++x) {
     const int i = place(x);
@@ -174,24 +197,27 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
       for (int e = 0; e < 4; ++e) {
         kv[x][c][e] = on ? kv[x][c][e] : 0.f;
         qv[x][c][e] = on ? qv[x][c][e] * a.scale : 0.f;
-        av[x][c][e] = on ? av[x][c][e] * kLog2e : 0.f;
+        av[x][c][e] = on ? av[x][c][e] : 0.f;
+        if constexpr (TILES) {
+          lv[x][c][e] = log2_units(av[x][c][e]);
+          gates = max(gates, abs_bits(av[x][c][e]));
+        }
       }
-      lv[x][c] = av[x][c];
-      if constexpr (TILES) *reinterpret_cast<f4*>(fl + i * LK + 64 * c + 4 * m) = lv[x][c];
+      if constexpr (TILES) *reinterpret_cast<u32x4*>(fl + i * LK + 64 * c + 4 * m) = lv[x][c];
     }
     if (m == 0) bet[i] = bt[x];
   }
   // sums along the paths, their lengths doubling: what a place has plus what the place above its own has
   int up = TILES && path != 0 ? parent : -1;
   while (__any(up >= 0)) {
-    f4 more[NPG][C4];
+    u32x4 more[NPG][C4];
     int ui[NPG];
     lds_barrier();
 #pragma unroll
     for (int x = 0; x < NPG; ++x) {
       ui[x] = __shfl(up, place(x), 64);
 #pragma unroll
-      for (int c = 0; c < C4; ++c) more[x][c] = *reinterpret_cast<const f4*>(fl + max(ui[x], 0) * LK + 64 * c + 4 * m);
+      for (int c = 0; c < C4; ++c) more[x][c] = *reinterpret_cast<const u32x4*>(fl + max(ui[x], 0) * LK + 64 * c + 4 * m);
     }
     lds_barrier();
 #pragma unroll
@@ -200,25 +226,26 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
 #pragma unroll
       for (int c = 0; c < C4; ++c) {
         lv[x][c] += more[x][c];
-        *reinterpret_cast<f4*>(fl + place(x) * LK + 64 * c + 4 * m) = lv[x][c];
+        *reinterpret_cast<u32x4*>(fl + place(x) * LK + 64 * c + 4 * m) = lv[x][c];
       }
     }
     const int next = __shfl(up, max(up, 0), 64);
     up = up >= 0 ? next : up;
   }
-  // Within 2^kWide the quotient may be two factors: gamma_i q_i times k_j / gamma_j, and
-  // the scores are products of tiles.  An addition of logarithms then rounds by 2^-18, 2.6e-6 of a
-  // factor, at most, and each has six; past it (or where one is not a number) the paths are walked.
-  constexpr float kWide = 80.f;
+  // Within 2^80 the quotient may be two factors: gamma_i q_i times k_j / gamma_j, and
+  // the scores are products of tiles; past it, or where a gate is not a number, the paths are walked.
+  // (Sums that pass 2^128 wrap, but not unseen: the places above have theirs, and a gate is less than
+  // the 96 by which one within 80 could reach another such.)
   bool far = !TILES;
-#pragma unroll
-  for (int x = 0; x < NPG; ++x)
-#pragma unroll
-    for (int c = 0; c < C4; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) far |= !(fabsf(lv[x][c][e]) <= kWide);
   if (TILES) {
-    const bool any = __any(far);
+    unsigned logs = 0;
+#pragma unroll
+    for (int x = 0; x < NPG; ++x)
+#pragma unroll
+      for (int c = 0; c < C4; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) logs = max(logs, lv[x][c][e] + kWide);
+    const bool any = __any(logs > 2 * kWide || gates > __float_as_uint(kWideGate));
     if (lane == 0) wide[wave] = any;
     lds_barrier();
     far = false;
@@ -233,8 +260,10 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
         f4 gm, in;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          gm[e] = fast_exp2(lv[x][c][e]);
-          in[e] = fast_exp2(-lv[x][c][e]);
+          float up, down;
+          exp2_units(lv[x][c][e], up, down);
+          gm[e] = up;
+          in[e] = down;
         }
         put_parts<NP, LP>(rk, place(x), c, m, gm * kv[x][c]);
         put_parts<NP, LP>(rq, place(x), c, m, gm * qv[x][c]);
@@ -292,7 +321,7 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
 #pragma unroll
       for (int c = 0; c < C4; ++c) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) av[x][c][e] = fast_exp2(av[x][c][e]);
+        for (int e = 0; e < 4; ++e) av[x][c][e] = fast_exp2(av[x][c][e] * kLog2e);
         *reinterpret_cast<f4*>(fk + place(x) * LK + 64 * c + 4 * m) = kv[x][c];
         *reinterpret_cast<f4*>(fq + place(x) * LK + 64 * c + 4 * m) = av[x][c];
       }
