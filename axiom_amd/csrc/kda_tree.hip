@@ -94,7 +94,7 @@ constexpr int kPa[6] = {0, 2, 1, 0, 1, 0}, kPb[6] = {2, 0, 1, 1, 0, 0};   // the
 // places far down a path is as good as their own few decays (a float of 64 or more has steps
 // of 2^-17, and a pair's decay would err by those of the whole path before it).  A gate's own
 // logarithm is off by 2^-25 whatever its size: what the product with log2 e rounds away is added.
-constexpr float kUnits = 16777216.f, kWideGate = 55.f;
+constexpr float kUnits = 16777216.f, kWideGate = 55.f, kLarge = 0x1p40f, kSmall = 0x1p-24f;
 constexpr unsigned kWide = 80u << 24;
 __device__ __forceinline__ unsigned log2_units(float g) {
   constexpr float low = 1.925963e-8f * kUnits;   // of log2 e, what the float lacks
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
 
   const u64 path = tree_paths(parent, N), live = __ballot(path != 0);
   u32x4 lv[NPG][C4];                     // log2 gamma of the places in hand, in units
-  unsigned gates = 0;
+  unsigned gates = 0, most = 0, least = ~0u;   // |g|; of the largest entries that a lane has of a k and of a scale q
 #pragma unroll
   for (int x = 0; x < NPG; ++x) {
     const int i = place(x);
@@ -204,6 +204,18 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
         }
       }
       if constexpr (TILES) *reinterpret_cast<u32x4*>(fl + i * LK + 64 * c + 4 * m) = lv[x][c];
+    }
+    if constexpr (TILES) {
+      unsigned tk = 0, tq = 0;
+#pragma unroll
+      for (int c = 0; c < C4; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          tk = max(tk, abs_bits(kv[x][c][e]));
+          tq = max(tq, abs_bits(qv[x][c][e]));
+        }
+      most = max(most, max(tk, tq));
+      least = min(least, min(tk - 1, tq - 1));   // of zeros only: none
     }
     if (m == 0) bet[i] = bt[x];
   }
@@ -234,6 +246,8 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
   }
   // Within 2^80 the quotient may be two factors: gamma_i q_i times k_j / gamma_j, and
   // the scores are products of tiles; past it, or where a gate is not a number, the paths are walked.
+  // So they are where q or k is so large that such a factor may overflow (2^40), or so small (2^-24) that
+  // its third part may be below 2^-126, which the matrix unit takes for 0: the pair's share need be neither.
   // (Sums that pass 2^128 wrap, but not unseen: the places above have theirs, and a gate is less than
   // the 96 by which one within 80 could reach another such.)
   bool far = !TILES;
@@ -245,7 +259,8 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
       for (int c = 0; c < C4; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) logs = max(logs, lv[x][c][e] + kWide);
-    const bool any = __any(logs > 2 * kWide || gates > __float_as_uint(kWideGate));
+    const bool any = __any(logs > 2 * kWide || gates > __float_as_uint(kWideGate) || most > __float_as_uint(kLarge) ||
+                           least < __float_as_uint(kSmall) - 1);
     if (lane == 0) wide[wave] = any;
     lds_barrier();
     far = false;

@@ -114,3 +114,46 @@ def test_sums_that_pass_the_range_several_times(cuda, strong):
     x = coherent(len(KINDS), 24, 2, 128, "fp32", 0.0, 0.5, seed=strong)
     x["g"][:, 3:3 + strong] -= 64 * 0.6931471805599453
     rows_right(x, one_root(trees(KINDS, 24, cuda, seed=strong)))
+
+
+SIZED = [(9, 128), (16, 64), (17, 128), (40, 64), (64, 128)]
+
+
+@pytest.mark.parametrize("N,d", SIZED)
+def test_large_keys_far_down_a_path(cuda, N, d):
+    """A key of 2^58 where the path has decayed to 2^-78: k / gamma has no float, the pair's share has."""
+    x = coherent(2, N, 2, d, "fp32", 54.0, 0.5, seed=N)
+    p = one_root(trees(["chain", "star"], N, cuda))
+    x["k"][0, -1] *= 2.0 ** 58                      # places that nothing continues
+    x["k"][1, N // 2:] *= 2.0 ** 58
+    rows_right(x, p)
+
+
+@pytest.mark.parametrize("N,d", SIZED)
+def test_small_queries_far_down_a_path(cuda, N, d):
+    """gamma q below the least float: the read-out of what the path itself wrote is as exact as ever."""
+    x = coherent(2, N, 2, d, "fp32", 50.0, 0.5, seed=N)
+    x["q"][0] *= 2.0 ** -60
+    x["q"][1, N // 2] *= 2.0 ** -70
+    rows_right(x, one_root(trees(["chain", "deep"], N, cuda)))
+
+
+@pytest.mark.parametrize("N,d", SIZED)
+def test_small_keys_behind_growing_gates(cuda, N, d):
+    """k / gamma below the least float, over a state of nothing."""
+    x = coherent(2, N, 2, d, "fp32", -50.0, 0.5, seed=N)
+    x["k"][0] *= 2.0 ** -60
+    x["k"][1, N // 2:] *= 2.0 ** -70
+    x["state"].zero_()
+    rows_right(x, one_root(trees(["chain", "star"], N, cuda)))
+
+
+def test_a_small_scale(cuda):
+    x = coherent(2, 33, 2, 128, "fp32", 50.0, 0.5, seed=1)
+    p = one_root(trees(["chain", "random"], 33, cuda))
+    ins = [x[n] for n in ("q", "k", "v", "g", "beta")]
+    o, u = axiom_amd.kda_tree_step(*ins, p, x["state"])
+    small, same = axiom_amd.kda_tree_step(*ins, p, x["state"], scale=2.0 ** -60)
+    want = O.step(*ins, p, x["state"])[0]
+    err = (small.cpu().double() * 2.0 ** 60 - want).norm(dim=-1) / want.norm(dim=-1)
+    assert err.max() <= ROW and ((u - same).norm(dim=-1) <= ROW * u.norm(dim=-1)).all()
