@@ -393,6 +393,20 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
     }
   }
 
+  // Third parts of entries under 2^-102 would be below 2^-126, the matrix unit's 0: a wave whose columns hold
+  // nothing of 2^-63 (an exponent with either of its two highest bits) takes 2^64 of them.
+  unsigned any = 0;
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) any |= __float_as_uint(S[s][e][0]) | __float_as_uint(S[s][e][1]);
+  const bool lift = !__any(any & 0x60000000u);
+  if (lift) {
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[s][e] *= 0x1p64f;
+  }
   f4 pk[NT][2], pq[NT][2];
 #pragma unroll
   for (int r = 0; r < NT; ++r)
@@ -425,6 +439,15 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
           pq[r][c] = mma32_bf16(pq[r][c], xq.p[kPa[k]], st[c].p[kPb[k]]);
         }
     }
+  }
+  if (lift) {
+#pragma unroll
+    for (int r = 0; r < NT; ++r)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        pk[r][c] *= 0x1p-64f;
+        pq[r][c] *= 0x1p-64f;
+      }
   }
   lds_barrier();                         // the inverses are there
   f4 u[NT][2];

@@ -157,3 +157,13 @@ def test_a_small_scale(cuda):
     want = O.step(*ins, p, x["state"])[0]
     err = (small.cpu().double() * 2.0 ** 60 - want).norm(dim=-1) / want.norm(dim=-1)
     assert err.max() <= ROW and ((u - same).norm(dim=-1) <= ROW * u.norm(dim=-1)).all()
+
+
+@pytest.mark.parametrize("size", [2.0 ** -110, 2.0 ** -118])
+@pytest.mark.parametrize("N,d", [(6, 128), (7, 64), (14, 128), (30, 64), (50, 128)])
+def test_a_state_near_the_least_float(cuda, N, d, size):
+    """Nothing but such a state is read out: no v."""
+    x = coherent(4, N, 2, d, "fp32", 0.0, 0.5, seed=N)
+    x["v"].zero_()
+    x["state"] *= size
+    rows_right(x, one_root(trees(KINDS, N, cuda, seed=N)), of_terms=True)
