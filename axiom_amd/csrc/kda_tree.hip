@@ -206,16 +206,16 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
       if constexpr (TILES) *reinterpret_cast<u32x4*>(fl + i * LK + 64 * c + 4 * m) = lv[x][c];
     }
     if constexpr (TILES) {
-      unsigned tk = 0, tq = 0;
+      float tk = 0.f, tq = 0.f;
 #pragma unroll
       for (int c = 0; c < C4; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          tk = max(tk, abs_bits(kv[x][c][e]));
-          tq = max(tq, abs_bits(qv[x][c][e]));
+          tk = fmaxf(tk, fabsf(kv[x][c][e]));
+          tq = fmaxf(tq, fabsf(qv[x][c][e]));
         }
-      most = max(most, max(tk, tq));
-      least = min(least, min(tk - 1, tq - 1));   // of zeros only: none
+      most = max(most, max(__float_as_uint(tk), __float_as_uint(tq)));
+      least = min(least, min(__float_as_uint(tk) - 1, __float_as_uint(tq) - 1));   // of zeros only: none
     }
     if (m == 0) bet[i] = bt[x];
   }
