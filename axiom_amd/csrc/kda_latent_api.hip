@@ -192,7 +192,9 @@ bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
 // A tree of drafts: the same, but that a tree has many row groups, so the runs a
 // sequence is cut into are no longer multiples of eight: as many as give each CU a
 // workgroup, dealt out so that the groups of a run meet in one XCD's L2.  25 groups:
-// 250 workgroups, 200 otherwise.  A sequence begun costs 64 rows' queries and 128 KiB
+// 250 workgroups, 200 otherwise.  With more groups whole runs leave CUs idle: 86 have two, 172 workgroups, 129 to
+// 255 have one (fp32, 64 heads, four sequences of up to 4096: 32 places 897 us, 33 places 1742;
+// bf16, 128 heads, up to 8192: 32 places 217, 43 places 384).  A sequence begun costs 64 rows' queries and 128 KiB
 // of parts, eight tiles' time: 32 sequences of up to 8192 tokens with 256 rows take
 // 77 us, 84 with pad = 4, 78 with 12 and 82 with 18; four of 32768 with 1600 rows alike.
 // Runs of four tiles at least: 17 and 19 us for two in small calls of many groups, with eight

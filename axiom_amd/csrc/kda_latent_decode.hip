@@ -105,6 +105,10 @@ __global__ __launch_bounds__(256) void kda_latent_append_kernel(LatentAppendArgs
 // fp32, with operands twice as large: two score waves and a ring of four.
 // 64 sequences of 1 to 8192 tokens, H16 R512 dr64 bf16: 28.8 us with the join, 3.0
 // TB/s of the cache's bytes, in fp32 66; one of 512 tokens 12.9 us, a chain of loads.
+// Of a tree (TREE), 32 sequences of up to 8192 tokens, R512 dr64: 16 rows in bf16 29 us and in fp32 60, 256 rows in
+// fp32 629, 42 TFLOP/s; one sequence of 512 13.8.  Page numbers of the tiles that hold places are loaded
+// behind the copies and waited for at once, so those tiles cost a round of loads each; the fp32 kernel
+// of a tree with R512 dr64 spills five registers (24 bytes a lane).
 template <int DT, int R, int DR>
 struct DecCfg {
   static constexpr int ES = El<DT>::ES;
@@ -586,7 +590,9 @@ __global__ __launch_bounds__(512) void kda_latent_decode16_kernel(LatentDecodeAr
 // the chain is per tile, not per key.
 // A tree of drafts (TREE) has many groups of 64 rows against the same cache.  25 drafts,
 // 64 heads, 4 sequences of 20000 to 32768 tokens, fp16: 370 to 400 us, 950 TFLOP/s over all
-// rows (800 over those that hold a draft).  What bounds it there is the copies: 36 KB a tile and CU go to
+// rows (800 over those that hold a draft: the others' are computed as well and thrown away).  Probabilities go to the output
+// waves in the inputs' type, as without a tree, since the products take no other: of an error of 2.1e-3 in bf16 the
+// output's own rounding is 1.7e-3.  What bounds it there is the copies: 36 KB a tile and CU go to
 // LDS at 21 to 28 bytes a clock, 1300 to 1750 of a tile's 2500 clocks, and nothing hides them whole.
 // Score waves of 32 rows (half the LDS reads of keys) took as long or longer in four
 // arrangements, 16 or 32 keys a tile, alternating or sharing tiles: 395 to 745 us.

@@ -115,8 +115,9 @@ __device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x
 // One workgroup a (sequence, head): D / 32 waves of 32 value columns each, whose
 // slice of the state waits in registers while the scores are made.
 //   1. 16 lanes a place: log2 gamma by doubling along the paths; A and L as products of tiles
-//      of gamma_i q_i and k_j / gamma_j (TILES).  Where a path decays by more than 2^-80 its pairs are
-//      taken one by one instead, the quotient being the product of a over the places between, so that
+//      of gamma_i q_i and k_j / gamma_j (TILES).  Where one channel of one path decays by more than 2^-80 (or
+//      grows by as much, or a q or k is very large or small) the whole workgroup takes its pairs one by
+//      one instead, the quotient being the product of a over the places between, so that
 //      nothing overflows however strong the decay.
 //   2. (gamma q)^T S and (gamma k)^T S, the state read once.  Both kinds of products are of
 //      fp32 factors in three bf16 parts; as 16x16x4 fp32 products they were 24 us of matrix
@@ -124,8 +125,10 @@ __device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x
 //   3. u tile of 16 places by tile: inverses of the diagonal tiles (I + beta L)^-1 times what the
 //      tiles before leave, o from A u, in fp32.  A tile's result is the next product's operand in
 //      the registers it was made in (row 4 gq + e of its four is step e's).
-// That call takes 40 us warm: the bytes, and phases of the two workgroups of a CU that overlap in part
-// (a third does not fit the LDS).  Few sequences: a chain of loads, walk, products, 8.4 us for B8 N6 H16.
+// That call takes 41 us (49 if every head has a path past 2^80): the bytes, and phases of the two workgroups of
+// a CU that overlap in part (a third does not fit the LDS).  33 to 64 places: 157 KB of LDS and one wave a SIMD, so
+// nothing overlaps: B16 chains of 64 29 us and 58 past 2^80, where gates of -0.9 a token bring them; B32 trees 57
+// and 88.  Few sequences: a chain of loads, walk, products, 8.4 us for B8 N6 H16.
 template <int D, int DT, int NT, bool TILES, int OUT>
 __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
   constexpr int NW = D / 32, NP = 16 * NT, G = 4 * NW, NPG = NP / G > 0 ? NP / G : 1;   // places of a group of 16 lanes
@@ -504,9 +507,11 @@ __global__ __launch_bounds__(2 * D) void kda_tree_step_kernel(TreeStepArgs a) {
 
 // The state after the path of place last[b], in place: two workgroups a (sequence,
 // head), each half of the value columns.  A thread holds four columns of D / 16
-// channels; the path's decayed keys go through LDS, the newest 16 places first,
-// while the state is on its way.  Bound by the state's bytes, read and written once: 64
-// sequences of 16 heads, trees of 32 places, 31.2 us, 4.5 TB/s; one sequence 3.5, its launch.
+// channels; the path's decayed keys go through LDS, the newest 16 places first.  Bound by the
+// state's bytes, read and written once: 64 sequences of 16 heads, trees of 32 places, 31.2 us, 4.5 TB/s.
+// A place's k and g are waited for before the next one's are asked for (the first time behind the state's
+// loads), then u two places at a time: one sequence 3.6 us for a path of two places, its launch, but
+// 5.4 for eight, 13.7 for 32 and 24.6 for 64; 16 sequences of 64 45.
 template <int D, int DT>
 __global__ __launch_bounds__(2 * D) void kda_tree_commit_kernel(TreeCommitArgs a) {
   constexpr int W = D / 2, NCQ = W / 4, RPT = D / 16, PIECE = 16;
@@ -568,8 +573,8 @@ hipError_t step_out(const TreeStepArgs& a, int out, hipStream_t s) {
 }
 template <int D, int DT>
 hipError_t step_places(const TreeStepArgs& a, int out, hipStream_t s) {
-  // Paths of up to eight places are walked: B8 N6 8.4 us and 8.7 with products, B2 N7 6.1 and 6.5; a
-  // chain of 16 (B4) 11.1 and 9.1, B32 N12 14.5 and 14.0, 32 places (B64) 47.4 and 39.7.
+  // Paths of up to eight places are walked: B8 N6 8.4 us and 9.0 with products, B64 N8 20.2 and 23.9; a
+  // chain of 16 (B4) 11.2 and 9.4, B32 N12 14.7 and 14.7, 32 places (B64) 48.4 and 40.6.
   if (a.N <= 8) return step_out<D, DT, 1, false>(a, out, s);
   if (a.N <= 16) return step_out<D, DT, 1, true>(a, out, s);
   return a.N <= 32 ? step_out<D, DT, 2, true>(a, out, s) : step_out<D, DT, 4, true>(a, out, s);

@@ -7,8 +7,12 @@
 // case in 2^40 or so.  Bound by rows: one of the target and of each draft refused for the next
 // token, and the same for every sibling asked after a refusal, since Z is a sum over the
 // vocabulary; the walk itself needs a few entries of the rows, a lane a place.  64 sequences
-// of 16 places and 128000 fp32 entries: 51 us, of which a pass over one pair of rows of all
-// is 13 of bytes, two to three are needed in turn, and 7 are the second launch.
+// of 16 places and 128000 fp32 entries: 52 us, of which a pass over one pair of rows of all
+// is 13 of bytes, two to three are needed in turn (a place has three children at most), and 7 are the
+// second launch.  R is not kept: after its k-th refusal among siblings a workgroup reads the target's row and
+// k of draft's, all of them whole, so k refused siblings cost k^2 / 2 rows one after the other.  Every child refused, 128000
+// fp32 entries, B1 and B64: 3 children 45 and 120 us, 8 220 and 685, 24 1.8 and 3.9 ms, 64 (B1) 12 ms.  Without
+// draft Z needs no row: 64 sequences of 16 places as trees 17 us, as stars 30.
 
 #include "kda_internal.h"
 #include "kda_tree.h"
@@ -412,8 +416,8 @@ __device__ __forceinline__ u64 best_of(const void* row, int lo, int hi) {
 
 // The largest entry of a slice of a row: a workgroup each, of every row that a walk can reach (which
 // one it does is known only after the rows before it).  Bound by their bytes where
-// there are many, 54 sequences of 2 places and 129186 entries 18 us; 16 of 8 places and 50021 bf16 7, and 3
-// of the walk's launch.
+// there are many, 64 sequences of 16 places and 128000 bf16 61 us for 279 MB, of which a walk over
+// three rows needs 49; 16 of 8 places and 50021 bf16 7, and 3 of the walk's launch.
 template <int DT>
 __global__ __launch_bounds__(256) void kda_tree_best_kernel(TreeVerifyArgs a) {
   constexpr int ES = DT == 0 ? 4 : 2;

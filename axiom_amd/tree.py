@@ -44,7 +44,8 @@ def kda_tree_step(q, k, v, g, beta, parents, state, scale: float = 1.0, out_dtyp
     S``, ``u_i = beta_i (v_i - S~^T k_i)``, ``S_i = S~ + k_i u_i^T`` and ``o_i =
     scale S_i^T q_i``.  ``o [B,N,H,dv]`` in ``out_dtype`` (fp32 or bf16), ``u
     [B,N,H,dv]`` fp32 for :func:`kda_tree_commit`.  ``out`` / ``u``: optional
-    preallocated outputs.
+    preallocated outputs.  A decay between two places is as exact as those of the places
+    between them, however far the path has decayed before.
     """
     return _ext().tree_step(q, k, v, g, beta, parents, state, scale, out_dtype, out, u)
 
@@ -111,7 +112,8 @@ def tree_verify(target, tokens, parents, uniforms=None, draft=None, workspace=No
     target's dtype), the distribution that the token was drawn from, or, without
     ``draft``, 1 at the token.  Where no child is left the next token is drawn from R
     with ``uniforms[N]``.  Accepted tokens and the next are then distributed as draws
-    from the target.  Sums and comparisons are in 64 bits.  A row without any positive
+    from the target.  Sums and comparisons are in 64 bits.  With ``draft`` the k-th refusal at
+    a row reads k + 1 rows of V again: many refused children of one place are slow.  A row without any positive
     entry gives -1; a token outside [0, V) is never accepted.
     """
     return _ext().tree_verify(target, tokens, parents, uniforms, draft, workspace)

@@ -34,7 +34,10 @@ extern "C" {
  *   o_i = scale S_i^T q_i.
  * o [B,N,H,dv] in out_dtype (F32 or BF16); u [B,N,H,dv] fp32, what
  * kda_tree_commit needs of the call.  dk == dv in {64, 128}.  Pointers aligned
- * to 16 bytes (beta and parents to their elements).
+ * to 16 bytes (beta and parents to their elements).  A decay between two places is
+ * as exact as those of the places between them, however far the path has decayed
+ * before; scale q_i and k_i times the decay of their whole path are read against
+ * `state` with fp32's bits down to 2^-102 (what is smaller by its bits to 2^-126).
  */
 KDA_API int kda_tree_step(hipStream_t stream, const void* q, const void* k, const void* v, const void* g,
                 const void* beta, const int32_t* parents, const float* state, void* o, float* u, int B, int N, int H,
@@ -106,7 +109,8 @@ KDA_API int kda_latent_tree_commit(hipStream_t stream, void* cache, const int32_
  * times the whole sum (where R has none, from the row as it was; -1 where
  * that has none; entries that are not positive count as 0).  So the accepted
  * tokens and the next are distributed as the target's own draws.  Sums,
- * products and comparisons in 64 bits.  A token outside [0, V) is never
+ * products and comparisons in 64 bits.  With draft the k-th refusal at a row
+ * reads k + 1 rows of V again: many refused children of one place are slow.  A token outside [0, V) is never
  * accepted.
  *
  * last int32 [B]: the last accepted place (-1: none); next int64 [B]: the
