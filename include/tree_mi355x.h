@@ -36,8 +36,9 @@ extern "C" {
  * kda_tree_commit needs of the call.  dk == dv in {64, 128}.  Pointers aligned
  * to 16 bytes (beta and parents to their elements).  A decay between two places is
  * as exact as those of the places between them, however far the path has decayed
- * before; scale q_i and k_i times the decay of their whole path are read against
- * `state` with fp32's bits down to 2^-102 (what is smaller by its bits to 2^-126).
+ * before.  In the read-out of `state` the bits of scale q_i and k_i times their
+ * path's decay end at 2^-126, and so do those of a state's entries beside ones of
+ * 2^-63 and more.
  */
 KDA_API int kda_tree_step(hipStream_t stream, const void* q, const void* k, const void* v, const void* g,
                 const void* beta, const int32_t* parents, const float* state, void* o, float* u, int B, int N, int H,
